@@ -41,6 +41,9 @@ EXPORTED = (
     "nls_profile_next",
     "nls_profile_next_generic", "nls_get_plan", "nls_status_string", "nls_last_error",
     "nls_lm_head_workspace", "nls_lm_head", "nls_lm_head_row_bytes", "nls_argmax",
+    "nls_rope_frequencies", "nls_rope", "nls_cache_append", "nls_paged_attention_workspace", "nls_paged_attention",
+    "nls_cache_workspace", "nls_cache_reserve", "nls_cache_fork", "nls_cache_release", "nls_cache_compact",
+    "nls_cache_copy_pages",
 )
 
 
@@ -49,6 +52,28 @@ class NlsLora(ctypes.Structure):
 
     _fields_ = [("d_a", ctypes.c_void_p), ("d_b", ctypes.c_void_p), ("rank", ctypes.c_int32),
                 ("scale", ctypes.c_float)]
+
+
+def _c_struct(doc, name, **fields):
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": list(fields.items())})
+
+
+_vp, _i32, _i64, _f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
+NlsHeads = _c_struct("nls_heads: rows of heads", "NlsHeads", d=_vp, token_stride=_i64, head_stride=_i64)
+NlsRopeScaling = _c_struct("nls_rope_scaling", "NlsRopeScaling", kind=_i32, base=_f64, factor=_f64, original_context=_f64,
+                           beta_fast=_f64, beta_slow=_f64, attn_factor=_f64, freq_factors=ctypes.POINTER(_f64))
+NlsRopePlan = _c_struct("nls_rope_plan", "NlsRopePlan", d_freqs=_vp, dim=_i32, interleaved=_i32,
+                        amplitude=ctypes.c_float)
+NlsPagedKv = _c_struct("nls_paged_kv: one layer of the cache", "NlsPagedKv", d_kv=_vp, type=_i32, pages=_i32,
+                       page_size=_i32, kv_heads=_i32, head_dim=_i32, page_stride=_i64, value_offset=_i64,
+                       head_stride=_i64, token_stride=_i64, d_table=_vp, table_stride=_i64, slots=_i32, max_pages=_i32,
+                       d_lens=_vp)
+NlsChunks = _c_struct("nls_chunks: the new tokens of a call", "NlsChunks", seqs=_i32, tokens=_i32, d_starts=_vp,
+                      d_slots=_vp)
+NlsPagePool = _c_struct("nls_page_pool: the pages of all layers", "NlsPagePool", d_kv=_vp, layers=_i32,
+                        page_bytes=_i64, layer_stride=_i64, page_stride=_i64)
+NlsPageTables = _c_struct("nls_page_tables: who holds which page", "NlsPageTables", d_table=_vp, table_stride=_i64,
+                          slots=_i32, max_pages=_i32, d_lens=_vp, d_refs=_vp, pages=_i32, page_size=_i32)
 
 
 class NlsParams(ctypes.Structure):
@@ -158,6 +183,21 @@ def lib():
         L.nls_lm_head.argtypes = [vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, vp, ctypes.c_int32, vp,
                                   ctypes.c_int32, P(NlsLora), vp, ctypes.c_size_t, vp]
         L.nls_lm_head.restype = ctypes.c_int32
+        i32, i64, hp, kp, cp = ctypes.c_int32, ctypes.c_int64, P(NlsHeads), P(NlsPagedKv), P(NlsChunks)
+        L.nls_rope_frequencies.argtypes = [P(NlsRopeScaling), i32, P(ctypes.c_double), P(ctypes.c_double)]
+        L.nls_rope.argtypes = [P(NlsRopePlan), i32, hp, hp, i32, i32, i32, vp, i32, vp]
+        L.nls_cache_append.argtypes = [kp, cp, P(NlsRopePlan), i32, hp, hp, i32, hp, hp, vp]
+        L.nls_paged_attention_workspace.argtypes = [kp, cp, i32, i32, i64, i32]
+        L.nls_paged_attention_workspace.restype = ctypes.c_size_t
+        L.nls_paged_attention.argtypes = [kp, cp, i32, hp, hp, i32, ctypes.c_float, i32, vp, vp, i32, i64] + ws
+        pp, tp = P(NlsPagePool), P(NlsPageTables)
+        L.nls_cache_workspace.argtypes = [tp, i32]
+        L.nls_cache_workspace.restype = ctypes.c_size_t
+        L.nls_cache_reserve.argtypes = [tp, vp, vp] + ws
+        L.nls_cache_fork.argtypes = [pp, tp, vp, vp, i32, vp] + ws
+        L.nls_cache_release.argtypes = [tp, vp, i32, vp] + ws
+        L.nls_cache_compact.argtypes = [pp, tp, vp] + ws
+        L.nls_cache_copy_pages.argtypes = [pp, i32, vp, vp, i32, vp]
         _lib = L
     return _lib
 
@@ -665,3 +705,306 @@ def lm_head(weight, ggml_type: int, rows: int, cols: int, x, exact: bool = False
                             ctypes.byref(lo) if lo is not None else None, ctypes.c_void_p(work.data_ptr()),
                             work.numel(), ctypes.c_void_p(stream)), "nls_lm_head")
     return out if x.dim() == 2 else out.reshape(rows)
+
+
+# ---------------------------------------------------------------- attention over a paged cache
+
+
+def _elem_type(t) -> int:
+    import torch
+
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(t.dtype)
+    if code is None:
+        raise SamplerError(f"element type {t.dtype} is not float32, float16 or bfloat16")
+    return code
+
+
+def _on(device, *tensors, dtype=None):
+    for t in tensors:
+        if t is None:
+            continue
+        assert t.is_cuda and t.device == device, "tensors of one call on different devices"
+        assert dtype is None or t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
+
+
+def _ints(device, *tensors):
+    import torch
+
+    _on(device, *tensors, dtype=torch.int32)
+    assert all(t is None or t.is_contiguous() for t in tensors), "int32 tensors are contiguous"
+
+
+def _heads(t):
+    """A [tokens, heads, head_dim] tensor as nls_heads."""
+    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] <= 1), "rows of heads: [tokens, heads, head_dim], elements side by side"
+    return NlsHeads(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _launch(device, call, *args, what):
+    """The call on the device's current stream, with that device current."""
+    import torch
+
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        check(call(*args, stream), what)
+    else:
+        with torch.cuda.device(device):
+            check(call(*args, stream), what)
+
+
+@dataclass
+class RopePlan:
+    """Rotary positions of a model: each pair's angle per position (float64 device
+    tensor [dim / 2]), whether pairs are neighbours (2j, 2j + 1) or halves
+    (j, j + dim / 2), and the amplitude."""
+
+    freqs: object
+    interleaved: bool = True
+    amplitude: float = 1.0
+
+    def _c(self, device):
+        import torch
+
+        _on(device, self.freqs, dtype=torch.float64)
+        assert self.freqs.dim() == 1 and self.freqs.is_contiguous()
+        return NlsRopePlan(self.freqs.data_ptr(), 2 * self.freqs.numel(), int(self.interleaved), self.amplitude)
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+
+
+def rope_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                     original_context: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     attn_factor: float = 1.0, freq_factors=None):
+    """(angles per position of the dim / 2 pairs, amplitude), on the host: the
+    rope.* keys of a GGUF file and its rope_freqs tensor (freq_factors)."""
+    if scaling not in ROPE_SCALINGS:
+        raise SamplerError(f"rope scaling {scaling!r} is none of {sorted(ROPE_SCALINGS)}")
+    n = max(dim // 2, 1)
+    ff = None
+    if freq_factors is not None:
+        ff = [float(f) for f in freq_factors]
+        assert len(ff) == dim // 2, f"freq_factors: {len(ff)} entries, dim / 2 = {dim // 2}"
+        ff = (ctypes.c_double * n)(*ff)
+    out, amp = (ctypes.c_double * n)(), ctypes.c_double()
+    s = NlsRopeScaling(ROPE_SCALINGS[scaling], base, factor, original_context, beta_fast, beta_slow, attn_factor, ff)
+    check(lib().nls_rope_frequencies(ctypes.byref(s), dim, out, ctypes.byref(amp)), "nls_rope_frequencies")
+    return list(out)[:dim // 2], amp.value
+
+
+def rope_plan(dim: int, interleaved: bool = True, device="cuda", **scaling) -> RopePlan:
+    """A RopePlan for the first `dim` elements of each head (rope_frequencies'
+    arguments); interleaved as llama's GGUF files have it, halves as qwen's."""
+    import torch
+
+    freqs, amp = rope_frequencies(dim, **scaling)
+    return RopePlan(torch.tensor(freqs, dtype=torch.float64, device=device), interleaved, amp)
+
+
+def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
+    """x [tokens, heads, head_dim] with the first elements of each head turned by
+    its token's position (int32 [tokens]); `inverse` takes a gradient back.
+    `out` may be x.  Returns out."""
+    import torch
+
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _on(x.device, x, out, dtype=x.dtype)
+    _ints(x.device, positions)
+    assert out.shape == x.shape and positions.numel() == x.shape[0]
+    _launch(x.device, lib().nls_rope, plan._c(x.device), _elem_type(x), _heads(x), _heads(out), x.shape[0], x.shape[1],
+            x.shape[2], positions.data_ptr(), int(inverse), what="nls_rope")
+    return out
+
+
+def _paged_kv(kv, table, lens):
+    assert kv.dim() == 5 and kv.shape[1] == 2 and kv.stride(4) == 1, (
+        "a layer of the cache: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
+    _on(kv.device, kv)
+    _ints(kv.device, lens)
+    _on(kv.device, table, dtype=lens.dtype)
+    assert table.dim() == 2 and table.stride(1) == 1 and lens.numel() == table.shape[0]
+    st = kv.stride()
+    return NlsPagedKv(kv.data_ptr(), _elem_type(kv), kv.shape[0], kv.shape[3], kv.shape[2], kv.shape[4], st[0], st[1],
+                      st[2], st[3], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], lens.data_ptr())
+
+
+def _chunks(x, starts, slots):
+    _ints(x.device, starts, slots)
+    seqs = starts.numel() - 1
+    assert seqs >= 0 and (slots is None or slots.numel() == seqs)
+    return NlsChunks(seqs, x.shape[0], starts.data_ptr(), _ptr(slots))
+
+
+def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan] = None, slots=None, out=None):
+    """The new tokens of a layer into the cache: k turned by `plan` (None: as it
+    is) and v, both [tokens, kv_heads, head_dim], to the pages of their
+    positions; q [tokens, heads, head_dim] turned into `out` (which may be q).
+    Sequence i's tokens are rows starts[i] .. starts[i + 1] and the last ones of
+    slot slots[i] (i when None), whose lens count them already.  Returns out."""
+    import torch
+
+    assert k.shape == v.shape and k.shape[1] == kv.shape[2] and k.shape[2] == kv.shape[4]
+    _on(kv.device, k, v, q, out, dtype=k.dtype)
+    heads = 0
+    if q is not None:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        heads = q.shape[1]
+        assert out.shape == q.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2]
+    else:
+        assert out is None, "out without q"
+    _launch(kv.device, lib().nls_cache_append, _paged_kv(kv, table, lens), _chunks(k, starts, slots),
+            None if plan is None else plan._c(kv.device), _elem_type(k), None if q is None else _heads(q),
+            None if q is None else _heads(out), heads, _heads(k), _heads(v), what="nls_cache_append")
+    return out
+
+
+def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, scale: Optional[float] = None,
+                    window: int = 0, first=None, slots=None, out=None, lse=None, work=None):
+    """Attention of the new tokens' q [tokens, heads, head_dim] over their slots'
+    cached keys and values (cache_append's arguments): causal, at most `window`
+    keys back when that is > 0, from key first[slot] on when given.  scale:
+    1 / sqrt(head_dim) by default.  max_new and max_len: what the caller knows of
+    the longest chunk and context (0: nothing); they choose how the work is
+    split, not what comes out.  lse: True, or a float32 [tokens, heads] tensor,
+    for the logarithm of each row's sum.  Rows of no sequence keep what `out` and
+    `lse` hold.  Returns out, or (out, lse)."""
+    import torch
+
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _on(kv.device, q, out, dtype=q.dtype)
+    assert out.shape == q.shape and q.dim() == 3 and q.shape[2] == kv.shape[4]
+    if lse is True:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    if lse is not None:
+        _on(kv.device, lse, dtype=torch.float32)
+        assert lse.is_contiguous() and lse.shape == q.shape[:2]
+    c, ch = _paged_kv(kv, table, lens), _chunks(q, starts, slots)
+    _ints(kv.device, first)
+    assert first is None or first.numel() == lens.numel()
+    heads = q.shape[1]
+    need = int(lib().nls_paged_attention_workspace(c, ch, heads, max_new, max_len, window))
+    if need and (work is None or work.numel() < need):
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch(kv.device, lib().nls_paged_attention, c, ch, _elem_type(q), _heads(q), _heads(out), heads,
+            q.shape[2] ** -0.5 if scale is None else scale, window, _ptr(first), _ptr(lse), max_new, max_len,
+            _ptr(work), 0 if work is None else work.numel(), what="nls_paged_attention")
+    return out if lse is None else (out, lse)
+
+
+PAGES_DONE, PAGES_NONE_LEFT, PAGES_ROW_FULL, PAGES_BAD_ENTRY = range(4)
+
+
+def _page_pool(kv):
+    assert kv.dim() == 6 and kv.shape[2] == 2 and (kv.shape[0] == 0 or kv[0, 0].is_contiguous()), (
+        "the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
+    n = kv.element_size()
+    return NlsPagePool(kv.data_ptr(), kv.shape[0], kv[0, 0].numel() * n, kv.stride(0) * n, kv.stride(1) * n)
+
+
+def _page_tables(table, lens, refs, page_size):
+    _ints(refs.device, lens, refs)
+    _on(refs.device, table, dtype=refs.dtype)
+    assert table.dim() == 2 and table.stride(1) == 1 and (lens is None or lens.numel() == table.shape[0])
+    return NlsPageTables(table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], _ptr(lens), refs.data_ptr(),
+                         refs.numel(), page_size)
+
+
+def _pages_call(what, refs, t, count, *args):
+    """One of the page calls with its workspace; returns its int32 word."""
+    import torch
+
+    need = int(lib().nls_cache_workspace(t, count))
+    work = torch.empty(max(need, 1), dtype=torch.uint8, device=refs.device)
+    word = torch.empty(1, dtype=torch.int32, device=refs.device)
+    _launch(refs.device, getattr(lib(), what), *args, word.data_ptr(), work.data_ptr(), need, what=what)
+    return word
+
+
+def cache_reserve(table, lens, refs, page_size: int, counts):
+    """Slot s grows by counts[s] (int32) tokens: the lowest free pages, in the
+    slots' order, and lens += counts.  Returns the status word (PAGES_DONE, or
+    why nothing was done) as an int32 device tensor [1]."""
+    _ints(refs.device, counts)
+    assert counts.numel() == table.shape[0]
+    t = _page_tables(table, lens, refs, page_size)
+    return _pages_call("nls_cache_reserve", refs, t, 0, t, counts.data_ptr())
+
+
+def cache_fork(kv, table, lens, refs, src, dst):
+    """The empty slots dst[i] (int32) become copies of the slots src[i]: full
+    pages shared, the last partial page copied in every layer of kv.  Returns the
+    status word."""
+    _ints(refs.device, src, dst)
+    _on(refs.device, kv)
+    assert src.numel() == dst.numel() and kv.shape[1] == refs.numel()
+    t = _page_tables(table, lens, refs, kv.shape[4])
+    return _pages_call("nls_cache_fork", refs, t, src.numel(), _page_pool(kv), t, _ptr(src), _ptr(dst), src.numel())
+
+
+def cache_release(table, lens, refs, slots, page_size: int):
+    """The slots (int32) let go of their pages and are empty.  Returns the
+    status word."""
+    _ints(refs.device, slots)
+    t = _page_tables(table, lens, refs, page_size)
+    return _pages_call("nls_cache_release", refs, t, 0, t, _ptr(slots), slots.numel())
+
+
+def cache_compact(kv, table, refs):
+    """Moves the held pages to the lowest ids, their contents in every layer and
+    the table's entries with them.  Returns how many are held, int32 [1]."""
+    _on(refs.device, kv)
+    assert kv.shape[1] == refs.numel()
+    t = _page_tables(table, None, refs, kv.shape[4])
+    return _pages_call("nls_cache_compact", refs, t, 0, _page_pool(kv), t)
+
+
+def cache_copy_pages(kv, src, dst):
+    """Page src[i] to page dst[i] (int32) in every layer of kv."""
+    _ints(kv.device, src, dst)
+    assert src.numel() == dst.numel()
+    _launch(kv.device, lib().nls_cache_copy_pages, _page_pool(kv), kv.shape[1], _ptr(src), _ptr(dst), src.numel(),
+            what="nls_cache_copy_pages")
+
+
+class PagedCache:
+    """Keys and values of `slots` contexts in pages: the device counterpart of the
+    dense cache of an nimllm context (src/nimllm/model.nim:300-302), for several
+    contexts that share one pool.
+
+    kv [layers, pages, 2, kv_heads, page_size, head_dim]; table [slots,
+    max_pages], lens [slots] and refs [pages] are int32.  A decoding step is
+    reserve(counts), then append and attend layer by layer; nothing of it waits
+    for the device, so it can be captured into a graph and replayed."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int,
+                 max_pages: int, dtype=None, device="cuda"):
+        import torch
+
+        device = torch.empty(0, device=device).device
+        self.kv = torch.zeros((layers, pages, 2, kv_heads, page_size, head_dim), dtype=dtype or torch.float32,
+                              device=device)
+        self.table = torch.full((slots, max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.page_size = page_size
+
+    def reserve(self, counts):
+        return cache_reserve(self.table, self.lens, self.refs, self.page_size, counts)
+
+    def append(self, layer: int, k, v, starts, q=None, plan=None, slots=None, out=None):
+        return cache_append(self.kv[layer], self.table, self.lens, starts, k, v, q=q, plan=plan, slots=slots, out=out)
+
+    def attend(self, layer: int, q, starts, **kw):
+        return paged_attention(q, self.kv[layer], self.table, self.lens, starts, **kw)
+
+    def fork(self, src, dst):
+        return cache_fork(self.kv, self.table, self.lens, self.refs, src, dst)
+
+    def release(self, slots):
+        return cache_release(self.table, self.lens, self.refs, slots, self.page_size)
+
+    def compact(self):
+        return cache_compact(self.kv, self.table, self.refs)

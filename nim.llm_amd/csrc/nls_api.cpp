@@ -34,6 +34,26 @@ int hip_fail(hipError_t e, const char* what) {
   return e == hipErrorOutOfMemory ? NLS_ERR_OUT_OF_MEMORY : NLS_ERR_HIP;
 }
 
+}  // namespace
+
+// The other translation units' errors (thrown strings stay inside).
+int nls::api_error(int status, const char* what) {
+  try {
+    g_last_error = what;
+  } catch (...) {
+  }
+  return status;
+}
+int nls::api_hip_error(hipError_t e, const char* what) {
+  try {
+    return hip_fail(e, what);
+  } catch (...) {
+    return e == hipErrorOutOfMemory ? NLS_ERR_OUT_OF_MEMORY : NLS_ERR_HIP;
+  }
+}
+
+namespace {
+
 #define NLS_HIP(call)                                   \
   do {                                                  \
     hipError_t e_ = (call);                             \

@@ -371,4 +371,8 @@ int lm_act_block_len(int type);
 bool lm_type_supported(int type);
 hipError_t launch_lm_head(const LmHeadCall& c, hipStream_t s);
 
+// nls_last_error's text and the status to return (nls_api.cpp)
+int api_error(int status, const char* what);
+int api_hip_error(hipError_t e, const char* what);
+
 }  // namespace nls
