@@ -1,0 +1,146 @@
+// nls_attend.h -- what the attention kernels share: element types as matrix
+// operands, the parts an fp32 number is split into, a row's place and its keys.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "nls_paged.h"
+
+namespace nls {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16x __attribute__((ext_vector_type(16)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float minus_inf() { return -__builtin_inff(); }
+
+template <typename TC>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+  typedef h8 vec;
+  static constexpr int kKeys = 32;  // keys per step of a wave: the depth of one product
+  // fp32 as two halves, 22 bits; the weights are up to 2^14, so that small
+  // ones stay clear of fp16's denormal range (2^-24 is 2^-38 of the largest)
+  static constexpr int kParts = 2;
+  static constexpr float kShift = 14.f;
+};
+template <>
+struct Elem<__bf16> {
+  typedef b8 vec;
+  static constexpr int kKeys = 32;
+  static constexpr int kParts = 3;  // fp32 as three times 8 bits, exactly
+  static constexpr float kShift = 0.f;
+};
+template <>
+struct Elem<float> {
+  typedef f4 vec;
+  static constexpr int kKeys = 16;
+  static constexpr int kParts = 1;
+  static constexpr float kShift = 0.f;
+};
+template <typename T, typename TC>
+constexpr int parts_of() {
+  return sizeof(T) == 4 ? Elem<TC>::kParts : 1;
+}
+
+__device__ __forceinline__ f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mma16(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// four elements of the depth per lane, one product each
+__device__ __forceinline__ f4 mma16(f4 a, f4 b, f4 c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+// x as N parts of the cache's type, largest first, into element j of p[0 .. N)
+template <int N>
+__device__ __forceinline__ void split(float x, h8* p, int j) {
+  const _Float16 hi = (_Float16)x;
+  p[0][j] = hi;
+  if constexpr (N > 1) p[1][j] = (_Float16)(x - (float)hi);
+}
+template <int N>
+__device__ __forceinline__ void split(float x, b8* p, int j) {
+  if constexpr (N == 1) {
+    p[0][j] = (__bf16)x;
+  } else {
+    // the upper 16 bits, cut: what is left is exact
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+      p[i][j] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(x) >> 16));
+      x -= hi;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void split(float x, f4* p, int j) {
+  p[0][j] = x;
+}
+
+// Which keys a sequence's tokens see: row r of kv head's group is token r /
+// group at position p, keys [low(p), p].
+struct Sees {
+  int64_t lo, p0;  // the first key of all; token 0's position
+  int window;
+  int64_t len;
+  __device__ int64_t low(int64_t p) const {
+    const int64_t w = p + 1 - window;
+    return window > 0 && w > lo ? w : lo;
+  }
+};
+__device__ __forceinline__ Sees sees_of(const AttendArgs& a, const Chunk& c) {
+  Sees s;
+  s.p0 = position_of(a.p, c, 0);
+  s.lo = a.first && c.slot >= 0 ? a.first[c.slot] : 0;
+  if (s.lo < 0) s.lo = 0;
+  s.window = a.window;
+  s.len = c.len;
+  return s;
+}
+
+// The keys that tokens t0 .. t1 see between them, from a multiple of 32 on, and
+// the parts of `keys` keys that they fall into (the last one takes the rest).
+struct Span {
+  int64_t lo, hi;
+  int parts;
+};
+__device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int64_t keys, int most) {
+  Span r;
+  r.lo = s.low(s.p0 + t0);
+  r.hi = s.p0 + t1 + 1 < s.len ? s.p0 + t1 + 1 : s.len;
+  r.lo &= ~int64_t{31};
+  const int64_t n = r.hi > r.lo ? (r.hi - r.lo + keys - 1) / keys : 1;
+  r.parts = (int)(n < most ? n : most);
+  return r;
+}
+
+// Where the parts of rows that are split over workgroups wait to be joined:
+// fp32 sums [part][row][D] relative to the part's largest score, and that
+// score (times log2 e) with the sum of the weights.
+struct Parts {
+  float* o;
+  float2* ml;
+  int64_t rows;   // of one part
+  int64_t keys;   // of one part
+  int most;       // parts at most; 1: none are used
+};
+
+// How a call's rows are dealt out.
+struct AttendPlan {
+  bool few, chunk;        // which kernels run
+  int few_tiles;          // of 16 rows per sequence and kv head (single tokens of wide groups: several)
+  int64_t few_rows, chunk_rows;
+  int64_t few_keys, chunk_keys;
+  int few_most, chunk_most;
+  int64_t chunk_tiles;
+  size_t few_bytes, chunk_bytes;
+};
+
+}  // namespace nls

@@ -129,6 +129,8 @@ def test_attention_refusals(pkg):
     # nothing to do is no error
     assert call(ch=_chunks(pkg, tokens=0, d_starts=None)) == OK
     assert call(ch=_chunks(pkg, seqs=0, d_starts=None)) == OK
+    for kw in (dict(tokens=0), dict(seqs=0)):
+        assert L.nls_paged_attention_workspace(_cache(pkg), _chunks(pkg, **kw), 4, 1, 1 << 20, 0) == 0
     # the workspace's own checks
     for kw in (dict(kv_heads=0), dict(head_dim=300), dict(page_size=5), dict(max_pages=0)):
         assert L.nls_paged_attention_workspace(_cache(pkg, **kw), _chunks(pkg), 4, 1, 100, 0) == 0
