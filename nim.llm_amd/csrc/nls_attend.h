@@ -19,6 +19,13 @@ constexpr float kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float minus_inf() { return -__builtin_inff(); }
 
+// x, computed no earlier than here: keeps what a rare path derives from it out
+// of the registers of the loop around it
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <typename TC>
 struct Elem;
 template <>
@@ -44,6 +51,14 @@ struct Elem<float> {
   static constexpr int kParts = 1;
   static constexpr float kShift = 0.f;
 };
+// 16-bit queries: the weights are rounded to the cache's type for the products.
+// The values are then divided by the sum of the rounded weights, which takes the
+// common part of the roundings out (all of it where one key has all the
+// weight); lse goes by the sum of the weights themselves.
+template <typename T, typename TC>
+constexpr bool rounds_weights() {
+  return sizeof(T) == 2;
+}
 template <typename T, typename TC>
 constexpr int parts_of() {
   return sizeof(T) == 4 ? Elem<TC>::kParts : 1;
@@ -82,6 +97,50 @@ __device__ __forceinline__ void split(float x, b8* p, int j) {
 template <int N>
 __device__ __forceinline__ void split(float x, f4* p, int j) {
   p[0][j] = x;
+}
+
+// c plus the elements of x, two products with 1 at a time
+__device__ __forceinline__ float plus_all(h8 x, float c) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2(h2{x[j], x[j + 1]}, h2{1, 1}, c, false);
+  return c;
+}
+__device__ __forceinline__ float plus_all(b8 x, float c) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) c = __builtin_amdgcn_fdot2_f32_bf16(b2{x[j], x[j + 1]}, b2{1.f, 1.f}, c, false);
+  return c;
+}
+
+// Values that are not finite meet weights of 0 in the rows that do not see
+// their keys, which would be NaN there.  Where rows see different keys they
+// leave the operand x, and what they stand for goes to the rows that see them
+// (`seen`: 1 for such a key and row, else 0): the products of indicators with
+// `seen` say which sums get an infinity or a NaN.
+template <typename V, typename Acc, typename Mma>
+__device__ __forceinline__ void only_seen(V& x, V seen, Acc& o, Mma&& mma) {
+  constexpr int n = sizeof(V) / sizeof(x[0]);
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < n; ++j) bad |= !(fabsf((float)x[j]) < __builtin_inff());
+  if (__ballot(bad) == 0) return;
+#pragma unroll 1
+  for (int kind = 0; kind < 3; ++kind) {  // infinity, minus infinity, NaN
+    const float it = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+    V is;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float f = (float)x[j];
+      is[j] = (kind == 2 ? f != f : f == it) ? 1.f : 0.f;
+    }
+    const Acc count = mma(is, seen, Acc{});
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(Acc) / 4); ++j) o[j] += count[j] > 0.f ? it : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < n; ++j)
+    if (!(fabsf((float)x[j]) < __builtin_inff())) x[j] = 0.f;
 }
 
 // Which keys a sequence's tokens see: row r of kv head's group is token r /
@@ -123,23 +182,31 @@ __device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int64_t k
 
 // Where the parts of rows that are split over workgroups wait to be joined:
 // fp32 sums [part][row][D] relative to the part's largest score, and that
-// score (times log2 e) with the sum of the weights.
+// score (times log2 e) with the sum of the weights, and of the weights as the
+// products took them.
 struct Parts {
   float* o;
-  float2* ml;
+  f4* ml;
   int64_t rows;   // of one part
   int64_t keys;   // of one part
   int most;       // parts at most; 1: none are used
 };
 
+constexpr int kChunkTile = 128;  // rows of a workgroup of the chunk kernel
+// log2 of the weight of a row's largest score: room for weights 2^8 larger
+template <typename TC>
+constexpr float chunk_shift() {
+  return __is_same(TC, _Float16) ? 7.f : 0.f;
+}
+hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+                        hipStream_t s);
+
 // How a call's rows are dealt out.
 struct AttendPlan {
   bool few, chunk;        // which kernels run
   int few_tiles;          // of 16 rows per sequence and kv head (single tokens of wide groups: several)
-  int64_t few_rows, chunk_rows;
-  int64_t few_keys, chunk_keys;
-  int few_most, chunk_most;
   int64_t chunk_tiles;
+  Parts few_parts, chunk_parts;  // (pointers unset)
   size_t few_bytes, chunk_bytes;
 };
 

@@ -39,6 +39,8 @@ constexpr int kFewThreads = 64 * kFewWaves;
 template <typename T, typename TC, int D>
 struct Few {
   static constexpr int kParts = parts_of<T, TC>();
+  // weights: 16-bit queries' too are two parts, since products cost nothing here
+  static constexpr int kWeightParts = sizeof(T) == 2 ? 2 : kParts;
   static constexpr int KT = Elem<TC>::kKeys, NSUB = KT / 16;
   static constexpr int KC = sizeof(TC) == 2 ? D / 32 : D / 16;   // K pieces of 16 bytes per lane and 16 keys
   static constexpr int KD = sizeof(TC) == 2 ? 8 : 4;             // elements of such a piece
@@ -56,8 +58,8 @@ template <typename T, typename TC, int D>
 __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts parts, int tiles, bool chunk_runs) {
   using F = Few<T, TC, D>;
   using vec = typename Elem<TC>::vec;
-  constexpr int NP = F::kParts, KT = F::KT, NSUB = F::NSUB;
-  extern __shared__ float few_lds[];  // [wave][16][D + 4] sums; before that, a step's weights
+  constexpr int NP = F::kParts, NW = F::kWeightParts, KT = F::KT, NSUB = F::NSUB;
+  extern __shared__ float few_lds[];  // [wave][16][D + 4] sums
   __shared__ float sh_m[kFewWaves][16], sh_l[kFewWaves][16];
 
   const int task = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
@@ -195,7 +197,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts pa
     for (int j = 0; j < NSUB * 4; ++j) top = vis[j] ? fmaxf(top, s_[j] * sc) : top;
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    top = fmaxf(top, m);
+    top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
     const float from = top == minus_inf() ? 0.f : top;
     const float shrink = exp2_(m - from);
     m = top;
@@ -209,73 +211,32 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts pa
 #pragma unroll
     for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
 
-    // A value that is not finite meets weights of 0 in the rows that do not see
-    // it: such steps, where rows see different keys, go key by key.
-    bool plain = true;
     if (!whole) {
-      bool odd = false;
 #pragma unroll
       for (int j = 0; j < NSUB * 4; ++j)
 #pragma unroll
-        for (int u = 0; u < F::U; ++u) {
+        for (int u = 0; u < F::U; ++u)
           if (!vok[j]) v[j][u] = VPiece<TC, F::E>{};
-#pragma unroll
-          for (int e = 0; e < F::E; ++e) odd |= !(fabsf((float)v[j][u].v[e]) < __builtin_inff());
-        }
-      plain = __ballot(odd) == 0;
     }
-    if (plain) {
-      if constexpr (sizeof(TC) == 2) {
-        vec p[NP];
+    constexpr int kDepth = sizeof(vec) / sizeof(TC);
+    vec p[NW], seen;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split<NP>(w[j], p, j);
-#pragma unroll
-        for (int u = 0; u < F::U; ++u)
-#pragma unroll
-          for (int e = 0; e < F::E; ++e) {
-            vec x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = v[j][u].v[e];
-#pragma unroll
-            for (int n = NP - 1; n >= 0; --n) o[u * F::E + e] = mma16(x, p[n], o[u * F::E + e]);
-          }
-      } else {
-#pragma unroll
-        for (int u = 0; u < F::U; ++u)
-#pragma unroll
-          for (int e = 0; e < F::E; ++e) {
-            f4 x, p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[j] = v[j][u].v[e];
-              p[j] = w[j];
-            }
-            o[u * F::E + e] = mma16(x, p, o[u * F::E + e]);
-          }
-      }
-    } else {
-      float* pw = few_lds + wave * 16 * (KT + 1);
-#pragma unroll
-      for (int j = 0; j < NSUB * 4; ++j) pw[i * (KT + 1) + (j >> 2) * 16 + g * 4 + (j & 3)] = vis[j] ? w[j] : -1.f;
-      __builtin_amdgcn_wave_barrier();
-      for (int n = 0; n < KT; ++n) {
-        const float x = pw[i * (KT + 1) + n];
-        const int64_t key = kb + n;
-        const int p = key < k1 ? page_of(a.p, c.slot, key) : -1;
-        if (p < 0 || x == -1.f) continue;
-        const TC* row_v = base + a.p.value_offset + (int64_t)p * a.p.page_stride + (key & mask) * a.p.token_stride;
-#pragma unroll
-        for (int u = 0; u < F::U; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int e = 0; e < F::E; ++e) {
-              const int d = u * 16 * F::E + (g * 4 + r) * F::E + e;
-              if (d < dim) o[u * F::E + e][r] += x * (float)row_v[d];
-            }
-      }
-      __builtin_amdgcn_wave_barrier();
+    for (int j = 0; j < kDepth; ++j) {
+      split<NW>(w[j], p, j);
+      seen[j] = vis[j] ? 1.f : 0.f;
     }
+#pragma unroll
+    for (int u = 0; u < F::U; ++u)
+#pragma unroll
+      for (int e = 0; e < F::E; ++e) {
+        vec x;
+#pragma unroll
+        for (int j = 0; j < kDepth; ++j) x[j] = v[j][u].v[e];
+        f4& sum_of = o[u * F::E + e];
+        if (!whole) only_seen(x, seen, sum_of, [](vec y, vec z, f4 c) { return mma16(y, z, c); });
+#pragma unroll
+        for (int n = NW - 1; n >= 0; --n) sum_of = mma16(x, p[n], sum_of);
+      }
   }
 
   // the waves' sums, relative to the largest of their maxima
@@ -320,7 +281,7 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts pa
     if (span.parts > 1) {
       const int64_t at = part * parts.rows + ((int64_t)task * a.p.kv_heads + kvh) * 16 + r;
       *reinterpret_cast<f4*>(parts.o + at * D + d) = s;
-      if (d == 0) parts.ml[at] = make_float2(rt, sum);
+      if (d == 0) parts.ml[at] = f4{rt, sum, sum, 0.f};
       continue;
     }
     const int rr = r0 + r, token = c.begin + rr / a.group, head = kvh * a.group + rr % a.group;
@@ -343,111 +304,96 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts pa
 // workgroup takes a row, D / 4 lanes across it and the parts side by side.
 constexpr int kJoinThreads = 256;
 
+// `tiles`: few_kernel's tiles per sequence; 0: the rows are chunk_kernel's.
 template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void few_join_kernel(AttendArgs a, Parts parts, int tiles, float shift) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts parts, int tiles, float shift) {
   constexpr int kAcross = D / 4, kSide = kJoinThreads / kAcross;
   __shared__ f4 sums[kSide][kAcross];
-  __shared__ float ls[kSide];
-  const int task = blockIdx.x / 16, r = blockIdx.x % 16, kvh = blockIdx.y;
-  const int seq = task / tiles, tile = task - seq * tiles;
+  __shared__ float ls[kSide], lrs[kSide];
+  const int size = tiles ? 16 : kChunkTile;
+  const int task = blockIdx.x / size, r = blockIdx.x % size, kvh = blockIdx.y;
+  int seq = -1, r0;
+  if (tiles) {
+    seq = task / tiles;
+    r0 = (task - seq * tiles) * 16;
+  } else {
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < a.p.seqs; s0 += 64) {
+      const int s = s0 + lane;
+      const int n = __popcll(__ballot(s < a.p.seqs && tile_base(a.p.starts[s < a.p.seqs ? s : 0], a.group, kChunkTile, s) <= task));
+      seq += n;
+      if (n < 64) break;
+    }
+    if (seq < 0) return;
+  }
   const Chunk c = chunk_of(a.p, seq);
   const int rows = c.n * a.group;
-  if ((rows > 16 && c.n != 1) || tile * 16 + r >= rows) return;
-  const int r0 = tile * 16, rn = rows - r0 < 16 ? rows - r0 : 16;
+  if ((rows <= 16 || c.n == 1) != (tiles > 0)) return;
+  if (!tiles) {
+    const int64_t x = (task - tile_base(c.begin, a.group, kChunkTile, seq)) * kChunkTile;
+    if (x < 0 || x >= rows) return;
+    r0 = (int)x;
+  }
+  if (r0 + r >= rows) return;
+  const int rn = rows - r0 < size ? rows - r0 : size;
   const Span span = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most);
   if (span.parts <= 1) return;
-  const int64_t at = ((int64_t)task * a.p.kv_heads + kvh) * 16 + r;
+  const int64_t at = ((int64_t)task * a.p.kv_heads + kvh) * size + r;
   float top = minus_inf();
-  for (int p = threadIdx.x & 63; p < span.parts; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at].x);
+  for (int p = threadIdx.x & 63; p < span.parts; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at][0]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float from = top == minus_inf() ? 0.f : top;
   const int x = threadIdx.x % kAcross, side = threadIdx.x / kAcross;
   f4 s{0, 0, 0, 0};
-  float l = 0.f;
+  float l = 0.f, lr = 0.f;
 #pragma unroll 4
   for (int p = side; p < span.parts; p += kSide) {
-    const float2 ml = parts.ml[p * parts.rows + at];
-    const float w = exp2_(ml.x - from);
+    const f4 ml = parts.ml[p * parts.rows + at];
+    const float w = exp2_(ml[0] - from);
     s += *reinterpret_cast<const f4*>(parts.o + (p * parts.rows + at) * D + x * 4) * w;
-    l += ml.y * w;
+    l += ml[1] * w;
+    lr += ml[2] * w;
   }
   sums[side][x] = s;
-  if (x == 0) ls[side] = l;
+  if (x == 0) {
+    ls[side] = l;
+    lrs[side] = lr;
+  }
   __syncthreads();
   if (side) return;
-  float sum = ls[0];
+  float sum = ls[0], sumr = lrs[0];
 #pragma unroll
   for (int y = 1; y < kSide; ++y) {
     s += sums[y][x];
     sum += ls[y];
+    sumr += lrs[y];
   }
   const int rr = r0 + r, token = c.begin + rr / a.group, head = kvh * a.group + rr % a.group;
   T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll
   for (int y = 0; y < 4; ++y)
-    if (x * 4 + y < a.p.dim) out[x * 4 + y] = (T)(sum == 0.f ? 0.f : s[y] / sum);
+    if (x * 4 + y < a.p.dim) out[x * 4 + y] = (T)(sumr == 0.f ? 0.f : s[y] / sumr);
   if (a.lse && x == 0)
     a.lse[(int64_t)token * a.heads + head] =
         sum == 0.f ? minus_inf() : (from + (__builtin_amdgcn_logf(sum) - shift)) * kLn2;
 }
 
-// ---------------------------------------------------------------- the others
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
-
-template <typename T, typename TC>
-__global__ __launch_bounds__(64) void attend_kernel(AttendArgs a) {
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  int seq = -1;
-  for (int s0 = 0; s0 < a.p.seqs + 1; s0 += 64) {
-    const int s = s0 + lane;
-    const int n = __popcll(__ballot(s <= a.p.seqs && a.p.starts[s <= a.p.seqs ? s : a.p.seqs] <= token));
-    seq += n;
-    if (n < 64) break;
-  }
-  if (seq < 0 || seq >= a.p.seqs) return;
-  const Chunk c = chunk_of(a.p, seq);
-  if (c.n * a.group <= 16 || c.n == 1) return;
-  const int64_t pos = position_of(a.p, c, token - c.begin);
-  int64_t lo = a.first && c.slot >= 0 ? a.first[c.slot] : 0, hi = pos + 1 < c.len ? pos + 1 : c.len;
-  if (lo < 0) lo = 0;
-  if (a.window > 0 && pos + 1 - a.window > lo) lo = pos + 1 - a.window;
-  const T* q = static_cast<const T*>(a.q.d) + token * a.q.token_stride + head * a.q.head_stride;
-  float x[4], o[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = lane + 64 * i < a.p.dim ? (float)q[lane + 64 * i] : 0.f;
-  float m = -__builtin_inff(), l = 0;
-  for (int64_t j = lo; j < hi; ++j) {
-    const int page = page_of(a.p, c.slot, j);
-    if (page < 0) continue;
-    const TC* k = static_cast<const TC*>(a.p.kv) + token_offset(a.p, page, j) + head / a.group * a.p.head_stride;
-    const TC* v = k + a.p.value_offset;
-    float s = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.p.dim) s += x[i] * (float)k[lane + 64 * i];
-    s = wave_sum(s) * a.scale;
-    if (s == -__builtin_inff()) continue;
-    const float top = fmaxf(m, s), f = expf(m - top), w = expf(s - top);
-    l = l * f + w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.p.dim) o[i] = o[i] * f + w * (float)v[lane + 64 * i];
-    m = top;
-  }
-  T* out = static_cast<T*>(a.out.d) + token * a.out.token_stride + head * a.out.head_stride;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.p.dim) out[lane + 64 * i] = (T)(l != 0 ? o[i] / l : 0.f);
-  if (a.lse && lane == 0) a.lse[(int64_t)token * a.heads + head] = l != 0 ? m + logf(l) : -__builtin_inff();
-}
-
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Parts of the keys, so that `tasks` workgroups become about `want`, but of no
+// fewer than `least` keys each and no more than `top`.
+Parts parts_of_keys(int64_t most, int64_t tasks, int64_t want, int64_t least, int64_t top) {
+  Parts p{};
+  const int64_t n = (want + tasks - 1) / tasks;
+  int64_t keys = (most + n - 1) / n;
+  if (keys > top) keys = top;
+  if (keys < least) keys = least;
+  p.keys = (keys + 127) / 128 * 128;
+  const int64_t m = (most + p.keys - 1) / p.keys;
+  p.most = (int)(m < 1 ? 1 : m > 4096 ? 4096 : m);
+  return p;
+}
 
 // How the call is dealt out, by its sizes and the caller's hints alone.
 AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
@@ -458,79 +404,90 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   if (max_len > 0 && max_len < most) most = max_len;
   int64_t longest = max_new > 0 && max_new < a.p.tokens ? max_new : a.p.tokens;
   if (a.window > 0 && most > (int64_t)a.window + longest) most = (int64_t)a.window + longest;
+  const size_t per_row = D * sizeof(float) + sizeof(f4);
   p.few = true;
   p.few_tiles = (a.group + 15) / 16;
   const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
   // Parts of at least 256 keys, and as many as give every CU three workgroups.
-  const int64_t want = (768 + tasks - 1) / tasks;
-  int64_t keys = (most + want - 1) / want;
-  if (keys > 2048) keys = 2048;
-  if (keys < 256) keys = 256;
-  p.few_keys = (keys + 127) / 128 * 128;
-  int64_t n = (most + p.few_keys - 1) / p.few_keys;
-  p.few_most = (int)(n < 1 ? 1 : n > 4096 ? 4096 : n);
-  p.few_rows = tasks * 16;
-  p.few_bytes = p.few_most > 1 ? (size_t)p.few_most * p.few_rows * (D * sizeof(float) + sizeof(float2)) : 0;
+  p.few_parts = parts_of_keys(most, tasks, 768, 256, 2048);
+  p.few_parts.rows = tasks * 16;
+  p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   p.chunk = longest > 1 && longest * a.group > 16;
+  if (p.chunk) {
+    p.chunk_tiles = tile_count(a.p.tokens, a.group, kChunkTile, a.p.seqs);
+    const int64_t wgs = p.chunk_tiles * a.p.kv_heads;
+    p.chunk_parts = parts_of_keys(most, wgs, 512, 512, most);
+    p.chunk_parts.rows = wgs * kChunkTile;
+    p.chunk_bytes = p.chunk_parts.most > 1 ? p.chunk_parts.most * p.chunk_parts.rows * per_row : 0;
+  }
+  return p;
+}
+
+Parts placed(Parts p, void* work, int D) {
+  p.o = static_cast<float*>(work);
+  p.ml = reinterpret_cast<f4*>(p.o + p.most * p.rows * D);
   return p;
 }
 
 template <typename T, typename TC, int D>
-hipError_t few_of(const AttendArgs& a, const AttendPlan& p, void* work, hipStream_t s) {
-  Parts parts{};
-  parts.rows = p.few_rows;
-  parts.keys = p.few_keys;
-  parts.most = p.few_most;
-  parts.o = static_cast<float*>(work);
-  parts.ml = reinterpret_cast<float2*>(parts.o + (int64_t)p.few_most * p.few_rows * D);
-  constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
-  if (lds > 60000) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
+hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
+  hipError_t e = hipSuccess;
+  if (p.few) {
+    const Parts parts = placed(p.few_parts, work, D);
+    constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
+    if (lds > 60000) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return e;
+    }
+    few_kernel<T, TC, D><<<dim3(a.p.seqs * p.few_tiles, a.p.kv_heads, parts.most), kFewThreads, lds, s>>>(
+        a, parts, p.few_tiles, p.chunk);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (parts.most > 1) {
+      join_kernel<T, D><<<dim3(a.p.seqs * p.few_tiles * 16, a.p.kv_heads), kJoinThreads, 0, s>>>(
+          a, parts, p.few_tiles, Elem<TC>::kShift);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
-  few_kernel<T, TC, D><<<dim3(a.p.seqs * p.few_tiles, a.p.kv_heads, p.few_most), kFewThreads, lds, s>>>(a, parts, p.few_tiles, p.chunk);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.few_most <= 1) return e;
-  few_join_kernel<T, D><<<dim3(a.p.seqs * p.few_tiles * 16, a.p.kv_heads), kJoinThreads, 0, s>>>(a, parts, p.few_tiles,
-                                                                                        Elem<TC>::kShift);
-  return hipGetLastError();
+  if (p.chunk) {
+    const Parts parts = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
+    if ((e = launch_chunk(a, type, cache_type, parts, p.chunk_tiles, s)) != hipSuccess) return e;
+    if (parts.most > 1) {
+      join_kernel<T, D><<<dim3((unsigned)(p.chunk_tiles * kChunkTile), a.p.kv_heads), kJoinThreads, 0, s>>>(
+          a, parts, 0, chunk_shift<TC>());
+      e = hipGetLastError();
+    }
+  }
+  return e;
 }
 
 template <typename T, typename TC>
-hipError_t attend_of(const AttendArgs& a, const AttendPlan& p, void* work, hipStream_t s) {
-  hipError_t e = hipSuccess;
-  if (p.few) {
-    switch (width_of(a.p.dim)) {
-      case 64: e = few_of<T, TC, 64>(a, p, work, s); break;
-      case 128: e = few_of<T, TC, 128>(a, p, work, s); break;
-      default: e = few_of<T, TC, 256>(a, p, work, s); break;
-    }
+hipError_t attend_types(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
+  switch (width_of(a.p.dim)) {
+    case 64: return attend_width<T, TC, 64>(a, p, type, cache_type, work, s);
+    case 128: return attend_width<T, TC, 128>(a, p, type, cache_type, work, s);
+    default: return attend_width<T, TC, 256>(a, p, type, cache_type, work, s);
   }
-  if (e == hipSuccess && p.chunk) {
-    attend_kernel<T, TC><<<dim3(a.p.tokens, a.heads), 64, 0, s>>>(a);
-    e = hipGetLastError();
-  }
-  return e;
 }
 
 }  // namespace
 
 size_t attend_workspace(const AttendArgs& a, int max_new, int64_t max_len) {
   const AttendPlan p = plan_of(a, max_new, max_len);
-  return p.few_bytes;
+  return (p.few_bytes + 255) / 256 * 256 + p.chunk_bytes;
 }
 
 hipError_t launch_attend(const AttendArgs& a, int type, int cache_type, int max_new, int64_t max_len, void* work,
                          hipStream_t s) {
   const AttendPlan p = plan_of(a, max_new, max_len);
+  char* w = static_cast<char*>(work);
   if (type == kF32) {
-    if (cache_type == kF32) return attend_of<float, float>(a, p, work, s);
-    if (cache_type == kF16) return attend_of<float, _Float16>(a, p, work, s);
-    return attend_of<float, __bf16>(a, p, work, s);
+    if (cache_type == kF32) return attend_types<float, float>(a, p, type, cache_type, w, s);
+    if (cache_type == kF16) return attend_types<float, _Float16>(a, p, type, cache_type, w, s);
+    return attend_types<float, __bf16>(a, p, type, cache_type, w, s);
   }
-  if (type == kF16) return attend_of<_Float16, _Float16>(a, p, work, s);
-  return attend_of<__bf16, __bf16>(a, p, work, s);
+  if (type == kF16) return attend_types<_Float16, _Float16>(a, p, type, cache_type, w, s);
+  return attend_types<__bf16, __bf16>(a, p, type, cache_type, w, s);
 }
 
 }  // namespace nls

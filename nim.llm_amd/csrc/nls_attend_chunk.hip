@@ -1,0 +1,411 @@
+// nls_attend_chunk.hip -- attention of chunks: sequences of more than 16 rows
+// (token, head of the group) per kv head.
+//
+// Bound by the products: 4 D per visible (row, key) on the matrix cores, times
+// the parts that fp32 queries and weights are split into.  A workgroup takes 128
+// rows of one (sequence, kv head), 32 per wave, and walks the keys in tiles: the
+// tile after next is requested into registers, the next one lies in LDS, the
+// current one is used by all four waves.  As for few rows, S^T = K Q^T and
+// O^T = V^T P^T, here with 32 x 32 products: a lane holds one row's scores of
+// keys 8 b + 4 h + 0 .. 3 (h = lane / 32), which are its weights' places in the
+// second product.
+//
+// LDS holds K and V rows as they are in memory, their 16-byte pieces permuted
+// within a row so that 16 lanes which read 16 rows (K), or 32 which read 4 rows
+// (V), meet all banks.  16-bit V is read with the transposing load: 4 keys of
+// one element per lane.
+//
+// The running maximum follows the scores only when it is passed by 2^8: until
+// then weights grow up to 2^8 times the largest one seen, which fp32 sums and
+// either 16-bit type hold without loss, and the sums need no rescaling.  It is
+// a whole number, so that what it is taken from and given back to is exact.
+#include "nls_attend.h"
+
+namespace nls {
+namespace {
+
+constexpr int kChunkWaves = 4;
+constexpr int kChunkThreads = 64 * kChunkWaves;
+static_assert(kChunkTile == 32 * kChunkWaves, "32 rows per wave");
+constexpr float kSlack = 8.f;
+
+__device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16x mma32(b8 a, b8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16x mma32(f4 a, f4 b, f16x c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T, typename TC, int D>
+struct Tile {
+  static constexpr bool kWide = sizeof(TC) == 4;               // an fp32 cache
+  static constexpr int NP = parts_of<T, TC>();
+  static constexpr int KT = kWide || D == 256 ? 32 : 64;       // keys per tile
+  static constexpr int KD = 16 / (int)sizeof(TC);              // elements of a 16-byte piece
+  static constexpr int kPieces = D / KD;                       // of a row
+  static constexpr int KC = kPieces / 2;                       // steps of the first product
+  static constexpr int kTiles = D / 32;                        // of O^T
+  static constexpr int kBytes = KT * D * (int)sizeof(TC);      // of K, or V
+  static constexpr int kStage = kBytes / 16 / kChunkThreads;   // pieces of K (or V) per thread
+  static constexpr int kRowsPerStep = kChunkThreads / kPieces; // rows that the workgroup fetches at a time
+  static constexpr float kShift = chunk_shift<TC>();
+  // the head's element of row x of O^T's tile t; kRun tiles hold neighbours
+  static constexpr int kRun = kWide ? (D == 64 ? 2 : 4) : 1;
+  static __device__ __forceinline__ constexpr int element(int t, int x) {
+    return kWide ? t / kRun * 32 * kRun + x * kRun + t % kRun : t * 32 + x;
+  }
+  // where piece c of row r lies within the row
+  static __device__ __forceinline__ int k_piece(int r, int c) {
+    return kPieces >= 16 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+  }
+  static __device__ __forceinline__ int v_piece(int r, int c) {
+    if (kWide) return c;
+    return kPieces >= 16 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
+  }
+};
+
+// The neighbouring elements of this lane's row among tiles t .. t + kRun - 1
+// and rows y .. of them: four (16-bit caches: rows y .. y + 3 of one tile).
+template <typename L, typename F>
+__device__ __forceinline__ void put_run(const f16x* o, int t, int y, int h, float f, F&& to) {
+  float x[4];
+  const int d = L::element(t, 8 * (y >> 2) + 4 * h + (y & 3));
+  if constexpr (L::kRun == 1) {
+#pragma unroll
+    for (int z = 0; z < 4; ++z) x[z] = o[t][y + z] * f;
+    to(d, x, 4);
+  } else {
+#pragma unroll
+    for (int z = 0; z < L::kRun; ++z) x[z] = o[t + z][y] * f;
+    to(d, x, L::kRun);
+  }
+}
+
+typedef short s4x __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4x* lds_s4x;
+
+template <typename T, typename TC, int D>
+__global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2) void chunk_kernel(AttendArgs a, Parts parts) {
+  using L = Tile<T, TC, D>;
+  using vec = typename Elem<TC>::vec;
+  constexpr int NP = L::NP, KT = L::KT, NS = KT / 32;
+  extern __shared__ __align__(16) char chunk_lds[];  // [2][K, V]
+  __shared__ uint8_t noted[2][KT][L::kPieces];       // bit j: element j of a piece of V was not finite
+  __shared__ int has_noted[2][kChunkWaves];
+
+  const int kvh = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, part = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
+
+  // the sequence whose tiles begin at or before this one
+  int seq = -1;
+  for (int s0 = 0; s0 < a.p.seqs; s0 += 64) {
+    const int s = s0 + lane;
+    const int n = __popcll(__ballot(s < a.p.seqs && tile_base(a.p.starts[s < a.p.seqs ? s : 0], a.group, kChunkTile, s) <= tile));
+    seq += n;
+    if (n < 64) break;
+  }
+  if (seq < 0) return;
+  const Chunk c = chunk_of(a.p, seq);
+  const int rows = c.n * a.group;
+  if (rows <= 16 || c.n == 1) return;  // few_kernel's
+  const int64_t r0l = (tile - tile_base(c.begin, a.group, kChunkTile, seq)) * kChunkTile;
+  if (r0l < 0 || r0l >= rows) return;
+  const int r0 = (int)r0l, rn = rows - r0 < kChunkTile ? rows - r0 : kChunkTile;
+  const Sees sees = sees_of(a, c);
+  const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
+  const Span span = span_of(sees, t0, t1, parts.keys, parts.most);
+  if (part >= span.parts) return;
+  const int64_t k0 = span.lo + part * parts.keys, k1 = part + 1 == span.parts ? span.hi : k0 + parts.keys;
+
+  const int w0 = wave * 32;
+  const bool busy = w0 < rn, row_ok = w0 + i < rn;
+  const int row = r0 + (row_ok ? w0 + i : 0);
+  const int64_t pos = sees.p0 + row / a.group, low = sees.low(pos);
+  // keys between these are seen by every row of this wave
+  const int last = r0 + (w0 + 31 < rn ? w0 + 31 : rn - 1);
+  const int64_t all_lo = sees.low(sees.p0 + last / a.group), all_hi = sees.p0 + (r0 + w0) / a.group;
+  const int64_t any_lo = sees.low(all_hi), any_hi = sees.p0 + last / a.group;  // and by some row
+  const int dim = a.p.dim;
+
+  vec q[L::KC][NP];
+  float qs = 1.f;
+  {
+    const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
+                   (int64_t)(kvh * a.group + row % a.group) * a.q.head_stride;
+    int e = 0;
+    if constexpr (NP == 2) {
+      float top = 0.f;
+      for (int d = h * L::KD; d < dim; d += 2 * L::KD)
+        for (int j = 0; j < L::KD; ++j) top = row_ok ? fmaxf(top, fabsf((float)src[d + j])) : 0.f;
+      top = fmaxf(top, __shfl_xor(top, 32));
+      e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
+      qs = ldexpf(1.f, e);
+    }
+#pragma unroll
+    for (int k = 0; k < L::KC; ++k)
+#pragma unroll
+      for (int j = 0; j < L::KD; ++j) {
+        const int d = (k * 2 + h) * L::KD + j;
+        float x = row_ok && d < dim ? (float)src[d] : 0.f;
+        if constexpr (NP == 2) x = ldexpf(x, -e);
+        split<NP>(x, q[k], j);
+      }
+  }
+  const float sc = a.scale * kLog2e * qs;
+
+  const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
+  const int64_t mask = (int64_t{1} << a.p.page_shift) - 1;
+  const int piece = threadIdx.x % L::kPieces, srow = threadIdx.x / L::kPieces;
+  const bool piece_ok = piece * L::KD < dim;
+
+  // a lane's key of a tile: its page, -1 where there is none
+  auto page_at = [&](int64_t kb) -> int {
+    const int64_t key = kb + (lane & (KT - 1));
+    return key < k1 ? page_of(a.p, c.slot, key) : -1;
+  };
+  u4 stage[L::kStage];  // K of the next tile, then its V
+  auto fetch = [&](int64_t kb, int page, int64_t what) {
+#pragma unroll
+    for (int n = 0; n < L::kStage; ++n) {
+      const int r = n * L::kRowsPerStep + srow;
+      const int p = __shfl(page, r);
+      // (a place that is no key reads page 0; it is not put)
+      stage[n] = *reinterpret_cast<const u4*>(base + what + (int64_t)(p < 0 ? 0 : p) * a.p.page_stride +
+                                              ((kb + r) & mask) * a.p.token_stride + (piece_ok ? piece * L::KD : 0));
+    }
+  };
+  auto put_k = [&](char* to, int page) {
+#pragma unroll
+    for (int n = 0; n < L::kStage; ++n) {
+      const int r = n * L::kRowsPerStep + srow;
+      const bool ok = piece_ok && __shfl(page, r) >= 0;
+      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::k_piece(r, piece)) * 16) = ok ? stage[n] : u4{0, 0, 0, 0};
+    }
+  };
+  // Values that are not finite meet weights of 0 in the rows that do not see
+  // their keys, which would be NaN there.  Where rows see different keys such a
+  // value is put as 0, and noted: the rows that see its key turn to NaN after
+  // the products.
+  auto put_v = [&](char* to, int page, int64_t kb, int buf) {
+    const bool edge = kb < sees.low(sees.p0 + t1) || kb + KT - 1 > sees.p0 + t0;
+    bool any = false;
+#pragma unroll
+    for (int n = 0; n < L::kStage; ++n) {
+      const int r = n * L::kRowsPerStep + srow;
+      const bool ok = piece_ok && __shfl(page, r) >= 0;
+      u4 x = ok ? stage[n] : u4{0, 0, 0, 0};
+      if (edge) {
+        TC e[L::KD];
+        __builtin_memcpy(e, &x, 16);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < L::KD; ++j)
+          if (!(fabsf((float)e[j]) < __builtin_inff())) {
+            bits |= 1u << j;
+            e[j] = 0.f;
+          }
+        __builtin_memcpy(&x, e, 16);
+        noted[buf][r][piece] = (uint8_t)bits;
+        any |= bits != 0;
+      }
+      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::v_piece(r, piece)) * 16) = x;
+    }
+    const bool wave_any = __ballot(any) != 0;
+    if (lane == 0) has_noted[buf][wave] = wave_any;
+  };
+
+  f16x o[L::kTiles];
+#pragma unroll
+  for (int t = 0; t < L::kTiles; ++t) o[t] = f16x{};
+  float m = minus_inf(), l = 0.f, lr = 0.f;  // (lr: of the rounded weights)
+
+  // 32 keys from kb + sub * 32 on; whole: every row sees all of them
+  auto step = [&](bool whole, int sub, const char* lk, const char* lv, int64_t kb, uint64_t there) {
+    f16x s{};
+    const char* row_k = lk + (sub * 32 + i) * L::kPieces * 16;
+#pragma unroll
+    for (int k = 0; k < L::KC; ++k) {
+      const vec x = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, k * 2 + h) * 16);
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n) s = mma32(x, q[k][n], s);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= sc;
+    if (!whole) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = sub * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+        const int64_t key = kb + n;
+        if (!((there >> n) & 1) || key < low || key > pos) s[r] = minus_inf();
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__ballot(top > m + kSlack || m == minus_inf())) {
+      const float to = ceilf(fmaxf(top, m)), from = to == minus_inf() ? 0.f : to;
+      const float shrink = exp2_(m - from);
+      m = to;
+      l *= shrink;
+      lr *= shrink;
+#pragma unroll
+      for (int t = 0; t < L::kTiles; ++t) o[t] *= shrink;
+    }
+    const float back = L::kShift - (m == minus_inf() ? 0.f : m);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = exp2_(s[r] + back);
+      l += s[r];
+    }
+    if constexpr (!L::kWide) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {  // 16 keys
+        vec p[NP];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) split<NP>(s[b * 8 + j], p, j);
+        if constexpr (rounds_weights<T, TC>()) lr = plus_all(p[0], lr);
+#pragma unroll
+        for (int t = 0; t < L::kTiles; ++t) {
+          // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
+          const int r = 4 * h + ((lane >> 2) & 3), e = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+          const char* at = lv + (sub * 32 + b * 16) * L::kPieces * 16 + (e & 7) * 2;
+          const s4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4x)(at + (r * L::kPieces + L::v_piece(r, e >> 3)) * 16));
+          const s4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4x)(at + ((r + 8) * L::kPieces + L::v_piece(r + 8, e >> 3)) * 16));
+          const vec x = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n) o[t] = mma32(x, p[n], o[t]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {  // 2 keys, one to each half of the wave
+        const char* at = lv + (sub * 32 + 8 * (r >> 2) + 4 * h + (r & 3)) * L::kPieces * 16;
+#pragma unroll
+        for (int t = 0; t < L::kTiles; t += L::kRun) {
+          float x[L::kRun];
+          __builtin_memcpy(x, __builtin_assume_aligned(at + L::element(t, i) * 4, 4 * L::kRun), 4 * L::kRun);
+#pragma unroll
+          for (int z = 0; z < L::kRun; ++z)
+            o[t + z] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[z], s[r], o[t + z], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  int page = page_at(k0), page1 = page_at(k0 + KT);
+  fetch(k0, page, 0);
+  put_k(chunk_lds, page);
+  fetch(k0, page, a.p.value_offset);
+  put_v(chunk_lds + L::kBytes, page, k0, 0);
+  int buf = 0;
+  for (int64_t kb = k0; kb < k1; kb += KT, buf ^= 1) {
+    const bool more = kb + KT < k1;
+    const int page2 = more ? page_at(kb + 2 * KT) : -1;
+    const char* lk = chunk_lds + buf * 2 * L::kBytes;
+    const char* lv = lk + L::kBytes;
+    char* next = chunk_lds + (buf ^ 1) * 2 * L::kBytes;
+    if (more) fetch(kb + KT, page1, 0);
+    __syncthreads();
+    const bool used = busy && kb <= any_hi && kb + KT > any_lo;
+    const uint64_t there = __ballot(page >= 0);  // (KT 32: twice the same)
+    const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && there == ~uint64_t{0};
+#pragma unroll 1
+    for (int sub = 0; sub < NS; ++sub) {
+      if (used) step(whole, sub, lk, lv, kb, there);
+      if (more && sub == 0) {
+        put_k(next, page1);
+        fetch(kb + KT, page1, a.p.value_offset);
+      }
+    }
+    if (more) put_v(next + L::kBytes, page1, kb + KT, buf ^ 1);
+    if (used && !whole && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
+#pragma unroll 1
+      for (int n = 0; n < KT; ++n) {
+        const int64_t key = kb + n;
+        const bool sees_it = ((there >> n) & 1) && key >= low && key <= pos;
+        const uint8_t* note = &noted[buf][n][0];
+#pragma unroll
+        for (int t = 0; t < L::kTiles; ++t)
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            const int d = L::element(t, 8 * (y >> 2) + 4 * here(h) + (y & 3));
+            if (sees_it && ((note[d / L::KD] >> (d % L::KD)) & 1)) o[t][y] = __builtin_nanf("");
+          }
+      }
+    }
+    page = page1;
+    page1 = page2;
+  }
+
+  if (!row_ok) return;
+  l += __shfl_xor(l, 32);
+  if constexpr (rounds_weights<T, TC>())
+    lr += __shfl_xor(lr, 32);
+  else
+    lr = l;
+  const float from = m == minus_inf() ? 0.f : m;
+  if (span.parts > 1) {
+    const int64_t at = part * parts.rows + ((int64_t)tile * a.p.kv_heads + kvh) * kChunkTile + w0 + i;
+#pragma unroll
+    for (int t = 0; t < L::kTiles; t += L::kRun)
+#pragma unroll
+      for (int y = 0; y < 16; y += L::kRun == 1 ? 4 : 1)
+        put_run<L>(o, t, y, h, 1.f, [&](int d, const float* x, int n) {
+          for (int z = 0; z < n; ++z) parts.o[at * D + d + z] = x[z];
+        });
+    if (h == 0) parts.ml[at] = f4{m, l, lr, 0.f};
+    return;
+  }
+  const int token = c.begin + row / a.group, head = kvh * a.group + row % a.group;
+  T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
+  const float f = lr == 0.f ? 0.f : 1.f / lr;
+#pragma unroll
+  for (int t = 0; t < L::kTiles; t += L::kRun)
+#pragma unroll
+    for (int y = 0; y < 16; y += L::kRun == 1 ? 4 : 1)
+      put_run<L>(o, t, y, h, f, [&](int d, const float* x, int n) {
+        if (d >= dim) return;
+        for (int z = 0; z < n; ++z) out[d + z] = (T)x[z];
+      });
+  if (a.lse && h == 0)
+    a.lse[(int64_t)token * a.heads + head] =
+        l == 0.f ? minus_inf() : (from + (__builtin_amdgcn_logf(l) - L::kShift)) * kLn2;
+}
+
+template <typename T, typename TC, int D>
+hipError_t chunk_of_width(const AttendArgs& a, const Parts& parts, int64_t tiles, hipStream_t s) {
+  constexpr int lds = 4 * Tile<T, TC, D>::kBytes;
+  if (lds > 60000) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_kernel<T, TC, D>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+  }
+  chunk_kernel<T, TC, D><<<dim3(a.p.kv_heads, (unsigned)tiles, parts.most), kChunkThreads, lds, s>>>(a, parts);
+  return hipGetLastError();
+}
+
+template <typename T, typename TC>
+hipError_t chunk_of_types(const AttendArgs& a, const Parts& parts, int64_t tiles, hipStream_t s) {
+  if (a.p.dim <= 64) return chunk_of_width<T, TC, 64>(a, parts, tiles, s);
+  if (a.p.dim <= 128) return chunk_of_width<T, TC, 128>(a, parts, tiles, s);
+  return chunk_of_width<T, TC, 256>(a, parts, tiles, s);
+}
+
+}  // namespace
+
+hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+                        hipStream_t s) {
+  if (type == kF32) {
+    if (cache_type == kF32) return chunk_of_types<float, float>(a, parts, tiles, s);
+    if (cache_type == kF16) return chunk_of_types<float, _Float16>(a, parts, tiles, s);
+    return chunk_of_types<float, __bf16>(a, parts, tiles, s);
+  }
+  if (type == kF16) return chunk_of_types<_Float16, _Float16>(a, parts, tiles, s);
+  return chunk_of_types<__bf16, __bf16>(a, parts, tiles, s);
+}
+
+}  // namespace nls
