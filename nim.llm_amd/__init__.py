@@ -710,46 +710,53 @@ def lm_head(weight, ggml_type: int, rows: int, cols: int, x, exact: bool = False
 # ---------------------------------------------------------------- attention over a paged cache
 
 
-def _elem_type(t) -> int:
-    import torch
+_ELEM_TYPES: dict = {}
 
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(t.dtype)
+
+def _elem_type(t) -> int:
+    code = _ELEM_TYPES.get(t.dtype)
     if code is None:
-        raise SamplerError(f"element type {t.dtype} is not float32, float16 or bfloat16")
+        import torch
+
+        _ELEM_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+        code = _ELEM_TYPES.get(t.dtype)
+        if code is None:
+            raise SamplerError(f"element type {t.dtype} is not float32, float16 or bfloat16")
     return code
 
 
-def _on(device, *tensors, dtype=None):
-    for t in tensors:
-        if t is None:
-            continue
-        assert t.is_cuda and t.device == device, "tensors of one call on different devices"
-        assert dtype is None or t.dtype == dtype, f"expected {dtype}, got {t.dtype}"
+def _ints(device: int, t):
+    """The address of a contiguous int32 tensor on the device (None: none)."""
+    if t is None:
+        return None
+    assert t.get_device() == device, "tensors of one call on different devices"
+    assert t.element_size() == 4 and not t.is_floating_point() and t.is_contiguous(), "int32 tensors, contiguous"
+    return t.data_ptr()
 
 
-def _ints(device, *tensors):
-    import torch
-
-    _on(device, *tensors, dtype=torch.int32)
-    assert all(t is None or t.is_contiguous() for t in tensors), "int32 tensors are contiguous"
-
-
-def _heads(t):
+def _heads(device: int, t, dtype):
     """A [tokens, heads, head_dim] tensor as nls_heads."""
-    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] <= 1), "rows of heads: [tokens, heads, head_dim], elements side by side"
-    return NlsHeads(t.data_ptr(), t.stride(0), t.stride(1))
+    assert t.get_device() == device and t.dtype == dtype, "tensors of one call: one device, one element type"
+    s = t.stride()
+    assert len(s) == 3 and (s[2] == 1 or t.shape[2] <= 1), "rows of heads: [tokens, heads, head_dim], elements side by side"
+    return NlsHeads(t.data_ptr(), s[0], s[1])
 
 
-def _launch(device, call, *args, what):
-    """The call on the device's current stream, with that device current."""
+def _launch(device: int, what: str, *args):
+    """The call on the device's current stream, with that device current.  (The
+    raw forms of torch.cuda.current_stream and current_device: 5 us less, of a
+    call that takes 10.)"""
     import torch
 
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        check(call(*args, stream), what)
+    C = torch._C
+    call = getattr(lib(), what)
+    if C._cuda_getDevice() == device:
+        status = call(*args, C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            check(call(*args, stream), what)
+            status = call(*args, C._cuda_getCurrentRawStream(device))
+    if status != NLS_OK:
+        check(status, what)
 
 
 @dataclass
@@ -762,12 +769,11 @@ class RopePlan:
     interleaved: bool = True
     amplitude: float = 1.0
 
-    def _c(self, device):
-        import torch
-
-        _on(device, self.freqs, dtype=torch.float64)
-        assert self.freqs.dim() == 1 and self.freqs.is_contiguous()
-        return NlsRopePlan(self.freqs.data_ptr(), 2 * self.freqs.numel(), int(self.interleaved), self.amplitude)
+    def _c(self, device: int):
+        f = self.freqs
+        assert f.get_device() == device and f.element_size() == 8 and f.is_floating_point() and f.dim() == 1 \
+            and f.is_contiguous(), "rope plan: float64 [dim / 2] on the call's device"
+        return NlsRopePlan(f.data_ptr(), 2 * f.numel(), self.interleaved, self.amplitude)
 
 
 ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
@@ -805,35 +811,35 @@ def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
     """x [tokens, heads, head_dim] with the first elements of each head turned by
     its token's position (int32 [tokens]); `inverse` takes a gradient back.
     `out` may be x.  Returns out."""
-    import torch
-
+    dev, dt = x.get_device(), x.dtype
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _on(x.device, x, out, dtype=x.dtype)
-    _ints(x.device, positions)
-    assert out.shape == x.shape and positions.numel() == x.shape[0]
-    _launch(x.device, lib().nls_rope, plan._c(x.device), _elem_type(x), _heads(x), _heads(out), x.shape[0], x.shape[1],
-            x.shape[2], positions.data_ptr(), int(inverse), what="nls_rope")
+        import torch
+
+        out = torch.empty(x.shape, dtype=dt, device=x.device)
+    tokens, heads, dim = x.shape
+    assert dev >= 0 and out.shape == x.shape and positions.numel() == tokens
+    _launch(dev, "nls_rope", plan._c(dev), _elem_type(x), _heads(dev, x, dt), _heads(dev, out, dt), tokens, heads, dim,
+            _ints(dev, positions), inverse)
     return out
 
 
-def _paged_kv(kv, table, lens):
-    assert kv.dim() == 5 and kv.shape[1] == 2 and kv.stride(4) == 1, (
-        "a layer of the cache: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
-    _on(kv.device, kv)
-    _ints(kv.device, lens)
-    _on(kv.device, table, dtype=lens.dtype)
-    assert table.dim() == 2 and table.stride(1) == 1 and lens.numel() == table.shape[0]
+def _paged_kv(dev: int, kv, table, lens):
+    pages, two, kv_heads, page_size, dim = kv.shape
     st = kv.stride()
-    return NlsPagedKv(kv.data_ptr(), _elem_type(kv), kv.shape[0], kv.shape[3], kv.shape[2], kv.shape[4], st[0], st[1],
-                      st[2], st[3], table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], lens.data_ptr())
+    assert dev >= 0 and two == 2 and st[4] == 1, (
+        "a layer of the cache on the GPU: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
+    slots, per = table.shape
+    ts = table.stride()
+    assert table.get_device() == dev and table.dtype == lens.dtype and ts[1] == 1 and lens.numel() == slots, (
+        "the page table: int32 [slots, pages], rows side by side")
+    return NlsPagedKv(kv.data_ptr(), _elem_type(kv), pages, page_size, kv_heads, dim, st[0], st[1], st[2], st[3],
+                      table.data_ptr(), ts[0], slots, per, _ints(dev, lens))
 
 
-def _chunks(x, starts, slots):
-    _ints(x.device, starts, slots)
+def _chunks(dev: int, tokens: int, starts, slots):
     seqs = starts.numel() - 1
     assert seqs >= 0 and (slots is None or slots.numel() == seqs)
-    return NlsChunks(seqs, x.shape[0], starts.data_ptr(), _ptr(slots))
+    return NlsChunks(seqs, tokens, _ints(dev, starts), _ints(dev, slots))
 
 
 def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan] = None, slots=None, out=None):
@@ -842,21 +848,22 @@ def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan]
     positions; q [tokens, heads, head_dim] turned into `out` (which may be q).
     Sequence i's tokens are rows starts[i] .. starts[i + 1] and the last ones of
     slot slots[i] (i when None), whose lens count them already.  Returns out."""
-    import torch
-
-    assert k.shape == v.shape and k.shape[1] == kv.shape[2] and k.shape[2] == kv.shape[4]
-    _on(kv.device, k, v, q, out, dtype=k.dtype)
-    heads = 0
+    dev, dt = kv.get_device(), k.dtype
+    tokens, kv_heads, dim = k.shape
+    assert k.shape == v.shape and kv_heads == kv.shape[2] and dim == kv.shape[4]
+    heads, cq, co = 0, None, None
     if q is not None:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            import torch
+
+            out = torch.empty(q.shape, dtype=dt, device=q.device)
         heads = q.shape[1]
-        assert out.shape == q.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2]
+        assert out.shape == q.shape and q.shape[0] == tokens and q.shape[2] == dim
+        cq, co = _heads(dev, q, dt), _heads(dev, out, dt)
     else:
         assert out is None, "out without q"
-    _launch(kv.device, lib().nls_cache_append, _paged_kv(kv, table, lens), _chunks(k, starts, slots),
-            None if plan is None else plan._c(kv.device), _elem_type(k), None if q is None else _heads(q),
-            None if q is None else _heads(out), heads, _heads(k), _heads(v), what="nls_cache_append")
+    _launch(dev, "nls_cache_append", _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots),
+            None if plan is None else plan._c(dev), _elem_type(k), cq, co, heads, _heads(dev, k, dt), _heads(dev, v, dt))
     return out
 
 
@@ -869,104 +876,113 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
     the longest chunk and context (0: nothing); they choose how the work is
     split, not what comes out.  lse: True, or a float32 [tokens, heads] tensor,
     for the logarithm of each row's sum.  Rows of no sequence keep what `out` and
-    `lse` hold.  Returns out, or (out, lse)."""
+    `lse` hold.  `work`: a preallocated uint8 workspace of
+    paged_attention_workspace() bytes.  Returns out, or (out, lse)."""
     import torch
 
+    dev, dt = kv.get_device(), q.dtype
+    tokens, heads, dim = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _on(kv.device, q, out, dtype=q.dtype)
-    assert out.shape == q.shape and q.dim() == 3 and q.shape[2] == kv.shape[4]
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
     if lse is True:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    if lse is not None:
-        _on(kv.device, lse, dtype=torch.float32)
-        assert lse.is_contiguous() and lse.shape == q.shape[:2]
-    c, ch = _paged_kv(kv, table, lens), _chunks(q, starts, slots)
-    _ints(kv.device, first)
-    assert first is None or first.numel() == lens.numel()
-    heads = q.shape[1]
-    need = int(lib().nls_paged_attention_workspace(c, ch, heads, max_new, max_len, window))
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+    elif lse is not None:
+        assert lse.get_device() == dev and lse.dtype == torch.float32 and lse.is_contiguous() \
+            and lse.shape == (tokens, heads), "lse: float32 [tokens, heads], contiguous"
+    assert out.shape == q.shape and dim == kv.shape[4] and (first is None or first.numel() == lens.numel())
+    c, ch = _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots)
+    cq, co, cf = _heads(dev, q, dt), _heads(dev, out, dt), _ints(dev, first)
+    need = lib().nls_paged_attention_workspace(c, ch, heads, max_new, max_len, window)
     if need and (work is None or work.numel() < need):
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _launch(kv.device, lib().nls_paged_attention, c, ch, _elem_type(q), _heads(q), _heads(out), heads,
-            q.shape[2] ** -0.5 if scale is None else scale, window, _ptr(first), _ptr(lse), max_new, max_len,
-            _ptr(work), 0 if work is None else work.numel(), what="nls_paged_attention")
+    elif work is not None:
+        assert work.get_device() == dev and work.dtype == torch.uint8 and work.is_contiguous()
+    _launch(dev, "nls_paged_attention", c, ch, _elem_type(q), cq, co, heads, dim ** -0.5 if scale is None else scale,
+            window, cf, None if lse is None else lse.data_ptr(), max_new, max_len, _ptr(work), need)
     return out if lse is None else (out, lse)
+
+
+def paged_attention_workspace(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, window: int = 0) -> int:
+    """Bytes of the workspace paged_attention takes for these arguments, for a
+    caller that keeps one (each call in flight needs its own)."""
+    return int(lib().nls_paged_attention_workspace(_paged_kv(kv.get_device(), kv, table, lens),
+                                                   _chunks(kv.get_device(), q.shape[0], starts, None), q.shape[1], max_new,
+                                                   max_len, window))
 
 
 PAGES_DONE, PAGES_NONE_LEFT, PAGES_ROW_FULL, PAGES_BAD_ENTRY = range(4)
 
 
-def _page_pool(kv):
-    assert kv.dim() == 6 and kv.shape[2] == 2 and (kv.shape[0] == 0 or kv[0, 0].is_contiguous()), (
+def _page_pool(dev: int, kv):
+    layers, _, two, heads, page_size, dim = kv.shape
+    st, n = kv.stride(), kv.element_size()
+    assert kv.get_device() == dev and two == 2 and sorted(st[2:]) == sorted(kv[0, 0].contiguous().stride()), (
         "the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
-    n = kv.element_size()
-    return NlsPagePool(kv.data_ptr(), kv.shape[0], kv[0, 0].numel() * n, kv.stride(0) * n, kv.stride(1) * n)
+    return NlsPagePool(kv.data_ptr(), layers, 2 * heads * page_size * dim * n, st[0] * n, st[1] * n)
 
 
-def _page_tables(table, lens, refs, page_size):
-    _ints(refs.device, lens, refs)
-    _on(refs.device, table, dtype=refs.dtype)
-    assert table.dim() == 2 and table.stride(1) == 1 and (lens is None or lens.numel() == table.shape[0])
-    return NlsPageTables(table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], _ptr(lens), refs.data_ptr(),
-                         refs.numel(), page_size)
+def _page_tables(dev: int, table, lens, refs, page_size: int):
+    slots, per = table.shape
+    ts = table.stride()
+    assert dev >= 0 and table.get_device() == dev and table.dtype == refs.dtype and ts[1] == 1 and (
+        lens is None or lens.numel() == slots), "the page table: int32 [slots, pages], rows side by side"
+    return NlsPageTables(table.data_ptr(), ts[0], slots, per, _ints(dev, lens), _ints(dev, refs), refs.numel(), page_size)
 
 
-def _pages_call(what, refs, t, count, *args):
+def _pages_call(dev: int, what: str, refs, t, count: int, *args):
     """One of the page calls with its workspace; returns its int32 word."""
     import torch
 
-    need = int(lib().nls_cache_workspace(t, count))
-    work = torch.empty(max(need, 1), dtype=torch.uint8, device=refs.device)
-    word = torch.empty(1, dtype=torch.int32, device=refs.device)
-    _launch(refs.device, getattr(lib(), what), *args, word.data_ptr(), work.data_ptr(), need, what=what)
-    return word
+    need = lib().nls_cache_workspace(t, count)
+    # the word, then the workspace from the next 256 bytes on
+    both = torch.empty(need // 4 + 64, dtype=torch.int32, device=refs.device)
+    at = both.data_ptr()
+    _launch(dev, what, *args, at, at + 256, need)
+    return both[:1]
 
 
 def cache_reserve(table, lens, refs, page_size: int, counts):
     """Slot s grows by counts[s] (int32) tokens: the lowest free pages, in the
     slots' order, and lens += counts.  Returns the status word (PAGES_DONE, or
     why nothing was done) as an int32 device tensor [1]."""
-    _ints(refs.device, counts)
+    dev = refs.get_device()
     assert counts.numel() == table.shape[0]
-    t = _page_tables(table, lens, refs, page_size)
-    return _pages_call("nls_cache_reserve", refs, t, 0, t, counts.data_ptr())
+    t = _page_tables(dev, table, lens, refs, page_size)
+    return _pages_call(dev, "nls_cache_reserve", refs, t, 0, t, _ints(dev, counts))
 
 
 def cache_fork(kv, table, lens, refs, src, dst):
     """The empty slots dst[i] (int32) become copies of the slots src[i]: full
     pages shared, the last partial page copied in every layer of kv.  Returns the
     status word."""
-    _ints(refs.device, src, dst)
-    _on(refs.device, kv)
-    assert src.numel() == dst.numel() and kv.shape[1] == refs.numel()
-    t = _page_tables(table, lens, refs, kv.shape[4])
-    return _pages_call("nls_cache_fork", refs, t, src.numel(), _page_pool(kv), t, _ptr(src), _ptr(dst), src.numel())
+    dev, n = refs.get_device(), src.numel()
+    assert n == dst.numel() and kv.shape[1] == refs.numel()
+    t = _page_tables(dev, table, lens, refs, kv.shape[4])
+    return _pages_call(dev, "nls_cache_fork", refs, t, n, _page_pool(dev, kv), t, _ints(dev, src), _ints(dev, dst), n)
 
 
 def cache_release(table, lens, refs, slots, page_size: int):
     """The slots (int32) let go of their pages and are empty.  Returns the
     status word."""
-    _ints(refs.device, slots)
-    t = _page_tables(table, lens, refs, page_size)
-    return _pages_call("nls_cache_release", refs, t, 0, t, _ptr(slots), slots.numel())
+    dev = refs.get_device()
+    t = _page_tables(dev, table, lens, refs, page_size)
+    return _pages_call(dev, "nls_cache_release", refs, t, 0, t, _ints(dev, slots), slots.numel())
 
 
 def cache_compact(kv, table, refs):
     """Moves the held pages to the lowest ids, their contents in every layer and
     the table's entries with them.  Returns how many are held, int32 [1]."""
-    _on(refs.device, kv)
+    dev = refs.get_device()
     assert kv.shape[1] == refs.numel()
-    t = _page_tables(table, None, refs, kv.shape[4])
-    return _pages_call("nls_cache_compact", refs, t, 0, _page_pool(kv), t)
+    t = _page_tables(dev, table, None, refs, kv.shape[4])
+    return _pages_call(dev, "nls_cache_compact", refs, t, 0, _page_pool(dev, kv), t)
 
 
 def cache_copy_pages(kv, src, dst):
     """Page src[i] to page dst[i] (int32) in every layer of kv."""
-    _ints(kv.device, src, dst)
-    assert src.numel() == dst.numel()
-    _launch(kv.device, lib().nls_cache_copy_pages, _page_pool(kv), kv.shape[1], _ptr(src), _ptr(dst), src.numel(),
-            what="nls_cache_copy_pages")
+    dev = kv.get_device()
+    assert dev >= 0 and src.numel() == dst.numel()
+    _launch(dev, "nls_cache_copy_pages", _page_pool(dev, kv), kv.shape[1], _ints(dev, src), _ints(dev, dst), src.numel())
 
 
 class PagedCache:

@@ -113,36 +113,6 @@ __device__ __forceinline__ float plus_all(b8 x, float c) {
   return c;
 }
 
-// Values that are not finite meet weights of 0 in the rows that do not see
-// their keys, which would be NaN there.  Where rows see different keys they
-// leave the operand x, and what they stand for goes to the rows that see them
-// (`seen`: 1 for such a key and row, else 0): the products of indicators with
-// `seen` say which sums get an infinity or a NaN.
-template <typename V, typename Acc, typename Mma>
-__device__ __forceinline__ void only_seen(V& x, V seen, Acc& o, Mma&& mma) {
-  constexpr int n = sizeof(V) / sizeof(x[0]);
-  bool bad = false;
-#pragma unroll
-  for (int j = 0; j < n; ++j) bad |= !(fabsf((float)x[j]) < __builtin_inff());
-  if (__ballot(bad) == 0) return;
-#pragma unroll 1
-  for (int kind = 0; kind < 3; ++kind) {  // infinity, minus infinity, NaN
-    const float it = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
-    V is;
-#pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const float f = (float)x[j];
-      is[j] = (kind == 2 ? f != f : f == it) ? 1.f : 0.f;
-    }
-    const Acc count = mma(is, seen, Acc{});
-#pragma unroll
-    for (int j = 0; j < (int)(sizeof(Acc) / 4); ++j) o[j] += count[j] > 0.f ? it : 0.f;
-  }
-#pragma unroll
-  for (int j = 0; j < n; ++j)
-    if (!(fabsf((float)x[j]) < __builtin_inff())) x[j] = 0.f;
-}
-
 // Which keys a sequence's tokens see: row r of kv head's group is token r /
 // group at position p, keys [low(p), p].
 struct Sees {

@@ -49,20 +49,53 @@ struct Few {
   static constexpr int kTiles = D / 16;  // tiles of O^T: (u, e)
 };
 
+// A lane's piece of a V row, as words; operand(): tile e's, for the keys of the
+// pieces v[0 ..], U pieces apart.
 template <typename TC, int E>
 struct VPiece {
-  TC v[E];
+  static constexpr int kWords = E * (int)sizeof(TC) / 4;
+  uint32_t w[kWords];
 };
+template <typename TC>
+constexpr uint32_t exponent_bits() {
+  return __is_same(TC, _Float16) ? 0x7c00u : __is_same(TC, __bf16) ? 0x7f80u : 0x7f800000u;
+}
+template <typename TC>
+constexpr uint32_t one_bits() {
+  return __is_same(TC, _Float16) ? 0x3c00u : __is_same(TC, __bf16) ? 0x3f80u : 0x3f800000u;
+}
+// the sign bit's place of each element of a word that is an infinity or NaN:
+// an exponent of ones and one more carries there
+template <typename TC>
+__device__ __forceinline__ uint32_t odd_elements(uint32_t w) {
+  constexpr uint32_t rep = sizeof(TC) == 4 ? 1u : 0x10001u, top = sizeof(TC) == 4 ? 0x80000000u : 0x8000u;
+  constexpr uint32_t e = exponent_bits<TC>();
+  return ((w & e * rep) + (top - e) * rep) & top * rep;
+}
+template <typename TC, typename V, int E, int U>
+__device__ __forceinline__ V operand(const VPiece<TC, E> (*v)[U], int u, int e) {
+  u4 x;
+  if constexpr (sizeof(TC) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = v[j][u].w[e];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = __builtin_amdgcn_perm(v[2 * j + 1][u].w[e / 2], v[2 * j][u].w[e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+  }
+  return __builtin_bit_cast(V, x);
+}
 
-template <typename T, typename TC, int D>
-__global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts parts, int tiles, bool chunk_runs) {
+// kPad: heads narrower than D
+template <typename T, typename TC, int D, bool kPad>
+__global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(AttendArgs a, Parts parts, int tiles, bool chunk_runs) {
   using F = Few<T, TC, D>;
   using vec = typename Elem<TC>::vec;
   constexpr int NP = F::kParts, NW = F::kWeightParts, KT = F::KT, NSUB = F::NSUB;
   extern __shared__ float few_lds[];  // [wave][16][D + 4] sums
   __shared__ float sh_m[kFewWaves][16], sh_l[kFewWaves][16];
 
-  const int task = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
+  const int kvh = blockIdx.x % a.p.kv_heads, task = blockIdx.x / a.p.kv_heads, part = blockIdx.z;
   const int seq = task / tiles, tile = task - seq * tiles;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const Chunk c = chunk_of(a.p, seq);
@@ -120,123 +153,186 @@ __global__ __launch_bounds__(kFewThreads) void few_kernel(AttendArgs a, Parts pa
   const float sc = a.scale * kLog2e * qs;
 
   const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
-  const int64_t mask = (int64_t{1} << a.p.page_shift) - 1;
+  const int mask = (1 << a.p.page_shift) - 1;
   f4 o[F::kTiles];
 #pragma unroll
   for (int t = 0; t < F::kTiles; ++t) o[t] = f4{0, 0, 0, 0};
   float m = minus_inf(), l = 0.f;
 
-  int page[NSUB];
+  // page[s]: that of key 16 s + i of a step, -1 where there is none (what is
+  // read there is page 0, and counts for nothing)
+  struct Pages {
+    int at[NSUB];
+  };
   auto pages_at = [&](int64_t kb) {
+    Pages p;
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
       const int64_t key = kb + s * 16 + i;
-      page[s] = key < k1 ? page_of(a.p, c.slot, key) : -1;
+      p.at[s] = key < k1 ? page_of(a.p, c.slot, key) : -1;
     }
+    return p;
   };
-  int64_t kb = k0 + wave * KT;
-  if (kb < k1) pages_at(kb);
-  for (; kb < k1; kb += kFewWaves * KT) {
-    vec k[NSUB][F::KC];
-    VPiece<TC, F::E> v[NSUB * 4][F::U];
-    bool whole = kb >= all_lo && kb + KT - 1 <= all_hi;
-    bool vok[NSUB * 4];
+  vec k[NSUB][F::KC];
+  using VP = VPiece<TC, F::E>;
+  VP v[NSUB * 4][F::U];
+  auto fetch_k = [&](int64_t kb, const Pages& pg) {
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
-      whole = whole && __ballot(page[s] >= 0) == ~uint64_t{0};
-      // (a place that is no key reads page 0, and what it reads counts for nothing)
-      const TC* row_k = base + (int64_t)(page[s] < 0 ? 0 : page[s]) * a.p.page_stride + ((kb + s * 16 + i) & mask) * a.p.token_stride;
+      const int off = ((int)kb + s * 16 + i) & mask;
+      const TC* row_k = base + (int64_t)(pg.at[s] < 0 ? 0 : pg.at[s]) * a.p.page_stride + off * a.p.token_stride + g * F::KD;
 #pragma unroll
       for (int x = 0; x < F::KC; ++x) {
-        const int d = x * 4 * F::KD + g * F::KD;
-        k[s][x] = *reinterpret_cast<const vec*>(row_k + (d < dim ? d : 0));
+        const int d = x * 4 * F::KD;
+        k[s][x] = *reinterpret_cast<const vec*>(row_k + (!kPad || d + g * F::KD < dim ? d : -g * F::KD));
       }
     }
+  };
+  auto fetch_v = [&](int64_t kb, const Pages& pg) {
 #pragma unroll
-    for (int s = 0; s < NSUB; ++s)
+    for (int s = 0; s < NSUB; ++s) {
+      const TC* row_v = nullptr;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int p = __shfl(page[s], g * 4 + r);
-        vok[s * 4 + r] = p >= 0;
-        const TC* row_v = base + a.p.value_offset + (int64_t)(p < 0 ? 0 : p) * a.p.page_stride +
-                          ((kb + s * 16 + g * 4 + r) & mask) * a.p.token_stride;
+        // keys 4 g .. 4 g + 3 share a page of at least 4 tokens
+        if (r == 0 || a.p.page_shift < 2) {
+          const int p = __shfl(pg.at[s], g * 4 + r);
+          const int off = ((int)kb + s * 16 + g * 4 + r) & mask;
+          row_v = base + a.p.value_offset + (int64_t)(p < 0 ? 0 : p) * a.p.page_stride + off * a.p.token_stride + i * F::E;
+        } else {
+          row_v += a.p.token_stride;
+        }
 #pragma unroll
         for (int u = 0; u < F::U; ++u) {
-          const int d = u * 16 * F::E + i * F::E;
-          __builtin_memcpy(&v[s * 4 + r][u], __builtin_assume_aligned(row_v + (d < dim ? d : 0), sizeof(TC) * F::E),
-                           sizeof(TC) * F::E);
+          const int d = u * 16 * F::E;
+          typedef uint32_t words __attribute__((ext_vector_type(VP::kWords)));
+          const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(row_v + (!kPad || d + i * F::E < dim ? d : -i * F::E)));
+#pragma unroll
+          for (int y = 0; y < VP::kWords; ++y) v[s * 4 + r][u].w[y] = x[y];
         }
       }
-    const int64_t next = kb + kFewWaves * KT;
-    bool vis[NSUB * 4];
-    float s_[NSUB * 4];
-    if (dim < D) {
-#pragma unroll
-      for (int s = 0; s < NSUB; ++s)
-#pragma unroll
-        for (int x = 0; x < F::KC; ++x)
-          if (x * 4 * F::KD + g * F::KD >= dim) k[s][x] = vec{};
     }
+  };
+
+  // K of a step is requested while the step before it is in its weights, V while
+  // it is in its scores, the page table two steps ahead.
+  constexpr int kStep = kFewWaves * KT;
+  int64_t kb = k0 + wave * KT;
+  Pages page, page1;
+  if (kb < k1) {
+    page = pages_at(kb);
+    page1 = pages_at(kb + kStep);
+    fetch_k(kb, page);
+    fetch_v(kb, page);
+  }
+  for (; kb < k1; kb += kStep) {
+    const bool more = kb + kStep < k1;
+    bool whole = kb >= all_lo && kb + KT - 1 <= all_hi;
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) whole = whole && __ballot(page.at[s] >= 0) == ~uint64_t{0};
+    float w[NSUB * 4];
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
       f4 acc{0, 0, 0, 0};
 #pragma unroll
-      for (int n = NP - 1; n >= 0; --n)
+      for (int x = 0; x < F::KC; ++x) {
+        vec kk = k[s][x];
+        if constexpr (kPad)
+          if (x * 4 * F::KD + g * F::KD >= dim) kk = vec{};
 #pragma unroll
-        for (int x = 0; x < F::KC; ++x) acc = mma16(k[s][x], q[x][n], acc);
+        for (int n = NP - 1; n >= 0; --n) acc = mma16(kk, q[x][n], acc);
+      }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t key = kb + s * 16 + g * 4 + r;
-        vis[s * 4 + r] = whole || (vok[s * 4 + r] && key >= low && key <= pos);
-        s_[s * 4 + r] = acc[r];
+      for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * sc;
+    }
+    if (more) fetch_k(kb + kStep, page1);
+    uint32_t vis = 0xffffffffu;
+    if (!whole) {
+      const int64_t from = low - kb, to = pos - kb;  // of this row's keys, within the step
+#pragma unroll
+      for (int j = 0; j < NSUB * 4; ++j) {
+        const int n = (j >> 2) * 16 + g * 4 + (j & 3);
+        const bool there = __shfl(page.at[j >> 2], g * 4 + (j & 3)) >= 0;
+        if (!there || n < from || n > to) {
+          vis &= ~(1u << j);
+          w[j] = minus_inf();
+        }
+        if (!there)
+#pragma unroll
+          for (int u = 0; u < F::U; ++u) v[j][u] = VP{};
       }
     }
-    if (next < k1) pages_at(next);
-    float top = minus_inf();
+    float top = w[0];
 #pragma unroll
-    for (int j = 0; j < NSUB * 4; ++j) top = vis[j] ? fmaxf(top, s_[j] * sc) : top;
+    for (int j = 1; j < NSUB * 4; ++j) top = fmaxf(top, w[j]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
-    const float from = top == minus_inf() ? 0.f : top;
-    const float shrink = exp2_(m - from);
-    m = top;
-    float w[NSUB * 4], sum = 0.f;
+    if (__ballot(top > m)) {
+      top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
+      const float shrink = exp2_(m - (top == minus_inf() ? 0.f : top));
+      m = top;
+      l *= shrink;
 #pragma unroll
-    for (int j = 0; j < NSUB * 4; ++j) {
-      w[j] = vis[j] ? exp2_(__builtin_fmaf(s_[j], sc, Elem<TC>::kShift - from)) : 0.f;
-      sum += w[j];
+      for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
     }
-    l = l * shrink + sum;
-#pragma unroll
-    for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
-
-    if (!whole) {
-#pragma unroll
-      for (int j = 0; j < NSUB * 4; ++j)
-#pragma unroll
-        for (int u = 0; u < F::U; ++u)
-          if (!vok[j]) v[j][u] = VPiece<TC, F::E>{};
-    }
+    const float back = Elem<TC>::kShift - (m == minus_inf() ? 0.f : m);
     constexpr int kDepth = sizeof(vec) / sizeof(TC);
-    vec p[NW], seen;
+    vec p[NW];
 #pragma unroll
     for (int j = 0; j < kDepth; ++j) {
-      split<NW>(w[j], p, j);
-      seen[j] = vis[j] ? 1.f : 0.f;
+      const float x = exp2_(w[j] + back);
+      l += x;
+      split<NW>(x, p, j);
+    }
+    // Values that are not finite meet weights of 0 in the rows that do not see
+    // their keys, which would be NaN there: where rows see different keys they
+    // count as 0, and the rows that see them turn to NaN.
+    if (!whole) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+        for (int u = 0; u < F::U; ++u)
+#pragma unroll
+          for (int y = 0; y < VP::kWords; ++y) odd |= odd_elements<TC>(v[j][u].w[y]);
+      if (__ballot(odd != 0)) {
+        vec seen;
+#pragma unroll
+        for (int j = 0; j < kDepth; ++j) seen[j] = (vis >> j) & 1 ? 1.f : 0.f;
+#pragma unroll
+        for (int u = 0; u < F::U; ++u) {
+          VP is[kDepth][1];
+#pragma unroll
+          for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+            for (int y = 0; y < VP::kWords; ++y) {
+              const uint32_t bad = odd_elements<TC>(here(v[j][u].w[y])) >> (sizeof(TC) == 4 ? 31 : 15);
+              is[j][0].w[y] = bad * one_bits<TC>();
+              v[j][u].w[y] &= ~(bad * (sizeof(TC) == 4 ? 0xffffffffu : 0xffffu));
+            }
+#pragma unroll
+          for (int e = 0; e < F::E; ++e) {
+            const f4 count = mma16(operand<TC, vec, F::E, 1>(is, 0, e), seen, f4{0, 0, 0, 0});
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (count[r] > 0.f) o[u * F::E + e][r] = __builtin_nanf("");
+          }
+        }
+      }
     }
 #pragma unroll
     for (int u = 0; u < F::U; ++u)
 #pragma unroll
       for (int e = 0; e < F::E; ++e) {
-        vec x;
+        const vec x = operand<TC, vec, F::E, F::U>(v, u, e);
 #pragma unroll
-        for (int j = 0; j < kDepth; ++j) x[j] = v[j][u].v[e];
-        f4& sum_of = o[u * F::E + e];
-        if (!whole) only_seen(x, seen, sum_of, [](vec y, vec z, f4 c) { return mma16(y, z, c); });
-#pragma unroll
-        for (int n = NW - 1; n >= 0; --n) sum_of = mma16(x, p[n], sum_of);
+        for (int n = NW - 1; n >= 0; --n) o[u * F::E + e] = mma16(x, p[n], o[u * F::E + e]);
       }
+    if (more) {
+      fetch_v(kb + kStep, page1);
+      page = page1;
+      page1 = pages_at(kb + 2 * kStep);
+    }
   }
 
   // the waves' sums, relative to the largest of their maxima
@@ -311,7 +407,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
   __shared__ f4 sums[kSide][kAcross];
   __shared__ float ls[kSide], lrs[kSide];
   const int size = tiles ? 16 : kChunkTile;
-  const int task = blockIdx.x / size, r = blockIdx.x % size, kvh = blockIdx.y;
+  const int64_t at = blockIdx.x;  // the row among a part's: task, kv head, row of the tile
+  const int r = (int)(at % size), kvh = (int)(at / size % a.p.kv_heads), task = (int)(at / size / a.p.kv_heads);
   int seq = -1, r0;
   if (tiles) {
     seq = task / tiles;
@@ -338,7 +435,6 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
   const int rn = rows - r0 < size ? rows - r0 : size;
   const Span span = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most);
   if (span.parts <= 1) return;
-  const int64_t at = ((int64_t)task * a.p.kv_heads + kvh) * size + r;
   float top = minus_inf();
   for (int p = threadIdx.x & 63; p < span.parts; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at][0]);
 #pragma unroll
@@ -381,17 +477,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
 
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Parts of the keys, so that `tasks` workgroups become about `want`, but of no
-// fewer than `least` keys each and no more than `top`.
+// Parts of the keys, so that `tasks` workgroups become about `want`, of no fewer
+// than `least` keys each and, so that long and short contexts of a batch take
+// their turns, no more than `top`; but not beyond 8192 workgroups, whose sums
+// wait in the workspace.
 Parts parts_of_keys(int64_t most, int64_t tasks, int64_t want, int64_t least, int64_t top) {
   Parts p{};
-  const int64_t n = (want + tasks - 1) / tasks;
+  const int64_t n = (want + tasks - 1) / tasks, cap = n > 8192 / tasks ? n : 8192 / tasks;
   int64_t keys = (most + n - 1) / n;
   if (keys > top) keys = top;
   if (keys < least) keys = least;
+  if (keys < (most + cap - 1) / cap) keys = (most + cap - 1) / cap;
   p.keys = (keys + 127) / 128 * 128;
   const int64_t m = (most + p.keys - 1) / p.keys;
-  p.most = (int)(m < 1 ? 1 : m > 4096 ? 4096 : m);
+  p.most = (int)(m < 1 ? 1 : m);
   return p;
 }
 
@@ -408,8 +507,8 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   p.few = true;
   p.few_tiles = (a.group + 15) / 16;
   const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
-  // Parts of at least 256 keys, and as many as give every CU three workgroups.
-  p.few_parts = parts_of_keys(most, tasks, 768, 256, 2048);
+  // Parts of at least 256 keys, and as many as give every CU two workgroups.
+  p.few_parts = parts_of_keys(most, tasks, 512, 256, 2048);
   p.few_parts.rows = tasks * 16;
   p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   p.chunk = longest > 1 && longest * a.group > 16;
@@ -429,22 +528,22 @@ Parts placed(Parts p, void* work, int D) {
   return p;
 }
 
-template <typename T, typename TC, int D>
+template <typename T, typename TC, int D, bool kPad>
 hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
   hipError_t e = hipSuccess;
   if (p.few) {
     const Parts parts = placed(p.few_parts, work, D);
     constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
     if (lds > 60000) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D>),
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D, kPad>),
                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (e != hipSuccess) return e;
     }
-    few_kernel<T, TC, D><<<dim3(a.p.seqs * p.few_tiles, a.p.kv_heads, parts.most), kFewThreads, lds, s>>>(
+    few_kernel<T, TC, D, kPad><<<dim3(a.p.kv_heads * a.p.seqs * p.few_tiles, 1, parts.most), kFewThreads, lds, s>>>(
         a, parts, p.few_tiles, p.chunk);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (parts.most > 1) {
-      join_kernel<T, D><<<dim3(a.p.seqs * p.few_tiles * 16, a.p.kv_heads), kJoinThreads, 0, s>>>(
+      join_kernel<T, D><<<(unsigned)parts.rows, kJoinThreads, 0, s>>>(
           a, parts, p.few_tiles, Elem<TC>::kShift);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
@@ -453,7 +552,7 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
     const Parts parts = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
     if ((e = launch_chunk(a, type, cache_type, parts, p.chunk_tiles, s)) != hipSuccess) return e;
     if (parts.most > 1) {
-      join_kernel<T, D><<<dim3((unsigned)(p.chunk_tiles * kChunkTile), a.p.kv_heads), kJoinThreads, 0, s>>>(
+      join_kernel<T, D><<<(unsigned)parts.rows, kJoinThreads, 0, s>>>(
           a, parts, 0, chunk_shift<TC>());
       e = hipGetLastError();
     }
@@ -463,11 +562,13 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
 
 template <typename T, typename TC>
 hipError_t attend_types(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
-  switch (width_of(a.p.dim)) {
-    case 64: return attend_width<T, TC, 64>(a, p, type, cache_type, work, s);
-    case 128: return attend_width<T, TC, 128>(a, p, type, cache_type, work, s);
-    default: return attend_width<T, TC, 256>(a, p, type, cache_type, work, s);
-  }
+  const int dim = a.p.dim;
+  if (dim == 64) return attend_width<T, TC, 64, false>(a, p, type, cache_type, work, s);
+  if (dim < 64) return attend_width<T, TC, 64, true>(a, p, type, cache_type, work, s);
+  if (dim == 128) return attend_width<T, TC, 128, false>(a, p, type, cache_type, work, s);
+  if (dim < 128) return attend_width<T, TC, 128, true>(a, p, type, cache_type, work, s);
+  if (dim == 256) return attend_width<T, TC, 256, false>(a, p, type, cache_type, work, s);
+  return attend_width<T, TC, 256, true>(a, p, type, cache_type, work, s);
 }
 
 }  // namespace

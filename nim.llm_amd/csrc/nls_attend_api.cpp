@@ -114,7 +114,11 @@ const char* check_sizes(const nls_paged_kv* kv, const nls_chunks* c, int heads, 
     return "cache: a size out of range";
   if (c->seqs < 0 || c->tokens < 0) return "chunks: a negative size";
   if (heads < 1 || heads % kv->kv_heads) return "heads is no multiple of the cache's";
-  if (heads > 65535 || (int64_t)c->tokens * heads > 0x7fffffff) return "more than 2^31 rows of heads";
+  // (a launch has fewer than 2^32 threads: one workgroup per sequence, kv head
+  // and 16 heads of its group, 16 rows each where parts are joined)
+  if (heads > 65535 || (int64_t)c->tokens * heads > 0x7fffffff ||
+      (int64_t)c->seqs * kv->kv_heads * ((heads / kv->kv_heads + 15) / 16) >= int64_t{1} << 20)
+    return "too many rows of heads (2^31), or sequences times heads (2^20)";
   if (max_new < 0 || max_len < 0 || window < 0) return "a negative size";
   return nullptr;
 }

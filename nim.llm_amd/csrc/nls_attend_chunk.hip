@@ -94,7 +94,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   __shared__ uint8_t noted[2][KT][L::kPieces];       // bit j: element j of a piece of V was not finite
   __shared__ int has_noted[2][kChunkWaves];
 
-  const int kvh = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, part = blockIdx.z;
+  const int kvh = blockIdx.x % a.p.kv_heads, tile = (gridDim.x - 1 - blockIdx.x) / a.p.kv_heads, part = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
 
   // the sequence whose tiles begin at or before this one
@@ -384,7 +384,7 @@ hipError_t chunk_of_width(const AttendArgs& a, const Parts& parts, int64_t tiles
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
   }
-  chunk_kernel<T, TC, D><<<dim3(a.p.kv_heads, (unsigned)tiles, parts.most), kChunkThreads, lds, s>>>(a, parts);
+  chunk_kernel<T, TC, D><<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), kChunkThreads, lds, s>>>(a, parts);
   return hipGetLastError();
 }
 
