@@ -159,7 +159,7 @@ struct Parts {
   f4* ml;
   int64_t rows;   // of one part
   int64_t keys;   // of one part
-  int most;       // parts at most; 1: none are used
+  int most;       // parts at most; 1 or 0: none are used
 };
 
 constexpr int kChunkTile = 128;  // rows of a workgroup of the chunk kernel

@@ -396,76 +396,85 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
 
 // ---------------------------------------------------------------- joining parts
 
-// One row's parts: weights from their maxima, then the weighted sum; a
-// workgroup takes a row, D / 4 lanes across it and the parts side by side.
+// One row's parts: weights from their maxima, then the weighted sum, D / 4 lanes
+// across the row and the parts side by side.  kWaves waves take a row: four
+// where rows are few and their parts many, else one.
 constexpr int kJoinThreads = 256;
 
-// `tiles`: few_kernel's tiles per sequence; 0: the rows are chunk_kernel's.
-template <typename T, int D>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts parts, int tiles, float shift) {
-  constexpr int kAcross = D / 4, kSide = kJoinThreads / kAcross;
-  __shared__ f4 sums[kSide][kAcross];
-  __shared__ float ls[kSide], lrs[kSide];
-  const int size = tiles ? 16 : kChunkTile;
-  const int64_t at = blockIdx.x;  // the row among a part's: task, kv head, row of the tile
-  const int r = (int)(at % size), kvh = (int)(at / size % a.p.kv_heads), task = (int)(at / size / a.p.kv_heads);
-  int seq = -1, r0;
-  if (tiles) {
-    seq = task / tiles;
-    r0 = (task - seq * tiles) * 16;
-  } else {
-    const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < a.p.seqs; s0 += 64) {
+template <typename T, int D, int kWaves>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int tiles,
+                                                            bool chunk_runs, float few_shift, float chunk_shift) {
+  constexpr int kAcross = D / 4, kSide = 64 * kWaves / kAcross;
+  constexpr int kRows = kJoinThreads / (64 * kWaves);  // of a workgroup
+  __shared__ f4 sums[kRows][kSide][kAcross];
+  __shared__ float ls[kRows][kSide][2];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x / (64 * kWaves), in = threadIdx.x % (64 * kWaves);
+  const int64_t index = (int64_t)blockIdx.x * kRows + sub;
+  const int token = (int)(index / a.heads), head = (int)(index % a.heads);
+  int parts_n = 0;
+  int64_t at = 0;
+  Parts parts = few;
+  float shift = few_shift;
+  int seq = -1;
+  if (token < a.p.tokens) {
+    for (int s0 = 0; s0 < a.p.seqs + 1; s0 += 64) {
       const int s = s0 + lane;
-      const int n = __popcll(__ballot(s < a.p.seqs && tile_base(a.p.starts[s < a.p.seqs ? s : 0], a.group, kChunkTile, s) <= task));
+      const int n = __popcll(__ballot(s <= a.p.seqs && a.p.starts[s <= a.p.seqs ? s : a.p.seqs] <= token));
       seq += n;
       if (n < 64) break;
     }
-    if (seq < 0) return;
+    if (seq >= 0 && seq < a.p.seqs) {
+      const Chunk c = chunk_of(a.p, seq);
+      const int rows = c.n * a.group, kvh = head / a.group, rr = (token - c.begin) * a.group + head % a.group;
+      const bool over = rows > 16 && c.n != 1;
+      int64_t task;
+      int size = 16;
+      if (over) {
+        parts = chunk;
+        shift = chunk_shift;
+        size = kChunkTile;
+        task = tile_base(c.begin, a.group, kChunkTile, seq) + rr / kChunkTile;
+      } else {
+        task = (int64_t)seq * tiles + rr / 16;
+      }
+      if (rr < rows && (!over || chunk_runs)) {
+        const int r0 = rr / size * size, rn = rows - r0 < size ? rows - r0 : size;
+        at = (task * a.p.kv_heads + kvh) * size + rr % size;
+        parts_n = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most).parts;
+      }
+    }
   }
-  const Chunk c = chunk_of(a.p, seq);
-  const int rows = c.n * a.group;
-  if ((rows <= 16 || c.n == 1) != (tiles > 0)) return;
-  if (!tiles) {
-    const int64_t x = (task - tile_base(c.begin, a.group, kChunkTile, seq)) * kChunkTile;
-    if (x < 0 || x >= rows) return;
-    r0 = (int)x;
-  }
-  if (r0 + r >= rows) return;
-  const int rn = rows - r0 < size ? rows - r0 : size;
-  const Span span = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most);
-  if (span.parts <= 1) return;
+  if (parts_n <= 1) parts_n = 0;  // (written by the kernel before)
   float top = minus_inf();
-  for (int p = threadIdx.x & 63; p < span.parts; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at][0]);
+  for (int p = lane; p < parts_n; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at][0]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float from = top == minus_inf() ? 0.f : top;
-  const int x = threadIdx.x % kAcross, side = threadIdx.x / kAcross;
+  const int x = in % kAcross, side = in / kAcross;
   f4 s{0, 0, 0, 0};
   float l = 0.f, lr = 0.f;
 #pragma unroll 4
-  for (int p = side; p < span.parts; p += kSide) {
+  for (int p = side; p < parts_n; p += kSide) {
     const f4 ml = parts.ml[p * parts.rows + at];
     const float w = exp2_(ml[0] - from);
     s += *reinterpret_cast<const f4*>(parts.o + (p * parts.rows + at) * D + x * 4) * w;
     l += ml[1] * w;
     lr += ml[2] * w;
   }
-  sums[side][x] = s;
+  sums[sub][side][x] = s;
   if (x == 0) {
-    ls[side] = l;
-    lrs[side] = lr;
+    ls[sub][side][0] = l;
+    ls[sub][side][1] = lr;
   }
   __syncthreads();
-  if (side) return;
-  float sum = ls[0], sumr = lrs[0];
+  if (side || parts_n == 0) return;
+  float sum = ls[sub][0][0], sumr = ls[sub][0][1];
 #pragma unroll
   for (int y = 1; y < kSide; ++y) {
-    s += sums[y][x];
-    sum += ls[y];
-    sumr += lrs[y];
+    s += sums[sub][y][x];
+    sum += ls[sub][y][0];
+    sumr += ls[sub][y][1];
   }
-  const int rr = r0 + r, token = c.begin + rr / a.group, head = kvh * a.group + rr % a.group;
   T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll
   for (int y = 0; y < 4; ++y)
@@ -507,8 +516,9 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   p.few = true;
   p.few_tiles = (a.group + 15) / 16;
   const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
-  // Parts of at least 256 keys, and as many as give every CU two workgroups.
-  p.few_parts = parts_of_keys(most, tasks, 512, 256, 2048);
+  // Parts of at least 256 keys, and as many as give every CU two workgroups; up
+  // to 768 keys are not split, since joining them takes longer.
+  p.few_parts = parts_of_keys(most, tasks, 512, most <= 768 ? 768 : 256, 2048);
   p.few_parts.rows = tasks * 16;
   p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   p.chunk = longest > 1 && longest * a.group > 16;
@@ -530,34 +540,29 @@ Parts placed(Parts p, void* work, int D) {
 
 template <typename T, typename TC, int D, bool kPad>
 hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
-  hipError_t e = hipSuccess;
-  if (p.few) {
-    const Parts parts = placed(p.few_parts, work, D);
-    constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
-    if (lds > 60000) {
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D, kPad>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-      if (e != hipSuccess) return e;
-    }
-    few_kernel<T, TC, D, kPad><<<dim3(a.p.kv_heads * a.p.seqs * p.few_tiles, 1, parts.most), kFewThreads, lds, s>>>(
-        a, parts, p.few_tiles, p.chunk);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (parts.most > 1) {
-      join_kernel<T, D><<<(unsigned)parts.rows, kJoinThreads, 0, s>>>(
-          a, parts, p.few_tiles, Elem<TC>::kShift);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+  if (!p.few) return hipSuccess;
+  const Parts few = placed(p.few_parts, work, D);
+  const Parts chunk = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
+  constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
+  hipError_t e;
+  if (lds > 60000) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D, kPad>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
   }
-  if (p.chunk) {
-    const Parts parts = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
-    if ((e = launch_chunk(a, type, cache_type, parts, p.chunk_tiles, s)) != hipSuccess) return e;
-    if (parts.most > 1) {
-      join_kernel<T, D><<<(unsigned)parts.rows, kJoinThreads, 0, s>>>(
-          a, parts, 0, chunk_shift<TC>());
-      e = hipGetLastError();
-    }
-  }
-  return e;
+  few_kernel<T, TC, D, kPad><<<dim3(a.p.kv_heads * a.p.seqs * p.few_tiles, 1, few.most), kFewThreads, lds, s>>>(
+      a, few, p.few_tiles, p.chunk);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  if (p.chunk && (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, s)) != hipSuccess) return e;
+  if (few.most <= 1 && chunk.most <= 1) return hipSuccess;
+  const int64_t rows = (int64_t)a.p.tokens * a.heads;
+  if (rows < 1024)
+    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, p.few_tiles, p.chunk,
+                                                                Elem<TC>::kShift, chunk_shift<TC>());
+  else
+    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, p.few_tiles, p.chunk,
+                                                                          Elem<TC>::kShift, chunk_shift<TC>());
+  return hipGetLastError();
 }
 
 template <typename T, typename TC>
