@@ -94,8 +94,8 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
 
 /* One layer's keys and values: the key of page p, head h, token t starts at
  * d_kv + p * page_stride + h * head_stride + t * token_stride (elements), the
- * value value_offset elements behind it.  All four strides are multiples of 8,
- * d_kv is 16-byte aligned, head_dim a multiple of 8 up to 256, page_size a
+ * value value_offset elements behind it.  All four strides are multiples of 8
+ * (page_stride and token_stride below 2^30), d_kv is 16-byte aligned, head_dim a multiple of 8 up to 256, page_size a
  * power of two up to 4096.  A table entry outside [0, pages) is no page: what
  * it would hold is neither read nor written, and attention sees no key there. */
 typedef struct nls_paged_kv {

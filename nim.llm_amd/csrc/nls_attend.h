@@ -134,19 +134,23 @@ __device__ __forceinline__ Sees sees_of(const AttendArgs& a, const Chunk& c) {
   return s;
 }
 
+// A position or key as an int: what is beyond the ints is beyond every key.
+__device__ __forceinline__ int as_int(int64_t x) { return x < -1 ? -1 : x > 0x7fffffff ? 0x7fffffff : (int)x; }
+
 // The keys that tokens t0 .. t1 see between them, from a multiple of 32 on, and
 // the parts of `keys` keys that they fall into (the last one takes the rest).
 struct Span {
-  int64_t lo, hi;
-  int parts;
+  int lo, hi, parts;
+  __device__ int begin(int part, int keys) const { return lo + part * keys; }
+  __device__ int end(int part, int keys) const { return part + 1 == parts ? hi : lo + (part + 1) * keys; }
 };
-__device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int64_t keys, int most) {
+__device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int keys, int most) {
   Span r;
-  r.lo = s.low(s.p0 + t0);
-  r.hi = s.p0 + t1 + 1 < s.len ? s.p0 + t1 + 1 : s.len;
-  r.lo &= ~int64_t{31};
-  const int64_t n = r.hi > r.lo ? (r.hi - r.lo + keys - 1) / keys : 1;
-  r.parts = (int)(n < most ? n : most);
+  const int64_t end = s.p0 + t1 + 1 < s.len ? s.p0 + t1 + 1 : s.len;
+  r.hi = as_int(end < 0 ? 0 : end);
+  r.lo = as_int(s.low(s.p0 + t0)) & ~31;
+  const uint32_t n = r.hi > r.lo ? ((uint32_t)(r.hi - r.lo) + (uint32_t)keys - 1) / (uint32_t)keys : 1;
+  r.parts = n < (uint32_t)most ? (int)n : most < 1 ? 1 : most;
   return r;
 }
 
@@ -158,7 +162,7 @@ struct Parts {
   float* o;
   f4* ml;
   int64_t rows;   // of one part
-  int64_t keys;   // of one part
+  int keys;       // of one part
   int most;       // parts at most; 1 or 0: none are used
 };
 

@@ -110,14 +110,15 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
   const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
   const Span span = span_of(sees, t0, t1, parts.keys, over ? 1 : parts.most);
   if (part >= span.parts) return;
-  const int64_t k0 = span.lo + part * parts.keys, k1 = part + 1 == span.parts ? span.hi : k0 + parts.keys;
+  const int k0 = span.begin(part, parts.keys), k1 = span.end(part, parts.keys);
 
   // this lane's row: column i of the transposed tiles
   const bool row_ok = i < rn;
   const int row = r0 + (row_ok ? i : 0);
-  const int64_t pos = sees.p0 + row / a.group, low = sees.low(pos);
+  const int64_t at_pos = sees.p0 + row / a.group;
+  const int pos = as_int(at_pos), low = as_int(sees.low(at_pos));
   // a step whose keys lie within these is seen whole by every row
-  const int64_t all_lo = sees.low(sees.p0 + t1), all_hi = sees.p0 + t0;
+  const int all_lo = as_int(sees.low(sees.p0 + t1)), all_hi = as_int(sees.p0 + t0);
   const int dim = a.p.dim;
 
   vec q[F::KC][NP];
@@ -164,23 +165,32 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
   struct Pages {
     int at[NSUB];
   };
-  auto pages_at = [&](int64_t kb) {
+  const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
+  const uint32_t page_bytes = (uint32_t)a.p.page_stride * (uint32_t)sizeof(TC);
+  const uint32_t token_bytes = (uint32_t)a.p.token_stride * (uint32_t)sizeof(TC);
+  auto row_at = [&](const char* from, int page, uint32_t key) {
+    return reinterpret_cast<const TC*>(from + (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
+                                       (uint64_t)(key & (uint32_t)mask) * token_bytes);
+  };
+  auto pages_at = [&](int kb) {
     Pages p;
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
-      const int64_t key = kb + s * 16 + i;
-      p.at[s] = key < k1 ? page_of(a.p, c.slot, key) : -1;
+      const uint32_t key = (uint32_t)kb + s * 16 + i;
+      p.at[s] = key < (uint32_t)k1 ? table[key >> a.p.page_shift] : -1;
+      if ((uint32_t)p.at[s] >= (uint32_t)a.p.pages) p.at[s] = -1;
     }
     return p;
   };
   vec k[NSUB][F::KC];
   using VP = VPiece<TC, F::E>;
   VP v[NSUB * 4][F::U];
-  auto fetch_k = [&](int64_t kb, const Pages& pg) {
+  const char* base_k = reinterpret_cast<const char*>(base + g * F::KD);
+  const char* base_v = reinterpret_cast<const char*>(base + a.p.value_offset + i * F::E);
+  auto fetch_k = [&](int kb, const Pages& pg) {
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
-      const int off = ((int)kb + s * 16 + i) & mask;
-      const TC* row_k = base + (int64_t)(pg.at[s] < 0 ? 0 : pg.at[s]) * a.p.page_stride + off * a.p.token_stride + g * F::KD;
+      const TC* row_k = row_at(base_k, pg.at[s], (uint32_t)kb + s * 16 + i);
 #pragma unroll
       for (int x = 0; x < F::KC; ++x) {
         const int d = x * 4 * F::KD;
@@ -188,7 +198,7 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
       }
     }
   };
-  auto fetch_v = [&](int64_t kb, const Pages& pg) {
+  auto fetch_v = [&](int kb, const Pages& pg) {
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
       const TC* row_v = nullptr;
@@ -196,9 +206,7 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
       for (int r = 0; r < 4; ++r) {
         // keys 4 g .. 4 g + 3 share a page of at least 4 tokens
         if (r == 0 || a.p.page_shift < 2) {
-          const int p = __shfl(pg.at[s], g * 4 + r);
-          const int off = ((int)kb + s * 16 + g * 4 + r) & mask;
-          row_v = base + a.p.value_offset + (int64_t)(p < 0 ? 0 : p) * a.p.page_stride + off * a.p.token_stride + i * F::E;
+          row_v = row_at(base_v, __shfl(pg.at[s], g * 4 + r), (uint32_t)kb + s * 16 + g * 4 + r);
         } else {
           row_v += a.p.token_stride;
         }
@@ -217,7 +225,7 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
   // K of a step is requested while the step before it is in its weights, V while
   // it is in its scores, the page table two steps ahead.
   constexpr int kStep = kFewWaves * KT;
-  int64_t kb = k0 + wave * KT;
+  int kb = k0 + wave * KT;
   Pages page, page1;
   if (kb < k1) {
     page = pages_at(kb);
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
     if (more) fetch_k(kb + kStep, page1);
     uint32_t vis = 0xffffffffu;
     if (!whole) {
-      const int64_t from = low - kb, to = pos - kb;  // of this row's keys, within the step
+      const int from = low - kb, to = pos - kb;  // of this row's keys, within the step
 #pragma unroll
       for (int j = 0; j < NSUB * 4; ++j) {
         const int n = (j >> 2) * 16 + g * 4 + (j & 3);
@@ -401,47 +409,44 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
 // where rows are few and their parts many, else one.
 constexpr int kJoinThreads = 256;
 
+// The first few_rows rows are (sequence, one of its first `per` tokens, head),
+// of few_kernel; the others all of the call's, of chunk_kernel.
 template <typename T, int D, int kWaves>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int tiles,
-                                                            bool chunk_runs, float few_shift, float chunk_shift) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int64_t few_rows,
+                                                            int per, int tiles, float few_shift, float chunk_shift) {
   constexpr int kAcross = D / 4, kSide = 64 * kWaves / kAcross;
   constexpr int kRows = kJoinThreads / (64 * kWaves);  // of a workgroup
   __shared__ f4 sums[kRows][kSide][kAcross];
   __shared__ float ls[kRows][kSide][2];
   const int lane = threadIdx.x & 63, sub = threadIdx.x / (64 * kWaves), in = threadIdx.x % (64 * kWaves);
   const int64_t index = (int64_t)blockIdx.x * kRows + sub;
-  const int token = (int)(index / a.heads), head = (int)(index % a.heads);
-  int parts_n = 0;
+  const bool is_few = index < few_rows;
+  const int64_t rest = is_few ? index : index - few_rows;
+  const int head = (int)(rest % a.heads), kvh = head / a.group, size = is_few ? 16 : kChunkTile;
+  const Parts parts = is_few ? few : chunk;
+  const float shift = is_few ? few_shift : chunk_shift;
+  int token = (int)(rest / a.heads), seq = -1, parts_n = 0;
   int64_t at = 0;
-  Parts parts = few;
-  float shift = few_shift;
-  int seq = -1;
-  if (token < a.p.tokens) {
+  if (is_few) {
+    seq = token / per;
+  } else if (token < a.p.tokens) {
     for (int s0 = 0; s0 < a.p.seqs + 1; s0 += 64) {
       const int s = s0 + lane;
       const int n = __popcll(__ballot(s <= a.p.seqs && a.p.starts[s <= a.p.seqs ? s : a.p.seqs] <= token));
       seq += n;
       if (n < 64) break;
     }
-    if (seq >= 0 && seq < a.p.seqs) {
-      const Chunk c = chunk_of(a.p, seq);
-      const int rows = c.n * a.group, kvh = head / a.group, rr = (token - c.begin) * a.group + head % a.group;
-      const bool over = rows > 16 && c.n != 1;
-      int64_t task;
-      int size = 16;
-      if (over) {
-        parts = chunk;
-        shift = chunk_shift;
-        size = kChunkTile;
-        task = tile_base(c.begin, a.group, kChunkTile, seq) + rr / kChunkTile;
-      } else {
-        task = (int64_t)seq * tiles + rr / 16;
-      }
-      if (rr < rows && (!over || chunk_runs)) {
-        const int r0 = rr / size * size, rn = rows - r0 < size ? rows - r0 : size;
-        at = (task * a.p.kv_heads + kvh) * size + rr % size;
-        parts_n = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most).parts;
-      }
+  }
+  if (seq >= 0 && seq < a.p.seqs) {
+    const Chunk c = chunk_of(a.p, seq);
+    const int rows = c.n * a.group;
+    if (is_few) token = c.begin + token % per;
+    const int rr = (token - c.begin) * a.group + head % a.group, r0 = rr / size * size;
+    if (token < c.begin + c.n && (rows > 16 && c.n != 1) != is_few) {
+      const int64_t task = is_few ? (int64_t)seq * tiles + rr / size : tile_base(c.begin, a.group, size, seq) + rr / size;
+      const int rn = rows - r0 < size ? rows - r0 : size;
+      at = (task * a.p.kv_heads + kvh) * size + rr % size;
+      parts_n = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most).parts;
     }
   }
   if (parts_n <= 1) parts_n = 0;  // (written by the kernel before)
@@ -453,7 +458,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
   const int x = in % kAcross, side = in / kAcross;
   f4 s{0, 0, 0, 0};
   float l = 0.f, lr = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int p = side; p < parts_n; p += kSide) {
     const f4 ml = parts.ml[p * parts.rows + at];
     const float w = exp2_(ml[0] - from);
@@ -497,7 +502,8 @@ Parts parts_of_keys(int64_t most, int64_t tasks, int64_t want, int64_t least, in
   if (keys > top) keys = top;
   if (keys < least) keys = least;
   if (keys < (most + cap - 1) / cap) keys = (most + cap - 1) / cap;
-  p.keys = (keys + 127) / 128 * 128;
+  if (keys > kMaxLen) keys = kMaxLen;
+  p.keys = (int)((keys + 127) / 128 * 128);
   const int64_t m = (most + p.keys - 1) / p.keys;
   p.most = (int)(m < 1 ? 1 : m);
   return p;
@@ -554,13 +560,15 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
       a, few, p.few_tiles, p.chunk);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (p.chunk && (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, s)) != hipSuccess) return e;
-  if (few.most <= 1 && chunk.most <= 1) return hipSuccess;
-  const int64_t rows = (int64_t)a.p.tokens * a.heads;
+  const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_kernel takes of a sequence
+  const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
+  const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
+  if (rows == 0) return hipSuccess;
   if (rows < 1024)
-    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, p.few_tiles, p.chunk,
+    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles,
                                                                 Elem<TC>::kShift, chunk_shift<TC>());
   else
-    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, p.few_tiles, p.chunk,
+    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles,
                                                                           Elem<TC>::kShift, chunk_shift<TC>());
   return hipGetLastError();
 }

@@ -66,6 +66,8 @@ const char* check_kv(const nls_paged_kv* kv) {
   const int64_t st[4] = {kv->page_stride, kv->value_offset, kv->head_stride, kv->token_stride};
   for (int64_t x : st)
     if (x < 0 || x > big || x % 8) return "cache: a stride is negative, too large or no multiple of 8";
+  if (kv->page_stride >= int64_t{1} << 30 || kv->token_stride >= int64_t{1} << 30)
+    return "cache: page_stride or token_stride is 2^30 elements or more";
   if (kv->value_offset < kv->head_dim || (kv->pages > 1 && kv->page_stride < kv->head_dim) ||
       (kv->kv_heads > 1 && kv->head_stride < kv->head_dim) || (kv->page_size > 1 && kv->token_stride < kv->head_dim))
     return "cache: strides overlap";

@@ -27,7 +27,6 @@ namespace {
 constexpr int kChunkWaves = 4;
 constexpr int kChunkThreads = 64 * kChunkWaves;
 static_assert(kChunkTile == 32 * kChunkWaves, "32 rows per wave");
-constexpr float kSlack = 8.f;
 
 __device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f16x mma32(b8 a, b8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -46,6 +45,8 @@ struct Tile {
   static constexpr int kPieces = D / KD;                       // of a row
   static constexpr int KC = kPieces / 2;                       // steps of the first product
   static constexpr int kTiles = D / 32;                        // of O^T
+  static constexpr int kGroup = 4;                               // K operands read at a time
+  static constexpr bool kEarly = false;      // V operands read before the exponentials
   static constexpr int kBytes = KT * D * (int)sizeof(TC);      // of K, or V
   static constexpr int kStage = kBytes / 16 / kChunkThreads;   // pieces of K (or V) per thread
   static constexpr int kRowsPerStep = kChunkThreads / kPieces; // rows that the workgroup fetches at a time
@@ -116,18 +117,22 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
   const Span span = span_of(sees, t0, t1, parts.keys, parts.most);
   if (part >= span.parts) return;
-  const int64_t k0 = span.lo + part * parts.keys, k1 = part + 1 == span.parts ? span.hi : k0 + parts.keys;
+  const int k0 = span.begin(part, parts.keys), k1 = span.end(part, parts.keys);
 
   const int w0 = wave * 32;
   const bool busy = w0 < rn, row_ok = w0 + i < rn;
   const int row = r0 + (row_ok ? w0 + i : 0);
-  const int64_t pos = sees.p0 + row / a.group, low = sees.low(pos);
+  const int64_t at = sees.p0 + row / a.group;
+  const int pos = as_int(at), low = as_int(sees.low(at));
   // keys between these are seen by every row of this wave
   const int last = r0 + (w0 + 31 < rn ? w0 + 31 : rn - 1);
-  const int64_t all_lo = sees.low(sees.p0 + last / a.group), all_hi = sees.p0 + (r0 + w0) / a.group;
-  const int64_t any_lo = sees.low(all_hi), any_hi = sees.p0 + last / a.group;  // and by some row
+  const int all_lo = as_int(sees.low(sees.p0 + last / a.group)), all_hi = as_int(sees.p0 + (r0 + w0) / a.group);
+  const int any_lo = as_int(sees.low(sees.p0 + (r0 + w0) / a.group)), any_hi = as_int(sees.p0 + last / a.group);  // and by some row
+  const int tile_lo = as_int(sees.low(sees.p0 + t1)), tile_hi = as_int(sees.p0 + t0);  // and by all of the workgroup's
   const int dim = a.p.dim;
 
+  // the scale's sign goes to the queries: a largest score is a largest product
+  const float flip = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
   vec q[L::KC][NP];
   float qs = 1.f;
   {
@@ -147,57 +152,79 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
 #pragma unroll
       for (int j = 0; j < L::KD; ++j) {
         const int d = (k * 2 + h) * L::KD + j;
-        float x = row_ok && d < dim ? (float)src[d] : 0.f;
+        float x = row_ok && d < dim ? (float)src[d] * flip : 0.f;
         if constexpr (NP == 2) x = ldexpf(x, -e);
         split<NP>(x, q[k], j);
       }
   }
-  const float sc = a.scale * kLog2e * qs;
+  const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e * qs;
 
-  const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
-  const int64_t mask = (int64_t{1} << a.p.page_shift) - 1;
   const int piece = threadIdx.x % L::kPieces, srow = threadIdx.x / L::kPieces;
   const bool piece_ok = piece * L::KD < dim;
+  // this thread's piece of a row
+  const char* base = reinterpret_cast<const char*>(static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride) +
+                     (piece_ok ? piece * 16 : 0);
+  const uint32_t page_bytes = (uint32_t)a.p.page_stride * (uint32_t)sizeof(TC);
+  const uint32_t token_bytes = (uint32_t)a.p.token_stride * (uint32_t)sizeof(TC);
+  const int64_t to_value = a.p.value_offset * (int64_t)sizeof(TC);
+  const uint32_t mask = (1u << a.p.page_shift) - 1;
+  const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
 
   // a lane's key of a tile: its page, -1 where there is none
-  auto page_at = [&](int64_t kb) -> int {
-    const int64_t key = kb + (lane & (KT - 1));
-    return key < k1 ? page_of(a.p, c.slot, key) : -1;
+  auto page_at = [&](int kb) -> int {
+    const uint32_t key = (uint32_t)kb + (lane & (KT - 1));
+    if (key >= (uint32_t)k1) return -1;
+    const int p = table[key >> a.p.page_shift];
+    return (uint32_t)p < (uint32_t)a.p.pages ? p : -1;
   };
   u4 stage[L::kStage];  // K of the next tile, then its V
-  auto fetch = [&](int64_t kb, int page, int64_t what) {
+  const char* row_of[L::kStage];
+  auto fetch_k = [&](int kb, int page) {
+    // (a place that is no key reads page 0; it is not put)
+    const uint64_t off = (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
+                         (uint64_t)(((uint32_t)kb + (lane & (KT - 1))) & mask) * token_bytes;
+    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
 #pragma unroll
     for (int n = 0; n < L::kStage; ++n) {
       const int r = n * L::kRowsPerStep + srow;
-      const int p = __shfl(page, r);
-      // (a place that is no key reads page 0; it is not put)
-      stage[n] = *reinterpret_cast<const u4*>(base + what + (int64_t)(p < 0 ? 0 : p) * a.p.page_stride +
-                                              ((kb + r) & mask) * a.p.token_stride + (piece_ok ? piece * L::KD : 0));
+      row_of[n] = base + ((uint64_t)(uint32_t)__shfl(lo, r) | (uint64_t)(uint32_t)__shfl(hi, r) << 32);
+      stage[n] = *reinterpret_cast<const u4*>(row_of[n]);
     }
   };
-  auto put_k = [&](char* to, int page) {
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int n = 0; n < L::kStage; ++n) stage[n] = *reinterpret_cast<const u4*>(row_of[n] + to_value);
+  };
+  // there: which keys of the tile there are
+  auto ok_at = [&](int n, uint64_t there) { return piece_ok && ((there >> (n * L::kRowsPerStep + srow)) & 1); };
+  auto put_k = [&](char* to, uint64_t there) {
+    if (there != ~uint64_t{0} || dim < D) {
+#pragma unroll
+      for (int n = 0; n < L::kStage; ++n)
+        if (!ok_at(n, there)) stage[n] = u4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int n = 0; n < L::kStage; ++n) {
       const int r = n * L::kRowsPerStep + srow;
-      const bool ok = piece_ok && __shfl(page, r) >= 0;
-      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::k_piece(r, piece)) * 16) = ok ? stage[n] : u4{0, 0, 0, 0};
+      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::k_piece(r, piece)) * 16) = stage[n];
     }
   };
   // Values that are not finite meet weights of 0 in the rows that do not see
   // their keys, which would be NaN there.  Where rows see different keys such a
   // value is put as 0, and noted: the rows that see its key turn to NaN after
   // the products.
-  auto put_v = [&](char* to, int page, int64_t kb, int buf) {
-    const bool edge = kb < sees.low(sees.p0 + t1) || kb + KT - 1 > sees.p0 + t0;
+  auto put_v = [&](char* to, uint64_t there, int kb, int buf) {
     bool any = false;
+    if (there != ~uint64_t{0} || dim < D) {
 #pragma unroll
-    for (int n = 0; n < L::kStage; ++n) {
-      const int r = n * L::kRowsPerStep + srow;
-      const bool ok = piece_ok && __shfl(page, r) >= 0;
-      u4 x = ok ? stage[n] : u4{0, 0, 0, 0};
-      if (edge) {
+      for (int n = 0; n < L::kStage; ++n)
+        if (!ok_at(n, there)) stage[n] = u4{0, 0, 0, 0};
+    }
+    if (kb < tile_lo || kb + KT - 1 > tile_hi) {
+#pragma unroll
+      for (int n = 0; n < L::kStage; ++n) {
         TC e[L::KD];
-        __builtin_memcpy(e, &x, 16);
+        __builtin_memcpy(e, &stage[n], 16);
         uint32_t bits = 0;
 #pragma unroll
         for (int j = 0; j < L::KD; ++j)
@@ -205,11 +232,15 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
             bits |= 1u << j;
             e[j] = 0.f;
           }
-        __builtin_memcpy(&x, e, 16);
-        noted[buf][r][piece] = (uint8_t)bits;
+        __builtin_memcpy(&stage[n], e, 16);
+        noted[buf][n * L::kRowsPerStep + srow][piece] = (uint8_t)bits;
         any |= bits != 0;
       }
-      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::v_piece(r, piece)) * 16) = x;
+    }
+#pragma unroll
+    for (int n = 0; n < L::kStage; ++n) {
+      const int r = n * L::kRowsPerStep + srow;
+      *reinterpret_cast<u4*>(to + (r * L::kPieces + L::v_piece(r, piece)) * 16) = stage[n];
     }
     const bool wave_any = __ballot(any) != 0;
     if (lane == 0) has_noted[buf][wave] = wave_any;
@@ -219,53 +250,29 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
 #pragma unroll
   for (int t = 0; t < L::kTiles; ++t) o[t] = f16x{};
   float m = minus_inf(), l = 0.f, lr = 0.f;  // (lr: of the rounded weights)
+  float back = __builtin_inff();             // kShift - m: what turns a score into its weight's exponent
+  constexpr float kSlack = __is_same(TC, _Float16) ? 32768.f : 256.f;  // 2^8, kShift included
 
   // 32 keys from kb + sub * 32 on; whole: every row sees all of them
-  auto step = [&](bool whole, int sub, const char* lk, const char* lv, int64_t kb, uint64_t there) {
-    f16x s{};
+  auto step = [&](bool whole, int sub, const char* lk, const char* lv, int kb, uint64_t there) {
     const char* row_k = lk + (sub * 32 + i) * L::kPieces * 16;
+    vec kf[L::kGroup];
+    f16x s{};
 #pragma unroll
-    for (int k = 0; k < L::KC; ++k) {
-      const vec x = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, k * 2 + h) * 16);
+    for (int k0 = 0; k0 < L::KC; k0 += L::kGroup) {
 #pragma unroll
-      for (int n = NP - 1; n >= 0; --n) s = mma32(x, q[k][n], s);
+      for (int k = 0; k < L::kGroup; ++k)
+        kf[k] = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, (k0 + k) * 2 + h) * 16);
+
+#pragma unroll
+      for (int k = 0; k < L::kGroup; ++k)
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) s = mma32(kf[k], q[k0 + k][n], s);
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= sc;
-    if (!whole) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = sub * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
-        const int64_t key = kb + n;
-        if (!((there >> n) & 1) || key < low || key > pos) s[r] = minus_inf();
-      }
-    }
-    float top = s[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__ballot(top > m + kSlack || m == minus_inf())) {
-      const float to = ceilf(fmaxf(top, m)), from = to == minus_inf() ? 0.f : to;
-      const float shrink = exp2_(m - from);
-      m = to;
-      l *= shrink;
-      lr *= shrink;
-#pragma unroll
-      for (int t = 0; t < L::kTiles; ++t) o[t] *= shrink;
-    }
-    const float back = L::kShift - (m == minus_inf() ? 0.f : m);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = exp2_(s[r] + back);
-      l += s[r];
-    }
-    if constexpr (!L::kWide) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {  // 16 keys
-        vec p[NP];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) split<NP>(s[b * 8 + j], p, j);
-        if constexpr (rounds_weights<T, TC>()) lr = plus_all(p[0], lr);
+    // this step's V is on its way during the exponentials
+    vec vf[L::kWide ? 1 : 2][L::kTiles];
+    auto read_v = [&](int b) {
+      if constexpr (!L::kWide) {
 #pragma unroll
         for (int t = 0; t < L::kTiles; ++t) {
           // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
@@ -275,10 +282,67 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
               (lds_s4x)(at + (r * L::kPieces + L::v_piece(r, e >> 3)) * 16));
           const s4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (lds_s4x)(at + ((r + 8) * L::kPieces + L::v_piece(r + 8, e >> 3)) * 16));
-          const vec x = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int n = NP - 1; n >= 0; --n) o[t] = mma32(x, p[n], o[t]);
+          vf[b][t] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
+      }
+    };
+    if constexpr (L::kEarly) {
+      read_v(0);
+      read_v(1);
+
+    }
+    if (!whole) {
+      const int lo = low - kb - sub * 32, hi = pos - kb - sub * 32;  // of the 32 keys
+      const int from = lo < 0 ? 0 : lo > 32 ? 32 : lo, to = hi < 0 ? 0 : hi > 31 ? 32 : hi + 1;
+      // bit n: this row sees key n
+      const uint32_t seen = (uint32_t)(there >> (sub * 32)) & (uint32_t)((uint64_t{1} << to) - 1) &
+                            ~(uint32_t)((uint64_t{1} << from) - 1);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!((seen >> (8 * (r >> 2) + 4 * h + (r & 3))) & 1)) s[r] = minus_inf();
+    }
+    // Weights from the maximum so far; when they add up to more than 2^8 of the
+    // largest (or to NaN), the maximum is brought up to date first.
+    float w[16], sum = 0.f;
+    auto weigh = [&](float from) {
+      sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        w[r] = exp2_(__builtin_fmaf(s[r], sc, from));
+        sum += w[r];
+      }
+    };
+    weigh(back);
+    if (__ballot(!(sum < kSlack))) {
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      top *= sc;
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float to = ceilf(fmaxf(top, m)), from = to == minus_inf() ? 0.f : to;
+      const float shrink = exp2_(m - from);
+      m = to;
+      back = L::kShift - from;
+      l *= shrink;
+      lr *= shrink;
+#pragma unroll
+      for (int t = 0; t < L::kTiles; ++t) o[t] *= shrink;
+      weigh(back);
+      if (to == minus_inf()) back = __builtin_inff();  // no key yet: the next one sets it
+    }
+    l += sum;
+    if constexpr (!L::kWide) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {  // 16 keys
+        if constexpr (!L::kEarly) read_v(b);
+        vec p[NP];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) split<NP>(w[b * 8 + j], p, j);
+        if constexpr (rounds_weights<T, TC>()) lr = plus_all(p[0], lr);
+#pragma unroll
+        for (int t = 0; t < L::kTiles; ++t)
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n) o[t] = mma32(vf[b][t], p[n], o[t]);
       }
     } else {
 #pragma unroll
@@ -290,42 +354,50 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
           __builtin_memcpy(x, __builtin_assume_aligned(at + L::element(t, i) * 4, 4 * L::kRun), 4 * L::kRun);
 #pragma unroll
           for (int z = 0; z < L::kRun; ++z)
-            o[t + z] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[z], s[r], o[t + z], 0, 0, 0);
+            o[t + z] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[z], w[r], o[t + z], 0, 0, 0);
         }
       }
     }
   };
 
-  int page = page_at(k0), page1 = page_at(k0 + KT);
-  fetch(k0, page, 0);
-  put_k(chunk_lds, page);
-  fetch(k0, page, a.p.value_offset);
-  put_v(chunk_lds + L::kBytes, page, k0, 0);
+  uint64_t there = 0, there1 = 0;  // (KT 32: each half is the tile)
+  int page1 = -1;                  // of the next tile
+  {
+    const int page = page_at(k0);
+    there = __ballot(page >= 0);
+    page1 = page_at(k0 + KT);
+    fetch_k(k0, page);
+    put_k(chunk_lds, there);
+    fetch_v();
+    put_v(chunk_lds + L::kBytes, there, k0, 0);
+  }
   int buf = 0;
-  for (int64_t kb = k0; kb < k1; kb += KT, buf ^= 1) {
+  for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
     const bool more = kb + KT < k1;
-    const int page2 = more ? page_at(kb + 2 * KT) : -1;
     const char* lk = chunk_lds + buf * 2 * L::kBytes;
     const char* lv = lk + L::kBytes;
     char* next = chunk_lds + (buf ^ 1) * 2 * L::kBytes;
-    if (more) fetch(kb + KT, page1, 0);
+    if (more) {
+      there1 = __ballot(page1 >= 0);
+      fetch_k(kb + KT, page1);
+      page1 = page_at(kb + 2 * KT);
+    }
     __syncthreads();
     const bool used = busy && kb <= any_hi && kb + KT > any_lo;
-    const uint64_t there = __ballot(page >= 0);  // (KT 32: twice the same)
     const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && there == ~uint64_t{0};
 #pragma unroll 1
     for (int sub = 0; sub < NS; ++sub) {
       if (used) step(whole, sub, lk, lv, kb, there);
       if (more && sub == 0) {
-        put_k(next, page1);
-        fetch(kb + KT, page1, a.p.value_offset);
+        put_k(next, there1);
+        fetch_v();
       }
     }
-    if (more) put_v(next + L::kBytes, page1, kb + KT, buf ^ 1);
+    if (more) put_v(next + L::kBytes, there1, kb + KT, buf ^ 1);
     if (used && !whole && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
 #pragma unroll 1
       for (int n = 0; n < KT; ++n) {
-        const int64_t key = kb + n;
+        const int key = kb + n;
         const bool sees_it = ((there >> n) & 1) && key >= low && key <= pos;
         const uint8_t* note = &noted[buf][n][0];
 #pragma unroll
@@ -337,8 +409,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
           }
       }
     }
-    page = page1;
-    page1 = page2;
+    there = there1;
   }
 
   if (!row_ok) return;

@@ -16,6 +16,7 @@ namespace nls {
 
 constexpr int kMaxHeadDim = 256;
 constexpr int kMaxPageSize = 4096;
+constexpr int kMaxLen = 0x7fffff00;  // tokens of a context: a step behind the last one is an int too
 constexpr int kMaxPages = 1 << 19;  // one bit and half a byte of LDS each in the page kernels
 
 enum ElemType { kF32 = 0, kF16 = 1, kBF16 = 30 };
@@ -51,7 +52,8 @@ NLS_HD Chunk chunk_of(const PagedArgs& a, int seq) {
   c.n = e - b;
   c.slot = a.slot_of ? a.slot_of[seq] : seq;
   if (c.slot < 0 || c.slot >= a.slots) c.slot = -1;
-  const int64_t most = (int64_t)a.max_pages << a.page_shift;
+  int64_t most = (int64_t)a.max_pages << a.page_shift;
+  if (most > kMaxLen) most = kMaxLen;
   int64_t len = c.slot < 0 ? 0 : a.lens[c.slot];
   c.len = len < 0 ? 0 : len > most ? most : len;
   return c;
