@@ -149,6 +149,7 @@ __device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int keys,
   const int64_t end = s.p0 + t1 + 1 < s.len ? s.p0 + t1 + 1 : s.len;
   r.hi = as_int(end < 0 ? 0 : end);
   r.lo = as_int(s.low(s.p0 + t0)) & ~31;
+  if (r.lo > r.hi) r.lo = r.hi;  // no key: no step begins behind the last one
   const uint32_t n = r.hi > r.lo ? ((uint32_t)(r.hi - r.lo) + (uint32_t)keys - 1) / (uint32_t)keys : 1;
   r.parts = n < (uint32_t)most ? (int)n : most < 1 ? 1 : most;
   return r;

@@ -45,8 +45,6 @@ struct Tile {
   static constexpr int kPieces = D / KD;                       // of a row
   static constexpr int KC = kPieces / 2;                       // steps of the first product
   static constexpr int kTiles = D / 32;                        // of O^T
-  static constexpr int kGroup = 4;                               // K operands read at a time
-  static constexpr bool kEarly = false;      // V operands read before the exponentials
   static constexpr int kBytes = KT * D * (int)sizeof(TC);      // of K, or V
   static constexpr int kStage = kBytes / 16 / kChunkThreads;   // pieces of K (or V) per thread
   static constexpr int kRowsPerStep = kChunkThreads / kPieces; // rows that the workgroup fetches at a time
@@ -256,41 +254,18 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   // 32 keys from kb + sub * 32 on; whole: every row sees all of them
   auto step = [&](bool whole, int sub, const char* lk, const char* lv, int kb, uint64_t there) {
     const char* row_k = lk + (sub * 32 + i) * L::kPieces * 16;
-    vec kf[L::kGroup];
     f16x s{};
+    // wide heads: products go before another wave's exponentials (D = 128: 1039
+    // -> 1010 us for 2048 tokens over 16384 keys; D = 64 is slower with it, 183
+    // -> 187 us for two prompts of 4001)
+    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int k0 = 0; k0 < L::KC; k0 += L::kGroup) {
+    for (int k = 0; k < L::KC; ++k) {
+      const vec x = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, k * 2 + h) * 16);
 #pragma unroll
-      for (int k = 0; k < L::kGroup; ++k)
-        kf[k] = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, (k0 + k) * 2 + h) * 16);
-
-#pragma unroll
-      for (int k = 0; k < L::kGroup; ++k)
-#pragma unroll
-        for (int n = NP - 1; n >= 0; --n) s = mma32(kf[k], q[k0 + k][n], s);
+      for (int n = NP - 1; n >= 0; --n) s = mma32(x, q[k][n], s);
     }
-    // this step's V is on its way during the exponentials
-    vec vf[L::kWide ? 1 : 2][L::kTiles];
-    auto read_v = [&](int b) {
-      if constexpr (!L::kWide) {
-#pragma unroll
-        for (int t = 0; t < L::kTiles; ++t) {
-          // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
-          const int r = 4 * h + ((lane >> 2) & 3), e = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-          const char* at = lv + (sub * 32 + b * 16) * L::kPieces * 16 + (e & 7) * 2;
-          const s4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s4x)(at + (r * L::kPieces + L::v_piece(r, e >> 3)) * 16));
-          const s4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s4x)(at + ((r + 8) * L::kPieces + L::v_piece(r + 8, e >> 3)) * 16));
-          vf[b][t] = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-      }
-    };
-    if constexpr (L::kEarly) {
-      read_v(0);
-      read_v(1);
-
-    }
+    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(0);
     if (!whole) {
       const int lo = low - kb - sub * 32, hi = pos - kb - sub * 32;  // of the 32 keys
       const int from = lo < 0 ? 0 : lo > 32 ? 32 : lo, to = hi < 0 ? 0 : hi > 31 ? 32 : hi + 1;
@@ -331,18 +306,27 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
       if (to == minus_inf()) back = __builtin_inff();  // no key yet: the next one sets it
     }
     l += sum;
+    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
     if constexpr (!L::kWide) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {  // 16 keys
-        if constexpr (!L::kEarly) read_v(b);
         vec p[NP];
 #pragma unroll
         for (int j = 0; j < 8; ++j) split<NP>(w[b * 8 + j], p, j);
         if constexpr (rounds_weights<T, TC>()) lr = plus_all(p[0], lr);
 #pragma unroll
-        for (int t = 0; t < L::kTiles; ++t)
+        for (int t = 0; t < L::kTiles; ++t) {
+          // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
+          const int r = 4 * h + ((lane >> 2) & 3), e = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+          const char* at = lv + (sub * 32 + b * 16) * L::kPieces * 16 + (e & 7) * 2;
+          const s4x lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4x)(at + (r * L::kPieces + L::v_piece(r, e >> 3)) * 16));
+          const s4x hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4x)(at + ((r + 8) * L::kPieces + L::v_piece(r + 8, e >> 3)) * 16));
+          const vec x = __builtin_bit_cast(vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n) o[t] = mma32(vf[b][t], p[n], o[t]);
+          for (int n = NP - 1; n >= 0; --n) o[t] = mma32(x, p[n], o[t]);
+        }
       }
     } else {
 #pragma unroll
@@ -358,6 +342,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
         }
       }
     }
+    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(0);
   };
 
   uint64_t there = 0, there1 = 0;  // (KT 32: each half is the tile)
@@ -385,7 +370,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
     __syncthreads();
     const bool used = busy && kb <= any_hi && kb + KT > any_lo;
     const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && there == ~uint64_t{0};
-#pragma unroll 1
+#pragma unroll
     for (int sub = 0; sub < NS; ++sub) {
       if (used) step(whole, sub, lk, lv, kb, there);
       if (more && sub == 0) {
