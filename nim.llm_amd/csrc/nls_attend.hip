@@ -172,14 +172,21 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
     return reinterpret_cast<const TC*>(from + (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
                                        (uint64_t)(key & (uint32_t)mask) * token_bytes);
   };
-  auto pages_at = [&](int kb) {
+  // (the entries as they are: what is done with them waits for the loads)
+  auto entries_at = [&](int kb) {
     Pages p;
 #pragma unroll
     for (int s = 0; s < NSUB; ++s) {
-      const uint32_t key = (uint32_t)kb + s * 16 + i;
-      p.at[s] = key < (uint32_t)k1 ? table[key >> a.p.page_shift] : -1;
-      if ((uint32_t)p.at[s] >= (uint32_t)a.p.pages) p.at[s] = -1;
+      const int key = kb + s * 16 + i;
+      p.at[s] = table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
     }
+    return p;
+  };
+  auto pages_of = [&](int kb, const Pages& e) {
+    Pages p;
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s)
+      p.at[s] = kb + s * 16 + i < k1 && (uint32_t)e.at[s] < (uint32_t)a.p.pages ? e.at[s] : -1;
     return p;
   };
   vec k[NSUB][F::KC];
@@ -226,10 +233,10 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
   // it is in its scores, the page table two steps ahead.
   constexpr int kStep = kFewWaves * KT;
   int kb = k0 + wave * KT;
-  Pages page, page1;
+  Pages page, page1, entry1;
   if (kb < k1) {
-    page = pages_at(kb);
-    page1 = pages_at(kb + kStep);
+    page = pages_of(kb, entries_at(kb));
+    entry1 = entries_at(kb + kStep);
     fetch_k(kb, page);
     fetch_v(kb, page);
   }
@@ -253,7 +260,11 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
 #pragma unroll
       for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * sc;
     }
-    if (more) fetch_k(kb + kStep, page1);
+    if (more) {
+      page1 = pages_of(kb + kStep, entry1);
+      entry1 = entries_at(kb + 2 * kStep);
+      fetch_k(kb + kStep, page1);
+    }
     uint32_t vis = 0xffffffffu;
     if (!whole) {
       const int from = low - kb, to = pos - kb;  // of this row's keys, within the step
@@ -339,7 +350,6 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
     if (more) {
       fetch_v(kb + kStep, page1);
       page = page1;
-      page1 = pages_at(kb + 2 * kStep);
     }
   }
 
@@ -417,7 +427,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
   constexpr int kAcross = D / 4, kSide = 64 * kWaves / kAcross;
   constexpr int kRows = kJoinThreads / (64 * kWaves);  // of a workgroup
   __shared__ f4 sums[kRows][kSide][kAcross];
-  __shared__ float ls[kRows][kSide][2];
+  __shared__ f4 ls[kRows][kSide];
   const int lane = threadIdx.x & 63, sub = threadIdx.x / (64 * kWaves), in = threadIdx.x % (64 * kWaves);
   const int64_t index = (int64_t)blockIdx.x * kRows + sub;
   const bool is_few = index < few_rows;
@@ -450,35 +460,51 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
     }
   }
   if (parts_n <= 1) parts_n = 0;  // (written by the kernel before)
-  float top = minus_inf();
-  for (int p = lane; p < parts_n; p += 64) top = fmaxf(top, parts.ml[p * parts.rows + at][0]);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float from = top == minus_inf() ? 0.f : top;
   const int x = in % kAcross, side = in / kAcross;
   f4 s{0, 0, 0, 0};
-  float l = 0.f, lr = 0.f;
-#pragma unroll 8
-  for (int p = side; p < parts_n; p += kSide) {
-    const f4 ml = parts.ml[p * parts.rows + at];
-    const float w = exp2_(ml[0] - from);
-    s += *reinterpret_cast<const f4*>(parts.o + (p * parts.rows + at) * D + x * 4) * w;
-    l += ml[1] * w;
-    lr += ml[2] * w;
+  float m = minus_inf(), l = 0.f, lr = 0.f;
+  constexpr int kBatch = kWaves == 4 ? 8 : 4;  // parts whose loads are in flight together
+  for (int p0 = side; p0 < parts_n; p0 += kBatch * kSide) {
+    f4 ml[kBatch], o[kBatch];
+#pragma unroll
+    for (int y = 0; y < kBatch; ++y) {
+      const int p = p0 + y * kSide < parts_n ? p0 + y * kSide : p0;
+      ml[y] = parts.ml[p * parts.rows + at];
+      o[y] = *reinterpret_cast<const f4*>(parts.o + (p * parts.rows + at) * D + x * 4);
+    }
+    float top = m;
+#pragma unroll
+    for (int y = 0; y < kBatch; ++y) top = fmaxf(top, ml[y][0]);
+    const float from = top == minus_inf() ? 0.f : top, f = exp2_(m - from);
+    s *= f;
+    l *= f;
+    lr *= f;
+    m = top;
+#pragma unroll
+    for (int y = 0; y < kBatch; ++y) {
+      if (p0 + y * kSide >= parts_n) break;
+      const float w = exp2_(ml[y][0] - from);
+      s += o[y] * w;
+      l += ml[y][1] * w;
+      lr += ml[y][2] * w;
+    }
   }
   sums[sub][side][x] = s;
-  if (x == 0) {
-    ls[sub][side][0] = l;
-    ls[sub][side][1] = lr;
-  }
+  if (x == 0) ls[sub][side] = f4{m, l, lr, 0.f};
   __syncthreads();
   if (side || parts_n == 0) return;
-  float sum = ls[sub][0][0], sumr = ls[sub][0][1];
 #pragma unroll
-  for (int y = 1; y < kSide; ++y) {
-    s += sums[sub][y][x];
-    sum += ls[sub][y][0];
-    sumr += ls[sub][y][1];
+  for (int y = 1; y < kSide; ++y) m = fmaxf(m, ls[sub][y][0]);
+  const float from = m == minus_inf() ? 0.f : m;
+  float sum = 0.f, sumr = 0.f;
+  s = f4{0, 0, 0, 0};
+#pragma unroll
+  for (int y = 0; y < kSide; ++y) {
+    const f4 ml = ls[sub][y];
+    const float w = exp2_(ml[0] - from);
+    s += sums[sub][y][x] * w;
+    sum += ml[1] * w;
+    sumr += ml[2] * w;
   }
   T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll

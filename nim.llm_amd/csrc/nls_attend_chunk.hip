@@ -168,12 +168,14 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   const uint32_t mask = (1u << a.p.page_shift) - 1;
   const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
 
-  // a lane's key of a tile: its page, -1 where there is none
-  auto page_at = [&](int kb) -> int {
-    const uint32_t key = (uint32_t)kb + (lane & (KT - 1));
-    if (key >= (uint32_t)k1) return -1;
-    const int p = table[key >> a.p.page_shift];
-    return (uint32_t)p < (uint32_t)a.p.pages ? p : -1;
+  // A lane's key of a tile: its entry of the table, as it is (what is done with
+  // it waits for the load), and its page, -1 where there is none.
+  auto entry_at = [&](int kb) -> int {
+    const int key = kb + (lane & (KT - 1));
+    return table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
+  };
+  auto page_of_entry = [&](int kb, int entry) -> int {
+    return kb + (lane & (KT - 1)) < k1 && (uint32_t)entry < (uint32_t)a.p.pages ? entry : -1;
   };
   u4 stage[L::kStage];  // K of the next tile, then its V
   const char* row_of[L::kStage];
@@ -346,11 +348,11 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   };
 
   uint64_t there = 0, there1 = 0;  // (KT 32: each half is the tile)
-  int page1 = -1;                  // of the next tile
-  {
-    const int page = page_at(k0);
+  int entry1 = 0;                  // of the next tile
+  if (k0 < k1) {
+    const int page = page_of_entry(k0, entry_at(k0));
+    entry1 = entry_at(k0 + KT);
     there = __ballot(page >= 0);
-    page1 = page_at(k0 + KT);
     fetch_k(k0, page);
     put_k(chunk_lds, there);
     fetch_v();
@@ -363,9 +365,10 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
     const char* lv = lk + L::kBytes;
     char* next = chunk_lds + (buf ^ 1) * 2 * L::kBytes;
     if (more) {
-      there1 = __ballot(page1 >= 0);
-      fetch_k(kb + KT, page1);
-      page1 = page_at(kb + 2 * KT);
+      const int page = page_of_entry(kb + KT, entry1);
+      there1 = __ballot(page >= 0);
+      entry1 = entry_at(kb + 2 * KT);
+      fetch_k(kb + KT, page);
     }
     __syncthreads();
     const bool used = busy && kb <= any_hi && kb + KT > any_lo;
