@@ -119,9 +119,10 @@ typedef struct nls_paged_kv {
 /* The new tokens of a call: sequence i's are rows [d_starts[i], d_starts[i+1])
  * of q, k, v and the outputs, and they are the last ones of slot d_slots[i]
  * (slot i when d_slots is NULL).  `tokens` rows are there in all; rows before
- * d_starts[0] and behind d_starts[seqs] belong to no sequence and are neither
- * read nor written.  d_starts never falls.  A sequence of a slot outside
- * [0, slots) has no keys, and its tokens are not appended. */
+ * d_starts[0] and behind d_starts[seqs] belong to no sequence, and none of the
+ * outputs' is written.  d_starts never falls.  A sequence of a slot outside
+ * [0, slots) has no keys, and its tokens are not appended.  Fewer than 2^24
+ * tokens, and fewer than 2^30 rows of heads. */
 typedef struct nls_chunks {
   int32_t seqs;
   int32_t tokens;
@@ -149,7 +150,8 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
  * lse[t, h] = ln sum_j exp(scale * q . k_j) where d_lse (fp32, [tokens, heads]
  * contiguous) is not NULL.  A row without a key, or whose every score is
  * -infinity, has out = 0 and lse = -infinity.  What a key that a row does not
- * see holds, infinities and NaN among it, does not reach that row.
+ * see holds, infinities and NaN among it, does not reach that row; an infinite
+ * value that it does see makes it infinite or NaN.
  * type (q and out): F32 with any cache type, F16 or BF16 with the same one.
  * Scores, statistics and sums are fp32: fp32 queries and weights meet 16-bit
  * keys and values as exact sums of 16-bit parts, 16-bit queries and weights

@@ -22,6 +22,8 @@ int elem_bytes(int t) { return t == kF32 ? 4 : 2; }
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 hipStream_t stream_of(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+constexpr int kMaxTokens = (1 << 24) - 1;  // a workgroup of 256 each: fewer than 2^32 threads
+
 // A strided view [tokens, heads, dim] whose elements side by side do not
 // overlap between heads or tokens when it is written.
 const char* check_heads(const nls_heads* x, int type, int heads, int tokens, int dim, bool written) {
@@ -79,6 +81,7 @@ const char* check_kv(const nls_paged_kv* kv) {
 const char* check_chunks(const nls_chunks* c) {
   if (!c) return "NULL chunks";
   if (c->seqs < 0 || c->tokens < 0) return "chunks: a negative size";
+  if (c->tokens > kMaxTokens) return "chunks: 2^24 tokens or more";
   if (c->seqs > 0 && c->tokens > 0 && (!c->d_starts || !aligned(c->d_starts, 4) || !aligned(c->d_slots, 4)))
     return "chunks: NULL or misaligned starts or slots";
   return nullptr;
@@ -118,9 +121,9 @@ const char* check_sizes(const nls_paged_kv* kv, const nls_chunks* c, int heads, 
   if (heads < 1 || heads % kv->kv_heads) return "heads is no multiple of the cache's";
   // (a launch has fewer than 2^32 threads: one workgroup per sequence, kv head
   // and 16 heads of its group, 16 rows each where parts are joined)
-  if (heads > 65535 || (int64_t)c->tokens * heads > 0x7fffffff ||
+  if (heads > 65535 || (int64_t)c->tokens * heads > 0x3fffffff ||
       (int64_t)c->seqs * kv->kv_heads * ((heads / kv->kv_heads + 15) / 16) >= int64_t{1} << 20)
-    return "too many rows of heads (2^31), or sequences times heads (2^20)";
+    return "too many rows of heads (2^30), or sequences times heads (2^20)";
   if (max_new < 0 || max_len < 0 || window < 0) return "a negative size";
   return nullptr;
 }
@@ -228,7 +231,8 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
                  int32_t heads, int32_t head_dim, const int32_t* d_positions, int32_t inverse, void* stream) {
   if (!plan) return bad("NULL plan");
   if (!elem_type(type)) return bad("rope: element type is not F32, F16 or BF16");
-  if (tokens < 0 || heads < 0 || head_dim < 1 || head_dim > kMaxHeadDim) return bad("rope: a size out of range");
+  if (tokens < 0 || tokens > kMaxTokens || heads < 0 || head_dim < 1 || head_dim > kMaxHeadDim)
+    return bad("rope: a size out of range");
   NLS_CHECK(check_plan(plan, head_dim));
   if (tokens == 0 || heads == 0) return NLS_OK;
   NLS_CHECK(check_heads(x, type, heads, tokens, head_dim, false));

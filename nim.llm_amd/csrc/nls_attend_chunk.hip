@@ -281,15 +281,15 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
     // Weights from the maximum so far; when they add up to more than 2^8 of the
     // largest (or to NaN), the maximum is brought up to date first.
     float w[16], sum = 0.f;
-    auto weigh = [&](float from) {
+    auto weigh = [&](float times, float from) {
       sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        w[r] = exp2_(__builtin_fmaf(s[r], sc, from));
+        w[r] = exp2_(__builtin_fmaf(s[r], times, from));
         sum += w[r];
       }
     };
-    weigh(back);
+    weigh(sc, back);
     if (__ballot(!(sum < kSlack))) {
       float top = s[0];
 #pragma unroll
@@ -304,7 +304,15 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
       lr *= shrink;
 #pragma unroll
       for (int t = 0; t < L::kTiles; ++t) o[t] *= shrink;
-      weigh(back);
+      // So large a product is off by whole numbers when rounded, as `top` was and
+      // the fused one is not: all are rounded, so that none passes the largest.
+      float times = sc;
+      if (__ballot(fabsf(from) > 1048576.f)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= sc;
+        times = 1.f;
+      }
+      weigh(times, back);
       if (to == minus_inf()) back = __builtin_inff();  // no key yet: the next one sets it
     }
     l += sum;

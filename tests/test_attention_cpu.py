@@ -73,7 +73,7 @@ def _cache(pkg, **kw):
 BAD_CACHES = [dict(d_kv=None), dict(d_kv=AT + 8), dict(type=2), dict(type=-1), dict(pages=0), dict(page_size=0),
               dict(page_size=24), dict(page_size=8192), dict(kv_heads=0), dict(head_dim=0), dict(head_dim=60),
               dict(head_dim=264), dict(page_stride=-8), dict(page_stride=4), dict(page_stride=8), dict(value_offset=8),
-              dict(value_offset=1028), dict(head_stride=8), dict(token_stride=8), dict(token_stride=1 << 50),
+              dict(value_offset=1028), dict(head_stride=8), dict(token_stride=8), dict(token_stride=1 << 50), dict(page_stride=1 << 30),
               dict(d_table=None), dict(d_table=AT + 2), dict(table_stride=4), dict(table_stride=-1), dict(slots=0),
               dict(max_pages=0), dict(d_lens=None), dict(d_lens=AT + 1)]
 BAD_CHUNKS = [dict(seqs=-1), dict(tokens=-1), dict(d_starts=None), dict(d_starts=AT + 2), dict(d_slots=AT + 1)]
@@ -112,7 +112,7 @@ def test_attention_refusals(pkg):
     for kw in OVERLAPS:
         assert call(out=_heads(pkg, **kw)) == INVALID, kw
     for kw in (dict(type=30), dict(type=8), dict(heads=0), dict(heads=3), dict(heads=-2), dict(heads=1 << 20),
-               dict(scale=math.inf), dict(scale=math.nan), dict(window=-1), dict(first=AT + 2), dict(lse=AT + 1),
+               dict(scale=math.inf), dict(scale=math.nan), dict(window=-1), dict(ch=_chunks(pkg, tokens=1 << 24)), dict(first=AT + 2), dict(lse=AT + 1),
                dict(max_new=-1), dict(max_len=-1)):
         assert call(**kw) == INVALID, kw
     need = L.nls_paged_attention_workspace(_cache(pkg), _chunks(pkg), 4, 1, 1 << 20, 0)
@@ -172,7 +172,7 @@ def test_append_and_rope_refusals(pkg):
         assert rope(y=_heads(pkg, **kw)) == INVALID, kw
     for p in bad_plans:
         assert rope(plan=p) == INVALID
-    for kw in (dict(type=3), dict(tokens=-1), dict(heads=-1), dict(dim=0), dict(dim=257), dict(pos=None), dict(pos=AT + 2),
+    for kw in (dict(type=3), dict(tokens=-1), dict(tokens=1 << 24), dict(heads=-1), dict(dim=0), dict(dim=257), dict(pos=None), dict(pos=AT + 2),
                dict(y=_heads(pkg, token_stride=512))):
         assert rope(**kw) == INVALID, kw
     assert L.nls_rope(None, 0, _heads(pkg), _heads(pkg), 1, 1, 64, AT, 0, None) == INVALID

@@ -302,6 +302,36 @@ def test_attention_large_scores(pkg):
     m.check(pkg, scale=m.scale, what="queries of 1e-9")
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+def test_attention_scales(pkg, dtype, cache):
+    """Negative scales, zero (every key weighs the same), and scores of 10^8 and
+    more, where a row goes to its largest score's value and stays finite."""
+    for scale in (-0.2, 0.0):
+        say(f"[attend] scale {scale} {NAME[dtype]}/{NAME[cache]}")
+        m = Made([300, 90], [1, 40], 4, 2, 64, 16, dtype, cache, seed=21)
+        m.scale = scale
+        m.check(pkg, scale=scale)
+    for scale in (1e8, 1e30, -1e30):
+        say(f"[attend] scale {scale} {NAME[dtype]}/{NAME[cache]}")
+        m = Made([300, 90], [1, 40], 4, 2, 64, 16, dtype, cache, seed=22)
+        got = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), 40, 300,
+                                  scale=scale).cpu()
+        assert bool(torch.isfinite(got).all())
+        seen = 0
+        for i in range(2):
+            for t in range(m.starts_l[i], m.starts_l[i + 1]):
+                n = m.lens_l[i] - m.starts_l[i + 1] + t + 1
+                rows = torch.stack([m.kv[m.table_l[i][j // 16], :, :, j % 16] for j in range(n)]).double()
+                for h in range(4):
+                    s = (rows[:, 0, h // 2] @ m.q[t, h].double()) * math.copysign(1.0, scale)
+                    two = s.topk(min(2, n)).values
+                    # products of 64 terms of up to 40: the fp32 scores are within 64 * 40 * 2^-23 of these
+                    if n == 1 or float(two[0] - two[1]) > 1e-3:
+                        assert torch.equal(got[t, h], rows[int(s.argmax()), 1, h // 2].to(dtype)), (i, t, h)
+                        seen += 1
+        assert seen > 100
+
+
 def test_attention_strided_rows_and_rows_of_no_sequence(pkg):
     for dtype, cache in PAIRS:
         say(f"[attend] strided {NAME[dtype]}/{NAME[cache]}")
