@@ -453,9 +453,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
     if (is_few) token = c.begin + token % per;
     const int rr = (token - c.begin) * a.group + head % a.group, r0 = rr / size * size;
     if (token < c.begin + c.n && (rows > 16 && c.n != 1) != is_few) {
-      const int64_t task = is_few ? (int64_t)seq * tiles + rr / size : tile_base(c.begin, a.group, size, seq) + rr / size;
       const int rn = rows - r0 < size ? rows - r0 : size;
-      at = (task * a.p.kv_heads + kvh) * size + rr % size;
+      at = is_few ? (((int64_t)seq * tiles + rr / size) * a.p.kv_heads + kvh) * size + rr % size : rest;
       parts_n = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most).parts;
     }
   }
@@ -556,9 +555,12 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   p.chunk = longest > 1 && longest * a.group > 16;
   if (p.chunk) {
     p.chunk_tiles = tile_count(a.p.tokens, a.group, kChunkTile, a.p.seqs);
-    const int64_t wgs = p.chunk_tiles * a.p.kv_heads;
+    // Two workgroups per CU, of the tiles that have rows when they are all of one
+    // sequence (509 tokens of 28 heads beside 16 that decode: 167 us when the
+    // empty tiles of those count too, 145 us so); parts of at least 512 keys.
+    const int64_t wgs = ((int64_t)a.p.tokens * a.group + kChunkTile - 1) / kChunkTile * a.p.kv_heads;
     p.chunk_parts = parts_of_keys(most, wgs, 512, 512, most);
-    p.chunk_parts.rows = wgs * kChunkTile;
+    p.chunk_parts.rows = (int64_t)a.p.tokens * a.heads;
     p.chunk_bytes = p.chunk_parts.most > 1 ? p.chunk_parts.most * p.chunk_parts.rows * per_row : 0;
   }
   return p;

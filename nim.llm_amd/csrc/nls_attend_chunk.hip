@@ -51,6 +51,7 @@ struct Tile {
   static constexpr float kShift = chunk_shift<TC>();
   // the head's element of row x of O^T's tile t; kRun tiles hold neighbours
   static constexpr int kRun = kWide ? (D == 64 ? 2 : 4) : 1;
+  static constexpr int kStore = kRun == 1 ? 4 : kRun;  // neighbouring elements that a lane stores
   static __device__ __forceinline__ constexpr int element(int t, int x) {
     return kWide ? t / kRun * 32 * kRun + x * kRun + t % kRun : t * 32 + x;
   }
@@ -73,11 +74,11 @@ __device__ __forceinline__ void put_run(const f16x* o, int t, int y, int h, floa
   if constexpr (L::kRun == 1) {
 #pragma unroll
     for (int z = 0; z < 4; ++z) x[z] = o[t][y + z] * f;
-    to(d, x, 4);
+    to(d, x);
   } else {
 #pragma unroll
     for (int z = 0; z < L::kRun; ++z) x[z] = o[t + z][y] * f;
-    to(d, x, L::kRun);
+    to(d, x);
   }
 }
 
@@ -415,28 +416,39 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   else
     lr = l;
   const float from = m == minus_inf() ? 0.f : m;
+  const int token = c.begin + row / a.group, head = kvh * a.group + row % a.group;
   if (span.parts > 1) {
-    const int64_t at = part * parts.rows + ((int64_t)tile * a.p.kv_heads + kvh) * kChunkTile + w0 + i;
+    const int64_t at = part * parts.rows + (int64_t)token * a.heads + head;
 #pragma unroll
     for (int t = 0; t < L::kTiles; t += L::kRun)
 #pragma unroll
       for (int y = 0; y < 16; y += L::kRun == 1 ? 4 : 1)
-        put_run<L>(o, t, y, h, 1.f, [&](int d, const float* x, int n) {
-          for (int z = 0; z < n; ++z) parts.o[at * D + d + z] = x[z];
+        put_run<L>(o, t, y, h, 1.f, [&](int d, const float* x) {
+          __builtin_memcpy(__builtin_assume_aligned(parts.o + at * D + d, 4 * L::kStore), x, 4 * L::kStore);
         });
     if (h == 0) parts.ml[at] = f4{m, l, lr, 0.f};
     return;
   }
-  const int token = c.begin + row / a.group, head = kvh * a.group + row % a.group;
   T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
   const float f = lr == 0.f ? 0.f : 1.f / lr;
+  const bool wide_out = ((reinterpret_cast<uintptr_t>(a.out.d) / sizeof(T) | (uint64_t)a.out.token_stride |
+                          (uint64_t)a.out.head_stride) & (L::kStore - 1)) == 0;
 #pragma unroll
   for (int t = 0; t < L::kTiles; t += L::kRun)
 #pragma unroll
     for (int y = 0; y < 16; y += L::kRun == 1 ? 4 : 1)
-      put_run<L>(o, t, y, h, f, [&](int d, const float* x, int n) {
+      put_run<L>(o, t, y, h, f, [&](int d, const float* x) {
         if (d >= dim) return;
-        for (int z = 0; z < n; ++z) out[d + z] = (T)x[z];
+        typedef T run __attribute__((ext_vector_type(L::kStore)));
+        run r;
+#pragma unroll
+        for (int z = 0; z < L::kStore; ++z) r[z] = (T)x[z];
+        if (wide_out) {
+          __builtin_memcpy(__builtin_assume_aligned(out + d, sizeof r), &r, sizeof r);
+        } else {
+#pragma unroll
+          for (int z = 0; z < L::kStore; ++z) out[d + z] = r[z];
+        }
       });
   if (a.lse && h == 0)
     a.lse[(int64_t)token * a.heads + head] =
