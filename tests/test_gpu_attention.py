@@ -351,6 +351,29 @@ def test_attention_strided_rows_and_rows_of_no_sequence(pkg):
         assert bool((rest == 7).all()) and bool((lse[:2] == 7).all()) and bool((lse[2 + n:] == 7).all())
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+def test_attention_one_sequence_among_padding(pkg, dtype, cache):
+    """One sequence of few rows in a batch padded to many, split over its keys;
+    a workspace of the caller's, and the same slot in two sequences."""
+    m = Made([3000], [2], 4, 2, 64, 16, dtype, cache, seed=31)
+    want, wl, ob, lb = R.attend(m.q, m.kv, m.table_l, m.lens_l, m.starts_l, m.scale)
+    q = torch.zeros(40, 4, 64, dtype=dtype, device="cuda")
+    q[5:7] = m.q.cuda()
+    out, lse = torch.full_like(q, 7.0), torch.full((40, 4), 7.0, device="cuda")
+    args = (m.kv_cuda(), m.table.cuda(), m.lens.cuda(), (m.starts + 5).cuda())
+    need = pkg.paged_attention_workspace(q, *args, max_len=3000)
+    assert need > 0
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    pkg.paged_attention(q, *args, max_len=3000, out=out, lse=lse, work=work)
+    near(out[5:7], want, ob)
+    near(lse[5:7], wl, lb)
+    assert bool((out[:5] == 7).all()) and bool((out[7:] == 7).all()) and bool((lse[7:] == 7).all())
+    # two sequences of one slot: each's rows are its last tokens
+    m.starts_l, m.starts = [0, 1, 2], torch.tensor([0, 1, 2], dtype=torch.int32)
+    m.new, m.slots_l, m.slots = [1, 1], [0, 0], torch.tensor([0, 0], dtype=torch.int32)
+    m.check(pkg)
+
+
 def test_attention_far_pages(pkg):
     """A cache of more than 2^32 elements: the pages in use are its last ones."""
     m = Made([100, 70], [1, 50], 4, 2, 64, 16, F32, F16, seed=12)
