@@ -186,7 +186,7 @@ typedef struct nls_page_pool {
 typedef struct nls_page_tables {
   int32_t* d_table;
   int64_t table_stride;
-  int32_t slots;
+  int32_t slots; /* at most 65536 */
   int32_t max_pages;
   int32_t* d_lens;
   int32_t* d_refs;

@@ -142,7 +142,7 @@ size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
 const char* check_tables(const nls_page_tables* t, bool lens) {
   if (!t) return "NULL tables";
   if (t->slots < 1 || t->max_pages < 1 || t->pages < 1) return "tables: a size is below 1";
-  if (t->pages > kMaxPages) return "tables: more than 524288 pages";
+  if (t->pages > kMaxPages || t->slots > kMaxSlots) return "tables: more than 524288 pages or 65536 slots";
   if (t->page_size < 1 || t->page_size > kMaxPageSize || (t->page_size & (t->page_size - 1)))
     return "tables: page_size is not a power of two up to 4096";
   if (t->table_stride < 0 || (t->slots > 1 && t->table_stride < t->max_pages) || t->table_stride > (int64_t{1} << 31) ||
@@ -175,10 +175,8 @@ PoolArgs pool(const nls_page_pool* p) {
 
 // int32 words of the page calls' work area (nls_pages.hip says what they hold)
 size_t page_words(const nls_page_tables* t, int count) {
-  const size_t reserve = (size_t)t->slots + t->pages;
-  const size_t fork = 1 + 3 * (size_t)count + t->slots;
-  const size_t compact = 1 + 3 * (size_t)t->pages;
-  size_t n = reserve > fork ? reserve : fork;
+  const size_t reserve = (size_t)t->slots, fork = 1 + 2 * (size_t)count, compact = 1 + 3 * (size_t)t->pages;
+  const size_t n = reserve > fork ? reserve : fork;
   return n > compact ? n : compact;
 }
 const char* check_work(const nls_page_tables* t, int count, const void* work, size_t bytes) {
@@ -365,7 +363,7 @@ int32_t nls_cache_release(const nls_page_tables* t, const int32_t* d_slots, int3
   NLS_CHECK(check_work(t, 0, d_work, work_bytes));
   if (!d_status || !aligned(d_status, 4) || (count > 0 && !d_slots) || !aligned(d_slots, 4))
     return bad("release: NULL or misaligned");
-  return done(launch_release(tables(t), d_slots, count, d_status, static_cast<int32_t*>(d_work), stream_of(stream)),
+  return done(launch_release(tables(t), d_slots, count, d_status, stream_of(stream)),
               "nls_cache_release");
 }
 

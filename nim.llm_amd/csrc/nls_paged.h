@@ -88,6 +88,8 @@ NLS_HD int64_t tile_count(int tokens, int group, int rows, int seqs) {
   return (int64_t)tokens * group / rows + seqs;
 }
 
+constexpr int kMaxSlots = 1 << 16;  // of a page table: one bit of LDS each
+
 // ---- rotary positions and the cache's writes (nls_rope.hip)
 
 struct HeadsView {
@@ -130,8 +132,7 @@ struct TableArgs {
 hipError_t launch_reserve(const TableArgs& t, const int32_t* counts, int32_t* status, int32_t* work, hipStream_t s);
 hipError_t launch_fork(const PoolArgs& p, const TableArgs& t, const int32_t* src, const int32_t* dst, int count,
                        int32_t* status, int32_t* work, hipStream_t s);
-hipError_t launch_release(const TableArgs& t, const int32_t* slots, int count, int32_t* status, int32_t* work,
-                          hipStream_t s);
+hipError_t launch_release(const TableArgs& t, const int32_t* slots, int count, int32_t* status, hipStream_t s);
 hipError_t launch_compact(const PoolArgs& p, const TableArgs& t, int32_t* live, int32_t* work, hipStream_t s);
 hipError_t launch_copy_pages(const PoolArgs& p, int pages, const int32_t* src, const int32_t* dst, int count,
                              hipStream_t s);

@@ -9,7 +9,7 @@
 // and 4.3 written, 1.69 ms, 5.1 TB/s.  Nothing depends on the order in which workgroups
 // run.
 //
-// Work area (int32): [0] pairs to move, then the ranks' pages or the pairs.
+// Work area (int32): [0] pairs to move, then the pairs; reserve's ranks.
 #include "nls_paged.h"
 
 namespace nls {
@@ -67,14 +67,31 @@ __device__ int free_bitmap(const int32_t* refs, int pages, uint64_t* bits, int* 
   return total;
 }
 
-// out[r] = the r-th free page, r < count
-__device__ void list_free(const uint64_t* bits, const int* ranks, int pages, int count, int32_t* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (pages + 63) >> 6;
-  for (int w = wave; w < words; w += kPlanWaves) {
-    const uint64_t b = bits[w];
-    const int r = ranks[w] + __popcll(b & ((uint64_t{1} << lane) - 1));
-    if (((b >> lane) & 1) && r < count) out[r] = w * 64 + lane;
+// The r-th free page, r below their number: the last word with no more than r
+// free pages before it, then the bit.  Each thread finds its own, so that no list
+// goes through memory.
+__device__ int free_page(const uint64_t* bits, const int* ranks, int pages, int r) {
+  int lo = 0, hi = ((pages + 63) >> 6) - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (ranks[mid] <= r)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
+  // (words without a free page have the rank of the next: the search ends behind them)
+  uint64_t b = bits[lo];
+  int n = r - ranks[lo], at = 0;
+#pragma unroll
+  for (int w = 32; w; w >>= 1) {
+    const int below = __popcll(b & ((uint64_t{1} << w) - 1));
+    if (n >= below) {
+      n -= below;
+      b >>= w;
+      at += w;
+    }
+  }
+  return lo * 64 + at;
 }
 
 struct PlanLds {
@@ -88,147 +105,191 @@ __device__ PlanLds plan_lds(int pages) {
 }
 size_t plan_lds_bytes(int pages) { return (size_t)((pages + 63) >> 6) * 12; }
 
-// need[s]: the pages that slot s takes, base[s]: the rank of its first one
+// Slots by kPlanThreads: what each takes and the rank of its first page among
+// the free ones (first in `work` where there are more slots than threads).
 __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(TableArgs t, const int32_t* counts, int32_t* status,
                                                                int32_t* work) {
   __shared__ int sh[kPlanWaves];
+  __shared__ int s_len[kPlanThreads], s_take[kPlanThreads], s_base[kPlanThreads];
   const PlanLds lds = plan_lds(t.pages);
-  int32_t* base = work;
-  int32_t* ids = work + t.slots;
-  const int64_t ps = int64_t{1} << t.page_shift;
+  const int ps = 1 << t.page_shift;
   int total = 0, full = 0, bad = 0;
   for (int s0 = 0; s0 < t.slots; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
-    int need = 0;
+    int need = 0, len = 0, n = 0;
     if (s < t.slots) {
-      const int64_t len = t.lens[s], n = counts[s];
-      const int64_t have = (len + ps - 1) >> t.page_shift, want = (len + n + ps - 1) >> t.page_shift;
+      len = t.lens[s];
+      n = counts[s];
+      const int64_t have = ((int64_t)len + ps - 1) >> t.page_shift, want = ((int64_t)len + n + ps - 1) >> t.page_shift;
       if (n < 0 || len < 0)
         bad = 1;
-      else if (want > t.max_pages || len + n > 0x7fffffff)
+      else if (want > t.max_pages || (int64_t)len + n > 0x7fffffff)
         full = 1;
       else
         need = (int)(want - have);
     }
     int sum;
-    const int b = block_scan(need, sh, &sum);
-    if (s < t.slots) base[s] = total + b;
+    const int b = total + block_scan(need, sh, &sum);
+    s_len[threadIdx.x] = len;
+    s_take[threadIdx.x] = n;
+    s_base[threadIdx.x] = b;
+    if (s < t.slots) work[s] = b;
     // (slots x max_pages is below 2^31, checked on the host)
+    total += sum;
+  }
+  const int free_pages = free_bitmap(t.refs, t.pages, lds.bits, lds.ranks, sh);
+  bad = __syncthreads_or(bad);
+  full = __syncthreads_or(full);
+  const int st = bad ? 3 : full ? 2 : free_pages < total ? 1 : 0;
+  if (threadIdx.x == 0) *status = st;
+  if (st) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int s0 = 0; s0 < t.slots; s0 += kPlanThreads) {
+    if (t.slots > kPlanThreads) {  // more than LDS holds: again, a block at a time
+      __syncthreads();
+      const int s = s0 + threadIdx.x;
+      if (s < t.slots) {
+        s_len[threadIdx.x] = t.lens[s];
+        s_take[threadIdx.x] = counts[s];
+        s_base[threadIdx.x] = work[s];
+      }
+      __syncthreads();
+    }
+    const int here = t.slots - s0 < kPlanThreads ? t.slots - s0 : kPlanThreads;
+    for (int i = wave; i < here; i += kPlanWaves) {
+      const int len = s_len[i], n = s_take[i], s = s0 + i;
+      if (n == 0) continue;
+      const int have = (int)(((int64_t)len + ps - 1) >> t.page_shift);
+      const int want = (int)(((int64_t)len + n + ps - 1) >> t.page_shift);
+      for (int j = lane; j < want - have; j += 64) {
+        const int page = free_page(lds.bits, lds.ranks, t.pages, s_base[i] + j);
+        t.table[s * t.table_stride + have + j] = page;
+        t.refs[page] = 1;
+      }
+      if (lane == 0) t.lens[s] = len + n;
+    }
+  }
+}
+
+// Forks by kPlanThreads.  work: [0] pairs to copy, [1 ..] sources, then
+// destinations.
+__global__ __launch_bounds__(kPlanThreads) void fork_kernel(TableArgs t, const int32_t* src, const int32_t* dst,
+                                                            int count, int32_t* status, int32_t* work) {
+  __shared__ int sh[kPlanWaves];
+  __shared__ uint32_t mark[kMaxSlots / 32];  // the slots that are destinations
+  __shared__ int s_src[kPlanThreads], s_dst[kPlanThreads], s_len[kPlanThreads], s_rank[kPlanThreads];
+  const PlanLds lds = plan_lds(t.pages);
+  int32_t* from = work + 1;
+  int32_t* to = from + count;
+  const int mask = (1 << t.page_shift) - 1;
+  for (int i = threadIdx.x; i < (t.slots + 31) / 32; i += kPlanThreads) mark[i] = 0;
+  __syncthreads();
+  int bad = 0, full = 0, total = 0;
+  for (int i = threadIdx.x; i < count; i += kPlanThreads) {
+    const int d = dst[i];
+    if ((uint32_t)d >= (uint32_t)t.slots || (uint32_t)src[i] >= (uint32_t)t.slots)
+      bad = 1;
+    else if (atomicOr(&mark[d >> 5], 1u << (d & 31)) >> (d & 31) & 1)
+      bad = 1;  // named twice
+  }
+  const int free_pages = free_bitmap(t.refs, t.pages, lds.bits, lds.ranks, sh);  // (its barriers end the marking)
+  for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    int s = 0, d = 0, len = 0;
+    if (i < count) {
+      s = src[i];
+      d = dst[i];
+      if ((uint32_t)d < (uint32_t)t.slots && (uint32_t)s < (uint32_t)t.slots) {
+        len = t.lens[s];
+        if (t.lens[d] != 0 || len < 0 || (mark[s >> 5] >> (s & 31) & 1)) bad = 1;
+        if (((int64_t)len + mask) >> t.page_shift > t.max_pages) full = 1;
+      }
+    }
+    int sum;
+    const int part = (len & mask) != 0, r = total + block_scan(part, sh, &sum);
+    s_src[threadIdx.x] = s;
+    s_dst[threadIdx.x] = d;
+    s_len[threadIdx.x] = len;
+    s_rank[threadIdx.x] = r;
     total += sum;
   }
   bad = __syncthreads_or(bad);
   full = __syncthreads_or(full);
-  const int free_pages = free_bitmap(t.refs, t.pages, lds.bits, lds.ranks, sh);
-  const int st = bad ? 3 : full ? 2 : free_pages < total ? 1 : 0;
-  if (threadIdx.x == 0) *status = st;
-  if (st) return;
-  list_free(lds.bits, lds.ranks, t.pages, total, ids);
-  __syncthreads();  // ids and base, written by other threads of this workgroup
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int s = wave; s < t.slots; s += kPlanWaves) {
-    const int64_t len = t.lens[s], n = counts[s];
-    if (n == 0) continue;
-    const int have = (int)((len + ps - 1) >> t.page_shift), want = (int)((len + n + ps - 1) >> t.page_shift);
-    for (int j = lane; j < want - have; j += 64) {
-      const int page = ids[base[s] + j];
-      t.table[s * t.table_stride + have + j] = page;
-      t.refs[page] = 1;
-    }
-    if (lane == 0) t.lens[s] = (int)(len + n);
-  }
-}
-
-// work: [0] pairs, [1 ..] sources, then destinations; then marks of the slots
-__global__ __launch_bounds__(kPlanThreads) void fork_kernel(TableArgs t, const int32_t* src, const int32_t* dst,
-                                                            int count, int32_t* status, int32_t* work) {
-  __shared__ int sh[kPlanWaves];
-  const PlanLds lds = plan_lds(t.pages);
-  int32_t* from = work + 1;
-  int32_t* to = from + count;
-  int32_t* rank = to + count;
-  int32_t* mark = rank + count;
-  const int mask = (1 << t.page_shift) - 1;
-  for (int s = threadIdx.x; s < t.slots; s += kPlanThreads) mark[s] = 0;
-  __syncthreads();
-  int bad = 0, full = 0;
-  for (int i = threadIdx.x; i < count; i += kPlanThreads) {
-    const int d = dst[i], s = src[i];
-    if ((uint32_t)d >= (uint32_t)t.slots || (uint32_t)s >= (uint32_t)t.slots) {
-      bad = 1;
-      continue;
-    }
-    if (t.lens[d] != 0 || t.lens[s] < 0) bad = 1;
-    if (((int64_t)t.lens[s] + mask) >> t.page_shift > t.max_pages) full = 1;
-    if (atomicAdd(&mark[d], 1)) bad = 1;
-  }
-  bad = __syncthreads_or(bad);
-  if (!bad)
-    for (int i = threadIdx.x; i < count; i += kPlanThreads)
-      // (an atomic reads where the atomics above wrote)
-      if (atomicAdd(&mark[src[i]], 0)) bad = 1;
-  bad = __syncthreads_or(bad);
-  full = __syncthreads_or(full);
-  int total = 0;
-  if (!bad)
-    for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
-      const int i = i0 + threadIdx.x;
-      const int part = i < count && (t.lens[src[i]] & mask) != 0;
-      int sum;
-      const int b = block_scan(part, sh, &sum);
-      if (i < count) rank[i] = part ? total + b : -1;
-      total += sum;
-    }
-  const int free_pages = free_bitmap(t.refs, t.pages, lds.bits, lds.ranks, sh);
   const int st = bad ? 3 : full ? 2 : free_pages < total ? 1 : 0;
   if (threadIdx.x == 0) {
     *status = st;
     work[0] = st ? 0 : total;
   }
   if (st) return;
-  list_free(lds.bits, lds.ranks, t.pages, total, to);
-  __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = wave; i < count; i += kPlanWaves) {
-    const int len = t.lens[src[i]], whole = len >> t.page_shift;
-    const int32_t* a = t.table + src[i] * t.table_stride;
-    int32_t* b = t.table + dst[i] * t.table_stride;
-    for (int j = lane; j < whole; j += 64) {
-      const int page = a[j];
-      b[j] = page;
-      if ((uint32_t)page < (uint32_t)t.pages) atomicAdd(&t.refs[page], 1);
+  int before = 0;
+  for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+    if (count > kPlanThreads) {  // more than LDS holds: again, a block at a time
+      const int i = i0 + threadIdx.x;
+      const int len = i < count ? t.lens[src[i]] : 0;
+      int sum;
+      const int r = before + block_scan((len & mask) != 0, sh, &sum);
+      s_src[threadIdx.x] = i < count ? src[i] : 0;
+      s_dst[threadIdx.x] = i < count ? dst[i] : 0;
+      s_len[threadIdx.x] = len;
+      s_rank[threadIdx.x] = r;
+      before += sum;
+      __syncthreads();
     }
-    if (lane == 0) {
-      const int r = rank[i];
-      if (r >= 0) {
-        from[r] = a[whole];
-        b[whole] = to[r];
-        t.refs[to[r]] = 1;
+    const int here = count - i0 < kPlanThreads ? count - i0 : kPlanThreads;
+    for (int i = wave; i < here; i += kPlanWaves) {
+      const int len = s_len[i], whole = len >> t.page_shift;
+      const int32_t* a = t.table + s_src[i] * t.table_stride;
+      int32_t* b = t.table + s_dst[i] * t.table_stride;
+      const bool part = (len & mask) != 0;
+      for (int j = lane; j < whole + part; j += 64) {
+        const int page = a[j];
+        if (j < whole) {
+          b[j] = page;
+          if ((uint32_t)page < (uint32_t)t.pages) atomicAdd(&t.refs[page], 1);
+        } else {
+          const int r = s_rank[i], mine = free_page(lds.bits, lds.ranks, t.pages, r);
+          from[r] = page;
+          to[r] = mine;
+          b[j] = mine;
+          t.refs[mine] = 1;
+        }
       }
-      t.lens[dst[i]] = len;
+      if (lane == 0) t.lens[s_dst[i]] = len;
     }
+    if (count > kPlanThreads) __syncthreads();  // the next block's numbers take the same LDS
   }
 }
 
 __global__ __launch_bounds__(kPlanThreads) void release_kernel(TableArgs t, const int32_t* slots, int count,
-                                                               int32_t* status, int32_t* work) {
+                                                               int32_t* status) {
+  __shared__ int s_slot[kPlanThreads], s_len[kPlanThreads];
   int bad = 0;
   for (int i = threadIdx.x; i < count; i += kPlanThreads) bad |= (uint32_t)slots[i] >= (uint32_t)t.slots;
   bad = __syncthreads_or(bad);
   if (threadIdx.x == 0) *status = bad ? 3 : 0;
   if (bad) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int i = wave; i < count; i += kPlanWaves) {
-    const int s = slots[i];
-    int len = 0;
-    if (lane == 0) len = atomicExch(&t.lens[s], 0);  // a slot named twice is one wave's
-    len = __shfl(len, 0);
-    int64_t n = ((int64_t)(len < 0 ? 0 : len) + (1 << t.page_shift) - 1) >> t.page_shift;
-    if (n > t.max_pages) n = t.max_pages;
-    for (int j = lane; j < n; j += 64) {
-      const int page = t.table[s * t.table_stride + j];
-      t.table[s * t.table_stride + j] = -1;
-      if ((uint32_t)page < (uint32_t)t.pages) atomicSub(&t.refs[page], 1);
+  for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    if (i < count) {
+      s_slot[threadIdx.x] = slots[i];
+      s_len[threadIdx.x] = atomicExch(&t.lens[slots[i]], 0);  // a slot named twice has its length once
     }
+    __syncthreads();
+    const int here = count - i0 < kPlanThreads ? count - i0 : kPlanThreads;
+    for (int e = wave; e < here; e += kPlanWaves) {
+      const int len = s_len[e];
+      int32_t* row = t.table + s_slot[e] * t.table_stride;
+      int64_t n = ((int64_t)(len < 0 ? 0 : len) + (1 << t.page_shift) - 1) >> t.page_shift;
+      if (n > t.max_pages) n = t.max_pages;
+      for (int j = lane; j < n; j += 64) {
+        const int page = row[j];
+        row[j] = -1;
+        if ((uint32_t)page < (uint32_t)t.pages) atomicSub(&t.refs[page], 1);
+      }
+    }
+    __syncthreads();  // the next block's numbers take the same LDS
   }
 }
 
@@ -320,7 +381,7 @@ __global__ __launch_bounds__(kCopyThreads) void move_kernel(PoolArgs p, TableArg
 
 hipError_t allow_lds(const void* f, int pages) {
   const size_t n = plan_lds_bytes(pages);
-  return n > 60000 ? hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)n) : hipSuccess;
+  return n > 32000 ? hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)n) : hipSuccess;
 }
 
 // Workgroups that copy `items` pieces of kCopyBytes: all at once up to what
@@ -350,9 +411,8 @@ hipError_t launch_fork(const PoolArgs& p, const TableArgs& t, const int32_t* src
   return hipGetLastError();
 }
 
-hipError_t launch_release(const TableArgs& t, const int32_t* slots, int count, int32_t* status, int32_t* work,
-                          hipStream_t s) {
-  release_kernel<<<1, kPlanThreads, 0, s>>>(t, slots, count, status, work);
+hipError_t launch_release(const TableArgs& t, const int32_t* slots, int count, int32_t* status, hipStream_t s) {
+  release_kernel<<<1, kPlanThreads, 0, s>>>(t, slots, count, status);
   return hipGetLastError();
 }
 

@@ -194,7 +194,7 @@ def test_page_call_refusals(pkg):
 
     big = 1 << 30
     bad_tables = [dict(d_table=None), dict(d_table=AT + 2), dict(table_stride=4), dict(slots=0), dict(max_pages=0),
-                  dict(d_refs=None), dict(d_refs=AT + 1), dict(pages=0), dict(pages=(1 << 19) + 1), dict(page_size=3),
+                  dict(d_refs=None), dict(d_refs=AT + 1), dict(pages=0), dict(pages=(1 << 19) + 1), dict(slots=(1 << 16) + 1), dict(page_size=3),
                   dict(page_size=0), dict(page_size=8192), dict(slots=1 << 16, max_pages=1 << 16, table_stride=1 << 16)]
     bad_pools = [dict(d_kv=None), dict(d_kv=AT + 8), dict(layers=0), dict(page_bytes=0), dict(page_bytes=24),
                  dict(layer_stride=8), dict(page_stride=2048), dict(page_stride=-16), dict(layer_stride=2048)]

@@ -552,7 +552,7 @@ def _same(cache, model, what):
 
 @pytest.mark.parametrize("slots,per,pages,ps,layers,d", [(6, 5, 20, 4, 3, 8), (3, 70, 200, 1, 1, 8), (40, 9, 150, 16, 2, 64),
                                                          (5, 40, 5000, 8, 1, 16), (1, 1, 1, 4096, 1, 8),
-                                                         (1100, 3, 2500, 2, 1, 8)])
+                                                         (1100, 3, 2500, 2, 1, 8), (4, 50, 1 << 19, 1, 1, 8)])
 def test_pages_follow_the_rules(pkg, slots, per, pages, ps, layers, d):
     """Random reserves, forks, releases and compactions, refused ones among them,
     against the rules on lists."""
@@ -597,6 +597,39 @@ def test_pages_follow_the_rules(pkg, slots, per, pages, ps, layers, d):
         seen.add((op, want if op != "compact" else 0))
         _same(c, model, f"step {step} {op}")
     assert ("reserve", 0) in seen and ("compact", 0) in seen
+
+
+def test_pages_of_many_slots_at_once(pkg):
+    """More forks and releases in one call than a workgroup has threads, against
+    the rules on lists; then one too many for the pages."""
+    slots, pages, ps = 2300, 1700, 4
+    c = pkg.PagedCache(2, pages, ps, 1, 8, slots, 3)
+    model = Pages(slots, 3, pages, ps)
+    c.kv.copy_((torch.tensor(model.label).float()[None, :] + 10000 * torch.arange(2)[:, None])
+               .reshape(2, pages, 1, 1, 1, 1).cuda().expand_as(c.kv))
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    rng = random.Random(8)
+    counts = [7, 8, 1] + [0] * (slots - 3)
+    assert int(c.reserve(ints(counts))) == model.reserve(counts) == 0
+    dst = list(range(3, slots))
+    rng.shuffle(dst)
+    src = [rng.randrange(3) for _ in dst]
+    say("[pages] 2297 forks")
+    assert int(c.fork(ints(src), ints(dst))) == model.fork(src, dst) == 0
+    _same(c, model, "forks")
+    gone = [s for s in range(slots) if s % 3] + [5, 4]
+    say("[pages] releases")
+    assert int(c.release(ints(gone))) == model.release(gone) == 0
+    _same(c, model, "releases")
+    assert int(c.compact()) == model.compact()
+    _same(c, model, "compact")
+    src, dst = [0] * len(gone[:-2]), gone[:-2]
+    say("[pages] too many forks")
+    assert int(c.fork(ints(src), ints(dst))) == model.fork(src, dst) == 1
+    _same(c, model, "too many")
+    dst[-1] = dst[0]
+    assert int(c.fork(ints(src), ints(dst))) == model.fork(src, dst) == 3
+    _same(c, model, "twice")
 
 
 def test_copy_pages(pkg):
