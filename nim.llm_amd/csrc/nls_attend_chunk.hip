@@ -219,7 +219,8 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   // Values that are not finite meet weights of 0 in the rows that do not see
   // their keys, which would be NaN there.  Where rows see different keys such a
   // value is put as 0, and noted: the rows that see its key turn to NaN after
-  // the products.
+  // the products.  (This wave's rows may see the whole tile all the same.)
+  auto mixed = [&](int kb) { return kb < tile_lo || kb + KT - 1 > tile_hi; };
   auto put_v = [&](char* to, uint64_t there, int kb, int buf) {
     bool any = false;
     if (there != ~uint64_t{0} || dim < D) {
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
       for (int n = 0; n < L::kStage; ++n)
         if (!ok_at(n, there)) stage[n] = u4{0, 0, 0, 0};
     }
-    if (kb < tile_lo || kb + KT - 1 > tile_hi) {
+    if (mixed(kb)) {
 #pragma unroll
       for (int n = 0; n < L::kStage; ++n) {
         TC e[L::KD];
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
       }
     }
     if (more) put_v(next + L::kBytes, there1, kb + KT, buf ^ 1);
-    if (used && !whole && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
+    if (used && mixed(kb) && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
 #pragma unroll 1
       for (int n = 0; n < KT; ++n) {
         const int key = kb + n;

@@ -265,6 +265,30 @@ def test_attention_masked_values_do_not_reach_a_row(pkg, dtype, cache):
     near(lse, clean[1], clean[3])
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lens,new", [([37, 60], [4, 2]), ([130, 90], [130, 60]), ([300], [300]), ([700, 40], [150, 1])])
+def test_attention_infinite_values_reach_the_rows_that_see_them(pkg, dtype, cache, lens, new):
+    """An infinity or NaN among the values alone: every row that sees its key is
+    infinite or NaN there, in that element and no other, and the rows that do not
+    see it come out as without it."""
+    say(f"[attend] infinite values {NAME[dtype]}/{NAME[cache]} lens {lens} new {new}")
+    m = Made(lens, new, 4, 2, 64, 16, dtype, cache, seed=9)
+    want, _, bound, _ = R.attend(m.q, m.kv, m.table_l, m.lens_l, m.starts_l, m.scale)
+    want, bound = want.clone(), bound.clone()
+    sees = torch.zeros(want.shape, dtype=torch.bool)
+    for s, j, h, e, value in ((0, 5, 0, 3, math.inf), (0, lens[0] - new[0] + new[0] // 2, 1, 40, math.nan),
+                              (0, lens[0] - 1, 1, 63, -math.inf), (len(lens) - 1, 0, 0, 17, math.inf)):
+        m.kv[m.table_l[s][j // 16], 1, h, j % 16, e] = value
+        for t in range(new[s]):
+            if lens[s] - new[s] + t >= j:
+                sees[m.starts_l[s] + t, 2 * h:2 * h + 2, e] = True
+    got = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), max(new),
+                              max(lens)).double().cpu()
+    assert not bool(torch.isfinite(got[sees]).any()), f"{int(torch.isfinite(got[sees]).sum())} of {int(sees.sum())} finite"
+    want[sees] = math.nan
+    near(got, want, bound)
+
+
 def test_attention_scores_of_minus_infinity(pkg):
     """A key whose score is -infinity weighs nothing; a row with none else is
     empty."""
