@@ -535,7 +535,6 @@ Parts parts_of_keys(int64_t most, int64_t tasks, int64_t want, int64_t least, in
   if (keys > top) keys = top;
   if (keys < least) keys = least;
   if (keys < (most + cap - 1) / cap) keys = (most + cap - 1) / cap;
-  if (keys > kMaxLen) keys = kMaxLen;
   p.keys = (int)((keys + 127) / 128 * 128);
   const int64_t m = (most + p.keys - 1) / p.keys;
   p.most = (int)(m < 1 ? 1 : m);
@@ -548,6 +547,7 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   if (a.p.seqs < 1 || a.p.tokens < 1) return p;
   const int D = width_of(a.p.dim);
   int64_t most = (int64_t)a.p.max_pages << a.p.page_shift;
+  if (most > kMaxLen) most = kMaxLen;  // (a longer table's rest is never used)
   if (max_len > 0 && max_len < most) most = max_len;
   int64_t longest = max_new > 0 && max_new < a.p.tokens ? max_new : a.p.tokens;
   if (a.window > 0 && most > (int64_t)a.window + longest) most = (int64_t)a.window + longest;

@@ -131,6 +131,14 @@ def test_attention_refusals(pkg):
     assert call(ch=_chunks(pkg, seqs=0, d_starts=None)) == OK
     for kw in (dict(tokens=0), dict(seqs=0)):
         assert L.nls_paged_attention_workspace(_cache(pkg), _chunks(pkg, **kw), 4, 1, 1 << 20, 0) == 0
+    # a table of more places than a context has tokens counts as its longest context
+    for tokens, heads, max_new in ((1 << 20, 32, 0), (3, 4, 1), (900, 4, 0)):
+        ch = _chunks(pkg, seqs=3, tokens=tokens)
+        size = lambda max_len, **kw: L.nls_paged_attention_workspace(_cache(pkg, page_size=4096, **kw), ch, heads, max_new,
+                                                                     max_len, 0)
+        assert size(0, max_pages=1 << 20) == size(1 << 40, max_pages=1 << 20) == size(0x7fffff00, max_pages=1 << 20)
+    assert L.nls_paged_attention_workspace(_cache(pkg, page_size=4096, max_pages=1 << 20), _chunks(pkg, seqs=1, tokens=1 << 20),
+                                           32, 0, 0, 0) == 0
     # the workspace's own checks
     for kw in (dict(kv_heads=0), dict(head_dim=300), dict(page_size=5), dict(max_pages=0)):
         assert L.nls_paged_attention_workspace(_cache(pkg, **kw), _chunks(pkg), 4, 1, 100, 0) == 0
