@@ -921,9 +921,13 @@ PAGES_DONE, PAGES_NONE_LEFT, PAGES_ROW_FULL, PAGES_BAD_ENTRY = range(4)
 def _page_pool(dev: int, kv):
     layers, _, two, heads, page_size, dim = kv.shape
     st, n = kv.stride(), kv.element_size()
-    assert kv.get_device() == dev and two == 2 and sorted(st[2:]) == sorted(kv[0, 0].contiguous().stride()), (
+    dense = 1  # elements of a page so far, in the order of the strides
+    for stride, size in sorted(zip(st[2:], kv.shape[2:])):
+        if size != 1:
+            dense = dense * size if stride == dense else 0
+    assert kv.get_device() == dev and two == 2 and dense == 2 * heads * page_size * dim, (
         "the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
-    return NlsPagePool(kv.data_ptr(), layers, 2 * heads * page_size * dim * n, st[0] * n, st[1] * n)
+    return NlsPagePool(kv.data_ptr(), layers, dense * n, st[0] * n, st[1] * n)
 
 
 def _page_tables(dev: int, table, lens, refs, page_size: int):

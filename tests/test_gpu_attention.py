@@ -667,6 +667,47 @@ def test_copy_pages(pkg):
     assert torch.equal(kv, want)
 
 
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (2, 0, 1, 3), (1, 2, 0, 3), (2, 1, 0, 3)])
+@pytest.mark.parametrize("kv_heads,ps,d", [(3, 4, 8), (1, 8, 16), (5, 1, 8)])
+def test_pages_in_any_dense_order(pkg, order, kv_heads, ps, d):
+    """Pages whose (key or value, head, token) come in any order: copied, forked
+    and compacted as the plain order is."""
+    say(f"[pages] order {order} {kv_heads} x {ps} x {d}")
+    sizes = (2, kv_heads, ps, d)
+    back = [order.index(i) for i in range(4)]
+    made = lambda: torch.zeros((2, 12) + tuple(sizes[i] for i in order), device="cuda").permute(0, 1, *[2 + i for i in back])
+    g = torch.Generator().manual_seed(3)
+    init = torch.randn((2, 12) + sizes, generator=g).cuda()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    kv = made().copy_(init)
+    assert kv.shape[2:] == sizes
+    pkg.cache_copy_pages(kv, ints([3, 7]), ints([1, 0]))
+    init[:, 1], init[:, 0] = init[:, 3].clone(), init[:, 7].clone()
+    assert torch.equal(kv, init)
+    c = pkg.PagedCache(2, 12, ps, kv_heads, d, 3, 8)
+    c.kv = kv
+    n = 2 * ps + ps // 2
+    assert int(c.reserve(ints([1, n, 0]))) == 0
+    assert int(c.fork(ints([1]), ints([2]))) == 0
+    assert int(c.release(ints([0]))) == 0
+    live = int(c.compact())
+    assert live == -(-n // ps) + (n % ps != 0)
+    for s in (1, 2):
+        assert c.table[s, :-(-n // ps)].max() < live
+        for j in range(n):
+            # pages 1 .. were slot 1's when the contents were made
+            assert torch.equal(kv[:, c.table[s, j // ps].item(), :, :, j % ps], init[:, 1 + j // ps, :, :, j % ps])
+
+
+def test_pages_that_are_not_dense_are_refused(pkg):
+    ints = torch.tensor([0], dtype=torch.int32).cuda()
+    wide = torch.zeros(2, 12, 2, 3, 4, 16, device="cuda")
+    for kv in (wide[..., :8], wide[:, :, :, :2], wide[:, :, :, :, ::2], wide[:, :, :, :1].expand(2, 12, 2, 3, 4, 16),
+               wide.as_strided((2, 12, 2, 4, 1, 8), (768, 64, 8, 32, 8, 1))):
+        with pytest.raises(AssertionError):
+            pkg.cache_copy_pages(kv, ints, ints)
+
+
 # ---------------------------------------------------------------- together
 
 
