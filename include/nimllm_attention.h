@@ -55,7 +55,7 @@ enum { NLS_ROPE_NONE = 0, NLS_ROPE_LINEAR = 1, NLS_ROPE_YARN = 2 };
  *           over original_context positions, as it is where it turns more than
  *           beta_fast times, blended in between; the amplitude is
  *           attn_factor * (0.1 ln(factor) + 1), attn_factor otherwise
- * and divided by freq_factors[j] (host, dim / 2 entries, or NULL), the
+ * and divided by freq_factors[j] (host, dim / 2 entries, none 0, or NULL), the
  * rope_freqs tensor of a GGUF file. */
 typedef struct nls_rope_scaling {
   int32_t kind;
@@ -95,8 +95,8 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
 /* One layer's keys and values: the key of page p, head h, token t starts at
  * d_kv + p * page_stride + h * head_stride + t * token_stride (elements), the
  * value value_offset elements behind it.  All four strides are multiples of 8
- * (page_stride and token_stride below 2^30), d_kv is 16-byte aligned, head_dim a multiple of 8 up to 256, page_size a
- * power of two up to 4096.  A table entry outside [0, pages) is no page: what
+ * (page_stride and token_stride below 2^30), d_kv is 16-byte aligned, head_dim a
+ * multiple of 8 up to 256, page_size a power of two up to 4096.  A table entry outside [0, pages) is no page: what
  * it would hold is neither read nor written, and attention sees no key there. */
 typedef struct nls_paged_kv {
   void* d_kv;
@@ -151,7 +151,8 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
  * contiguous) is not NULL.  A row without a key, or whose every score is
  * -infinity, has out = 0 and lse = -infinity.  What a key that a row does not
  * see holds, infinities and NaN among it, does not reach that row; an infinite
- * value that it does see makes it infinite or NaN.
+ * value that it does see makes it infinite or NaN.  (An infinite key that it
+ * sees makes its score infinite, or NaN where fp32 queries meet 16-bit keys.)
  * type (q and out): F32 with any cache type, F16 or BF16 with the same one.
  * Scores, statistics and sums are fp32: fp32 queries and weights meet 16-bit
  * keys and values as exact sums of 16-bit parts, 16-bit queries and weights

@@ -889,7 +889,9 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
     tokens, heads, dim = q.shape
     if out is None:
         out = torch.empty(q.shape, dtype=dt, device=q.device)
-    if lse is True:
+    if lse is False:
+        lse = None
+    elif lse is True:
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
     elif lse is not None:
         assert lse.get_device() == dev and lse.dtype == torch.float32 and lse.is_contiguous() \

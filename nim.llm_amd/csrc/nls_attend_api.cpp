@@ -200,6 +200,8 @@ int32_t nls_rope_frequencies(const nls_rope_scaling* s, int32_t dim, double* fre
     return bad("rope: no such scaling");
   if (!(s->base > 0) || !std::isfinite(s->base) || !std::isfinite(s->attn_factor)) return bad("rope: base or attn_factor");
   if (s->kind != NLS_ROPE_NONE && (!(s->factor > 0) || !std::isfinite(s->factor))) return bad("rope: factor");
+  for (int j = 0; s->freq_factors && j < dim / 2; ++j)
+    if (!(std::fabs(s->freq_factors[j]) > 0)) return bad("rope: a frequency factor is 0 or NaN");
   double lo = 0, hi = 0;
   if (s->kind == NLS_ROPE_YARN) {
     if (!(s->original_context > 0) || !(s->beta_fast > 0) || !(s->beta_slow > 0) || !(s->base > 1) ||

@@ -49,7 +49,8 @@ def test_rope_frequencies_refusals(pkg):
            dict(dim=64, scaling="yarn", factor=4.0), dict(dim=64, scaling="yarn", factor=4.0, original_context=math.inf),
            dict(dim=64, scaling="yarn", factor=4.0, original_context=4096.0, beta_fast=0.0),
            dict(dim=64, scaling="yarn", factor=4.0, original_context=4096.0, base=1.0),
-           dict(dim=64, attn_factor=math.nan), dict(dim=64, scaling="other")]
+           dict(dim=64, attn_factor=math.nan), dict(dim=64, scaling="other"),
+           dict(dim=4, freq_factors=[1.0, 0.0]), dict(dim=4, freq_factors=[math.nan, 1.0])]
     for kw in bad:
         with pytest.raises(pkg.SamplerError):
             pkg.rope_frequencies(**kw)

@@ -310,6 +310,32 @@ def test_attention_scores_of_minus_infinity(pkg):
     del want
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lens,new", [([150, 40], [150, 3]), ([400, 70], [100, 1])])
+def test_attention_keys_of_minus_infinity(pkg, dtype, cache, lens, new):
+    """Keys of -infinity under queries above 0 are as if they were not there; fp32
+    queries over 16-bit keys may have NaN for them, and only in rows that see one."""
+    say(f"[attend] keys of -infinity {NAME[dtype]}/{NAME[cache]} lens {lens}")
+    m = Made(lens, new, 4, 2, 64, 1, dtype, cache, seed=12)
+    m.q = m.q.abs() + 0.125
+    gone = [(0, j) for j in (0, 1, 7, 63, 64, 100, lens[0] - 1)] + [(1, j) for j in range(0, 40, 2)]
+    without = [list(r) for r in m.table_l]
+    for s, j in gone:
+        without[s][j] = -1
+    want, lse, ob, lb = R.attend(m.q, m.kv, without, m.lens_l, m.starts_l, m.scale)
+    for s, j in gone:
+        m.kv[m.table_l[s][j], 0, :, 0] = -math.inf
+    got, l = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), max(new),
+                                 max(lens), lse=True)
+    if dtype == F32 and cache != F32:
+        # (the first key is -infinity: every row sees one)
+        got, l = got.double().cpu(), l.double().cpu()
+        want, lse = want.clone(), lse.clone()
+        want[torch.isnan(got)], lse[torch.isnan(l)] = math.nan, math.nan
+    near(got, want, ob)
+    near(l, lse, lb)
+
+
 def test_attention_large_scores(pkg):
     """Scores of hundreds, either sign, and queries beyond fp16's range: the
     maximum leaves before the exponential."""
@@ -396,6 +422,17 @@ def test_attention_one_sequence_among_padding(pkg, dtype, cache):
     m.starts_l, m.starts = [0, 1, 2], torch.tensor([0, 1, 2], dtype=torch.int32)
     m.new, m.slots_l, m.slots = [1, 1], [0, 0], torch.tensor([0, 0], dtype=torch.int32)
     m.check(pkg)
+
+
+def test_attention_with_and_without_lse(pkg):
+    m = Made([33, 5], [20, 1], 4, 2, 64, 16, F32, F16, seed=4)
+    args = (m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda())
+    got, lse = pkg.paged_attention(*args, lse=True)
+    mine = torch.full_like(lse, 7.0)
+    again, same = pkg.paged_attention(*args, lse=mine)
+    assert same is mine and torch.equal(mine, lse) and torch.equal(got, again)
+    for none in (None, False):
+        assert torch.equal(pkg.paged_attention(*args, lse=none), got)
 
 
 def test_attention_far_pages(pkg):
