@@ -20,11 +20,12 @@
 // either 16-bit type hold without loss, and the sums need no rescaling.  It is
 // a whole number, so that what it is taken from and given back to is exact.
 //
-// 2048 tokens over 16384 keys, 32 heads of 128, fp32 over fp16: 960 us, 1073
+// 2048 tokens over 16384 keys, 32 heads of 128, fp32 over fp16: 928 us, 1110
 // TFLOP/s of products, which is what a large fp16 matrix product reaches on
-// this card.  Two prompts of 4001, heads of 64, bf16: 170 us, 590 TFLOP/s, bound
-// by the 16 exponentials and about 100 other vector instructions beside each 8
-// products.
+// this card.  Two prompts of 4001, heads of 64, bf16: 160 us, 630 TFLOP/s: 16
+// exponentials and about 90 other vector instructions stand beside each 8
+// products.  (There, both halves of a tile in turn under each other's
+// exponentials take 191 registers, and 206 us.)
 #include "nls_attend.h"
 
 namespace nls {
@@ -91,8 +92,17 @@ __device__ __forceinline__ void put_run(const f16x* o, int t, int y, int h, floa
 typedef short s4x __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4x* lds_s4x;
 
+// Waves per SIMD that registers are kept for.  Narrow heads of 16-bit queries
+// have so many instructions beside their products that four waves hide each
+// other's best (two prompts of 4001: 171 us with three, 166 with four).
 template <typename T, typename TC, int D>
-__global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2) void chunk_kernel(AttendArgs a, Parts parts, bool alone) {
+constexpr int chunk_waves() {
+  return sizeof(TC) == 4 || D == 256 ? 1 : D == 64 && sizeof(T) == 2 ? 4 : 2;
+}
+
+template <typename T, typename TC, int D>
+__global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void chunk_kernel(AttendArgs a, Parts parts,
+                                                                                        bool alone) {
   using L = Tile<T, TC, D>;
   using vec = typename Elem<TC>::vec;
   constexpr int NP = L::NP, KT = L::KT, NS = KT / 32;
@@ -185,7 +195,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
     return kb + (lane & (KT - 1)) < k1 && (uint32_t)entry < (uint32_t)a.p.pages ? entry : -1;
   };
   u4 stage[L::kStage];  // K of the next tile, then its V
-  const char* row_of[L::kStage];
+  uint64_t row_of[L::kStage];  // from `base` on
   auto fetch_k = [&](int kb, int page) {
     // (a place that is no key reads page 0; it is not put)
     const uint64_t off = (uint64_t)(uint32_t)(page < 0 ? 0 : page) * page_bytes +
@@ -194,13 +204,13 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
 #pragma unroll
     for (int n = 0; n < L::kStage; ++n) {
       const int r = n * L::kRowsPerStep + srow;
-      row_of[n] = base + ((uint64_t)(uint32_t)__shfl(lo, r) | (uint64_t)(uint32_t)__shfl(hi, r) << 32);
-      stage[n] = *reinterpret_cast<const u4*>(row_of[n]);
+      row_of[n] = (uint64_t)(uint32_t)__shfl(lo, r) | (uint64_t)(uint32_t)__shfl(hi, r) << 32;
+      stage[n] = *reinterpret_cast<const u4*>(base + row_of[n]);
     }
   };
   auto fetch_v = [&]() {
 #pragma unroll
-    for (int n = 0; n < L::kStage; ++n) stage[n] = *reinterpret_cast<const u4*>(row_of[n] + to_value);
+    for (int n = 0; n < L::kStage; ++n) stage[n] = *reinterpret_cast<const u4*>(base + (row_of[n] + to_value));
   };
   // there: which keys of the tile there are
   auto ok_at = [&](int n, uint64_t there) { return piece_ok && ((there >> (n * L::kRowsPerStep + srow)) & 1); };
@@ -265,26 +275,27 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
   auto step = [&](bool whole, int sub, const char* lk, const char* lv, int kb, uint64_t there) {
     const char* row_k = lk + (sub * 32 + i) * L::kPieces * 16;
     f16x s{};
-    // wide heads: products go before another wave's exponentials (D = 128: 1039
-    // -> 1010 us for 2048 tokens over 16384 keys; D = 64 is slower with it, 183
-    // -> 187 us for two prompts of 4001)
-    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
+    // Products go before another wave's exponentials (2048 tokens over 16384 keys:
+    // 1039 -> 1010 us; two prompts of 4001, heads of 64: 166 -> 160 us; the first
+    // product's alone: 952 and 166).
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int k = 0; k < L::KC; ++k) {
       const vec x = *reinterpret_cast<const vec*>(row_k + L::k_piece(i, k * 2 + h) * 16);
 #pragma unroll
       for (int n = NP - 1; n >= 0; --n) s = mma32(x, q[k][n], s);
     }
-    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_setprio(0);
     if (!whole) {
       const int lo = low - kb - sub * 32, hi = pos - kb - sub * 32;  // of the 32 keys
       const int from = lo < 0 ? 0 : lo > 32 ? 32 : lo, to = hi < 0 ? 0 : hi > 31 ? 32 : hi + 1;
       // bit n: this row sees key n
       const uint32_t seen = (uint32_t)(there >> (sub * 32)) & (uint32_t)((uint64_t{1} << to) - 1) &
                             ~(uint32_t)((uint64_t{1} << from) - 1);
+      const uint32_t mine = seen >> (4 * h);  // (shifted once: 16 bits by number, not 16 registers)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (!((seen >> (8 * (r >> 2) + 4 * h + (r & 3))) & 1)) s[r] = minus_inf();
+        if (!((mine >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = minus_inf();
     }
     // Weights from the maximum so far; when they add up to more than 2^8 of the
     // largest (or to NaN), the maximum is brought up to date first.
@@ -324,7 +335,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
       if (to == minus_inf()) back = __builtin_inff();  // no key yet: the next one sets it
     }
     l += sum;
-    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_s_setprio(1);
     if constexpr (!L::kWide) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {  // 16 keys
@@ -360,7 +371,7 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
         }
       }
     }
-    if constexpr (D >= 128) __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_setprio(0);
   };
 
   uint64_t there = 0, there1 = 0;  // (KT 32: each half is the tile)
@@ -390,14 +401,15 @@ __global__ __launch_bounds__(kChunkThreads, sizeof(TC) == 4 || D == 256 ? 1 : 2)
     const bool used = busy && kb <= any_hi && kb + KT > any_lo;
     const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && there == ~uint64_t{0};
 #pragma unroll
-    for (int sub = 0; sub < NS; ++sub) {
+    for (int sub = 0; sub < NS; ++sub)
       if (used) step(whole, sub, lk, lv, kb, there);
-      if (more && sub == 0) {
-        put_k(next, there1);
-        fetch_v();
-      }
+    // (behind the steps, not between them: 945 -> 932 us for 2048 tokens over
+    // 16384 keys)
+    if (more) {
+      put_k(next, there1);
+      fetch_v();
+      put_v(next + L::kBytes, there1, kb + KT, buf ^ 1);
     }
-    if (more) put_v(next + L::kBytes, there1, kb + KT, buf ^ 1);
     if (used && mixed(kb) && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
 #pragma unroll 1
       for (int n = 0; n < KT; ++n) {
