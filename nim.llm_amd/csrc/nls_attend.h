@@ -174,9 +174,16 @@ template <typename TC>
 constexpr float chunk_shift() {
   return __is_same(TC, _Float16) ? 7.f : 0.f;
 }
-// alone: sequences of few rows are its too
-hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles, bool alone,
-                        hipStream_t s);
+// Where few rows and chunks share a launch: where registers for as many waves
+// suit both (one SIMD takes two of either, or one).
+template <typename TC, int D>
+constexpr bool together() {
+  return D == 256 || (D == 128 && sizeof(TC) == 2);
+}
+// few: the parts of the sequences of few rows, which the launch takes too where
+// they go together; NULL: those are chunks as well
+hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+                        const Parts* few, int few_tiles, hipStream_t s);
 
 // How a call's rows are dealt out.
 struct AttendPlan {

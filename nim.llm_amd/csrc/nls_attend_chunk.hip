@@ -26,7 +26,7 @@
 // exponentials and about 90 other vector instructions stand beside each 8
 // products.  (There, both halves of a tile in turn under each other's
 // exponentials take 191 registers, and 206 us.)
-#include "nls_attend.h"
+#include "nls_attend_few.h"
 
 namespace nls {
 namespace {
@@ -101,8 +101,8 @@ constexpr int chunk_waves() {
 }
 
 template <typename T, typename TC, int D>
-__global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void chunk_kernel(AttendArgs a, Parts parts,
-                                                                                        bool alone) {
+__device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& parts, bool alone, int group_at,
+                                           int groups, int part) {
   using L = Tile<T, TC, D>;
   using vec = typename Elem<TC>::vec;
   constexpr int NP = L::NP, KT = L::KT, NS = KT / 32;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void chun
   __shared__ uint8_t noted[2][KT][L::kPieces];       // bit j: element j of a piece of V was not finite
   __shared__ int has_noted[2][kChunkWaves];
 
-  const int kvh = blockIdx.x % a.p.kv_heads, tile = (gridDim.x - 1 - blockIdx.x) / a.p.kv_heads, part = blockIdx.z;
+  const int kvh = group_at % a.p.kv_heads, tile = (groups - 1 - group_at) / a.p.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
 
   // the sequence whose tiles begin at or before this one
@@ -474,36 +474,76 @@ __global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void chun
         l == 0.f ? minus_inf() : (from + (__builtin_amdgcn_logf(l) - L::kShift)) * kLn2;
 }
 
+// alone: sequences of few rows are its too
 template <typename T, typename TC, int D>
-hipError_t chunk_of_width(const AttendArgs& a, const Parts& parts, int64_t tiles, bool alone, hipStream_t s) {
-  constexpr int lds = 4 * Tile<T, TC, D>::kBytes;
-  if (lds > 60000) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_kernel<T, TC, D>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-  }
-  chunk_kernel<T, TC, D><<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), kChunkThreads, lds, s>>>(a, parts, alone);
+__global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void chunk_kernel(AttendArgs a, Parts parts,
+                                                                                        bool alone) {
+  chunk_rows<T, TC, D>(a, parts, alone, blockIdx.x, gridDim.x, blockIdx.z);
+}
+
+// Chunks, and the sequences of few rows behind them in the grid: those fill the
+// GPU while the chunks' last workgroups end, and read while others multiply.
+template <typename T, typename TC, int D, bool kPad>
+__global__ __launch_bounds__(kChunkThreads, (chunk_waves<T, TC, D>())) void both_kernel(AttendArgs a, Parts chunk,
+                                                                                       Parts few, int few_tiles,
+                                                                                       int chunk_groups, int few_groups) {
+  static_assert(kChunkThreads == kFewThreads, "one workgroup for both");
+  const int b = blockIdx.x, n = chunk_groups * chunk.most;
+  if (b < n)
+    chunk_rows<T, TC, D>(a, chunk, false, b % chunk_groups, chunk_groups, b / chunk_groups);
+  else
+    few_rows<T, TC, D, kPad>(a, few, few_tiles, true, (b - n) % few_groups, (b - n) / few_groups);
+}
+
+hipError_t allow_lds(const void* f, size_t lds) {
+  return lds > 60000 ? hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) : hipSuccess;
+}
+
+template <typename T, typename TC, int D, bool kPad>
+hipError_t both_of(const AttendArgs& a, const Parts& parts, int64_t tiles, const Parts& few, int few_tiles,
+                   hipStream_t s) {
+  constexpr size_t chunk_lds = 4 * Tile<T, TC, D>::kBytes, lds = chunk_lds > few_lds_bytes(D) ? chunk_lds : few_lds_bytes(D);
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(both_kernel<T, TC, D, kPad>), lds);
+  if (e != hipSuccess) return e;
+  const int chunk_groups = (int)(tiles * a.p.kv_heads), few_groups = a.p.seqs * few_tiles * a.p.kv_heads;
+  const int64_t all = (int64_t)chunk_groups * parts.most + (int64_t)few_groups * few.most;
+  both_kernel<T, TC, D, kPad><<<(unsigned)all, kChunkThreads, lds, s>>>(a, parts, few, few_tiles, chunk_groups, few_groups);
+  return hipGetLastError();
+}
+
+template <typename T, typename TC, int D>
+hipError_t chunk_of_width(const AttendArgs& a, const Parts& parts, int64_t tiles, const Parts* few, int few_tiles,
+                          hipStream_t s) {
+  if constexpr (together<TC, D>())
+    if (few)
+      return a.p.dim == D ? both_of<T, TC, D, false>(a, parts, tiles, *few, few_tiles, s)
+                          : both_of<T, TC, D, true>(a, parts, tiles, *few, few_tiles, s);
+  constexpr size_t lds = 4 * Tile<T, TC, D>::kBytes;
+  const hipError_t e = allow_lds(reinterpret_cast<const void*>(chunk_kernel<T, TC, D>), lds);
+  if (e != hipSuccess) return e;
+  chunk_kernel<T, TC, D><<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), kChunkThreads, lds, s>>>(a, parts, !few);
   return hipGetLastError();
 }
 
 template <typename T, typename TC>
-hipError_t chunk_of_types(const AttendArgs& a, const Parts& parts, int64_t tiles, bool alone, hipStream_t s) {
-  if (a.p.dim <= 64) return chunk_of_width<T, TC, 64>(a, parts, tiles, alone, s);
-  if (a.p.dim <= 128) return chunk_of_width<T, TC, 128>(a, parts, tiles, alone, s);
-  return chunk_of_width<T, TC, 256>(a, parts, tiles, alone, s);
+hipError_t chunk_of_types(const AttendArgs& a, const Parts& parts, int64_t tiles, const Parts* few, int few_tiles,
+                          hipStream_t s) {
+  if (a.p.dim <= 64) return chunk_of_width<T, TC, 64>(a, parts, tiles, few, few_tiles, s);
+  if (a.p.dim <= 128) return chunk_of_width<T, TC, 128>(a, parts, tiles, few, few_tiles, s);
+  return chunk_of_width<T, TC, 256>(a, parts, tiles, few, few_tiles, s);
 }
 
 }  // namespace
 
-hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles, bool alone,
-                        hipStream_t s) {
+hipError_t launch_chunk(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+                        const Parts* few, int few_tiles, hipStream_t s) {
   if (type == kF32) {
-    if (cache_type == kF32) return chunk_of_types<float, float>(a, parts, tiles, alone, s);
-    if (cache_type == kF16) return chunk_of_types<float, _Float16>(a, parts, tiles, alone, s);
-    return chunk_of_types<float, __bf16>(a, parts, tiles, alone, s);
+    if (cache_type == kF32) return chunk_of_types<float, float>(a, parts, tiles, few, few_tiles, s);
+    if (cache_type == kF16) return chunk_of_types<float, _Float16>(a, parts, tiles, few, few_tiles, s);
+    return chunk_of_types<float, __bf16>(a, parts, tiles, few, few_tiles, s);
   }
-  if (type == kF16) return chunk_of_types<_Float16, _Float16>(a, parts, tiles, alone, s);
-  return chunk_of_types<__bf16, __bf16>(a, parts, tiles, alone, s);
+  if (type == kF16) return chunk_of_types<_Float16, _Float16>(a, parts, tiles, few, few_tiles, s);
+  return chunk_of_types<__bf16, __bf16>(a, parts, tiles, few, few_tiles, s);
 }
 
 }  // namespace nls

@@ -435,6 +435,30 @@ def test_attention_with_and_without_lse(pkg):
         assert torch.equal(pkg.paged_attention(*args, lse=none), got)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_many_empty_sequences(pkg, d):
+    """Thousands of sequences of no rows around a chunk and single tokens, with
+    hints of far longer contexts."""
+    seqs, at = 4000, {3: (700, 90), 1999: (300, 1), 3999: (65, 20)}
+    m = Made([n for n, _ in at.values()], [k for _, k in at.values()], 16, 8, d, 16, F32, BF16, seed=6)
+    want, lse, ob, lb = R.attend(m.q, m.kv, m.table_l, m.lens_l, m.starts_l, m.scale)
+    starts, slots = [0], []
+    for s in range(seqs):
+        starts.append(starts[-1] + at.get(s, (0, 0))[1])
+        slots.append(sorted(at).index(s) if s in at else s % 5 - 1)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    say(f"[attend] {seqs} sequences, heads of {d}")
+    got, l = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), ints(starts), slots=ints(slots),
+                                 max_new=90, max_len=700, lse=True)
+    near(got, want, ob)
+    near(l, lse, lb)
+    wide = torch.full((3, 1 << 16), -1, dtype=torch.int32)  # room for contexts of a million tokens
+    wide[:, :m.table.shape[1]] = m.table
+    got, l = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), wide.cuda(), m.lens.cuda(), ints(starts), slots=ints(slots), lse=True)
+    near(got, want, ob)
+    near(l, lse, lb)
+
+
 def test_attention_far_pages(pkg):
     """A cache of more than 2^32 elements: the pages in use are its last ones."""
     m = Made([100, 70], [1, 50], 4, 2, 64, 16, F32, F16, seed=12)
