@@ -156,7 +156,7 @@ __device__ __forceinline__ Span span_of(const Sees& s, int t0, int t1, int keys,
 }
 
 // Where the parts of rows that are split over workgroups wait to be joined
-// (rows: few_kernel's 16 of each task, chunk_kernel's token times heads + head):
+// (rows: few_rows' 16 of each task, chunk_rows' token times heads + head):
 // fp32 sums [part][row][D] relative to the part's largest score, and that
 // score (times log2 e) with the sum of the weights, and of the weights as the
 // products took them.

@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) void few_kernel(Atte
 constexpr int kJoinThreads = 256;
 
 // The first few_rows rows are (sequence, one of its first `per` tokens, head),
-// of few_kernel; the others all of the call's, of chunk_kernel.
+// of few_rows; the others all of the call's, of chunk_rows.
 template <typename T, int D, int kWaves>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int64_t few_rows,
                                                             int per, int tiles, bool alone, float few_shift,
@@ -223,7 +223,7 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
   if (p.chunk &&
       (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, p.few ? &few : nullptr, p.few_tiles, s)) != hipSuccess)
     return e;
-  const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_kernel takes of a sequence
+  const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_rows takes of a sequence
   const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
   const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
   if (rows == 0) return hipSuccess;

@@ -20,8 +20,8 @@
 // either 16-bit type hold without loss, and the sums need no rescaling.  It is
 // a whole number, so that what it is taken from and given back to is exact.
 //
-// 2048 tokens over 16384 keys, 32 heads of 128, fp32 over fp16: 928 us, 1110
-// TFLOP/s of products, which is what a large fp16 matrix product reaches on
+// 2048 tokens over 16384 keys, 32 heads of 128, fp32 over fp16: 930 to
+// 960 us, 1073 to 1110 TFLOP/s of products, which is what a large fp16 matrix product reaches on
 // this card.  Two prompts of 4001, heads of 64, bf16: 160 us, 630 TFLOP/s: 16
 // exponentials and about 90 other vector instructions stand beside each 8
 // products.  (There, both halves of a tile in turn under each other's
@@ -124,7 +124,7 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
   if (seq < 0) return;
   const Chunk c = chunk_of(a.p, seq);
   const int rows = c.n * a.group;
-  if (!alone && (rows <= 16 || c.n == 1)) return;  // few_kernel's
+  if (!alone && (rows <= 16 || c.n == 1)) return;  // few_rows'
   const int64_t r0l = (tile - tile_base(c.begin, a.group, kChunkTile, seq)) * kChunkTile;
   if (r0l < 0 || r0l >= rows) return;
   const int r0 = (int)r0l, rn = rows - r0 < kChunkTile ? rows - r0 : kChunkTile;
