@@ -424,6 +424,17 @@ def test_attention_one_sequence_among_padding(pkg, dtype, cache):
     m.check(pkg)
 
 
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 80), (4, 2, 128), (6, 3, 200), (2, 1, 256), (20, 1, 128)])
+def test_attention_mixed_batches(pkg, dtype, cache, heads, kv_heads, d):
+    """Chunks and sequences of few rows in one call, all of them split over their
+    keys, with a window and without."""
+    say(f"[attend] mixed {NAME[dtype]}/{NAME[cache]} {heads}/{kv_heads} heads of {d}")
+    lens, new = [1100, 40, 1300, 3, 900], [1, 40, 70, 3, 2]
+    Made(lens, new, heads, kv_heads, d, 16, dtype, cache, seed=11).check(pkg, what="mixed")
+    Made(lens, new, heads, kv_heads, d, 16, dtype, cache, seed=13).check(pkg, window=777, hints=False, what="window")
+
+
 def test_attention_with_and_without_lse(pkg):
     m = Made([33, 5], [20, 1], 4, 2, 64, 16, F32, F16, seed=4)
     args = (m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda())
