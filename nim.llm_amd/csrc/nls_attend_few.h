@@ -283,12 +283,14 @@ __device__ __forceinline__ void few_rows(const AttendArgs& a, const Parts& parts
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) o[t] *= shrink;
       }
-      const float back = Elem<TC>::kShift - (m == minus_inf() ? 0.f : m);
+      // (the shift behind the difference, which is exact: it would be rounded within
+      // a maximum of 2^24 or more, and weights of 2^16 are beyond fp16)
+      const float from = m == minus_inf() ? 0.f : m;
       constexpr int kDepth = sizeof(vec) / sizeof(TC);
       vec p[NW];
 #pragma unroll
       for (int j = 0; j < kDepth; ++j) {
-        const float x = exp2_(w[j] + back);
+        const float y = w[j] - from, x = exp2_(Elem<TC>::kShift == 0.f ? y : y + Elem<TC>::kShift);
         l += x;
         split<NW>(x, p, j);
       }

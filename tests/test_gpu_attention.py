@@ -971,3 +971,48 @@ def test_refused_calls(pkg):
     assert bool((out == 7).all())
 
 
+
+
+def _goes_to_its_largest(pkg, m, scale):
+    """Scores so far apart that a row is the value of its largest one, rows of
+    near ties aside.  Returns how many rows were looked at."""
+    got, lse = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), max(m.new),
+                                   max(m.lens_l), scale=scale, lse=True)
+    got, lse = got.cpu(), lse.cpu()
+    assert bool(torch.isfinite(got).all()) and bool(torch.isfinite(lse).all())
+    heads, kv_heads, d = m.q.shape[1], m.kv.shape[2], m.q.shape[2]
+    seen = 0
+    for i in range(len(m.new)):
+        for t in range(m.starts_l[i], m.starts_l[i + 1]):
+            n = m.lens_l[i] - m.starts_l[i + 1] + t + 1
+            rows = torch.stack([m.kv[m.table_l[i][j // m.page], :, :, j % m.page] for j in range(n)]).double()
+            for h in range(heads):
+                k, v, x = rows[:, 0, h // (heads // kv_heads)], rows[:, 1, h // (heads // kv_heads)], m.q[t, h].double()
+                s = (k @ x) * scale
+                # an fp32 score may be off by this: d products and sums, the parts
+                # of a query, the scale and log2 e
+                ds = float(((k.abs() @ x.abs()) * abs(scale)).max()) * ((d + 4) * 2.0 ** -24 + 2.0 ** -22)
+                two = s.topk(min(2, n)).values
+                # lse: the score's error, the whole number and logarithm it is made
+                # of (2^-24 of it, four times), and the other keys' weights (at most n)
+                assert abs(float(lse[t, h]) - float(two[0])) <= ds + 4 * abs(float(two[0])) * 2.0 ** -24 + math.log(n) + 1e-6
+                if n > 1 and float(two[0] - two[1]) <= 2 * ds + 40:
+                    continue
+                # a weight of one key: 22 bits or more (fp32 queries) or 16 of it
+                # enter the product, the quotient is rounded, then the output
+                want = v[int(s.argmax())]
+                bound = want.abs() * (2.0 ** -20 if m.q.dtype == F32 else 2 * R.HALF[m.q.dtype]) + n * math.exp(-40) * v.abs().max()
+                near(got[t, h], want, bound + R.tiny(m.q.dtype), f"row {i} {t} {h}")
+                seen += 1
+    return seen
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lens,new", [([300, 90], [1, 3]), ([1300, 60], [1, 2]), ([300, 90], [20, 40])])
+def test_attention_scores_around_whole_fp32_numbers(pkg, dtype, cache, lens, new):
+    """Scores of 10^6 to 10^9: fp32 holds whole numbers there, or every second to
+    sixteenth one, and what is added to a maximum is rounded."""
+    for scale in (1e5, 3e5, 1e6, 2e6, -2e6, 4e6, 8e6, 1.6e7):
+        say(f"[attend] scale {scale} {NAME[dtype]}/{NAME[cache]} lens {lens} new {new}")
+        m = Made(lens, new, 4, 2, 64, 16, dtype, cache, seed=22)
+        assert _goes_to_its_largest(pkg, m, scale) > 10
