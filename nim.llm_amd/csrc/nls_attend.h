@@ -99,6 +99,15 @@ __device__ __forceinline__ void split(float x, f4* p, int j) {
   p[0][j] = x;
 }
 
+// fp32 queries over fp16: the exponent of the power of two that a row is divided
+// by, from its largest element.  That comes into [2^13, 2^14): its lower part
+// keeps 11 bits too.  (The power is a normal number: rows of denormals stay
+// below, at 2^-23 or more.)
+__device__ __forceinline__ int query_exponent(float top) {
+  const int e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
+  return e < -126 ? -126 : e;
+}
+
 // c plus the elements of x, two products with 1 at a time
 __device__ __forceinline__ float plus_all(h8 x, float c) {
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));

@@ -109,6 +109,7 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
   extern __shared__ __align__(16) char chunk_lds[];  // [2][K, V]
   __shared__ uint8_t noted[2][KT][L::kPieces];       // bit j: element j of a piece of V was not finite
   __shared__ int has_noted[2][kChunkWaves];
+  __shared__ float max_times[NP == 2 ? kChunkTile : 1];
 
   const int kvh = group_at % a.p.kv_heads, tile = (groups - 1 - group_at) / a.p.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
@@ -148,6 +149,7 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
 
   // the scale's sign goes to the queries: a largest score is a largest product
   const float flip = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   vec q[L::KC][NP];
   float qs = 1.f;
   {
@@ -159,7 +161,11 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
       for (int d = h * L::KD; d < dim; d += 2 * L::KD)
         for (int j = 0; j < L::KD; ++j) top = row_ok ? fmaxf(top, fabsf((float)src[d + j])) : 0.f;
       top = fmaxf(top, __shfl_xor(top, 32));
-      e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
+      // The scale times the power stays a normal number: masked scores would be
+      // -infinity times 0.  (Scores are below 2^-80 then, whatever the queries lose.)
+      const int least = -126 - ilogbf(scale2);
+      e = query_exponent(top);
+      e = e < least ? least : e;
       qs = ldexpf(1.f, e);
     }
 #pragma unroll
@@ -172,7 +178,17 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
         split<NP>(x, q[k], j);
       }
   }
-  const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e * qs;
+  float sc = scale2 * qs;
+  if constexpr (NP == 2) {
+    // Nor does it pass fp32's range, where scores are 0, infinite or 2^70 apart:
+    // the weights are the same, and the maximum gets back what was left out.
+    float rest = 1.f;
+    if (sc > 0x1p127f) {
+      sc = 0x1p127f;
+      rest = scale2 * 0x1p-127f * qs;
+    }
+    if (h == 0) max_times[w0 + i] = rest;  // (read by this wave alone)
+  }
 
   const int piece = threadIdx.x % L::kPieces, srow = threadIdx.x / L::kPieces;
   const bool piece_ok = piece * L::KD < dim;
@@ -434,6 +450,7 @@ __device__ __forceinline__ void chunk_rows(const AttendArgs& a, const Parts& par
     lr += __shfl_xor(lr, 32);
   else
     lr = l;
+  if constexpr (NP == 2) m *= max_times[w0 + i];
   const float from = m == minus_inf() ? 0.f : m;
   const int token = c.begin + row / a.group, head = kvh * a.group + row % a.group;
   if (span.parts > 1) {

@@ -125,8 +125,7 @@ __device__ __forceinline__ void few_rows(const AttendArgs& a, const Parts& parts
       if constexpr (sizeof(T) == 4 && __is_same(TC, _Float16)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        // the largest element into [2^13, 2^14): its lower part keeps 11 bits too
-        const int e = top > 0.f && top < __builtin_inff() ? ilogbf(top) - 13 : 0;
+        const int e = query_exponent(top);
         qs = ldexpf(1.f, e);
 #pragma unroll
         for (int k = 0; k < F::KC; ++k)
@@ -138,7 +137,7 @@ __device__ __forceinline__ void few_rows(const AttendArgs& a, const Parts& parts
 #pragma unroll
         for (int j = 0; j < F::KD; ++j) split<NP>(x[k][j], q[k], j);
     }
-    const float sc = a.scale * kLog2e * qs;
+    const float sc = a.scale * kLog2e;  // (behind qs: times it, it may leave fp32's range where the score does not)
 
     const TC* base = static_cast<const TC*>(a.p.kv) + (int64_t)kvh * a.p.head_stride;
     const int mask = (1 << a.p.page_shift) - 1;
@@ -247,7 +246,7 @@ __device__ __forceinline__ void few_rows(const AttendArgs& a, const Parts& parts
           for (int n = NP - 1; n >= 0; --n) acc = mma16(kk, q[x][n], acc);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * sc;
+        for (int r = 0; r < 4; ++r) w[s * 4 + r] = acc[r] * qs * sc;
       }
       if (more) {
         page1 = pages_of(kb + kStep, entry1);

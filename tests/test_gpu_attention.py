@@ -990,8 +990,11 @@ def _goes_to_its_largest(pkg, m, scale):
                 k, v, x = rows[:, 0, h // (heads // kv_heads)], rows[:, 1, h // (heads // kv_heads)], m.q[t, h].double()
                 s = (k @ x) * scale
                 # an fp32 score may be off by this: d products and sums, the parts
-                # of a query, the scale and log2 e
-                ds = float(((k.abs() @ x.abs()) * abs(scale)).max()) * ((d + 4) * 2.0 ** -24 + 2.0 ** -22)
+                # of a query, the scale and log2 e.  (Sums of fp16 products are
+                # aligned by the operands' exponents, and a denormal's is that of
+                # 2^-14: 24 bits of it hold what 2^-14 times the query is held by.)
+                size = k.abs().clamp(min=2.0 ** -14) if m.kv.dtype == F16 else k.abs()
+                ds = float(((size @ x.abs()) * abs(scale)).max()) * ((d + 4) * 2.0 ** -24 + 2.0 ** -22)
                 two = s.topk(min(2, n)).values
                 # lse: the score's error, the whole number and logarithm it is made
                 # of (2^-24 of it, four times), and the other keys' weights (at most n)
@@ -1016,3 +1019,34 @@ def test_attention_scores_around_whole_fp32_numbers(pkg, dtype, cache, lens, new
         say(f"[attend] scale {scale} {NAME[dtype]}/{NAME[cache]} lens {lens} new {new}")
         m = Made(lens, new, 4, 2, 64, 16, dtype, cache, seed=22)
         assert _goes_to_its_largest(pkg, m, scale) > 10
+
+
+@pytest.mark.parametrize("dtype,cache", PAIRS, ids=lambda t: NAME[t])
+@pytest.mark.parametrize("lens,new", [([300, 90, 33], [20, 40, 2]), ([1300, 60], [1, 2])])
+def test_attention_scores_next_to_zero(pkg, dtype, cache, lens, new):
+    """Scales and queries down to the least fp32 numbers: every visible key weighs
+    the same, in masked tiles too."""
+    for scale, spread in ((1e-45, 2.0), (-1e-45, 2.0), (1e-41, 2.0), (1e-38, 2.0), (0.125, 1e-42), (0.125, 1e-44), (1e-20, 1e-30),
+                          (1.0, 1e-36), (1e-45, 1e-44)):
+        if dtype != F32 and spread < 1.0:
+            continue
+        say(f"[attend] scale {scale} queries of {spread} {NAME[dtype]}/{NAME[cache]} lens {lens}")
+        m = Made(lens, new, 4, 2, 64, 16, dtype, cache, seed=22, spread=spread)
+        m.scale = scale
+        m.check(pkg, scale=scale)
+        m.check(pkg, scale=scale, window=21)
+
+
+@pytest.mark.parametrize("lens,new", [([300, 90, 33], [20, 40, 2]), ([1300, 60], [1, 2]), ([1300, 70], [50, 60])])
+def test_attention_large_queries_over_zeros(pkg, lens, new):
+    """Queries of 1e30 under a scale of 1e13: keys of zeros have scores of 0, and
+    one of fp16's least numbers has a finite score that takes all of the weight."""
+    say(f"[attend] large queries over zeros, lens {lens}")
+    m = Made(lens, new, 4, 2, 64, 16, F32, F16, seed=23)
+    m.q = m.q.abs() * 1e30 + 1e29
+    m.kv[:, 0] = 0.0
+    m.scale = 1e13
+    m.check(pkg, scale=1e13, what="zeros")
+    for s, n in enumerate(lens):
+        m.kv[m.table_l[s][0], 0, :, 0] = 2.0 ** -24
+    assert _goes_to_its_largest(pkg, m, 1e13) == 4 * sum(new)
