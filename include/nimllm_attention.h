@@ -153,6 +153,7 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
  * see holds, infinities and NaN among it, does not reach that row; an infinite
  * value that it does see makes it infinite or NaN.  (An infinite key that it
  * sees makes its score infinite, or NaN where fp32 queries meet 16-bit keys.)
+ * scale: finite, up to 2.3e38 either way (log2 e times it is finite too).
  * type (q and out): F32 with any cache type, F16 or BF16 with the same one.
  * Scores, statistics and sums are fp32: fp32 queries and weights meet 16-bit
  * keys and values as exact sums of 16-bit parts, 16-bit queries and weights

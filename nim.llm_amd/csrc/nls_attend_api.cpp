@@ -314,7 +314,8 @@ int32_t nls_paged_attention(const nls_paged_kv* kv, const nls_chunks* chunks, in
   NLS_CHECK(check_sizes(kv, chunks, heads, max_new, max_len, window));
   if (!elem_type(type) || (type != kF32 && type != kv->type))
     return bad("attention: q and out are F32, or of the cache's type");
-  if (!std::isfinite(scale)) return bad("attention: scale is not finite");
+  // (the kernels take exponents of base 2: an infinite factor times a score of 0 is NaN)
+  if (!std::isfinite(scale * 1.4426950408889634f)) return bad("attention: scale, or scale times log2 e, is not finite");
   if (chunks->tokens == 0 || chunks->seqs == 0) return NLS_OK;
   NLS_CHECK(check_heads(q, type, heads, chunks->tokens, kv->head_dim, false));
   NLS_CHECK(check_heads(out, type, heads, chunks->tokens, kv->head_dim, true));

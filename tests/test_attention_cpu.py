@@ -234,3 +234,18 @@ def test_page_call_refusals(pkg):
     assert copy(pages=0) == copy(a=None) == copy(b=AT + 1) == copy(n=-1) == INVALID
     assert copy(n=0) == OK
     assert L.nls_cache_workspace(None, 0) == 0 and L.nls_cache_workspace(t, -1) == 0
+
+
+def test_scales_beyond_the_exponents_base_are_refused(pkg):
+    """A scale that is finite, but infinite in exponents of base 2, would make a
+    score of 0 NaN."""
+    call = lambda scale: pkg.lib().nls_paged_attention(_cache(pkg), _chunks(pkg), 0, _heads(pkg), _heads(pkg), 4, scale, 0, None,
+                                                       None, 1, 80, None, 0, None)
+    for scale in (2.4e38, -2.4e38, 3.4e38):
+        assert call(scale) == INVALID, scale
+        assert b"log2" in pkg.lib().nls_last_error()
+    # (below the limit the call goes on to its other checks: its rows are none)
+    none = _chunks(pkg, tokens=0, d_starts=None)
+    for scale in (2.3e38, -2.3e38, 1e-45, 0.0):
+        assert pkg.lib().nls_paged_attention(_cache(pkg), none, 0, _heads(pkg), _heads(pkg), 4, scale, 0, None, None, 1, 80, None,
+                                             0, None) == OK
