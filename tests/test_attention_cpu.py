@@ -249,3 +249,30 @@ def test_scales_beyond_the_exponents_base_are_refused(pkg):
     for scale in (2.3e38, -2.3e38, 1e-45, 0.0):
         assert pkg.lib().nls_paged_attention(_cache(pkg), none, 0, _heads(pkg), _heads(pkg), 4, scale, 0, None, None, 1, 80, None,
                                              0, None) == OK
+
+
+@pytest.mark.parametrize("chunks,heads,max_new,max_len", [
+    (dict(seqs=2, tokens=2), 4, 1, 0),                  # single tokens, the keys split over workgroups
+    (dict(seqs=2, tokens=2), 4, 1, 1 << 15),
+    (dict(seqs=2, tokens=2), 4, 0, 0),
+    (dict(seqs=1, tokens=90), 4, 0, 0),                 # one chunk
+    (dict(seqs=2, tokens=90), 4, 80, 40000),            # a chunk and few rows
+    (dict(seqs=2, tokens=90), 32, 0, 0)])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_attention_workspace_refusals(pkg, chunks, heads, max_new, max_len, head_dim):
+    """Calls whose parts wait in the workspace: none, a misaligned one and one a
+    byte too short are refused before any device work."""
+    L = pkg.lib()
+    c = _cache(pkg, max_pages=4096, table_stride=4096, head_dim=head_dim, head_stride=16 * head_dim, token_stride=head_dim,
+               value_offset=2 * 16 * head_dim, page_stride=4 * 16 * head_dim)
+    ch = _chunks(pkg, **chunks)
+    rows = _heads(pkg, token_stride=heads * head_dim, head_stride=head_dim)
+    need = L.nls_paged_attention_workspace(c, ch, heads, max_new, max_len, 0)
+    assert need > 0 and need % 256 == 0
+    call = lambda work, size: L.nls_paged_attention(c, ch, 0, rows, rows, heads, 0.125, 0, None, None, max_new, max_len, work,
+                                                    size, None)
+    for work, size in ((None, need), (AT, need - 1), (AT, 0), (AT + 16, need), (AT + 128, 1 << 40)):
+        assert call(work, size) == INVALID, (work, size)
+        assert b"workspace" in L.nls_last_error()
+    # a window shortens what is split, and with it the workspace
+    assert L.nls_paged_attention_workspace(c, ch, heads, max_new, max_len, 64) < need
