@@ -730,20 +730,29 @@ def _elem_type(t) -> int:
     return code
 
 
+# The checks below are raised, not asserted: the C ABI sees addresses alone, and
+# what is wrong in lengths, types or devices would be read on the GPU, under
+# python -O too.
+
+
 def _ints(device: int, t):
     """The address of a contiguous int32 tensor on the device (None: none)."""
     if t is None:
         return None
-    assert t.get_device() == device, "tensors of one call on different devices"
-    assert t.element_size() == 4 and not t.is_floating_point() and t.is_contiguous(), "int32 tensors, contiguous"
+    if t.get_device() != device:
+        raise AssertionError("tensors of one call on different devices")
+    if not (t.element_size() == 4 and not t.is_floating_point() and t.is_contiguous()):
+        raise AssertionError("int32 tensors, contiguous")
     return t.data_ptr()
 
 
 def _heads(device: int, t, dtype):
     """A [tokens, heads, head_dim] tensor as nls_heads."""
-    assert t.get_device() == device and t.dtype == dtype, "tensors of one call: one device, one element type"
+    if not (t.get_device() == device and t.dtype == dtype):
+        raise AssertionError("tensors of one call: one device, one element type")
     s = t.stride()
-    assert len(s) == 3 and (s[2] == 1 or t.shape[2] <= 1), "rows of heads: [tokens, heads, head_dim], elements side by side"
+    if not (len(s) == 3 and (s[2] == 1 or t.shape[2] <= 1)):
+        raise AssertionError("rows of heads: [tokens, heads, head_dim], elements side by side")
     return NlsHeads(t.data_ptr(), s[0], s[1])
 
 
@@ -776,8 +785,9 @@ class RopePlan:
 
     def _c(self, device: int):
         f = self.freqs
-        assert f.get_device() == device and f.element_size() == 8 and f.is_floating_point() and f.dim() == 1 \
-            and f.is_contiguous(), "rope plan: float64 [dim / 2] on the call's device"
+        if not (f.get_device() == device and f.element_size() == 8 and f.is_floating_point() and f.dim() == 1 and
+                f.is_contiguous()):
+            raise AssertionError("rope plan: float64 [dim / 2] on the call's device")
         return NlsRopePlan(f.data_ptr(), 2 * f.numel(), self.interleaved, self.amplitude)
 
 
@@ -795,7 +805,8 @@ def rope_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", fac
     ff = None
     if freq_factors is not None:
         ff = [float(f) for f in freq_factors]
-        assert len(ff) == dim // 2, f"freq_factors: {len(ff)} entries, dim / 2 = {dim // 2}"
+        if len(ff) != dim // 2:
+            raise AssertionError(f"freq_factors: {len(ff)} entries, dim / 2 = {dim // 2}")
         ff = (ctypes.c_double * n)(*ff)
     out, amp = (ctypes.c_double * n)(), ctypes.c_double()
     s = NlsRopeScaling(ROPE_SCALINGS[scaling], base, factor, original_context, beta_fast, beta_slow, attn_factor, ff)
@@ -822,7 +833,8 @@ def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
 
         out = torch.empty(x.shape, dtype=dt, device=x.device)
     tokens, heads, dim = x.shape
-    assert dev >= 0 and out.shape == x.shape and positions.numel() == tokens
+    if not (dev >= 0 and out.shape == x.shape and positions.numel() == tokens):
+        raise AssertionError("rope: x on the GPU, out of its shape, a position per token")
     _launch(dev, "nls_rope", plan._c(dev), _elem_type(x), _heads(dev, x, dt), _heads(dev, out, dt), tokens, heads, dim,
             _ints(dev, positions), inverse)
     return out
@@ -831,19 +843,20 @@ def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
 def _paged_kv(dev: int, kv, table, lens):
     pages, two, kv_heads, page_size, dim = kv.shape
     st = kv.stride()
-    assert dev >= 0 and two == 2 and st[4] == 1, (
-        "a layer of the cache on the GPU: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
+    if not (dev >= 0 and two == 2 and st[4] == 1):
+        raise AssertionError("a layer of the cache on the GPU: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
     slots, per = table.shape
     ts = table.stride()
-    assert table.get_device() == dev and table.dtype == lens.dtype and ts[1] == 1 and lens.numel() == slots, (
-        "the page table: int32 [slots, pages], rows side by side")
+    if not (table.get_device() == dev and table.dtype == lens.dtype and ts[1] == 1 and lens.numel() == slots):
+        raise AssertionError("the page table: int32 [slots, pages], rows side by side")
     return NlsPagedKv(kv.data_ptr(), _elem_type(kv), pages, page_size, kv_heads, dim, st[0], st[1], st[2], st[3],
                       table.data_ptr(), ts[0], slots, per, _ints(dev, lens))
 
 
 def _chunks(dev: int, tokens: int, starts, slots):
     seqs = starts.numel() - 1
-    assert seqs >= 0 and (slots is None or slots.numel() == seqs)
+    if not (seqs >= 0 and (slots is None or slots.numel() == seqs)):
+        raise AssertionError("starts [sequences + 1], slots [sequences]")
     return NlsChunks(seqs, tokens, _ints(dev, starts), _ints(dev, slots))
 
 
@@ -855,7 +868,8 @@ def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan]
     slot slots[i] (i when None), whose lens count them already.  Returns out."""
     dev, dt = kv.get_device(), k.dtype
     tokens, kv_heads, dim = k.shape
-    assert k.shape == v.shape and kv_heads == kv.shape[2] and dim == kv.shape[4]
+    if not (k.shape == v.shape and kv_heads == kv.shape[2] and dim == kv.shape[4]):
+        raise AssertionError("k and v: [tokens, kv_heads, head_dim] of the cache's heads")
     heads, cq, co = 0, None, None
     if q is not None:
         if out is None:
@@ -863,10 +877,12 @@ def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan]
 
             out = torch.empty(q.shape, dtype=dt, device=q.device)
         heads = q.shape[1]
-        assert out.shape == q.shape and q.shape[0] == tokens and q.shape[2] == dim
+        if not (out.shape == q.shape and q.shape[0] == tokens and q.shape[2] == dim):
+            raise AssertionError("q and out: [tokens, heads, head_dim] of k's tokens and head_dim")
         cq, co = _heads(dev, q, dt), _heads(dev, out, dt)
     else:
-        assert out is None, "out without q"
+        if out is not None:
+            raise AssertionError("out without q")
     _launch(dev, "nls_cache_append", _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots),
             None if plan is None else plan._c(dev), _elem_type(k), cq, co, heads, _heads(dev, k, dt), _heads(dev, v, dt))
     return out
@@ -894,16 +910,19 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
     elif lse is True:
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
     elif lse is not None:
-        assert lse.get_device() == dev and lse.dtype == torch.float32 and lse.is_contiguous() \
-            and lse.shape == (tokens, heads), "lse: float32 [tokens, heads], contiguous"
-    assert out.shape == q.shape and dim == kv.shape[4] and (first is None or first.numel() == lens.numel())
+        if not (lse.get_device() == dev and lse.dtype == torch.float32 and lse.is_contiguous() and
+                lse.shape == (tokens, heads)):
+            raise AssertionError("lse: float32 [tokens, heads], contiguous")
+    if not (out.shape == q.shape and dim == kv.shape[4] and (first is None or first.numel() == lens.numel())):
+        raise AssertionError("out: q's shape; q: the cache's head_dim; first: a key per slot")
     c, ch = _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots)
     cq, co, cf = _heads(dev, q, dt), _heads(dev, out, dt), _ints(dev, first)
     need = lib().nls_paged_attention_workspace(c, ch, heads, max_new, max_len, window)
     if need and (work is None or work.numel() < need):
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif work is not None:
-        assert work.get_device() == dev and work.dtype == torch.uint8 and work.is_contiguous()
+        if not (work.get_device() == dev and work.dtype == torch.uint8 and work.is_contiguous()):
+            raise AssertionError("work: uint8, contiguous, on the call's device")
     _launch(dev, "nls_paged_attention", c, ch, _elem_type(q), cq, co, heads, dim ** -0.5 if scale is None else scale,
             window, cf, None if lse is None else lse.data_ptr(), max_new, max_len, _ptr(work), need)
     return out if lse is None else (out, lse)
@@ -927,16 +946,17 @@ def _page_pool(dev: int, kv):
     for stride, size in sorted(zip(st[2:], kv.shape[2:])):
         if size != 1:
             dense = dense * size if stride == dense else 0
-    assert kv.get_device() == dev and two == 2 and dense == 2 * heads * page_size * dim, (
-        "the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
+    if not (kv.get_device() == dev and two == 2 and dense == 2 * heads * page_size * dim):
+        raise AssertionError("the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
     return NlsPagePool(kv.data_ptr(), layers, dense * n, st[0] * n, st[1] * n)
 
 
 def _page_tables(dev: int, table, lens, refs, page_size: int):
     slots, per = table.shape
     ts = table.stride()
-    assert dev >= 0 and table.get_device() == dev and table.dtype == refs.dtype and ts[1] == 1 and (
-        lens is None or lens.numel() == slots), "the page table: int32 [slots, pages], rows side by side"
+    if not (dev >= 0 and table.get_device() == dev and table.dtype == refs.dtype and ts[1] == 1 and
+            (lens is None or lens.numel() == slots)):
+        raise AssertionError("the page table: int32 [slots, pages], rows side by side")
     return NlsPageTables(table.data_ptr(), ts[0], slots, per, _ints(dev, lens), _ints(dev, refs), refs.numel(), page_size)
 
 
@@ -957,7 +977,8 @@ def cache_reserve(table, lens, refs, page_size: int, counts):
     slots' order, and lens += counts.  Returns the status word (PAGES_DONE, or
     why nothing was done) as an int32 device tensor [1]."""
     dev = refs.get_device()
-    assert counts.numel() == table.shape[0]
+    if counts.numel() != table.shape[0]:
+        raise AssertionError("counts: one per slot")
     t = _page_tables(dev, table, lens, refs, page_size)
     return _pages_call(dev, "nls_cache_reserve", refs, t, 0, t, _ints(dev, counts))
 
@@ -967,7 +988,8 @@ def cache_fork(kv, table, lens, refs, src, dst):
     pages shared, the last partial page copied in every layer of kv.  Returns the
     status word."""
     dev, n = refs.get_device(), src.numel()
-    assert n == dst.numel() and kv.shape[1] == refs.numel()
+    if not (n == dst.numel() and kv.shape[1] == refs.numel()):
+        raise AssertionError("src and dst of one length; refs: one per page of kv")
     t = _page_tables(dev, table, lens, refs, kv.shape[4])
     return _pages_call(dev, "nls_cache_fork", refs, t, n, _page_pool(dev, kv), t, _ints(dev, src), _ints(dev, dst), n)
 
@@ -984,7 +1006,8 @@ def cache_compact(kv, table, refs):
     """Moves the held pages to the lowest ids, their contents in every layer and
     the table's entries with them.  Returns how many are held, int32 [1]."""
     dev = refs.get_device()
-    assert kv.shape[1] == refs.numel()
+    if kv.shape[1] != refs.numel():
+        raise AssertionError("refs: one per page of kv")
     t = _page_tables(dev, table, None, refs, kv.shape[4])
     return _pages_call(dev, "nls_cache_compact", refs, t, 0, _page_pool(dev, kv), t)
 
@@ -992,7 +1015,8 @@ def cache_compact(kv, table, refs):
 def cache_copy_pages(kv, src, dst):
     """Page src[i] to page dst[i] (int32) in every layer of kv."""
     dev = kv.get_device()
-    assert dev >= 0 and src.numel() == dst.numel()
+    if not (dev >= 0 and src.numel() == dst.numel()):
+        raise AssertionError("copies: kv on the GPU, src and dst of one length")
     _launch(dev, "nls_cache_copy_pages", _page_pool(dev, kv), kv.shape[1], _ints(dev, src), _ints(dev, dst), src.numel())
 
 

@@ -5,6 +5,7 @@ import ctypes
 import math
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -276,3 +277,91 @@ def test_attention_workspace_refusals(pkg, chunks, heads, max_new, max_len, head
         assert b"workspace" in L.nls_last_error()
     # a window shortens what is split, and with it the workspace
     assert L.nls_paged_attention_workspace(c, ch, heads, max_new, max_len, 64) < need
+
+
+_REFUSED = '''
+import importlib.util, sys
+import torch
+spec = importlib.util.spec_from_file_location("nimllm_amd", sys.argv[1], submodule_search_locations=[])
+m = importlib.util.module_from_spec(spec)
+sys.modules["nimllm_amd"] = m
+spec.loader.exec_module(m)
+if __debug__:
+    sys.exit("run with -O")
+
+
+class OnGpu(torch.Tensor):
+    """Host memory that says it is device 0's; nothing is launched."""
+    def get_device(self):
+        return 0
+
+
+launched = []
+m._launch = lambda device, what, *args: launched.append(what)
+gpu = lambda t: t.as_subclass(OnGpu)
+ints = lambda n, dtype=torch.int32: gpu(torch.zeros(n, dtype=dtype))
+real = lambda *shape, dtype=torch.float32: gpu(torch.zeros(shape, dtype=dtype))
+kv, table, lens, starts = real(6, 2, 2, 16, 64), ints((3, 4)), ints(3), ints(3)
+q, k = real(5, 4, 64), real(5, 2, 64)
+pool, refs = real(1, 6, 2, 2, 16, 64), ints(6)
+plan = m.RopePlan(gpu(torch.ones(32, dtype=torch.float64)))
+attend = dict(q=q, kv=kv, table=table, lens=lens, starts=starts, out=q.clone())
+append = dict(kv=kv, table=table, lens=lens, starts=starts, k=k, v=k, q=q, plan=plan, out=q)
+calls = {
+    m.rope: (dict(x=q, positions=ints(5), plan=plan, out=q), [
+        dict(positions=ints(4)), dict(positions=ints(5, torch.int64)), dict(positions=gpu(torch.zeros(10, dtype=torch.int32)[::2])),
+        dict(positions=torch.zeros(5, dtype=torch.int32)), dict(out=real(5, 4, 32)), dict(out=real(5, 4, 64, dtype=torch.float16)),
+        dict(x=torch.zeros(5, 4, 64), out=torch.zeros(5, 4, 64)), dict(plan=m.RopePlan(real(32))),
+        dict(plan=m.RopePlan(torch.ones(32, dtype=torch.float64))), dict(x=gpu(torch.zeros(5, 64, 4).transpose(1, 2)))]),
+    m.paged_attention: (attend, [
+        dict(first=ints(2)), dict(slots=ints(3)), dict(lens=ints(2)), dict(lens=ints(3, torch.int64)), dict(table=ints((3, 4), torch.int64)),
+        dict(table=gpu(torch.zeros((4, 3), dtype=torch.int32).t())), dict(starts=ints(0)), dict(starts=torch.zeros(3, dtype=torch.int32)),
+        dict(q=real(5, 4, 32), out=real(5, 4, 32)), dict(out=real(4, 4, 64)), dict(lse=real(5, 3)), dict(lse=real(5, 4, dtype=torch.float16)),
+        dict(lse=torch.zeros(5, 4)), dict(kv=real(6, 1, 2, 16, 64)), dict(kv=torch.zeros(6, 2, 2, 16, 64)), dict(max_len=64, work=torch.zeros(1 << 20)),
+        dict(kv=gpu(torch.zeros(6, 2, 2, 64, 16).transpose(3, 4)))]),
+    m.cache_append: (append, [
+        dict(v=real(4, 2, 64)), dict(k=real(5, 1, 64), v=real(5, 1, 64)), dict(k=real(5, 2, 32), v=real(5, 2, 32)), dict(q=real(4, 4, 64), out=real(4, 4, 64)),
+        dict(out=real(5, 3, 64)), dict(q=None), dict(v=real(5, 2, 64, dtype=torch.float16)), dict(slots=ints(1)), dict(lens=ints(4))]),
+    m.cache_reserve: (dict(table=table, lens=lens, refs=refs, page_size=16, counts=ints(3)), [
+        dict(counts=ints(2)), dict(counts=ints(3, torch.int64)), dict(lens=ints(2)), dict(refs=ints(6, torch.int64))]),
+    m.cache_fork: (dict(kv=pool, table=table, lens=lens, refs=refs, src=ints(1), dst=ints(1)), [
+        dict(dst=ints(2)), dict(refs=ints(5)), dict(kv=pool[..., :32]), dict(lens=ints(2))]),
+    m.cache_release: (dict(table=table, lens=lens, refs=refs, slots=ints(2), page_size=16), [
+        dict(slots=ints(2, torch.int64)), dict(lens=ints(4)), dict(slots=torch.zeros(2, dtype=torch.int32))]),
+    m.cache_compact: (dict(kv=pool, table=table, refs=refs), [dict(refs=ints(7)), dict(kv=pool[:, :, :, :1])]),
+    m.cache_copy_pages: (dict(kv=pool, src=ints(2), dst=ints(2)), [
+        dict(src=ints(3)), dict(kv=torch.zeros(1, 6, 2, 2, 16, 64)), dict(kv=pool[..., ::2])]),
+}
+bad = []
+for call, (good, wrong) in calls.items():
+    call(**good)
+    if not launched:
+        bad.append((call.__name__, "the right call was not made"))
+    for i, kw in enumerate(wrong):
+        del launched[:]
+        try:
+            call(**{**good, **kw})
+            bad.append((call.__name__, i, sorted(kw), "was taken"))
+        except (AssertionError, m.SamplerError):
+            pass
+        if launched:
+            bad.append((call.__name__, i, sorted(kw), "was launched"))
+    del launched[:]
+try:
+    m.rope_frequencies(64, freq_factors=[1.0] * 31)
+    bad.append("freq_factors")
+except AssertionError:
+    pass
+print(bad or "all refused")
+'''
+
+
+@pytest.mark.parametrize("flag", ["-O", "-OO"])
+def test_python_refusals_without_asserts(tmp_path, flag):
+    """What the C ABI cannot see is refused by the Python entry points under
+    python -O as well."""
+    script = tmp_path / "refused.py"
+    script.write_text(_REFUSED)
+    done = subprocess.run([sys.executable, flag, str(script), os.path.join(ROOT, "nim.llm_amd", "__init__.py")],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "all refused", done.stdout + done.stderr[-2000:]
