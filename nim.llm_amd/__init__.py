@@ -853,6 +853,12 @@ def _paged_kv(dev: int, kv, table, lens):
                       table.data_ptr(), ts[0], slots, per, _ints(dev, lens))
 
 
+def _in_range(window: int, max_new: int, max_len: int):
+    """Numbers that the C ABI takes whole: ctypes cuts others to 32 bits."""
+    if not (0 <= window < 1 << 31 and 0 <= max_new < 1 << 31 and 0 <= max_len < 1 << 63):
+        raise AssertionError("window and max_new: 0 .. 2^31 - 1, max_len: 0 .. 2^63 - 1")
+
+
 def _chunks(dev: int, tokens: int, starts, slots):
     seqs = starts.numel() - 1
     if not (seqs >= 0 and (slots is None or slots.numel() == seqs)):
@@ -903,6 +909,7 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
 
     dev, dt = kv.get_device(), q.dtype
     tokens, heads, dim = q.shape
+    _in_range(window, max_new, max_len)
     if out is None:
         out = torch.empty(q.shape, dtype=dt, device=q.device)
     if lse is False:
@@ -931,6 +938,7 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
 def paged_attention_workspace(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, window: int = 0) -> int:
     """Bytes of the workspace paged_attention takes for these arguments, for a
     caller that keeps one (each call in flight needs its own)."""
+    _in_range(window, max_new, max_len)
     return int(lib().nls_paged_attention_workspace(_paged_kv(kv.get_device(), kv, table, lens),
                                                    _chunks(kv.get_device(), q.shape[0], starts, None), q.shape[1], max_new,
                                                    max_len, window))
@@ -954,6 +962,8 @@ def _page_pool(dev: int, kv):
 def _page_tables(dev: int, table, lens, refs, page_size: int):
     slots, per = table.shape
     ts = table.stride()
+    if not 0 < page_size <= 4096:
+        raise AssertionError("page_size: a power of two up to 4096")
     if not (dev >= 0 and table.get_device() == dev and table.dtype == refs.dtype and ts[1] == 1 and
             (lens is None or lens.numel() == slots)):
         raise AssertionError("the page table: int32 [slots, pages], rows side by side")

@@ -365,3 +365,33 @@ def test_python_refusals_without_asserts(tmp_path, flag):
     done = subprocess.run([sys.executable, flag, str(script), os.path.join(ROOT, "nim.llm_amd", "__init__.py")],
                           capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and done.stdout.strip() == "all refused", done.stdout + done.stderr[-2000:]
+
+
+def test_numbers_beyond_32_bits_are_refused(pkg, monkeypatch):
+    """ctypes would cut them: a window of 2^32 + 5 would be one of 5."""
+    import torch
+
+    class OnGpu(torch.Tensor):
+        def get_device(self):
+            return 0
+
+    launched = []
+    monkeypatch.setattr(pkg, "_launch", lambda device, what, *args: launched.append(what))
+    ints = lambda *n: torch.zeros(n, dtype=torch.int32).as_subclass(OnGpu)
+    real = lambda *n: torch.zeros(n).as_subclass(OnGpu)
+    q, args = real(2, 4, 64), (real(6, 2, 2, 16, 64), ints(3, 4), ints(3), ints(3))
+    for kw in (dict(window=(1 << 32) + 5), dict(window=1 << 32), dict(window=1 << 31), dict(window=-(1 << 32)), dict(window=-1),
+               dict(max_new=(1 << 32) + 1), dict(max_new=-1), dict(max_len=1 << 64), dict(max_len=-1)):
+        with pytest.raises(AssertionError):
+            pkg.paged_attention(q, *args, out=real(2, 4, 64), **kw)
+        with pytest.raises(AssertionError):
+            pkg.paged_attention_workspace(q, *args, **kw)
+    for page in ((1 << 32) + 16, 0, -16, 8192):
+        with pytest.raises(AssertionError):
+            pkg.cache_reserve(ints(3, 4), ints(3), ints(6), page, ints(3))
+        with pytest.raises(AssertionError):
+            pkg.cache_release(ints(3, 4), ints(3), ints(6), ints(1), page)
+    assert not launched
+    pkg.paged_attention(q, *args, out=real(2, 4, 64), window=(1 << 31) - 1, max_new=(1 << 31) - 1, max_len=(1 << 63) - 1)
+    pkg.cache_reserve(ints(3, 4), ints(3), ints(6), 16, ints(3))
+    assert launched == ["nls_paged_attention", "nls_cache_reserve"]
