@@ -1050,3 +1050,92 @@ def test_attention_large_queries_over_zeros(pkg, lens, new):
     for s, n in enumerate(lens):
         m.kv[m.table_l[s][0], 0, :, 0] = 2.0 ** -24
     assert _goes_to_its_largest(pkg, m, 1e13) == 4 * sum(new)
+
+
+@pytest.mark.parametrize("dtype,cache,heads,kv_heads,d", [(F32, F32, 4, 2, 128), (F32, F16, 8, 2, 128), (F32, BF16, 4, 1, 256),
+                                                          (BF16, BF16, 8, 2, 64), (F16, F16, 4, 2, 256)])
+def test_mixed_batches_captured_and_replayed(pkg, dtype, cache, heads, kv_heads, d):
+    """Chunks and single tokens of wide heads, all split and joined, in two graphs
+    of one set of tensors, replayed in turn with new inputs, other lengths and
+    eager calls between: each replay as the eager call."""
+    say(f"[graph] {NAME[dtype]}/{NAME[cache]} {heads}/{kv_heads} heads of {d}")
+    m = Made([1500, 700, 40, 900], [1, 90, 40, 3], heads, kv_heads, d, 16, dtype, cache, seed=17)
+    q, kv, table, lens, starts = m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda()
+    call = lambda window: pkg.paged_attention(q, kv, table, lens, starts, 90, 1500, window=window, lse=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0), call(600)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for window in (0, 600):
+        graphs.append((torch.cuda.CUDAGraph(), window))
+        with torch.cuda.graph(graphs[-1][0]):
+            graphs[-1] += (call(window),)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for i in range(12):
+        say(f"[graph] replay {i}")
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda") * 2)
+        lens[0] = 1500 - 100 * i
+        lens[1] = 90 + 50 * i
+        graph, window, got = graphs[i % 2]
+        graph.replay()
+        if i % 3 == 0:
+            graphs[(i + 1) % 2][0].replay()
+        want = call(window)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_page_calls_captured_and_replayed(pkg):
+    """A pool whose bitmap takes more LDS than a kernel has unasked: reserve, fork,
+    release and compact in one graph, as the eager calls on a second cache."""
+    make = lambda: pkg.PagedCache(1, 400000, 2, 1, 8, 12, 500, dtype=F16)
+    a, b = make(), make()
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    grow, src, dst, gone = ints([3, 5, 0, 7] + [0] * 8), ints([0, 1]), ints([4, 5]), ints([4, 5, 0])
+
+    def step(c):
+        return c.reserve(grow), c.fork(src, dst), c.release(gone), c.compact()
+
+    step(b)  # kernels loaded before the capture
+    torch.cuda.synchronize()
+    for x, y in ((b.table, a.table), (b.lens, a.lens), (b.refs, a.refs), (b.kv, a.kv)):
+        x.copy_(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(a)
+    for i in range(8):
+        say(f"[graph] pages, replay {i}")
+        noise = torch.randn(a.kv.shape, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").half()
+        a.kv.copy_(noise), b.kv.copy_(noise)
+        grow[6 + i % 4] = 1 + i
+        graph.replay()
+        want = step(b)
+        torch.cuda.synchronize()
+        assert [int(x) for x in got] == [int(x) for x in want] and [int(x) for x in got[:3]] == [0, 0, 0]
+        assert torch.equal(a.table, b.table) and torch.equal(a.lens, b.lens) and torch.equal(a.refs, b.refs)
+        assert torch.equal(a.kv, b.kv)
+
+
+def test_forks_share_pages_and_attend_as_their_parent(pkg):
+    """Contexts that share a prompt's pages: the same query has the same bits in
+    each, for single tokens and chunks, whatever the others' tokens are."""
+    cache = pkg.PagedCache(1, 400, 16, 2, 128, 24, 80, dtype=BF16)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32).cuda()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache.kv.normal_(generator=g)
+    assert int(cache.reserve(ints([1003] + [0] * 23))) == 0
+    assert int(cache.fork(ints([0] * 23), ints(list(range(1, 24))))) == 0
+    assert int((cache.refs > 1).sum()) == 1003 // 16 and int(cache.refs.max()) == 24
+    for n in (1, 33):
+        say(f"[forks] {n} tokens each")
+        assert int(cache.reserve(ints([n] * 24))) == 0
+        q, k, v = (torch.randn(n, h, 128, generator=g, device="cuda").bfloat16().repeat(24, 1, 1) for h in (8, 2, 2))
+        starts = ints([n * i for i in range(25)])
+        q = cache.append(0, k, v, starts, q=q, plan=pkg.rope_plan(128))
+        out = cache.attend(0, q, starts, max_new=n, max_len=1100).view(24, n, 8, 128)
+        assert all(torch.equal(out[i], out[0]) for i in range(24))
+        alone = pkg.paged_attention(q[:n], cache.kv[0], cache.table[:1], cache.lens[:1], starts[:2], max_new=n, max_len=1100)
+        # (split otherwise: the same sums in another order, bf16 weights rounded from other maxima)
+        assert float((alone.float() - out[0].float()).abs().max()) <= 4 * R.HALF[BF16] * float(cache.kv.abs().max())
