@@ -1139,3 +1139,31 @@ def test_forks_share_pages_and_attend_as_their_parent(pkg):
         alone = pkg.paged_attention(q[:n], cache.kv[0], cache.table[:1], cache.lens[:1], starts[:2], max_new=n, max_len=1100)
         # (split otherwise: the same sums in another order, bf16 weights rounded from other maxima)
         assert float((alone.float() - out[0].float()).abs().max()) <= 4 * R.HALF[BF16] * float(cache.kv.abs().max())
+
+
+def test_rope_next_to_quarter_turns(pkg):
+    """Angles next to whole quarters of a turn, where the sine or the cosine is
+    next to 0: it is right to its own last places, as a table in 64 bits is."""
+    quarter = math.pi / 2
+    pos = torch.tensor([1, 2, 3, 5, 1001, 40002, 99999], dtype=torch.int32)
+    freqs = [quarter * (1 + e) for e in (0.0, 3e-9, -1e-8, 5e-8, 1e-7, -4e-7, 1e-6, 2e-3)]
+    plan = pkg.RopePlan(torch.tensor(freqs, dtype=torch.float64).cuda(), True, 1.0)
+    x = torch.zeros(len(pos), 1, 16)
+    x[..., 0::2] = 1.0  # turned: (cos, sin) of the angle
+    got = pkg.rope(x.cuda(), pos.cuda(), plan).cpu().double().view(-1, 8, 2)
+    angle = np.asarray(pos, dtype=np.float64)[:, None] * np.asarray(freqs)[None, :]
+    want = torch.from_numpy(np.stack([np.cos(angle), np.sin(angle)], -1))
+    # the float64 angle's product and reduction (2^-52 of it, twice), sine and
+    # cosine to 4 units of 2^-24, the turn by what is behind 24 bits (its square's
+    # half, 2^-47, a rounding more), the product with 1
+    bound = torch.from_numpy(angle)[..., None] * 2.0 ** -51 + want.abs() * 8 * 2.0 ** -24 + 2.0 ** -46
+    near(got, want, bound, "quarters")
+    # and on the way into the cache, at positions behind others
+    kv = torch.zeros((1, 2, 1, 8, 16), device="cuda")
+    one = lambda *v: torch.tensor(v, dtype=torch.int32).cuda()
+    q = pkg.cache_append(kv, one(0).reshape(1, 1), one(6), one(0, 5), x[:5].cuda(), x[:5].cuda(), q=x[:5].cuda(), plan=plan)
+    angle = np.arange(1, 6)[:, None] * np.asarray(freqs)[None, :]
+    want = torch.from_numpy(np.stack([np.cos(angle), np.sin(angle)], -1))
+    bound = 2.0 ** -48 + want.abs() * 8 * 2.0 ** -24 + 2.0 ** -46
+    near(q.cpu().double().view(-1, 8, 2), want, bound, "q")
+    near(kv[0, 0, 0, 1:6].cpu().double().view(-1, 8, 2), want, bound, "k")
