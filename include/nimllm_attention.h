@@ -84,8 +84,8 @@ typedef struct nls_rope_plan {
 /*
  * y[t, h, :] = x[t, h, :] turned by positions[t] * freqs (`inverse`: by minus
  * that, with the same amplitude, which takes a gradient of y to one of x).
- * Angles and their reduction are float64, the products fp32, rounded once to
- * `type`.  y may be x.  d_positions: int32 [tokens], any value.
+ * Angles and their reduction are float64, sines, cosines and products fp32,
+ * rounded once to `type`.  y may be x.  d_positions: int32 [tokens], any value.
  */
 int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, const nls_heads* y, int32_t tokens,
                  int32_t heads, int32_t head_dim, const int32_t* d_positions, int32_t inverse, void* stream);
@@ -155,9 +155,14 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
  * sees makes its score infinite, or NaN where fp32 queries meet 16-bit keys.)
  * scale: finite, up to 2.3e38 either way (log2 e times it is finite too).
  * type (q and out): F32 with any cache type, F16 or BF16 with the same one.
- * Scores, statistics and sums are fp32: fp32 queries and weights meet 16-bit
- * keys and values as exact sums of 16-bit parts, 16-bit queries and weights
- * rounded to the cache's type.
+ * Scores, statistics and sums are fp32.  fp32 queries and weights meet 16-bit
+ * keys and values as sums of 16-bit parts: three of bf16, which are exact, or two
+ * of fp16, 22 bits (or 2^-38 of the row's largest element).  16-bit queries'
+ * weights are rounded to the cache's type in sequences of more than 16 rows
+ * (tokens times heads per kv head), and to 16 bits or more in others, so a token
+ * may come out a rounding apart in another batch.  Weighted values are summed
+ * before they are divided: in an fp32 or bf16 cache, values beyond 2^88 may
+ * overflow in long sums.
  * max_new and max_len say what the caller expects of the longest chunk and
  * context (0: not known).  They choose how the work is split; results hold
  * whatever the true values are.
@@ -205,7 +210,9 @@ enum {
   NLS_PAGES_BAD_ENTRY = 3  /* a slot out of range or named where it may not be, or a negative count */
 };
 
-/* Device workspace of the calls below, 256-byte aligned. */
+/* Device workspace of the calls below, 256-byte aligned: one size for all of
+ * them, so that one buffer serves each in turn (compact's three words per page
+ * are the most of it; release checks it as the others do and uses none). */
 size_t nls_cache_workspace(const nls_page_tables* tables, int32_t count);
 
 /* Slot s grows by counts[s] (int32 [slots]) tokens: pages for them, the lowest

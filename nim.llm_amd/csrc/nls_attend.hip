@@ -168,11 +168,12 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   if (p.few) {
     p.few_tiles = (a.group + 15) / 16;
     const int64_t tasks = (int64_t)a.p.seqs * p.few_tiles * a.p.kv_heads;
-    // Parts of at least 256 keys, and as many as give every CU two workgroups (one
-    // token over 131071 keys: 101 us so, 119 with three, 138 with parts of 512);
-    // up to 768 keys are not split: the second launch costs the host the 5 us that
-    // it saves the GPU (517 keys: 14.6 us whole, 12.5 in three parts; 24 contexts
-    // of 517: 12.9 whole, 19.2 split).
+    // Parts of at least 256 keys (one token over 8000 fp32 keys, heads of 64: 17.7
+    // us, with parts of 512 20.8), and as many as give every CU two workgroups (one
+    // token over 131071 keys: 94.1 us so, 96.8 with three); up to 768 keys are not
+    // split: the second launch costs the host more than it saves the GPU (517 keys:
+    // 13.2 us a call whole, 17.2 in three parts, 12.8 and 12.3 in a graph; 24
+    // contexts of 517: 17.4 and 18.4, 17.8 and 18.8 in a graph).
     p.few_parts = parts_of_keys(most, tasks, (512 + tasks - 1) / tasks, most <= 768 ? 768 : 256, 2048);
     p.few_parts.rows = tasks * 16;
     p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
@@ -181,12 +182,16 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
     p.chunk_tiles = tile_count(a.p.tokens, a.group, kChunkTile, a.p.seqs);
     // Two workgroups per CU (heads of up to 64: three), of the tiles that have rows
     // when they are all of one sequence (509 tokens of 28 heads beside 16 that
-    // decode: 167 us when the empty tiles of those count too, 145 us so); parts of
-    // at least 512 keys.  No more than that, so that none waits for a second turn
-    // and few rows find room, unless a quarter of the places stayed empty (that
-    // batch, few rows in the same launch: 135 us when rounded up, 126 so; 512
-    // tokens beside 32 over 8000 keys, bf16: 249 and 210; 1600 tokens over 16000:
-    // 577 and 513; but 300 tokens over 4000 fp32 keys: 227 and 261).
+    // decode: 141 us when the empty tiles of those count too, 126 us so); parts of
+    // at least 512 keys.  No more than that, so that few rows find room, and none
+    // waits for a second turn where that many run at once (fp32 queries over a
+    // 16-bit cache, and 16-bit ones in heads of 72 to 128), unless a quarter of the
+    // places stayed empty (that batch, few rows in the same launch: 135 us when
+    // rounded up, 126 so; 512 tokens beside 32 over 8000 keys, bf16: 249 and 210;
+    // 1600 tokens over 16000: 582 and 516).  One number for all types: registers let
+    // four run at once of 16-bit queries in heads of up to 64, two and one (heads of
+    // 72 to 128) over an fp32 cache, one of wider heads (300 tokens over 4000 fp32
+    // keys, heads of 128: 227 us when rounded up, 262 so).
     const int64_t wgs = ((int64_t)a.p.tokens * a.group + kChunkTile - 1) / kChunkTile * a.p.kv_heads;
     const int64_t places = D == 64 ? 768 : 512, down = places / wgs > 1 ? places / wgs : 1;
     // (tiles of no rows are launched too: sequences beyond number do not multiply)

@@ -3,12 +3,13 @@
 //
 // Bound by the products: 4 D per visible (row, key) on the matrix cores, times
 // the parts that fp32 queries and weights are split into.  A workgroup takes 128
-// rows of one (sequence, kv head), 32 per wave, and walks the keys in tiles: the
-// tile after next is requested into registers, the next one lies in LDS, the
-// current one is used by all four waves.  As for few rows, S^T = K Q^T and
-// O^T = V^T P^T, here with 32 x 32 products: a lane holds one row's scores of
-// keys 8 b + 4 h + 0 .. 3 (h = lane / 32), which are its weights' places in the
-// second product.
+// rows of one (sequence, kv head), 32 per wave, and walks the keys in tiles, two
+// of which have room in LDS: while all four waves use the current one, K of the
+// next is on its way into registers; then it goes to LDS, and V after it, whose
+// wait the CU's other waves fill.  As for few rows, S^T = K Q^T and O^T = V^T P^T,
+// here with 32 x 32 products: a lane holds one row's scores of keys
+// 8 b + 4 h + 0 .. 3 (h = lane / 32), which are its weights' places in the second
+// product.
 //
 // LDS holds K and V rows as they are in memory, their 16-byte pieces permuted
 // within a row so that 16 lanes which read 16 rows (K), or 32 which read 4 rows
@@ -21,11 +22,16 @@
 // a whole number, so that what it is taken from and given back to is exact.
 //
 // 2048 tokens over 16384 keys, 32 heads of 128, fp32 over fp16: 930 to
-// 960 us, 1073 to 1110 TFLOP/s of products, which is what a large fp16 matrix product reaches on
-// this card.  Two prompts of 4001, heads of 64, bf16: 160 us, 630 TFLOP/s: 16
+// 960 us, 1073 to 1110 TFLOP/s of products, which is what a large fp16 matrix
+// product reaches on this card.  Two prompts of 4001, heads of 64, bf16: 160 us, 630 TFLOP/s: 16
 // exponentials and about 90 other vector instructions stand beside each 8
 // products.  (There, both halves of a tile in turn under each other's
 // exponentials take 191 registers, and 206 us.)
+//
+// Registers that do not suffice, in bytes of scratch per lane: fp32 over bf16 in
+// heads of 72 to 128 40, 16-bit queries in heads of up to 64 28 (for the fourth
+// wave), and heads beyond 128, one wave per SIMD, 332 (fp32 over bf16), 276 (over
+// fp32) and 108 (over fp16).
 #include "nls_attend_few.h"
 
 namespace nls {

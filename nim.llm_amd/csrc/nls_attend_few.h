@@ -207,8 +207,11 @@ __device__ __forceinline__ void few_rows(const AttendArgs& a, const Parts& parts
           for (int u = 0; u < F::U; ++u) {
             const int d = u * 16 * F::E;
             typedef uint32_t words __attribute__((ext_vector_type(VP::kWords)));
-            // (past the caches: 102 -> 92 us for one token over 131071 keys; K's
-          // 64-byte pieces of a row meet in the cache and are not)
+            // (past the caches: one token over 131071 keys 104 -> 89 us, 48 contexts
+            // of 4000 147 -> 133; shared pages lose less: 48 forks of 4000 67.6 us
+            // either way, of 16000 235 -> 246, groups of 32 heads 34.5 -> 35.2 (8 of
+            // 16000) and 89.2 -> 89.8 (64 of 4000).  K's 64-byte pieces of a row meet
+            // in the cache and are not)
           const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(row_v + (!kPad || d + i * F::E < dim ? d : -i * F::E)));
 #pragma unroll
             for (int y = 0; y < VP::kWords; ++y) v[s * 4 + r][u].w[y] = x[y];

@@ -17,7 +17,7 @@ namespace nls {
 constexpr int kMaxHeadDim = 256;
 constexpr int kMaxPageSize = 4096;
 constexpr int kMaxLen = 0x7fffff00;  // tokens of a context: a step behind the last one is an int too
-constexpr int kMaxPages = 1 << 19;  // one bit and half a byte of LDS each in the page kernels
+constexpr int kMaxPages = 1 << 19;  // one bit and half a bit of LDS each in the page kernels
 
 enum ElemType { kF32 = 0, kF16 = 1, kBF16 = 30 };
 
@@ -109,8 +109,8 @@ struct TurnArgs {
 };
 
 #ifdef __HIPCC__
-// width: elements per load; a divisor of what the call's sizes, strides and
-// pointers allow
+// wide: 8 elements at a time (rope's fp32: 4), where pointers, strides and the
+// turned part allow it; else one
 hipError_t launch_rope(const TurnArgs& t, int type, bool wide, hipStream_t s);
 hipError_t launch_append(const TurnArgs& t, const PagedArgs& a, int type, int cache_type, bool wide, hipStream_t s);
 
