@@ -98,6 +98,12 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
  * (page_stride and token_stride below 2^30), d_kv is 16-byte aligned, head_dim a
  * multiple of 8 up to 256, page_size a power of two up to 4096.  A table entry outside [0, pages) is no page: what
  * it would hold is neither read nor written, and attention sees no key there. */
+/* type NLS_GGML_Q8_0 or NLS_GGML_Q4_0: blocks of 32 elements of a head, an fp16
+ * factor d and a whole number c each, value d c, as GGUF's types of those names
+ * hold (Q8_0 -127 .. 127, Q4_0 -8 .. 7), but with codes and factors apart and in
+ * the order that the kernels take them.  A page is then nls_cache_page_bytes()
+ * bytes; page_stride counts bytes (a multiple of 16), the three strides within a
+ * page are 0, head_dim is a multiple of 32 and page_size at least 16. */
 typedef struct nls_paged_kv {
   void* d_kv;
   int32_t type;
@@ -115,6 +121,10 @@ typedef struct nls_paged_kv {
   int32_t max_pages;
   const int32_t* d_lens; /* [slots]: tokens of each context, this call's among them */
 } nls_paged_kv;
+
+/* Bytes of a page's keys and values, or -1 for a type or size that a cache
+ * cannot have. */
+int64_t nls_cache_page_bytes(int32_t type, int32_t kv_heads, int32_t page_size, int32_t head_dim);
 
 /* The new tokens of a call: sequence i's are rows [d_starts[i], d_starts[i+1])
  * of q, k, v and the outputs, and they are the last ones of slot d_slots[i]
@@ -136,10 +146,26 @@ typedef struct nls_chunks {
  * converted to the cache's type.  plan may be NULL (nothing is turned).
  * `type` is that of q, k and v.  Two tokens never share a place, unless a slot
  * is named twice or a page is held twice: then either's row may stay.
+ * Blocks (type is then any of the three): the turned elements, unrounded, give
+ *   Q8_0  d = fp16(max |x| * (1 / 127)),                  c = rint(x * (1 / d))
+ *   Q4_0  d = fp16(max(max x * (1 / 7), min x * (-1 / 8))), c within -8 .. 7
+ * in fp32, each operation rounded once (d at most 65504: larger elements are
+ * cut; all c are 0 where d is 0).  A block with an element that is not finite
+ * has d = NaN.
  */
 int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const nls_rope_plan* plan, int32_t type,
                          const nls_heads* q, const nls_heads* q_out, int32_t heads, const nls_heads* k,
                          const nls_heads* v, void* stream);
+
+/*
+ * The rows back: k[t] and v[t] ([tokens, kv_heads, head_dim], `type` any of the
+ * three) are what the cache holds for the tokens of `chunks`, the last ones of
+ * their slots, converted with one rounding (a block's d c is one product).
+ * Rows of a sequence that have no place (no page, a slot out of range or
+ * shorter than its rows) are 0; rows of no sequence are left as they were.
+ */
+int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t type, const nls_heads* k,
+                       const nls_heads* v, void* stream);
 
 /*
  * out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the keys j of

@@ -48,7 +48,7 @@ EXPORTED = (
     "nls_lm_head_workspace", "nls_lm_head", "nls_lm_head_row_bytes", "nls_argmax",
     "nls_rope_frequencies", "nls_rope", "nls_cache_append", "nls_paged_attention_workspace", "nls_paged_attention",
     "nls_cache_workspace", "nls_cache_reserve", "nls_cache_fork", "nls_cache_release", "nls_cache_compact",
-    "nls_cache_copy_pages",
+    "nls_cache_copy_pages", "nls_cache_page_bytes", "nls_cache_read",
 )
 
 
@@ -196,6 +196,9 @@ def lib():
         L.nls_paged_attention_workspace.restype = ctypes.c_size_t
         L.nls_paged_attention.argtypes = [kp, cp, i32, hp, hp, i32, ctypes.c_float, i32, vp, vp, i32, i64] + ws
         pp, tp = P(NlsPagePool), P(NlsPageTables)
+        L.nls_cache_page_bytes.argtypes = [i32, i32, i32, i32]
+        L.nls_cache_page_bytes.restype = i64
+        L.nls_cache_read.argtypes = [kp, cp, i32, hp, hp, vp]
         L.nls_cache_workspace.argtypes = [tp, i32]
         L.nls_cache_workspace.restype = ctypes.c_size_t
         L.nls_cache_reserve.argtypes = [tp, vp, vp] + ws
@@ -840,16 +843,57 @@ def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
     return out
 
 
-def _paged_kv(dev: int, kv, table, lens):
-    pages, two, kv_heads, page_size, dim = kv.shape
+@dataclass(frozen=True)
+class PageFormat:
+    """Pages whose keys and values are blocks of 32 elements of a head, an fp16
+    factor and a code of 8 or 4 bits each: kind "q8_0" or "q4_0", as GGUF's types
+    of those names hold.  One layer of such a cache is a uint8 tensor [pages,
+    page_bytes], whose pages are 16-byte aligned."""
+
+    kind: str
+    kv_heads: int
+    page_size: int
+    head_dim: int
+
+    @property
+    def type(self) -> int:
+        t = {"q8_0": 8, "q4_0": 2}.get(self.kind)
+        if t is None:
+            raise SamplerError(f"page format {self.kind!r} is neither q8_0 nor q4_0")
+        return t
+
+    @property
+    def page_bytes(self) -> int:
+        n = -1
+        if 0 < self.kv_heads < 1 << 31 and 0 < self.page_size <= 4096 and 0 < self.head_dim <= 256:
+            n = int(lib().nls_cache_page_bytes(self.type, self.kv_heads, self.page_size, self.head_dim))
+        if n < 0:
+            raise SamplerError(f"{self}: pages of 16 to 4096 tokens (a power of two), heads of a multiple of 32 up to 256")
+        return n
+
+
+def _kv_dims(kv, fmt):
+    """(kv_heads, page_size, head_dim) of a layer."""
+    return (kv.shape[2], kv.shape[3], kv.shape[4]) if fmt is None else (fmt.kv_heads, fmt.page_size, fmt.head_dim)
+
+
+def _paged_kv(dev: int, kv, table, lens, fmt=None):
     st = kv.stride()
-    if not (dev >= 0 and two == 2 and st[4] == 1):
-        raise AssertionError("a layer of the cache on the GPU: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
+    if fmt is not None:
+        if not (dev >= 0 and kv.dim() == 2 and kv.element_size() == 1 and st[1] == 1 and kv.shape[1] == fmt.page_bytes):
+            raise AssertionError("a layer of blocks on the GPU: uint8 [pages, page_bytes] of its format")
+        pages, kv_heads, page_size, dim = kv.shape[0], fmt.kv_heads, fmt.page_size, fmt.head_dim
+        st, kind = (st[0], 0, 0, 0), fmt.type
+    else:
+        pages, two, kv_heads, page_size, dim = kv.shape
+        if not (dev >= 0 and two == 2 and st[4] == 1):
+            raise AssertionError("a layer of the cache on the GPU: [pages, 2, kv_heads, page_size, head_dim], elements side by side")
+        kind = _elem_type(kv)
     slots, per = table.shape
     ts = table.stride()
     if not (table.get_device() == dev and table.dtype == lens.dtype and ts[1] == 1 and lens.numel() == slots):
         raise AssertionError("the page table: int32 [slots, pages], rows side by side")
-    return NlsPagedKv(kv.data_ptr(), _elem_type(kv), pages, page_size, kv_heads, dim, st[0], st[1], st[2], st[3],
+    return NlsPagedKv(kv.data_ptr(), kind, pages, page_size, kv_heads, dim, st[0], st[1], st[2], st[3],
                       table.data_ptr(), ts[0], slots, per, _ints(dev, lens))
 
 
@@ -866,15 +910,18 @@ def _chunks(dev: int, tokens: int, starts, slots):
     return NlsChunks(seqs, tokens, _ints(dev, starts), _ints(dev, slots))
 
 
-def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan] = None, slots=None, out=None):
+def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan] = None, slots=None, out=None,
+                 fmt: Optional[PageFormat] = None):
     """The new tokens of a layer into the cache: k turned by `plan` (None: as it
     is) and v, both [tokens, kv_heads, head_dim], to the pages of their
     positions; q [tokens, heads, head_dim] turned into `out` (which may be q).
     Sequence i's tokens are rows starts[i] .. starts[i + 1] and the last ones of
-    slot slots[i] (i when None), whose lens count them already.  Returns out."""
+    slot slots[i] (i when None), whose lens count them already.  fmt: the format
+    of a cache of blocks.  Returns out."""
     dev, dt = kv.get_device(), k.dtype
     tokens, kv_heads, dim = k.shape
-    if not (k.shape == v.shape and kv_heads == kv.shape[2] and dim == kv.shape[4]):
+    of = _kv_dims(kv, fmt)
+    if not (k.shape == v.shape and kv_heads == of[0] and dim == of[2]):
         raise AssertionError("k and v: [tokens, kv_heads, head_dim] of the cache's heads")
     heads, cq, co = 0, None, None
     if q is not None:
@@ -889,13 +936,34 @@ def cache_append(kv, table, lens, starts, k, v, q=None, plan: Optional[RopePlan]
     else:
         if out is not None:
             raise AssertionError("out without q")
-    _launch(dev, "nls_cache_append", _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots),
+    _launch(dev, "nls_cache_append", _paged_kv(dev, kv, table, lens, fmt), _chunks(dev, tokens, starts, slots),
             None if plan is None else plan._c(dev), _elem_type(k), cq, co, heads, _heads(dev, k, dt), _heads(dev, v, dt))
     return out
 
 
+def cache_read(kv, table, lens, starts, tokens: int, dtype=None, k=None, v=None, slots=None,
+               fmt: Optional[PageFormat] = None):
+    """The cached keys and values of the sequences' last tokens (cache_append's
+    starts and slots) as rows again: (k, v), both [tokens, kv_heads, head_dim] of
+    `dtype` (float32 by default, or that of a k and v given).  Rows without a
+    place in the cache are 0, rows of no sequence are left as they were."""
+    import torch
+
+    dev, of = kv.get_device(), _kv_dims(kv, fmt)
+    shape = (tokens, of[0], of[2])
+    given = k if k is not None else v
+    dt = dtype or (torch.float32 if given is None else given.dtype)
+    k, v = (torch.empty(shape, dtype=dt, device=kv.device) if x is None else x for x in (k, v))
+    if not (k.shape == shape and v.shape == shape):
+        raise AssertionError("k and v: [tokens, kv_heads, head_dim] of the cache's heads")
+    _launch(dev, "nls_cache_read", _paged_kv(dev, kv, table, lens, fmt), _chunks(dev, tokens, starts, slots), _elem_type(k),
+            _heads(dev, k, dt), _heads(dev, v, dt))
+    return k, v
+
+
 def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, scale: Optional[float] = None,
-                    window: int = 0, first=None, slots=None, out=None, lse=None, work=None):
+                    window: int = 0, first=None, slots=None, out=None, lse=None, work=None,
+                    fmt: Optional[PageFormat] = None):
     """Attention of the new tokens' q [tokens, heads, head_dim] over their slots'
     cached keys and values (cache_append's arguments): causal, at most `window`
     keys back when that is > 0, from key first[slot] on when given.  scale:
@@ -904,7 +972,8 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
     split, not what comes out.  lse: True, or a float32 [tokens, heads] tensor,
     for the logarithm of each row's sum.  Rows of no sequence keep what `out` and
     `lse` hold.  `work`: a preallocated uint8 workspace of
-    paged_attention_workspace() bytes.  Returns out, or (out, lse)."""
+    paged_attention_workspace() bytes.  fmt: the format of a cache of blocks.
+    Returns out, or (out, lse)."""
     import torch
 
     dev, dt = kv.get_device(), q.dtype
@@ -920,9 +989,9 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
         if not (lse.get_device() == dev and lse.dtype == torch.float32 and lse.is_contiguous() and
                 lse.shape == (tokens, heads)):
             raise AssertionError("lse: float32 [tokens, heads], contiguous")
-    if not (out.shape == q.shape and dim == kv.shape[4] and (first is None or first.numel() == lens.numel())):
+    if not (out.shape == q.shape and dim == _kv_dims(kv, fmt)[2] and (first is None or first.numel() == lens.numel())):
         raise AssertionError("out: q's shape; q: the cache's head_dim; first: a key per slot")
-    c, ch = _paged_kv(dev, kv, table, lens), _chunks(dev, tokens, starts, slots)
+    c, ch = _paged_kv(dev, kv, table, lens, fmt), _chunks(dev, tokens, starts, slots)
     cq, co, cf = _heads(dev, q, dt), _heads(dev, out, dt), _ints(dev, first)
     need = lib().nls_paged_attention_workspace(c, ch, heads, max_new, max_len, window)
     if need and (work is None or work.numel() < need):
@@ -935,11 +1004,12 @@ def paged_attention(q, kv, table, lens, starts, max_new: int = 0, max_len: int =
     return out if lse is None else (out, lse)
 
 
-def paged_attention_workspace(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, window: int = 0) -> int:
+def paged_attention_workspace(q, kv, table, lens, starts, max_new: int = 0, max_len: int = 0, window: int = 0,
+                              fmt: Optional[PageFormat] = None) -> int:
     """Bytes of the workspace paged_attention takes for these arguments, for a
     caller that keeps one (each call in flight needs its own)."""
     _in_range(window, max_new, max_len)
-    return int(lib().nls_paged_attention_workspace(_paged_kv(kv.get_device(), kv, table, lens),
+    return int(lib().nls_paged_attention_workspace(_paged_kv(kv.get_device(), kv, table, lens, fmt),
                                                    _chunks(kv.get_device(), q.shape[0], starts, None), q.shape[1], max_new,
                                                    max_len, window))
 

@@ -19,6 +19,7 @@
 // that type, each with a product of its own, so that nothing is rounded to 16
 // bits.  An fp32 cache goes through the fp32 products (16 x 16 x 4).
 #include "nls_attend_few.h"
+#include "nls_attend_quant.h"
 
 namespace nls {
 namespace {
@@ -161,7 +162,7 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   int64_t longest = max_new > 0 && max_new < a.p.tokens ? max_new : a.p.tokens;
   if (a.window > 0 && most > (int64_t)a.window + longest) most = (int64_t)a.window + longest;
   const size_t per_row = D * sizeof(float) + sizeof(f4);
-  p.chunk = longest > 1 && longest * a.group > 16;
+  p.chunk = longest > 1 && longest * a.group > 16 && !quant_type(a.cache_type);
   // One sequence that may be a chunk is taken for one: its rows are few only
   // where the others belong to no sequence.
   p.few = !(p.chunk && a.p.seqs == 1);
@@ -209,6 +210,23 @@ Parts placed(Parts p, void* work, int D) {
   return p;
 }
 
+// The rows whose keys were split.
+template <typename T, int D>
+hipError_t join(const AttendArgs& a, const AttendPlan& p, const Parts& few, const Parts& chunk, float few_shift,
+                float chunk_shift, hipStream_t s) {
+  const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_rows takes of a sequence
+  const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
+  const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
+  if (rows == 0) return hipSuccess;
+  if (rows < 1024)
+    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
+                                                                few_shift, chunk_shift);
+  else
+    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
+                                                                          few_shift, chunk_shift);
+  return hipGetLastError();
+}
+
 template <typename T, typename TC, int D, bool kPad>
 hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
   const Parts few = placed(p.few_parts, work, D);
@@ -228,17 +246,7 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
   if (p.chunk &&
       (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, p.few ? &few : nullptr, p.few_tiles, s)) != hipSuccess)
     return e;
-  const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_rows takes of a sequence
-  const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
-  const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
-  if (rows == 0) return hipSuccess;
-  if (rows < 1024)
-    join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
-                                                                Elem<TC>::kShift, chunk_shift<TC>());
-  else
-    join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
-                                                                          Elem<TC>::kShift, chunk_shift<TC>());
-  return hipGetLastError();
+  return join<T, D>(a, p, few, chunk, Elem<TC>::kShift, chunk_shift<TC>(), s);
 }
 
 template <typename T, typename TC>
@@ -252,6 +260,24 @@ hipError_t attend_types(const AttendArgs& a, const AttendPlan& p, int type, int 
   return attend_width<T, TC, 256, true>(a, p, type, cache_type, work, s);
 }
 
+// Pages of blocks.
+template <typename T, int D>
+hipError_t attend_quant_width(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work,
+                              hipStream_t s) {
+  const Parts few = placed(p.few_parts, work, D);
+  const Parts chunk = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
+  const hipError_t e = p.few ? launch_few_quant(a, type, cache_type, few, p.few_tiles, p.chunk, s) : hipSuccess;
+  if (e != hipSuccess) return e;
+  return join<T, D>(a, p, few, chunk, kQuantShift, kQuantShift, s);
+}
+
+template <typename T>
+hipError_t attend_quant(const AttendArgs& a, const AttendPlan& p, int type, int cache_type, char* work, hipStream_t s) {
+  if (a.p.dim <= 64) return attend_quant_width<T, 64>(a, p, type, cache_type, work, s);
+  if (a.p.dim <= 128) return attend_quant_width<T, 128>(a, p, type, cache_type, work, s);
+  return attend_quant_width<T, 256>(a, p, type, cache_type, work, s);
+}
+
 }  // namespace
 
 size_t attend_workspace(const AttendArgs& a, int max_new, int64_t max_len) {
@@ -263,6 +289,12 @@ hipError_t launch_attend(const AttendArgs& a, int type, int cache_type, int max_
                          hipStream_t s) {
   const AttendPlan p = plan_of(a, max_new, max_len);
   char* w = static_cast<char*>(work);
+  if (quant_type(cache_type)) {
+    if (a.p.seqs < 1 || a.p.tokens < 1) return hipSuccess;
+    if (type == kF32) return attend_quant<float>(a, p, type, cache_type, w, s);
+    if (type == kF16) return attend_quant<_Float16>(a, p, type, cache_type, w, s);
+    return attend_quant<__bf16>(a, p, type, cache_type, w, s);
+  }
   if (type == kF32) {
     if (cache_type == kF32) return attend_types<float, float>(a, p, type, cache_type, w, s);
     if (cache_type == kF16) return attend_types<float, _Float16>(a, p, type, cache_type, w, s);

@@ -9,6 +9,7 @@
 #include "../../include/nimllm_sampler.h"
 #include "nls_internal.h"
 #include "nls_paged.h"
+#include "nls_quant.h"
 
 using namespace nls;
 
@@ -53,18 +54,38 @@ const char* check_plan(const nls_rope_plan* p, int dim) {
   return nullptr;
 }
 
+// Bytes of a page: sizes that check_kv takes
+int64_t page_bytes_of(int type, int kv_heads, int page_size, int head_dim) {
+  if (quant_type(type)) return quant_page_bytes(quant_shape(type, head_dim, page_size), kv_heads);
+  return (int64_t)2 * kv_heads * page_size * head_dim * elem_bytes(type);
+}
+
 const char* check_kv(const nls_paged_kv* kv) {
   if (!kv) return "NULL cache";
-  if (!elem_type(kv->type)) return "cache: element type is not F32, F16 or BF16";
+  const bool quant = quant_type(kv->type);
+  if (!elem_type(kv->type) && !quant) return "cache: type is not F32, F16, BF16, Q8_0 or Q4_0";
   if (kv->pages < 1 || kv->slots < 1 || kv->max_pages < 1 || kv->kv_heads < 1) return "cache: a size is below 1";
   if (kv->page_size < 1 || kv->page_size > kMaxPageSize || (kv->page_size & (kv->page_size - 1)))
     return "cache: page_size is not a power of two up to 4096";
   if (kv->head_dim < 8 || kv->head_dim > kMaxHeadDim || kv->head_dim % 8)
     return "cache: head_dim is not a multiple of 8 up to 256";
+  if (quant && (kv->head_dim % 32 || kv->page_size < kMinQuantPage))
+    return "cache of blocks: head_dim is no multiple of 32, or pages of fewer than 16 tokens";
   if (!kv->d_kv || !aligned(kv->d_kv, 16)) return "cache: NULL or misaligned d_kv";
   if (!kv->d_table || !kv->d_lens || !aligned(kv->d_table, 4) || !aligned(kv->d_lens, 4))
     return "cache: NULL or misaligned table or lens";
   const int64_t big = int64_t{1} << 40;
+  if (kv->table_stride < 0 || kv->table_stride > big || (kv->slots > 1 && kv->table_stride < kv->max_pages))
+    return "cache: table_stride is shorter than max_pages";
+  if (quant) {
+    const int64_t bytes = page_bytes_of(kv->type, kv->kv_heads, kv->page_size, kv->head_dim);
+    if (bytes >= int64_t{1} << 30) return "cache of blocks: a page of 2^30 bytes or more";
+    if (kv->page_stride % 16 || kv->page_stride < 0 || kv->page_stride > big || (kv->pages > 1 && kv->page_stride < bytes))
+      return "cache of blocks: page_stride (bytes) is negative, too large, no multiple of 16 or shorter than a page";
+    if (kv->value_offset || kv->head_stride || kv->token_stride)
+      return "cache of blocks: the strides within a page are not 0";
+    return nullptr;
+  }
   const int64_t st[4] = {kv->page_stride, kv->value_offset, kv->head_stride, kv->token_stride};
   for (int64_t x : st)
     if (x < 0 || x > big || x % 8) return "cache: a stride is negative, too large or no multiple of 8";
@@ -73,8 +94,6 @@ const char* check_kv(const nls_paged_kv* kv) {
   if (kv->value_offset < kv->head_dim || (kv->pages > 1 && kv->page_stride < kv->head_dim) ||
       (kv->kv_heads > 1 && kv->head_stride < kv->head_dim) || (kv->page_size > 1 && kv->token_stride < kv->head_dim))
     return "cache: strides overlap";
-  if (kv->table_stride < 0 || kv->table_stride > big || (kv->slots > 1 && kv->table_stride < kv->max_pages))
-    return "cache: table_stride is shorter than max_pages";
   return nullptr;
 }
 
@@ -117,6 +136,7 @@ const char* check_sizes(const nls_paged_kv* kv, const nls_chunks* c, int heads, 
   if (kv->kv_heads < 1 || kv->head_dim < 8 || kv->head_dim > kMaxHeadDim || kv->head_dim % 8 || kv->max_pages < 1 ||
       kv->page_size < 1 || kv->page_size > kMaxPageSize || (kv->page_size & (kv->page_size - 1)))
     return "cache: a size out of range";
+  if (quant_type(kv->type) && (kv->head_dim % 32 || kv->page_size < kMinQuantPage)) return "cache of blocks: a size out of range";
   if (c->seqs < 0 || c->tokens < 0) return "chunks: a negative size";
   if (heads < 1 || heads % kv->kv_heads) return "heads is no multiple of the cache's";
   // (a launch has fewer than 2^32 threads: one workgroup per sequence, kv head
@@ -131,6 +151,7 @@ const char* check_sizes(const nls_paged_kv* kv, const nls_chunks* c, int heads, 
 AttendArgs attend_args(const nls_paged_kv* kv, const nls_chunks* c, int heads, int window) {
   AttendArgs a{};
   a.p = paged(kv, c);
+  a.cache_type = kv->type;
   a.heads = heads;
   a.group = heads / kv->kv_heads;
   a.window = window;
@@ -263,8 +284,8 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
                          const nls_heads* v, void* stream) {
   NLS_CHECK(check_kv(kv));
   NLS_CHECK(check_chunks(chunks));
-  if (!elem_type(type) || (type != kF32 && type != kv->type))
-    return bad("append: q, k and v are F32, or of the cache's type");
+  if (!elem_type(type) || (type != kF32 && type != kv->type && !quant_type(kv->type)))
+    return bad("append: q, k and v are F32, or of the cache's type (any, where that is of blocks)");
   if (heads < 0 || (int64_t)heads * kv->head_dim > 0x1fffffff || (int64_t)kv->kv_heads * kv->head_dim > 0x1fffffff)
     return bad("append: heads out of range");
   if (plan) NLS_CHECK(check_plan(plan, kv->head_dim));
@@ -296,7 +317,32 @@ int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const
   t.v = view(v);
   const bool wide = (heads == 0 || (wide_ok(q, type, 8) && wide_ok(q_out, type, 8))) && wide_ok(k, type, 8) &&
                     wide_ok(v, type, 8) && t.rot % 16 == 0;
-  return done(launch_append(t, paged(kv, chunks), type, kv->type, wide, stream_of(stream)), "nls_cache_append");
+  const hipError_t e = quant_type(kv->type)
+                           ? launch_append_quant(t, paged(kv, chunks), type, kv->type, wide, stream_of(stream))
+                           : launch_append(t, paged(kv, chunks), type, kv->type, wide, stream_of(stream));
+  return done(e, "nls_cache_append");
+}
+
+int64_t nls_cache_page_bytes(int32_t type, int32_t kv_heads, int32_t page_size, int32_t head_dim) {
+  if ((!elem_type(type) && !quant_type(type)) || kv_heads < 1 || page_size < 1 || page_size > kMaxPageSize ||
+      (page_size & (page_size - 1)) || head_dim < 8 || head_dim > kMaxHeadDim || head_dim % 8)
+    return -1;
+  if (quant_type(type) && (head_dim % 32 || page_size < kMinQuantPage)) return -1;
+  return page_bytes_of(type, kv_heads, page_size, head_dim);
+}
+
+int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t type, const nls_heads* k,
+                       const nls_heads* v, void* stream) {
+  NLS_CHECK(check_kv(kv));
+  NLS_CHECK(check_chunks(chunks));
+  if (!elem_type(type)) return bad("read: k and v are F32, F16 or BF16");
+  if ((int64_t)kv->kv_heads * kv->head_dim > 0x1fffffff) return bad("read: heads out of range");
+  if (chunks->tokens == 0 || chunks->seqs == 0) return NLS_OK;
+  NLS_CHECK(check_heads(k, type, kv->kv_heads, chunks->tokens, kv->head_dim, true));
+  NLS_CHECK(check_heads(v, type, kv->kv_heads, chunks->tokens, kv->head_dim, true));
+  ReadArgs a{paged(kv, chunks), view(k), view(v)};
+  const bool wide = wide_ok(k, type, 8) && wide_ok(v, type, 8);
+  return done(launch_read(a, type, kv->type, wide, stream_of(stream)), "nls_cache_read");
 }
 
 size_t nls_paged_attention_workspace(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t heads, int32_t max_new,
@@ -312,8 +358,8 @@ int32_t nls_paged_attention(const nls_paged_kv* kv, const nls_chunks* chunks, in
   NLS_CHECK(check_kv(kv));
   NLS_CHECK(check_chunks(chunks));
   NLS_CHECK(check_sizes(kv, chunks, heads, max_new, max_len, window));
-  if (!elem_type(type) || (type != kF32 && type != kv->type))
-    return bad("attention: q and out are F32, or of the cache's type");
+  if (!elem_type(type) || (type != kF32 && type != kv->type && !quant_type(kv->type)))
+    return bad("attention: q and out are F32, or of the cache's type (any, where that is of blocks)");
   // (the kernels take exponents of base 2: an infinite factor times a score of 0 is NaN)
   if (!std::isfinite(scale * 1.4426950408889634f)) return bad("attention: scale, or scale times log2 e, is not finite");
   if (chunks->tokens == 0 || chunks->seqs == 0) return NLS_OK;

@@ -1,0 +1,58 @@
+// nls_attend_quant.hip -- attention of few rows over pages of blocks, in
+// launches of its own.
+#include "nls_attend_quant.h"
+
+namespace nls {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T, int kBits, int GT, bool kPad>
+__global__ __launch_bounds__(kThreads, GT == 8 ? 1 : 2) void few_quant_kernel(AttendArgs a, Parts parts, int tiles,
+                                                                              bool chunk_runs) {
+  few_quant_rows<T, kBits, GT, kPad>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
+}
+
+template <typename T, int kBits, int GT, bool kPad>
+hipError_t few_of(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs, hipStream_t s) {
+  constexpr size_t lds = (size_t)4 * 16 * (32 * GT + 4) * sizeof(float);
+  if (lds > 60000) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_quant_kernel<T, kBits, GT, kPad>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  few_quant_kernel<T, kBits, GT, kPad>
+      <<<dim3(a.p.kv_heads * a.p.seqs * tiles, 1, parts.most), kThreads, lds, s>>>(a, parts, tiles, chunk_runs);
+  return hipGetLastError();
+}
+
+template <typename T, int kBits>
+hipError_t few_width(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs, hipStream_t s) {
+  switch (a.p.dim / 32) {
+    case 1: return few_of<T, kBits, 2, true>(a, parts, tiles, chunk_runs, s);
+    case 2: return few_of<T, kBits, 2, false>(a, parts, tiles, chunk_runs, s);
+    case 3: return few_of<T, kBits, 4, true>(a, parts, tiles, chunk_runs, s);
+    case 4: return few_of<T, kBits, 4, false>(a, parts, tiles, chunk_runs, s);
+    case 8: return few_of<T, kBits, 8, false>(a, parts, tiles, chunk_runs, s);
+    default: return few_of<T, kBits, 8, true>(a, parts, tiles, chunk_runs, s);
+  }
+}
+
+template <typename T>
+hipError_t few_type(const AttendArgs& a, int cache_type, const Parts& parts, int tiles, bool chunk_runs, hipStream_t s) {
+  return cache_type == kQ8_0 ? few_width<T, 8>(a, parts, tiles, chunk_runs, s)
+                             : few_width<T, 4>(a, parts, tiles, chunk_runs, s);
+}
+
+}  // namespace
+
+hipError_t launch_few_quant(const AttendArgs& a, int type, int cache_type, const Parts& parts, int few_tiles,
+                            bool chunk_runs, hipStream_t s) {
+  switch (type) {
+    case kF32: return few_type<float>(a, cache_type, parts, few_tiles, chunk_runs, s);
+    case kF16: return few_type<_Float16>(a, cache_type, parts, few_tiles, chunk_runs, s);
+    default: return few_type<__bf16>(a, cache_type, parts, few_tiles, chunk_runs, s);
+  }
+}
+
+}  // namespace nls

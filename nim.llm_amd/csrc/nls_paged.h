@@ -141,6 +141,7 @@ hipError_t launch_copy_pages(const PoolArgs& p, int pages, const int32_t* src, c
 
 struct AttendArgs {
   PagedArgs p;
+  int cache_type;
   HeadsView q, out;
   int heads, group;
   float scale;

@@ -9,6 +9,7 @@
 // each to a few units of its own last place.
 // 8191 tokens of 32 heads of 128, bf16 (134 MB): 24.6 us, 5.4 TB/s.
 #include "nls_paged.h"
+#include "nls_quant.h"
 
 namespace nls {
 namespace {
@@ -220,7 +221,214 @@ hipError_t append_width(const TurnArgs& t, const PagedArgs& a, bool wide, hipStr
   return wide ? append_of<T, TC, 8>(t, a, s) : append_of<T, TC, 1>(t, a, s);
 }
 
+// ---------------------------------------------------------------- pages of blocks
+
+// The largest and least of a block's elements, whose lanes are `lanes`
+// neighbours, and whether one is not finite.
+template <int kLanes>
+__device__ __forceinline__ void over_block(float& hi, float& lo, int& odd) {
+#pragma unroll
+  for (int d = 1; d < kLanes; d <<= 1) {
+    hi = fmaxf(hi, __shfl_xor(hi, d));
+    lo = fminf(lo, __shfl_xor(lo, d));
+    odd |= __shfl_xor(odd, d);
+  }
+}
+
+// A block's factor, and what its elements are multiplied by.
+template <int kBits>
+__device__ __forceinline__ _Float16 factor_of(float hi, float lo, int odd, float* step) {
+  const float t = kBits == 8 ? fmaxf(hi, -lo) * 0.007874015718698502f : fmaxf(hi * 0.1428571492433548f, lo * -0.125f);
+  const _Float16 d = (_Float16)fminf(t, 65504.f);
+  *step = (float)d > 0.f ? 1.f / (float)d : 0.f;
+  return odd ? (_Float16)__builtin_nanf("") : d;
+}
+
+// The element's code as it is held.
+template <int kBits>
+__device__ __forceinline__ uint32_t code_of(float x, float step) {
+  constexpr float kLow = kBits == 8 ? -127.f : -8.f, kHigh = kBits == 8 ? 127.f : 7.f;
+  const float c = __builtin_rintf(x * step);
+  return (uint32_t)((int)fminf(fmaxf(c, kLow), kHigh) + (kBits == 8 ? 128 : 8));  // (NaN: the lowest)
+}
+
+// 8 neighbouring elements of a row from d on, turned.
+enum Turn { kNoTurn, kNeighbours, kHalves };
+template <typename T, bool kWide, Turn kTurn>
+__device__ __forceinline__ void turned8(const T* row, int d, int rot, const float2* cs, float (&x)[8]) {
+  if constexpr (kWide) {
+    const Pack<T, 8> p = load_pack<T, 8>(row + d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_f(p.v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = to_f(row[d + e]);
+  }
+  if constexpr (kTurn == kNeighbours) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      if (d + e >= rot) break;
+      const float2 c = cs[(d + e) / 2];
+      const float a = x[e], b = x[e + 1];
+      x[e] = a * c.x - b * c.y;
+      x[e + 1] = b * c.x + a * c.y;
+    }
+  }
+  if constexpr (kTurn == kHalves) {
+    const int half = rot / 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (d + e >= rot) break;
+      const bool low = d + e < half;
+      const int j = low ? d + e : d + e - half;
+      const float2 c = cs[j];
+      const float other = to_f(row[low ? d + e + half : j]);
+      x[e] = low ? x[e] * c.x - other * c.y : x[e] * c.x + other * c.y;
+    }
+  }
+}
+
+// One token's k and v into a page of blocks, and its q turned.  A key's block
+// is four lanes of 8 elements, a value's 16 lanes of 2; each lane's codes are
+// one piece of the row (nls_quant.h).  Factors and codes come of fp32 products
+// alone, each rounded once, so that they are the same numbers wherever they
+// are computed.
+template <typename T, int kBits, bool kWide, Turn kTurn>
+__global__ __launch_bounds__(kTurnThreads) void append_quant_kernel(TurnArgs t, PagedArgs a) {
+  constexpr int N = kWide ? 8 : 1;
+  constexpr bool kInterleaved = kTurn == kNeighbours;
+  __shared__ float2 cs[kMaxHeadDim / 2];
+  const int token = blockIdx.x;
+  const int rot = kTurn == kNoTurn ? 0 : t.rot;
+  const int pairs = rot / (2 * N), units = pairs + (t.dim - rot) / N;
+  const int qu = t.heads ? (t.x.d == t.y.d ? pairs : units) : 0;
+  const int lane = threadIdx.x & 63;
+  int seq = -1;
+  for (int s0 = 0; s0 < a.seqs + 1; s0 += 64) {
+    const int s = s0 + lane;
+    const int n = __popcll(__ballot(s <= a.seqs && a.starts[s <= a.seqs ? s : a.seqs] <= token));
+    seq += n;
+    if (n < 64) break;
+  }
+  if (seq < 0 || seq >= a.seqs) return;  // a row of no sequence
+  const Chunk c = chunk_of(a, seq);
+  const int64_t pos = position_of(a, c, token - c.begin);
+  const int page = page_of(a, c.slot, pos);
+  if constexpr (kTurn != kNoTurn) {
+    turn_table(t, pos, cs);
+    __syncthreads();
+  }
+  if (qu) {
+    const T* x = static_cast<const T*>(t.x.d) + token * t.x.token_stride;
+    T* y = static_cast<T*>(t.y.d) + token * t.y.token_stride;
+    for (int w = threadIdx.x; w < qu * t.heads; w += kTurnThreads)
+      store_unit<T, T, N, kInterleaved>(load_unit<T, N, kInterleaved>(x + w / qu * t.x.head_stride, w % qu, rot),
+                                        y + w / qu * t.y.head_stride, w % qu, rot, cs);
+  }
+  if (page < 0) return;
+  const QuantShape s = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, t.dim, 1 << a.page_shift);
+  const int place = (int)(pos & ((1 << a.page_shift) - 1)), size = 1 << a.page_shift;
+  char* home = static_cast<char*>(a.kv) + (int64_t)page * a.page_stride;
+  const int planes = plane_count(s.groups);
+  // keys by four lanes to a block, then (from a multiple of 16 on) values by 16 to a plane
+  const int nk = 4 * s.groups * a.kv_heads, v0 = (nk + 15) & ~15, all = v0 + 16 * planes * a.kv_heads;
+  for (int w = threadIdx.x; w < all; w += kTurnThreads) {
+    if (w < nk) {
+      const int head = w / (4 * s.groups), u = w % (4 * s.groups), x = u >> 2, g = u & 3;
+      float e[8];
+      turned8<T, kWide, kTurn>(static_cast<const T*>(t.k.d) + token * t.k.token_stride + head * t.k.head_stride,
+                               32 * x + 8 * g, rot, cs, e);
+      float hi = e[0], lo = e[0];
+      int odd = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hi = fmaxf(hi, e[j]);
+        lo = fminf(lo, e[j]);
+        odd |= !(fabsf(e[j]) < __builtin_inff());
+      }
+      over_block<4>(hi, lo, odd);
+      float step;
+      const _Float16 d = factor_of<kBits>(hi, lo, odd, &step);
+      char* to = home + quant_base(s, head, 0);
+      if constexpr (kBits == 8) {
+        uint32_t r[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j / 4] |= code_of<8>(e[j], step) << (8 * (j & 3));
+        __builtin_memcpy(__builtin_assume_aligned(to + place * s.row + key_at(s, x, g), 8), r, 8);
+      } else {
+        uint32_t r = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r |= code_of<4>(e[j], step) << (4 * nibble_of(j));
+        *reinterpret_cast<uint32_t*>(to + place * s.row + key_at(s, x, g)) = r;
+      }
+      if (g == 0) reinterpret_cast<_Float16*>(to + s.codes)[x * size + place] = d;
+    } else if (w >= v0) {
+      const int n = (w - v0) >> 4, i = w & 15, head = n / planes;
+      const Plane p = plane_of(s.groups, n % planes);
+      const T* row = static_cast<const T*>(t.v.d) + token * t.v.token_stride + head * t.v.head_stride + 32 * p.first + i;
+      char* to = home + quant_base(s, head, 1);
+      float e[8];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        e[2 * x] = x < p.wide ? to_f(row[32 * x]) : 0.f;
+        e[2 * x + 1] = x < p.wide ? to_f(row[32 * x + 16]) : 0.f;
+      }
+      uint32_t r[2] = {0, 0};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (x >= p.wide) break;
+        float hi = fmaxf(e[2 * x], e[2 * x + 1]), lo = fminf(e[2 * x], e[2 * x + 1]);
+        int odd = !(fabsf(e[2 * x]) < __builtin_inff()) || !(fabsf(e[2 * x + 1]) < __builtin_inff());
+        over_block<16>(hi, lo, odd);
+        float step;
+        const _Float16 d = factor_of<kBits>(hi, lo, odd, &step);
+        const uint32_t a0 = code_of<kBits>(e[2 * x], step), a1 = code_of<kBits>(e[2 * x + 1], step);
+        if constexpr (kBits == 8)
+          r[x / 2] |= (a0 | a1 << 8) << (16 * (x & 1));
+        else
+          r[0] |= (a0 | a1 << 4) << (8 * x);
+        if (i == 0) reinterpret_cast<_Float16*>(to + s.codes)[(p.first + x) * size + place] = d;
+      }
+      char* at = to + place * s.row + value_at(s, p, i);
+      const int bytes = p.wide * kBits / 4;
+      if (bytes == 8) {
+        __builtin_memcpy(__builtin_assume_aligned(at, 8), r, 8);
+      } else if (bytes == 4) {
+        *reinterpret_cast<uint32_t*>(at) = r[0];
+      } else if (bytes == 2) {
+        *reinterpret_cast<uint16_t*>(at) = (uint16_t)r[0];
+      } else {
+        *reinterpret_cast<uint8_t*>(at) = (uint8_t)r[0];
+      }
+    }
+  }
+}
+
+template <typename T, int kBits, bool kWide>
+hipError_t append_quant_of(const TurnArgs& t, const PagedArgs& a, hipStream_t s) {
+  if (!t.freqs)
+    append_quant_kernel<T, kBits, kWide, kNoTurn><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+  else if (t.interleaved)
+    append_quant_kernel<T, kBits, kWide, kNeighbours><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+  else
+    append_quant_kernel<T, kBits, kWide, kHalves><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+  return hipGetLastError();
+}
+template <typename T>
+hipError_t append_quant_type(const TurnArgs& t, const PagedArgs& a, int cache_type, bool wide, hipStream_t s) {
+  if (cache_type == kQ8_0) return wide ? append_quant_of<T, 8, true>(t, a, s) : append_quant_of<T, 8, false>(t, a, s);
+  return wide ? append_quant_of<T, 4, true>(t, a, s) : append_quant_of<T, 4, false>(t, a, s);
+}
+
 }  // namespace
+
+hipError_t launch_append_quant(const TurnArgs& t, const PagedArgs& a, int type, int cache_type, bool wide, hipStream_t s) {
+  switch (type) {
+    case kF32: return append_quant_type<float>(t, a, cache_type, wide, s);
+    case kF16: return append_quant_type<_Float16>(t, a, cache_type, wide, s);
+    default: return append_quant_type<__bf16>(t, a, cache_type, wide, s);
+  }
+}
 
 hipError_t launch_rope(const TurnArgs& t, int type, bool wide, hipStream_t s) {
   switch (type) {
