@@ -227,7 +227,7 @@ typedef struct nls_page_tables {
   int32_t page_size;
 } nls_page_tables;
 
-/* What reserve, fork and release write to *d_status: all of the call was done,
+/* What reserve, fork, release and reorder write to *d_status: all of the call was done,
  * or none of it for the reason given. */
 enum {
   NLS_PAGES_DONE = 0,
@@ -257,6 +257,17 @@ int32_t nls_cache_fork(const nls_page_pool* pool, const nls_page_tables* tables,
  * released once. */
 int32_t nls_cache_release(const nls_page_tables* tables, const int32_t* d_slots, int32_t count, int32_t* d_status,
                           void* d_work, size_t work_bytes, void* stream);
+
+/* Every slot s becomes what slot d_parents[s] (int32 [slots]) was: itself, another
+ * one, or, where that is -1, empty.  Full pages are shared.  The partial last
+ * page of a parent stays with the parent if it is its own child, else goes to
+ * its first child; the other children take copies, in the order of the slots, on
+ * the lowest pages that nobody holds any more.  What no slot goes on from is let
+ * go of.  A status as above: BAD_ENTRY for a parent or a length out of range.
+ * d_work: nls_cache_reorder_workspace() bytes, 256-byte aligned. */
+size_t nls_cache_reorder_workspace(const nls_page_tables* tables);
+int32_t nls_cache_reorder(const nls_page_pool* pool, const nls_page_tables* tables, const int32_t* d_parents,
+                          int32_t* d_status, void* d_work, size_t work_bytes, void* stream);
 
 /* Moves pages so that the held ones are 0 .. *d_live - 1: the held pages from
  * there on, in ascending order, to the free ones below it, in ascending

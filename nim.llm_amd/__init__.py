@@ -49,6 +49,7 @@ EXPORTED = (
     "nls_rope_frequencies", "nls_rope", "nls_cache_append", "nls_paged_attention_workspace", "nls_paged_attention",
     "nls_cache_workspace", "nls_cache_reserve", "nls_cache_fork", "nls_cache_release", "nls_cache_compact",
     "nls_cache_copy_pages", "nls_cache_page_bytes", "nls_cache_read",
+    "nls_cache_reorder_workspace", "nls_cache_reorder", "nls_beam_workspace", "nls_beam_select",
 )
 
 
@@ -205,6 +206,12 @@ def lib():
         L.nls_cache_fork.argtypes = [pp, tp, vp, vp, i32, vp] + ws
         L.nls_cache_release.argtypes = [tp, vp, i32, vp] + ws
         L.nls_cache_compact.argtypes = [pp, tp, vp] + ws
+        L.nls_cache_reorder_workspace.argtypes = [tp]
+        L.nls_cache_reorder_workspace.restype = ctypes.c_size_t
+        L.nls_cache_reorder.argtypes = [pp, tp, vp, vp] + ws
+        L.nls_beam_workspace.argtypes = [i32, i32, i64]
+        L.nls_beam_workspace.restype = ctypes.c_size_t
+        L.nls_beam_select.argtypes = [vp, i32, i32, i64, vp, vp, vp, i32, vp, vp, vp, vp] + ws
         L.nls_cache_copy_pages.argtypes = [pp, i32, vp, vp, i32, vp]
         _lib = L
     return _lib
@@ -1017,9 +1024,13 @@ def paged_attention_workspace(q, kv, table, lens, starts, max_new: int = 0, max_
 PAGES_DONE, PAGES_NONE_LEFT, PAGES_ROW_FULL, PAGES_BAD_ENTRY = range(4)
 
 
-def _page_pool(dev: int, kv):
-    layers, _, two, heads, page_size, dim = kv.shape
+def _page_pool(dev: int, kv, fmt=None):
     st, n = kv.stride(), kv.element_size()
+    if fmt is not None:
+        if not (kv.get_device() == dev and kv.dim() == 3 and n == 1 and st[2] == 1 and kv.shape[2] == fmt.page_bytes):
+            raise AssertionError("a cache of blocks: uint8 [layers, pages, page_bytes] of its format")
+        return NlsPagePool(kv.data_ptr(), kv.shape[0], kv.shape[2], st[0], st[1])
+    layers, _, two, heads, page_size, dim = kv.shape
     dense = 1  # elements of a page so far, in the order of the strides
     for stride, size in sorted(zip(st[2:], kv.shape[2:])):
         if size != 1:
@@ -1027,6 +1038,10 @@ def _page_pool(dev: int, kv):
     if not (kv.get_device() == dev and two == 2 and dense == 2 * heads * page_size * dim):
         raise AssertionError("the cache: [layers, pages, 2, kv_heads, page_size, head_dim], each page's contents side by side")
     return NlsPagePool(kv.data_ptr(), layers, dense * n, st[0] * n, st[1] * n)
+
+
+def _page_size(kv, fmt) -> int:
+    return kv.shape[4] if fmt is None else fmt.page_size
 
 
 def _page_tables(dev: int, table, lens, refs, page_size: int):
@@ -1040,11 +1055,11 @@ def _page_tables(dev: int, table, lens, refs, page_size: int):
     return NlsPageTables(table.data_ptr(), ts[0], slots, per, _ints(dev, lens), _ints(dev, refs), refs.numel(), page_size)
 
 
-def _pages_call(dev: int, what: str, refs, t, count: int, *args):
-    """One of the page calls with its workspace; returns its int32 word."""
+def _pages_call(dev: int, what: str, refs, need: int, *args):
+    """One of the page calls with its workspace of `need` bytes; returns its int32
+    word."""
     import torch
 
-    need = lib().nls_cache_workspace(t, count)
     # the word, then the workspace from the next 256 bytes on
     both = torch.empty(need // 4 + 64, dtype=torch.int32, device=refs.device)
     at = both.data_ptr()
@@ -1060,18 +1075,19 @@ def cache_reserve(table, lens, refs, page_size: int, counts):
     if counts.numel() != table.shape[0]:
         raise AssertionError("counts: one per slot")
     t = _page_tables(dev, table, lens, refs, page_size)
-    return _pages_call(dev, "nls_cache_reserve", refs, t, 0, t, _ints(dev, counts))
+    return _pages_call(dev, "nls_cache_reserve", refs, lib().nls_cache_workspace(t, 0), t, _ints(dev, counts))
 
 
-def cache_fork(kv, table, lens, refs, src, dst):
+def cache_fork(kv, table, lens, refs, src, dst, fmt: Optional[PageFormat] = None):
     """The empty slots dst[i] (int32) become copies of the slots src[i]: full
-    pages shared, the last partial page copied in every layer of kv.  Returns the
+    pages shared, the last partial page copied in every layer of kv (fmt: the
+    format of a cache of blocks, uint8 [layers, pages, page_bytes]).  Returns the
     status word."""
     dev, n = refs.get_device(), src.numel()
     if not (n == dst.numel() and kv.shape[1] == refs.numel()):
         raise AssertionError("src and dst of one length; refs: one per page of kv")
-    t = _page_tables(dev, table, lens, refs, kv.shape[4])
-    return _pages_call(dev, "nls_cache_fork", refs, t, n, _page_pool(dev, kv), t, _ints(dev, src), _ints(dev, dst), n)
+    t = _page_tables(dev, table, lens, refs, _page_size(kv, fmt))
+    return _pages_call(dev, "nls_cache_fork", refs, lib().nls_cache_workspace(t, n), _page_pool(dev, kv, fmt), t, _ints(dev, src), _ints(dev, dst), n)
 
 
 def cache_release(table, lens, refs, slots, page_size: int):
@@ -1079,25 +1095,38 @@ def cache_release(table, lens, refs, slots, page_size: int):
     status word."""
     dev = refs.get_device()
     t = _page_tables(dev, table, lens, refs, page_size)
-    return _pages_call(dev, "nls_cache_release", refs, t, 0, t, _ints(dev, slots), slots.numel())
+    return _pages_call(dev, "nls_cache_release", refs, lib().nls_cache_workspace(t, 0), t, _ints(dev, slots), slots.numel())
 
 
-def cache_compact(kv, table, refs):
+def cache_reorder(kv, table, lens, refs, parents, fmt: Optional[PageFormat] = None):
+    """Every slot s becomes what slot parents[s] (int32 [slots]; -1: nothing) was:
+    full pages shared, a parent's last partial page kept by itself or its first
+    child and copied for the others, in every layer of kv.  Returns the status
+    word."""
+    dev = refs.get_device()
+    if not (parents.numel() == table.shape[0] and kv.shape[1] == refs.numel()):
+        raise AssertionError("parents: one per slot; refs: one per page of kv")
+    t = _page_tables(dev, table, lens, refs, _page_size(kv, fmt))
+    return _pages_call(dev, "nls_cache_reorder", refs, lib().nls_cache_reorder_workspace(t), _page_pool(dev, kv, fmt), t,
+                       _ints(dev, parents))
+
+
+def cache_compact(kv, table, refs, fmt: Optional[PageFormat] = None):
     """Moves the held pages to the lowest ids, their contents in every layer and
     the table's entries with them.  Returns how many are held, int32 [1]."""
     dev = refs.get_device()
     if kv.shape[1] != refs.numel():
         raise AssertionError("refs: one per page of kv")
-    t = _page_tables(dev, table, None, refs, kv.shape[4])
-    return _pages_call(dev, "nls_cache_compact", refs, t, 0, _page_pool(dev, kv), t)
+    t = _page_tables(dev, table, None, refs, _page_size(kv, fmt))
+    return _pages_call(dev, "nls_cache_compact", refs, lib().nls_cache_workspace(t, 0), _page_pool(dev, kv, fmt), t)
 
 
-def cache_copy_pages(kv, src, dst):
+def cache_copy_pages(kv, src, dst, fmt: Optional[PageFormat] = None):
     """Page src[i] to page dst[i] (int32) in every layer of kv."""
     dev = kv.get_device()
     if not (dev >= 0 and src.numel() == dst.numel()):
         raise AssertionError("copies: kv on the GPU, src and dst of one length")
-    _launch(dev, "nls_cache_copy_pages", _page_pool(dev, kv), kv.shape[1], _ints(dev, src), _ints(dev, dst), src.numel())
+    _launch(dev, "nls_cache_copy_pages", _page_pool(dev, kv, fmt), kv.shape[1], _ints(dev, src), _ints(dev, dst), src.numel())
 
 
 class PagedCache:
@@ -1106,17 +1135,23 @@ class PagedCache:
     contexts that share one pool.
 
     kv [layers, pages, 2, kv_heads, page_size, head_dim]; table [slots,
-    max_pages], lens [slots] and refs [pages] are int32.  A decoding step is
-    reserve(counts), then append and attend layer by layer; nothing of it waits
-    for the device, so it can be captured into a graph and replayed."""
+    max_pages], lens [slots] and refs [pages] are int32.  dtype may be a torch
+    type, or "q8_0" or "q4_0": blocks of 8 or 4 bits, kv then uint8 [layers,
+    pages, page_bytes] in the format `fmt`.  A decoding step is reserve(counts),
+    then append and attend layer by layer; nothing of it waits for the device, so
+    it can be captured into a graph and replayed."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int,
                  max_pages: int, dtype=None, device="cuda"):
         import torch
 
         device = torch.empty(0, device=device).device
-        self.kv = torch.zeros((layers, pages, 2, kv_heads, page_size, head_dim), dtype=dtype or torch.float32,
-                              device=device)
+        self.fmt = PageFormat(dtype, kv_heads, page_size, head_dim) if isinstance(dtype, str) else None
+        if self.fmt is None:
+            self.kv = torch.zeros((layers, pages, 2, kv_heads, page_size, head_dim), dtype=dtype or torch.float32,
+                                  device=device)
+        else:
+            self.kv = torch.zeros((layers, pages, self.fmt.page_bytes), dtype=torch.uint8, device=device)
         self.table = torch.full((slots, max_pages), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(slots, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
@@ -1126,16 +1161,70 @@ class PagedCache:
         return cache_reserve(self.table, self.lens, self.refs, self.page_size, counts)
 
     def append(self, layer: int, k, v, starts, q=None, plan=None, slots=None, out=None):
-        return cache_append(self.kv[layer], self.table, self.lens, starts, k, v, q=q, plan=plan, slots=slots, out=out)
+        return cache_append(self.kv[layer], self.table, self.lens, starts, k, v, q=q, plan=plan, slots=slots, out=out,
+                            fmt=self.fmt)
+
+    def read(self, layer: int, starts, tokens: int, **kw):
+        return cache_read(self.kv[layer], self.table, self.lens, starts, tokens, fmt=self.fmt, **kw)
 
     def attend(self, layer: int, q, starts, **kw):
-        return paged_attention(q, self.kv[layer], self.table, self.lens, starts, **kw)
+        return paged_attention(q, self.kv[layer], self.table, self.lens, starts, fmt=self.fmt, **kw)
 
     def fork(self, src, dst):
-        return cache_fork(self.kv, self.table, self.lens, self.refs, src, dst)
+        return cache_fork(self.kv, self.table, self.lens, self.refs, src, dst, fmt=self.fmt)
+
+    def reorder(self, parents):
+        return cache_reorder(self.kv, self.table, self.lens, self.refs, parents, fmt=self.fmt)
 
     def release(self, slots):
         return cache_release(self.table, self.lens, self.refs, slots, self.page_size)
 
     def compact(self):
-        return cache_compact(self.kv, self.table, self.refs)
+        return cache_compact(self.kv, self.table, self.refs, fmt=self.fmt)
+
+
+# ---------------------------------------------------------------- beam search
+
+
+def beam_select(logits, scores, ended=None, eog=None, out=None, work=None):
+    """The next beams of each group: of all continuations (r, v) of its rows,
+    worth scores[r] + ln softmax(logits[r])[v], the best ones in descending order
+    (of equal ones the lowest).  logits: float32 [groups * beams, V] (or [groups,
+    beams, V]), scores: float32 [groups, beams].  ended (int32 [groups, beams]):
+    beams that stand for themselves alone; eog (int32): the ids that end one.
+
+    Returns (parents, tokens, scores, ended), [groups, beams] each: parents are
+    rows of `logits`, tokens -1 where a beam had ended or there were too few
+    continuations (its score is -infinity then, its parent its own row).  `out`:
+    four such tensors; scores and ended may be those given.  `work`: a
+    preallocated uint8 workspace of nls_beam_workspace() bytes."""
+    import torch
+
+    dev = logits.get_device()
+    groups, beams = scores.shape
+    vocab = logits.shape[-1]
+    if not (dev >= 0 and logits.dtype == torch.float32 and logits.is_contiguous() and
+            logits.numel() == groups * beams * vocab):
+        raise AssertionError("beams: logits float32 [groups * beams, V] on the GPU, contiguous")
+    if not (vocab < 1 << 29 and groups * beams < 1 << 24):
+        raise AssertionError("beams: V below 2^29, fewer than 2^24 rows")
+    if out is None:
+        # (one buffer: an allocation less for each of the others)
+        ints = torch.empty((3, groups, beams), dtype=torch.int32, device=logits.device)
+        out = ints[0], ints[1], torch.empty_like(scores), ints[2]
+    parents, tokens, worth, over = out
+    for x in (scores, worth):
+        if not (x.get_device() == dev and x.dtype == torch.float32 and x.is_contiguous() and x.shape == scores.shape):
+            raise AssertionError("beams: scores float32 [groups, beams], contiguous, on the logits' device")
+    for x in (parents, tokens, over, ended):
+        if x is not None and x.shape != scores.shape:
+            raise AssertionError("beams: parents, tokens and ended of the scores' shape")
+    need = lib().nls_beam_workspace(groups, beams, vocab)
+    if work is None or work.numel() < need:
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=logits.device)
+    elif not (work.get_device() == dev and work.dtype == torch.uint8 and work.is_contiguous()):
+        raise AssertionError("work: uint8, contiguous, on the call's device")
+    _launch(dev, "nls_beam_select", logits.data_ptr(), groups, beams, vocab, scores.data_ptr(), _ints(dev, ended),
+            _ints(dev, eog), 0 if eog is None else eog.numel(), _ints(dev, parents), _ints(dev, tokens),
+            worth.data_ptr(), _ints(dev, over), work.data_ptr(), work.numel())
+    return out

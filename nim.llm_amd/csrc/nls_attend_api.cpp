@@ -426,6 +426,22 @@ int32_t nls_cache_compact(const nls_page_pool* p, const nls_page_tables* t, int3
               "nls_cache_compact");
 }
 
+size_t nls_cache_reorder_workspace(const nls_page_tables* t) {
+  if (check_tables(t, true)) return 0;
+  return align256(4 * (2 + 5 * (size_t)t->slots + (size_t)t->slots * t->max_pages));
+}
+
+int32_t nls_cache_reorder(const nls_page_pool* p, const nls_page_tables* t, const int32_t* d_parents, int32_t* d_status,
+                          void* d_work, size_t work_bytes, void* stream) {
+  NLS_CHECK(check_tables(t, true));
+  NLS_CHECK(check_pool(p, t->pages));
+  if (!d_work || !aligned(d_work, 256) || work_bytes < nls_cache_reorder_workspace(t))
+    return bad("workspace: NULL, misaligned or too small");
+  if (!d_parents || !d_status || !aligned(d_parents, 4) || !aligned(d_status, 4)) return bad("reorder: NULL or misaligned");
+  return done(launch_reorder(pool(p), tables(t), d_parents, d_status, static_cast<int32_t*>(d_work), stream_of(stream)),
+              "nls_cache_reorder");
+}
+
 int32_t nls_cache_copy_pages(const nls_page_pool* p, int32_t pages, const int32_t* d_src, const int32_t* d_dst,
                              int32_t count, void* stream) {
   if (pages < 1 || count < 0) return bad("copy: a size out of range");

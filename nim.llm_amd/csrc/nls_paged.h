@@ -134,6 +134,8 @@ hipError_t launch_fork(const PoolArgs& p, const TableArgs& t, const int32_t* src
                        int32_t* status, int32_t* work, hipStream_t s);
 hipError_t launch_release(const TableArgs& t, const int32_t* slots, int count, int32_t* status, hipStream_t s);
 hipError_t launch_compact(const PoolArgs& p, const TableArgs& t, int32_t* live, int32_t* work, hipStream_t s);
+hipError_t launch_reorder(const PoolArgs& p, const TableArgs& t, const int32_t* src, int32_t* status, int32_t* work,
+                          hipStream_t s);
 hipError_t launch_copy_pages(const PoolArgs& p, int pages, const int32_t* src, const int32_t* dst, int count,
                              hipStream_t s);
 

@@ -43,16 +43,8 @@ __device__ int block_scan(int x, int* sh, int* total) {
   return base + s - x;
 }
 
-// bits[w]: the free pages among 64 w .. 64 w + 63; ranks[w]: how many are free
-// below them.  Returns the number of free pages.
-__device__ int free_bitmap(const int32_t* refs, int pages, uint64_t* bits, int* ranks, int* sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (pages + 63) >> 6;
-  for (int w = wave; w < words; w += kPlanWaves) {
-    const int p = w * 64 + lane;
-    const uint64_t b = __ballot(p < pages && refs[p < pages ? p : 0] == 0);
-    if (lane == 0) bits[w] = b;
-  }
-  __syncthreads();
+// ranks[w]: how many bits of bits[0 .. w) are set.  Returns how many are in all.
+__device__ int rank_bitmap(int words, const uint64_t* bits, int* ranks, int* sh) {
   const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = threadIdx.x * per;
   int n = 0;
   for (int i = 0; i < per; ++i)
@@ -66,6 +58,19 @@ __device__ int free_bitmap(const int32_t* refs, int pages, uint64_t* bits, int* 
     }
   __syncthreads();
   return total;
+}
+
+// bits[w]: the free pages among 64 w .. 64 w + 63; ranks[w]: how many are free
+// below them.  Returns the number of free pages.
+__device__ int free_bitmap(const int32_t* refs, int pages, uint64_t* bits, int* ranks, int* sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (pages + 63) >> 6;
+  for (int w = wave; w < words; w += kPlanWaves) {
+    const int p = w * 64 + lane;
+    const uint64_t b = __ballot(p < pages && refs[p < pages ? p : 0] == 0);
+    if (lane == 0) bits[w] = b;
+  }
+  __syncthreads();
+  return rank_bitmap(words, bits, ranks, sh);
 }
 
 // The r-th free page, r below their number: the last word with no more than r
@@ -384,6 +389,127 @@ __global__ __launch_bounds__(kCopyThreads) void move_kernel(PoolArgs p, TableArg
   copy_pairs(p, t.pages, work + 1, work + 1 + t.pages, work[0], blockIdx.x - table_blocks, gridDim.x - table_blocks);
 }
 
+// Where reorder's work area has what: [0] the status, [1] pairs to copy, then
+// their sources and destinations, each slot's old length, the page its partial
+// last one is copied to (-1: none), its first child, and the old table.
+struct ReorderWork {
+  int32_t *head, *from, *to, *len, *fresh, *first, *rows;
+  __device__ __host__ ReorderWork(int32_t* w, int slots)
+      : head(w), from(w + 2), to(from + slots), len(to + slots), fresh(len + slots), first(fresh + slots),
+        rows(first + slots) {}
+};
+// Pages of a context (whose length may be all that an int holds).
+__device__ __forceinline__ int pages_of(int len, int shift) { return (int)(((uint32_t)len + ((1u << shift) - 1)) >> shift); }
+// (written by this workgroup before a barrier, with atomics among it)
+__device__ __forceinline__ int settled(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// What goes where.  A page is free for a copy when nobody held it, or only
+// slots whose contexts end here: it is marked by those, and the mark is taken off
+// by every row as it will be.
+__global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, const int32_t* src, int32_t* status,
+                                                               int32_t* work) {
+  __shared__ int sh[kPlanWaves];
+  const PlanLds lds = plan_lds(t.pages);
+  const ReorderWork w(work, t.slots);
+  const int mask = (1 << t.page_shift) - 1;
+  int bad = 0;
+  for (int s = threadIdx.x; s < t.slots; s += kPlanThreads) {
+    const int len = t.lens[s], p = src[s];
+    if (p < -1 || p >= t.slots || len < 0 || ((int64_t)len + mask) >> t.page_shift > t.max_pages) bad = 1;
+    w.len[s] = len;
+    __hip_atomic_store(&w.first[s], t.slots, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  bad = __syncthreads_or(bad);
+  if (bad) {
+    if (threadIdx.x == 0) *status = w.head[0] = 3;
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (t.pages + 63) >> 6;
+  for (int i = wave; i < words; i += kPlanWaves) {
+    const int p = i * 64 + lane;
+    const uint64_t b = __ballot(p < t.pages && t.refs[p < t.pages ? p : 0] == 0);
+    if (lane == 0) lds.bits[i] = b;
+  }
+  // the partial page of a parent stays with itself, else with its first child
+  for (int s = threadIdx.x; s < t.slots; s += kPlanThreads)
+    if (src[s] >= 0) atomicMin(&w.first[src[s]], src[s] == s ? -1 : s);
+  __syncthreads();
+  const uint32_t all = (uint32_t)t.slots * (uint32_t)t.max_pages, per = t.max_pages;  // (below 2^31)
+  uint32_t* marks = reinterpret_cast<uint32_t*>(lds.bits);
+  for (uint32_t e = threadIdx.x; e < all; e += kPlanThreads) {
+    const int s = (int)(e / per), j = (int)(e % per);
+    if (j >= pages_of(w.len[s], t.page_shift)) continue;
+    const int page = t.table[s * t.table_stride + j];
+    w.rows[e] = page;
+    if (src[s] != s && (uint32_t)page < (uint32_t)t.pages) atomicOr(&marks[page >> 5], 1u << (page & 31));
+  }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < all; e += kPlanThreads) {
+    const int s = (int)(e / per), j = (int)(e % per), p = src[s];
+    if (p < 0) continue;
+    const int len = w.len[p], whole = len >> t.page_shift;
+    const int first = settled(&w.first[p]);
+    if (j >= whole + ((len & mask) != 0 && (first == s || p == s))) continue;
+    const int page = t.table[p * t.table_stride + j];
+    if ((uint32_t)page < (uint32_t)t.pages) atomicAnd(&marks[page >> 5], ~(1u << (page & 31)));
+  }
+  __syncthreads();
+  const int free_pages = rank_bitmap(words, lds.bits, lds.ranks, sh);
+  int total = 0;
+  for (int s0 = 0; s0 < t.slots; s0 += kPlanThreads) {
+    const int s = s0 + threadIdx.x;
+    int copies = 0, p = -1;
+    if (s < t.slots && (p = src[s]) >= 0)
+      copies = (w.len[p] & mask) != 0 && p != s && settled(&w.first[p]) != s;
+    int sum;
+    const int r = total + block_scan(copies, sh, &sum);
+    if (s < t.slots) {
+      int mine = -1;
+      if (copies && r < free_pages) {
+        mine = free_page(lds.bits, lds.ranks, t.pages, r);
+        w.from[r] = t.table[p * t.table_stride + (w.len[p] >> t.page_shift)];
+        w.to[r] = mine;
+      }
+      w.fresh[s] = mine;
+    }
+    total += sum;
+  }
+  if (threadIdx.x == 0) {
+    const int st = free_pages < total ? 1 : 0;
+    *status = w.head[0] = st;
+    w.head[1] = st ? 0 : total;
+  }
+}
+
+// The tables as planned, and the copies.
+__global__ __launch_bounds__(kCopyThreads) void reorder_apply_kernel(PoolArgs p, TableArgs t, const int32_t* src,
+                                                                     int32_t* work, int table_blocks) {
+  const ReorderWork w(work, t.slots);
+  if (w.head[0]) return;
+  if ((int)blockIdx.x >= table_blocks) {
+    copy_pairs(p, t.pages, w.from, w.to, w.head[1], blockIdx.x - table_blocks, gridDim.x - table_blocks);
+    return;
+  }
+  const uint32_t n = (uint32_t)t.slots * (uint32_t)t.max_pages, per = t.max_pages;  // (below 2^31)
+  for (uint32_t e = blockIdx.x * kCopyThreads + threadIdx.x; e < n; e += table_blocks * kCopyThreads) {
+    const int s = (int)(e / per), j = (int)(e % per), from = src[s];
+    if (from == s) continue;
+    const int had = pages_of(w.len[s], t.page_shift), len = from < 0 ? 0 : w.len[from];
+    const int whole = len >> t.page_shift, has = pages_of(len, t.page_shift);
+    if (j == 0) t.lens[s] = len;
+    if (j >= had && j >= has) continue;
+    const int was = j < had ? w.rows[e] : -1;
+    int page = -1;
+    if (j < has) page = j < whole || w.fresh[s] < 0 ? w.rows[(int64_t)from * t.max_pages + j] : w.fresh[s];
+    if (page == was) continue;
+    t.table[(int64_t)s * t.table_stride + j] = page;
+    if ((uint32_t)was < (uint32_t)t.pages) atomicSub(&t.refs[was], 1);
+    if ((uint32_t)page < (uint32_t)t.pages) atomicAdd(&t.refs[page], 1);
+  }
+}
+
 hipError_t allow_lds(const void* f, int pages) {
   const size_t n = plan_lds_bytes(pages);
   return n > 32000 ? hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)n) : hipSuccess;
@@ -430,6 +556,18 @@ hipError_t launch_compact(const PoolArgs& p, const TableArgs& t, int32_t* live, 
   const int tb = (int)(entries < 1 ? 0 : entries > 64 * kCopyThreads * 8 ? 64 : (entries + kCopyThreads * 8 - 1) / (kCopyThreads * 8));
   // (at most half of the pages move)
   move_kernel<<<tb + copy_blocks(copy_items(p, (t.pages + 1) / 2)), kCopyThreads, 0, s>>>(p, t, work, tb);
+  return hipGetLastError();
+}
+
+hipError_t launch_reorder(const PoolArgs& p, const TableArgs& t, const int32_t* src, int32_t* status, int32_t* work,
+                          hipStream_t s) {
+  hipError_t e = allow_lds(reinterpret_cast<const void*>(reorder_kernel), t.pages);
+  if (e != hipSuccess) return e;
+  reorder_kernel<<<1, kPlanThreads, plan_lds_bytes(t.pages), s>>>(t, src, status, work);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const int64_t entries = (int64_t)t.slots * t.max_pages;
+  const int tb = (int)(entries > 256 * kCopyThreads ? 256 : (entries + kCopyThreads - 1) / kCopyThreads);
+  reorder_apply_kernel<<<tb + copy_blocks(copy_items(p, t.slots)), kCopyThreads, 0, s>>>(p, t, src, work, tb);
   return hipGetLastError();
 }
 

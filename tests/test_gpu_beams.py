@@ -1,0 +1,338 @@
+"""Beam search: the selection over beams and vocabulary, the contexts that
+follow it, and both together over a cache, against their definitions."""
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import quant_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+# ---------------------------------------------------------------- selection
+
+
+def select(logits, scores, ended=None, eog=()):
+    """The definition in float64, group by group: parents, tokens, scores, ended;
+    and how near the nearest two candidates of different rows are among the
+    first beams + 1."""
+    groups, beams = scores.shape
+    x = logits.astype(np.float64).reshape(groups, beams, -1)
+    out = [np.zeros((groups, beams), dtype=t) for t in (np.int64, np.int64, np.float64, np.int64)]
+    gap = math.inf
+    for g in range(groups):
+        all_ = []
+        for b in range(beams):
+            s = float(scores[g, b])
+            if not s > -math.inf:
+                continue
+            if ended is not None and ended[g, b]:
+                all_.append((-s, b, -1))
+                continue
+            row = np.where(np.isnan(x[g, b]), -np.inf, x[g, b])
+            m = row.max()
+            if m == -np.inf:
+                continue
+            d = np.where(row == m, 0.0, row - m)
+            c = d - math.log(np.exp(d).sum()) + s
+            near = np.argsort(-c, kind="stable")[:beams + 1]
+            all_ += [(-c[v], b, int(v)) for v in near if c[v] > -np.inf]
+        all_.sort()
+        for one, two in zip(all_[:beams], all_[1:beams + 1]):
+            if one[1] != two[1] and one[0] != two[0]:
+                gap = min(gap, two[0] - one[0])
+        for j in range(beams):
+            if j < len(all_):
+                c, b, v = all_[j]
+                done = (ended is not None and bool(ended[g, b])) or v in eog
+                out[0][g, j], out[1][g, j], out[2][g, j], out[3][g, j] = g * beams + b, v, -c, done
+            else:
+                out[0][g, j], out[1][g, j], out[2][g, j] = g * beams + j, -1, -math.inf
+    return out, gap
+
+
+# A row's sum: 32 terms of 2^-22 each one after another and 9 more sums in fp32,
+# the rest in float64; then one rounding of the score.
+LSE = 2.0 ** -22 + 41 * 2.0 ** -24
+
+
+def check(pkg, logits, scores, ended=None, eog=(), **kw):
+    (parents, tokens, worth, over), gap = select(logits, scores, ended, set(eog))
+    assert gap > 2 * LSE, gap  # else the order were not decided
+    to = lambda a, t: None if a is None else torch.from_numpy(np.ascontiguousarray(a, dtype=t)).cuda()
+    got = pkg.beam_select(to(logits, np.float32), to(scores, np.float32), ended=to(ended, np.int32),
+                          eog=to(list(eog), np.int32) if eog else None, **kw)
+    p, t, s, e = (x.cpu().numpy() for x in got)
+    assert np.array_equal(p, parents) and np.array_equal(t, tokens) and np.array_equal(e, over)
+    live = np.isfinite(worth)
+    assert np.array_equal(s[~live], worth[~live])
+    assert (np.abs(s[live] - worth[live]) <= LSE + 2.0 ** -24 * np.abs(worth[live]) * (1 + LSE)).all()
+    return got
+
+
+def made(seed, groups, beams, vocab, spread=3.0):
+    g = np.random.default_rng(seed)
+    return (g.standard_normal((groups * beams, vocab)) * spread).astype(np.float32), \
+        (g.standard_normal((groups, beams)) * 2 - 30).astype(np.float32)
+
+
+@pytest.mark.parametrize("groups,beams,vocab", [(1, 1, 1), (1, 2, 1), (3, 4, 2), (2, 5, 7), (1, 4, 32000), (5, 3, 8191),
+                                                (2, 8, 8192), (2, 8, 8193), (1, 64, 1000), (2, 16, 50257), (3, 2, 300),
+                                                (1, 64, 50), (1, 7, 151936), (40, 2, 999), (1, 1, 100001)])
+def test_selection(pkg, groups, beams, vocab):
+    say(f"[beams] {groups}x{beams}x{vocab}")
+    logits, scores = made(groups * 1000 + beams + vocab, groups, beams, vocab)
+    check(pkg, logits, scores)
+    rng = np.random.default_rng(1)
+    ended = (rng.random((groups, beams)) < 0.4).astype(np.int32)
+    check(pkg, logits, scores, ended)
+    eog = sorted({0, vocab - 1, int(logits.reshape(-1, vocab)[0].argmax())})
+    check(pkg, logits, scores, ended, eog)
+
+
+def test_first_step(pkg):
+    """One live beam a group: its best continuations, also beyond what the merge
+    holds at a time."""
+    for beams, vocab in ((4, 32000), (32, 128256), (64, 300001), (64, 70)):
+        logits, scores = made(beams, 2, beams, vocab)
+        scores[:] = -np.inf
+        scores[0, 0] = scores[1, beams - 1] = 0.0
+        check(pkg, logits, scores)
+
+
+@pytest.mark.parametrize("beams,vocab", [(4, 3), (8, 5000), (64, 40000), (5, 20000)])
+def test_equal_candidates_go_by_the_lowest(pkg, beams, vocab):
+    logits, scores = np.zeros((2 * beams, vocab), dtype=np.float32), np.full((2, beams), -3.0, dtype=np.float32)
+    check(pkg, logits, scores)
+    logits[:, vocab // 2:] = 1.0
+    check(pkg, logits, scores)
+    logits[:, ::3] = 2.0  # many of them on each bound
+    check(pkg, logits, scores)
+    # ended beams worth as much as continuations of others
+    logits[:] = -np.inf
+    logits[:, vocab - 1] = 5.0
+    check(pkg, logits, scores, np.tile(np.arange(beams) % 2, (2, 1)))
+
+
+def test_unusual_logits_and_scores(pkg):
+    beams, vocab = 4, 9001
+    logits, scores = made(3, 6, beams, vocab)
+    x = logits.reshape(6, beams, vocab)
+    x[0, 0, ::2] = -np.inf
+    x[0, 1] = -np.inf
+    x[0, 2, 5:] = np.nan
+    x[0, 3] = np.nan
+    x[1, :, 1:] = -np.inf          # one candidate each
+    x[2] = -np.inf                 # none
+    x[3, 0, 77] = x[3, 0, 8500] = np.inf
+    x[3, 1, :] = np.inf
+    x[4, 2] = 3e38
+    x[4, 3] = -3e38
+    scores[5] = [np.nan, -np.inf, -1.0, 0.0]
+    check(pkg, logits, scores)
+    x[:, :, 4096:] = -np.inf       # a slice without any
+    check(pkg, logits, scores)
+
+
+def test_far_scores_and_steep_rows(pkg):
+    logits, scores = made(9, 3, 6, 40000, spread=300.0)
+    check(pkg, logits, scores)
+    logits, scores = made(10, 3, 6, 40000, spread=1e-3)
+    scores = scores * 1e4
+    check(pkg, logits, scores)
+
+
+def test_scores_and_ended_in_place(pkg):
+    logits, scores = made(5, 7, 8, 12345)
+    rng = np.random.default_rng(2)
+    ended = (rng.random((7, 8)) < 0.3).astype(np.int32)
+    want = check(pkg, logits, scores, ended, [5, 17])
+    x, s, e = torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda(), torch.from_numpy(ended).cuda()
+    p, t = torch.empty_like(e), torch.empty_like(e)
+    work = torch.empty(pkg.lib().nls_beam_workspace(7, 8, 12345), dtype=torch.uint8, device="cuda")
+    got = pkg.beam_select(x.view(7, 8, -1), s, ended=e, eog=torch.tensor([5, 17], dtype=torch.int32).cuda(), out=(p, t, s, e), work=work)
+    assert got[2] is s and got[3] is e
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_rows_off_16_bytes(pkg):
+    logits, scores = made(6, 2, 3, 10007)
+    want = check(pkg, logits, scores)
+    far = torch.zeros(logits.size + 3, device="cuda")
+    far[3:] = torch.from_numpy(logits).cuda().view(-1)
+    got = pkg.beam_select(far[3:].view(6, 10007), torch.from_numpy(scores).cuda())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- contexts follow
+
+
+class Model:
+    """The page tables by their rules, and what every place of every slot's
+    context holds (a number per token, the same in all layers)."""
+
+    def __init__(self, slots, per, pages, ps):
+        self.per, self.ps = per, ps
+        self.table, self.lens, self.refs = [[-1] * per for _ in range(slots)], [0] * slots, [0] * pages
+        self.held = [[] for _ in range(slots)]
+
+    def lowest(self):
+        return self.refs.index(0)
+
+    def reserve(self, counts, tokens):
+        for s, n in enumerate(counts):
+            for j in range(-(-self.lens[s] // self.ps), -(-(self.lens[s] + n) // self.ps)):
+                p = self.lowest()
+                self.table[s][j], self.refs[p] = p, 1
+            self.lens[s] += n
+            self.held[s] = self.held[s] + tokens[s]
+
+    def reorder(self, src):
+        ps, slots = self.ps, range(len(src))
+        refs, new, copies = list(self.refs), [], []
+        first = {}
+        for s in slots:
+            if src[s] >= 0 and (src[s] not in first or src[s] == s):
+                if first.get(src[s]) != src[s]:
+                    first[src[s]] = s
+        for s in slots:
+            for p in self.table[s]:
+                if p >= 0:
+                    refs[p] -= 1
+        for s in slots:
+            row = [-1] * self.per
+            if src[s] >= 0:
+                n = self.lens[src[s]]
+                keep = -(-n // ps) if first[src[s]] == s else n // ps
+                row[:keep] = self.table[src[s]][:keep]
+                for p in row[:keep]:
+                    refs[p] += 1
+                if n % ps and first[src[s]] != s:
+                    copies.append((s, n // ps))
+            new.append(row)
+        if refs.count(0) < len(copies):
+            return 1
+        for s, j in copies:
+            p = refs.index(0)
+            new[s][j], refs[p] = p, 1
+        self.lens = [self.lens[p] if p >= 0 else 0 for p in src]
+        self.held = [list(self.held[p]) if p >= 0 else [] for p in src]
+        self.table, self.refs = new, refs
+        return 0
+
+    def same(self, c):
+        assert c.lens.tolist() == self.lens
+        assert c.table.tolist() == self.table
+        assert c.refs.tolist() == self.refs
+
+
+def put(c, m, counts):
+    """The new tokens' numbers into every layer of the cache."""
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    x = [t for s, n in enumerate(counts) for t in m.held[s][len(m.held[s]) - n:]]
+    kvh, d = (c.fmt.kv_heads, c.fmt.head_dim) if c.fmt else (c.kv.shape[3], c.kv.shape[5])
+    k = torch.tensor(x, dtype=torch.float32).view(-1, 1, 1).expand(-1, kvh, d).contiguous().cuda()
+    for layer in range(c.kv.shape[0]):
+        c.append(layer, k + layer, -k, torch.from_numpy(starts).cuda())
+
+
+def holds(c, m):
+    """Every context is what its history says, in every layer."""
+    starts = torch.from_numpy(np.concatenate([[0], np.cumsum(m.lens)]).astype(np.int32)).cuda()
+    want = np.array([t for h in m.held for t in h], dtype=np.float32)
+    for layer in range(c.kv.shape[0]):
+        k, v = (x.cpu().numpy() for x in c.read(layer, starts, len(want)))
+        for got, w in ((k, want + layer), (v, -want)):
+            if c.fmt:  # equal elements of a block: one factor, one code
+                w = R.values(*R.blocks(np.repeat(w[:, None], 32, 1), c.fmt.kind))[:, 0]
+            else:
+                w = torch.from_numpy(w).to(c.kv.dtype).double().numpy()
+            assert (got == w[:, None, None]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, "q8_0", "q4_0"], ids=str)
+@pytest.mark.parametrize("slots,per,pages,ps,layers", [(4, 6, 30, 16, 2), (12, 9, 120, 16, 1), (1, 3, 4, 32, 3), (33, 4, 140, 16, 1)])
+def test_contexts_follow(pkg, dtype, slots, per, pages, ps, layers):
+    rng = random.Random(slots)
+    c = pkg.PagedCache(layers, pages, ps, 2, 32, slots, per, dtype=dtype)
+    m = Model(slots, per, pages, ps)
+    for step in range(25):
+        counts = [rng.choice([0, 1, 1, 2, 5, ps]) if n + ps <= per * ps else 0 for n in m.lens]
+        need = sum(-(-(n + k) // ps) - -(-n // ps) for n, k in zip(m.lens, counts))
+        if m.refs.count(0) >= need:
+            m.reserve(counts, [[float(rng.randint(1, 99)) for _ in range(k)] for k in counts])
+            assert c.reserve(torch.tensor(counts, dtype=torch.int32).cuda()).item() == 0
+            put(c, m, counts)
+        kind = step % 5
+        src = [rng.randrange(slots) for _ in range(slots)]
+        if kind == 1:
+            src = [s if rng.random() < 0.7 else rng.randrange(-1, slots) for s in range(slots)]
+        elif kind == 2:
+            src = [slots - 1 - s for s in range(slots)]  # all change places
+        elif kind == 3:
+            src = [rng.randrange(slots)] * slots         # all go on from one
+        elif kind == 4 and step > 20:
+            src = [-1] * slots
+        say(f"[reorder] step {step} {src}")
+        st = m.reorder(src)
+        got = c.reorder(torch.tensor(src, dtype=torch.int32).cuda()).item()
+        assert got == st
+        m.same(c)
+        holds(c, m)
+
+
+def test_reorder_does_all_or_nothing(pkg):
+    c = pkg.PagedCache(1, 5, 16, 1, 32, 3, 4)
+    c.reserve(torch.tensor([20, 5, 5], dtype=torch.int32).cuda())  # 4 of 5 pages
+    state = [x.clone() for x in (c.table, c.lens, c.refs, c.kv)]
+    same = lambda: all(torch.equal(a, b) for a, b in zip(state, (c.table, c.lens, c.refs, c.kv)))
+    go = lambda *src: c.reorder(torch.tensor(src, dtype=torch.int32).cuda()).item()
+    for src in ((0, 1, 3), (-2, 1, 2), (0, 1, 1 << 30)):
+        assert go(*src) == pkg.PAGES_BAD_ENTRY and same()
+    c.refs[4] = 1  # held by someone else
+    state[2] = c.refs.clone()
+    assert go(0, 0, 2) == pkg.PAGES_DONE  # slot 1's page serves the copy
+    assert c.refs.tolist() == [2, 1, 1, 1, 1] and c.lens.tolist() == [20, 20, 5]
+    state = [x.clone() for x in (c.table, c.lens, c.refs, c.kv)]
+    assert go(0, 1, 0) == pkg.PAGES_DONE
+    assert c.refs.tolist() == [3, 1, 1, 1, 1]
+    c.lens[1] = -1
+    state = [x.clone() for x in (c.table, c.lens, c.refs, c.kv)]
+    assert go(0, 0, 0) == pkg.PAGES_BAD_ENTRY and same()
+    c.lens[1] = 4 * 16 + 1
+    state[1] = c.lens.clone()
+    assert go(0, 0, 0) == pkg.PAGES_BAD_ENTRY and same()
+    # none left: two contexts with partial pages, all pages held
+    c = pkg.PagedCache(1, 3, 16, 1, 32, 3, 2)
+    c.reserve(torch.tensor([5, 5, 0], dtype=torch.int32).cuda())
+    c.refs[2] = 7
+    state = [x.clone() for x in (c.table, c.lens, c.refs, c.kv)]
+    assert go(0, 1, 1) == pkg.PAGES_NONE_LEFT and same()
+    assert go(0, -1, 0) == pkg.PAGES_DONE and c.refs.tolist() == [1, 1, 7]
+
+
+def test_reorder_many_slots(pkg):
+    """More slots than the plan's threads, long rows, pages shared by many."""
+    slots, per, ps = 2500, 7, 16
+    c = pkg.PagedCache(1, 9000, ps, 1, 32, slots, per, dtype="q4_0")
+    m = Model(slots, per, 9000, ps)
+    rng = random.Random(8)
+    counts = [rng.choice([0, 3, 16, 40]) for _ in range(slots)]
+    m.reserve(counts, [[float(rng.randint(1, 99)) for _ in range(k)] for k in counts])
+    assert c.reserve(torch.tensor(counts, dtype=torch.int32).cuda()).item() == 0
+    put(c, m, counts)
+    for _ in range(2):
+        src = [rng.randrange(max(-1, s // 8 * 8 - 1), min(slots, s // 8 * 8 + 8)) for s in range(slots)]
+        assert m.reorder(src) == 0
+        assert c.reorder(torch.tensor(src, dtype=torch.int32).cuda()).item() == 0
+        m.same(c)
+        holds(c, m)
