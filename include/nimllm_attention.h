@@ -149,8 +149,8 @@ typedef struct nls_chunks {
  * Blocks (type is then any of the three): the turned elements, unrounded, give
  *   Q8_0  d = fp16(max |x| * (1 / 127)),                  c = rint(x * (1 / d))
  *   Q4_0  d = fp16(max(max x * (1 / 7), min x * (-1 / 8))), c within -8 .. 7
- * in fp32, each operation rounded once (d at most 65504: larger elements are
- * cut; all c are 0 where d is 0).  A block with an element that is not finite
+ * in fp32, each operation rounded once.  d is at most 515.5 and 8188, so that
+ * fp16 holds d c: elements beyond its range are cut.  All c are 0 where d is 0.  A block with an element that is not finite
  * has d = NaN.
  */
 int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const nls_rope_plan* plan, int32_t type,

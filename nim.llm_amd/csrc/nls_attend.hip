@@ -162,7 +162,7 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
   int64_t longest = max_new > 0 && max_new < a.p.tokens ? max_new : a.p.tokens;
   if (a.window > 0 && most > (int64_t)a.window + longest) most = (int64_t)a.window + longest;
   const size_t per_row = D * sizeof(float) + sizeof(f4);
-  p.chunk = longest > 1 && longest * a.group > 16 && !quant_type(a.cache_type);
+  p.chunk = longest > 1 && longest * a.group > 16;
   // One sequence that may be a chunk is taken for one: its rows are few only
   // where the others belong to no sequence.
   p.few = !(p.chunk && a.p.seqs == 1);
@@ -266,9 +266,10 @@ hipError_t attend_quant_width(const AttendArgs& a, const AttendPlan& p, int type
                               hipStream_t s) {
   const Parts few = placed(p.few_parts, work, D);
   const Parts chunk = placed(p.chunk_parts, work + (p.few_bytes + 255) / 256 * 256, D);
-  const hipError_t e = p.few ? launch_few_quant(a, type, cache_type, few, p.few_tiles, p.chunk, s) : hipSuccess;
-  if (e != hipSuccess) return e;
-  return join<T, D>(a, p, few, chunk, kQuantShift, kQuantShift, s);
+  hipError_t e;
+  if (p.few && (e = launch_few_quant(a, type, cache_type, few, p.few_tiles, p.chunk, s)) != hipSuccess) return e;
+  if (p.chunk && (e = launch_chunk_quant(a, type, cache_type, chunk, p.chunk_tiles, !p.few, s)) != hipSuccess) return e;
+  return join<T, D>(a, p, few, chunk, kQuantShift, chunk_shift<_Float16>(), s);
 }
 
 template <typename T>

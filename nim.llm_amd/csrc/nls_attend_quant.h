@@ -406,5 +406,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 // Launched by launch_attend (nls_attend.hip), which joins the parts.
 hipError_t launch_few_quant(const AttendArgs& a, int type, int cache_type, const Parts& parts, int few_tiles,
                             bool chunk_runs, hipStream_t s);
+hipError_t launch_chunk_quant(const AttendArgs& a, int type, int cache_type, const Parts& parts, int64_t tiles,
+                              bool alone, hipStream_t s);
 
 }  // namespace nls

@@ -239,7 +239,7 @@ __device__ __forceinline__ void over_block(float& hi, float& lo, int& odd) {
 template <int kBits>
 __device__ __forceinline__ _Float16 factor_of(float hi, float lo, int odd, float* step) {
   const float t = kBits == 8 ? fmaxf(hi, -lo) * 0.007874015718698502f : fmaxf(hi * 0.1428571492433548f, lo * -0.125f);
-  const _Float16 d = (_Float16)fminf(t, 65504.f);
+  const _Float16 d = (_Float16)fminf(t, kBits == 8 ? 515.5f : 8188.f);  // (so that fp16 holds d c)
   *step = (float)d > 0.f ? 1.f / (float)d : 0.f;
   return odd ? (_Float16)__builtin_nanf("") : d;
 }

@@ -20,7 +20,7 @@ def blocks(x, kind):
             t, low, high = np.maximum(hi, -lo) * (np.float32(1) / np.float32(127)), -127, 127
         else:
             t, low, high = np.maximum(hi * (np.float32(1) / np.float32(7)), lo * np.float32(-0.125)), -8, 7
-        d = np.minimum(t, np.float32(65504)).astype(np.float16)
+        d = np.minimum(t, np.float32(515.5 if kind == "q8_0" else 8188)).astype(np.float16)  # (fp16 holds d c)
         step = np.where(d > 0, np.float32(1) / d.astype(np.float32), np.float32(0)).astype(np.float32)
         c = np.clip(np.nan_to_num(np.rint(b * step[..., None]), nan=low, posinf=high, neginf=low), low, high)
         d = np.where(np.isfinite(b).all(-1), d, np.float16(np.nan))
