@@ -24,19 +24,37 @@ __device__ __forceinline__ uint32_t less(uint32_t x, float by) {
   const h2 r = __builtin_bit_cast(h2, x) - h2{(_Float16)by, (_Float16)by};
   return __builtin_bit_cast(uint32_t, r);
 }
-__device__ __forceinline__ uint32_t low_nibbles(uint32_t x) { return less((x & 0x000f000fu) | 0x64006400u, 1032.f); }
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t x) { return less((x & 0x00f000f0u) | 0x54005400u, 72.f); }
+// (a number that the compiler does not know is one register and one instruction
+// with the mask; a constant would be an instruction of its own)
+template <uint32_t kWord>
+__device__ __forceinline__ uint32_t word() {
+  uint32_t x;
+  asm("v_mov_b32 %0, %1" : "=v"(x) : "i"(kWord));
+  return x;
+}
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t x) { return less((x & 0x000f000fu) | word<0x64006400u>(), 1032.f); }
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t x) { return less((x & 0x00f000f0u) | word<0x54005400u>(), 72.f); }
 
 // (a value, not an element of a vector: of that __builtin_bit_cast takes the
 // vector's first)
 __device__ __forceinline__ h2 halves(uint32_t x) { return __builtin_bit_cast(h2, x); }
 
-// A product as the fp32 number that it is: where it is split, the compiler else
-// rounds it to fp16 from its factors for one part and from fp32 for the other,
-// and in one of some thousands the two do not belong together.
-__device__ __forceinline__ float settled(float x) {
-  asm("" : "+v"(x));
-  return x;
+// Eight numbers as two halves each.  The first is what both come from: let alone,
+// the compiler rounds a product to fp16 from its factors for one and from fp32
+// for the other, and in one of some thousands the two do not belong together.
+__device__ __forceinline__ void in_two(const float* x, h8* p) {
+  u4 hi, lo;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    uint32_t r = __builtin_bit_cast(uint32_t, h2{(_Float16)x[2 * n], (_Float16)x[2 * n + 1]});
+    asm("" : "+v"(r));
+    const h2 h = halves(r);
+    const h2 rest{(_Float16)__builtin_fmaf((float)h[0], -1.f, x[2 * n]), (_Float16)__builtin_fmaf((float)h[1], -1.f, x[2 * n + 1])};
+    hi[n] = r;
+    lo[n] = __builtin_bit_cast(uint32_t, rest);
+  }
+  p[0] = __builtin_bit_cast(h8, hi);
+  p[1] = __builtin_bit_cast(h8, lo);
 }
 
 // A key unit's 8 elements.
@@ -65,23 +83,40 @@ __device__ __forceinline__ uint32_t value_codes(const uint32_t* a, const uint32_
   return h ? high_nibbles(pair) : low_nibbles(pair);
 }
 
-// fp32 queries and weights times factors: two fp16 parts, 22 bits.  16-bit ones:
-// one, which holds fp16 and bf16 queries whole and 11 bits of a weight.
+// fp32 queries are two fp16 parts, 22 bits; one holds fp16 and bf16 queries whole.
 template <typename T>
 constexpr int quant_parts() {
   return sizeof(T) == 4 ? 2 : 1;
 }
+// Weights times factors, likewise; for bf16 queries they are rounded to fp16 (an
+// eighth of the output's own step).
+template <typename T>
+constexpr int weight_parts() {
+  return __is_same(T, __bf16) ? 1 : 2;
+}
+// Numbers and truth values as types.
+template <int N>
+struct Nth {
+  __device__ constexpr operator int() const { return N; }
+};
+template <bool B>
+struct Is {
+  __device__ constexpr operator bool() const { return B; }
+};
+
 constexpr float kQuantShift = 14.f;  // log2 of the largest weight times factor
 
 // kPad: heads of fewer than GT blocks
 template <typename T, int kBits, int GT, bool kPad>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,
                                                int group_at, int part) {
-  constexpr int NP = quant_parts<T>(), D = 32 * GT, kWaves = 4, kThreads = 256;
+  constexpr int NP = quant_parts<T>(), NW = weight_parts<T>(), D = 32 * GT, kWaves = 4, kThreads = 256;
   constexpr int KW = kBits / 4;                       // words of a key unit
+  constexpr int kWide = GT < 4 ? GT : 4;              // blocks of a plane
   constexpr int VW = (GT * kBits / 4 + 3) / 4;        // words of a lane's piece of a value row
   extern __shared__ float quant_lds[];                // [wave][16][D + 4] sums
   __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
+  __shared__ __align__(16) uint32_t sh_f[kWaves][32 * GT];  // a step's factors, of keys, then of values: [2 GT][32 tokens]
 
   const int kvh = group_at % a.p.kv_heads, task = group_at / a.p.kv_heads;
   const int seq = task / tiles, tile = task - seq * tiles;
@@ -115,14 +150,25 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
                      (int64_t)(kvh * a.group + row % a.group) * a.q.head_stride;
       float x[GT][8], top = 0.f;
+      const bool wide = ((reinterpret_cast<uintptr_t>(a.q.d) / sizeof(T) | (uint64_t)a.q.token_stride | (uint64_t)a.q.head_stride) &
+                         (16 / sizeof(T) - 1)) == 0;
 #pragma unroll
-      for (int b = 0; b < GT; ++b)
+      for (int b = 0; b < GT; ++b) {
+        T y[8];
+        if (!kPad || b < groups) {
+          if (wide) {
+            __builtin_memcpy(y, __builtin_assume_aligned(src + b * 32 + g * 8, 16), sizeof y);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = src[b * 32 + g * 8 + j];
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int d = b * 32 + g * 8 + j;
-          x[b][j] = row_ok && d < dim ? (float)src[d] : 0.f;
+          x[b][j] = row_ok && (!kPad || b < groups) ? (float)y[j] : 0.f;
           top = fmaxf(top, fabsf(x[b][j]));
         }
+      }
       int e = 0;
       if constexpr (!__is_same(T, _Float16)) {
         top = fmaxf(top, __shfl_xor(top, 16));
@@ -140,24 +186,21 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     f4 o[2 * GT];
 #pragma unroll
     for (int t = 0; t < 2 * GT; ++t) o[t] = f4{0, 0, 0, 0};
-    // The weights are taken from m + up: `up` is a power of two no less than any
-    // value's factor so far, so that a weight times a factor is at most 1.
-    float m = minus_inf(), l = 0.f, most = 0.f;  // (most = 2^up, or 0)
-    float up = -24.f;                            // (fp16's least number is 2^-24)
+    // The weights are taken from m + up: 2^up is above any value's factor so far,
+    // so that a weight times a factor is at most 1.  (One part: not below 2^0, so
+    // that the weight itself is too.)  most: that bound as fp16's bits.
+    float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f;
+    uint32_t most = NW == 1 ? 0x3bffu : 0u;
 
-    // A step's 32 keys are two runs of 16, each within a page: its first byte of
-    // this head, in the same registers for the wave.
-    struct Step {
-      const char* at[2];
-      bool there[2];
+    // A step's 32 keys are two runs of 16, each within a page (-1: none; what is
+    // read there is page 0, and counts for nothing).
+    struct Pages {
+      int at[2];
     };
     const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
     const char* base = static_cast<const char*>(a.p.kv) + quant_base(shape, kvh, 0);
-    struct Entries {
-      int at[2];
-    };
     auto entries_at = [&](int kb) {
-      Entries e;
+      Pages e;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int key = kb + s * 16;
@@ -165,55 +208,72 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       }
       return e;
     };
-    auto step_of = [&](int kb, const Entries& e) {
-      Step p;
+    auto pages_of = [&](int kb, const Pages& e) {
+      Pages p;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int page = __builtin_amdgcn_readfirstlane(e.at[s]);
-        p.there[s] = kb + s * 16 < k1 && (uint32_t)page < (uint32_t)a.p.pages;
-        p.at[s] = base + (int64_t)(p.there[s] ? page : 0) * a.p.page_stride;
+        p.at[s] = kb + s * 16 < k1 && (uint32_t)page < (uint32_t)a.p.pages ? page : -1;
       }
       return p;
     };
-    uint32_t kc[2][GT][KW], vc[8][VW];
-    u2 kd[2][GT], vd[2][GT];  // factors of 4 keys
-    auto fetch_k = [&](int kb, const Step& p) {
+    auto home = [&](int page) { return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride; };
+
+    // Two steps of a wave are on their way while one is worked on.
+    uint32_t kc[2][2][GT][KW], vc[2][8][VW];
+    // A lane's factors: GT tokens' of one block, keys' for the first 32 lanes and
+    // values' for the others; 16 lanes of the operands want each, out of LDS.
+    constexpr int FW = GT / 2, kAcross = 32 / GT;
+    uint32_t fc[2][FW];
+    Pages page[2], entry[2];  // of the steps in flight; of those behind them
+    const int f_x = lane / kAcross % GT, f_token = lane % kAcross * GT;
+    const bool f_there = !kPad || f_x < groups;
+    uint32_t* factors = sh_f[wave];
+    // (one address for the wave and 32 bits for the lane)
+    const uint32_t lane_k = i * row_bytes + g * groups * kBits, lane_v = g * 4 * row_bytes + (kPad ? 0 : i * kWide * kBits / 4);
+    const uint32_t lane_f = (lane < 32 ? 0 : shape.half) + shape.codes + ((f_there ? f_x : 0) * size + (f_token & 15)) * 2;
+    auto fetch_k = [&](auto set, int kb) {
+      constexpr int B = set;
+      const uint32_t at_k = here(lane_k);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int place = (kb + s * 16) & (size - 1);
-        const char* codes = p.at[s] + (place + i) * row_bytes + g * groups * kBits;
-        const char* factors = p.at[s] + shape.codes + (place + g * 4) * 2;
+        const char* codes = home(page[B].at[s]) + place * row_bytes;
         if constexpr (!kPad) {
-          __builtin_memcpy(kc[s], __builtin_assume_aligned(codes, GT * kBits < 16 ? GT * kBits : 16), GT * kBits);
+          __builtin_memcpy(kc[B][s], __builtin_assume_aligned(codes + at_k, GT * kBits < 16 ? GT * kBits : 16), GT * kBits);
         } else {
 #pragma unroll
           for (int x = 0; x < GT; ++x)
-            if (x < groups) __builtin_memcpy(kc[s][x], __builtin_assume_aligned(codes + x * kBits, kBits), kBits);
+            if (x < groups)
+              __builtin_memcpy(kc[B][s][x], __builtin_assume_aligned(codes + x * kBits + at_k, kBits), kBits);
         }
-#pragma unroll
-        for (int x = 0; x < GT; ++x)
-          if (!kPad || x < groups) kd[s][x] = *reinterpret_cast<const u2*>(factors + x * size * 2);
       }
     };
-    auto fetch_v = [&](int kb, const Step& p) {
+    auto fetch_f = [&](auto set, int kb) {
+      constexpr int B = set;
+      const bool second = f_token >= 16;
+      const char* from = home(second ? page[B].at[1] : page[B].at[0]) + ((kb + (second ? 16 : 0)) & (size - 1)) * 2;
+      __builtin_memcpy(fc[B], __builtin_assume_aligned(from + lane_f, 2 * GT), 2 * GT);
+    };
+    auto fetch_v = [&](auto set, int kb) {
+      constexpr int B = set;
+      const uint32_t at_v = here(lane_v);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int place = (kb + s * 16) & (size - 1);
-        const char* codes = p.at[s] + shape.half + (place + g * 4) * row_bytes;
-        const char* factors = p.at[s] + shape.half + shape.codes + (place + g * 4) * 2;
+        const char* codes = home(page[B].at[s]) + shape.half + place * row_bytes;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          uint32_t* to = vc[s * 4 + r];
+          uint32_t* to = vc[B][s * 4 + r];
           const char* from = codes + r * row_bytes;
           if constexpr (!kPad) {
-            constexpr int kWide = GT < 4 ? GT : 4, kBytes = kWide * kBits / 4;  // of a plane
+            constexpr int kBytes = kWide * kBits / 4;  // of a plane
             if constexpr (kBytes == 2) {
-              to[0] = *reinterpret_cast<const uint16_t*>(from + i * 2);
+              to[0] = *reinterpret_cast<const uint16_t*>(from + at_v);
             } else {
 #pragma unroll
               for (int n = 0; n < GT / kWide; ++n)
-                __builtin_memcpy(to + n * kBytes / 4, __builtin_assume_aligned(from + n * 16 * kBytes + i * kBytes, kBytes),
-                                 kBytes);
+                __builtin_memcpy(to + n * kBytes / 4, __builtin_assume_aligned(from + n * 16 * kBytes + at_v, kBytes), kBytes);
             }
           } else {
 #pragma unroll
@@ -223,7 +283,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
               if (x >= groups) break;
               const int fours = groups & ~3, first = x < fours ? x & ~3 : x < fours + (groups & 2) ? fours : x;
               const int wide = x < fours ? 4 : x < fours + (groups & 2) ? 2 : 1;
-              const char* at = from + (first * 16 + i * wide + x - first) * (kBits / 4);
+              const char* at = from + (first * 16 + x - first) * (kBits / 4) + (at_v + i * (uint32_t)wide * (kBits / 4));
               if constexpr (kBits == 8)
                 to[x / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(at) << (16 * (x & 1));
               else
@@ -231,25 +291,41 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
             }
           }
         }
-#pragma unroll
-        for (int x = 0; x < GT; ++x)
-          if (!kPad || x < groups) vd[s][x] = *reinterpret_cast<const u2*>(factors + x * size * 2);
       }
     };
+    // 4 tokens' factors of a plane of sh_f
+    auto factors_of = [&](int plane, int s) { return *reinterpret_cast<const u2*>(factors + plane * 16 + s * 8 + g * 2); };
 
     constexpr int kStep = kWaves * 32;
-    int kb = k0 + wave * 32;
-    Step step, step1;
-    Entries entry1;
-    if (kb < k1) {
-      step = step_of(kb, entries_at(kb));
-      entry1 = entries_at(kb + kStep);
-      fetch_k(kb, step);
-      fetch_v(kb, step);
-    }
-    for (; kb < k1; kb += kStep) {
-      const bool more = kb + kStep < k1;
-      const bool whole = kb >= all_lo && kb + 31 <= all_hi && kb + 32 <= k1 && step.there[0] && step.there[1];
+    auto body = [&](auto set, const int kb) {
+      constexpr int B = set;
+      const Pages now = page[B];
+      const bool both = now.at[0] >= 0 && now.at[1] >= 0 && kb + 32 <= k1;
+      const bool whole = kb >= all_lo && kb + 31 <= all_hi && both;
+      const bool more = kb + 2 * kStep < k1;
+      // The factors, those of tokens that are not there as 0 (the memory there may
+      // hold anything).
+      if (!f_there || (!both && (f_token < 16 ? now.at[0] : now.at[1]) < 0)) {
+#pragma unroll
+        for (int n = 0; n < FW; ++n) fc[B][n] = 0;
+      } else if (!both) {
+        const int left = k1 - kb - f_token;  // of this lane's tokens
+#pragma unroll
+        for (int n = 0; n < FW; ++n) fc[B][n] &= (2 * n < left ? 0xffffu : 0u) | (2 * n + 1 < left ? 0xffff0000u : 0u);
+      }
+      // (bits of numbers that are not negative, in order; a block that is not finite
+      // is above them all, and has no say)
+      typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+      us2 dm{0, 0};
+#pragma unroll
+      for (int n = 0; n < FW; ++n) dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[B][n])));
+      uint32_t dtop = dm[0] > dm[1] ? dm[0] : dm[1];
+      dtop = lane < 32 ? 0 : dtop;
+      __builtin_memcpy(__builtin_assume_aligned(factors + (lane < 32 ? 0 : GT * 16) + (f_x * 32 + f_token) / 2, 2 * GT), fc[B],
+                       2 * GT);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+
       float w[8];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -257,11 +333,12 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
         for (int x = 0; x < GT; ++x) {
           if (kPad && x >= groups) break;
-          const h8 codes = key_codes<kBits>(kc[s][x]);
+          const h8 codes = key_codes<kBits>(kc[B][s][x]);
           f4 acc{0, 0, 0, 0};
 #pragma unroll
           for (int n = NP - 1; n >= 0; --n) acc = mma16(codes, q[x][n], acc);
-          const h2 d01 = halves(kd[s][x][0]), d23 = halves(kd[s][x][1]);
+          const u2 d = factors_of(x, s);
+          const h2 d01 = halves(d[0]), d23 = halves(d[1]);
           sum[0] = __builtin_fmaf((float)d01[0], acc[0], sum[0]);
           sum[1] = __builtin_fmaf((float)d01[1], acc[1], sum[1]);
           sum[2] = __builtin_fmaf((float)d23[0], acc[2], sum[2]);
@@ -271,34 +348,23 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         for (int r = 0; r < 4; ++r) w[s * 4 + r] = sum[r] * qs * sc;
       }
       if (more) {
-        step1 = step_of(kb + kStep, entry1);
-        entry1 = entries_at(kb + 2 * kStep);
-        fetch_k(kb + kStep, step1);
+        page[B] = pages_of(kb + 2 * kStep, entry[B]);
+        entry[B] = entries_at(kb + 4 * kStep);
+        fetch_f(set, kb + 2 * kStep);
+        fetch_k(set, kb + 2 * kStep);
       }
+      uint32_t vis = 0xff;  // bit j: this row sees key j of this lane
       if (!whole) {
-        // What this row does not see weighs nothing, and its values' factors,
-        // which may be anything there, count as 0 in this lane's products.
         const int from = low - kb, to = (pos < k1 ? pos : k1 - 1) - kb;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int n = (j >> 2) * 16 + g * 4 + (j & 3);
-          if (!step.there[j >> 2] || n < from || n > to) {
+          if (now.at[j >> 2] < 0 || n < from || n > to) {
             w[j] = minus_inf();
-#pragma unroll
-            for (int x = 0; x < GT; ++x) vd[j >> 2][x][(j & 3) / 2] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+            vis &= ~(1u << j);
           }
         }
       }
-      // the factors' bound
-      h2 dm{0, 0};
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int x = 0; x < GT; ++x)
-          if (!kPad || x < groups)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) dm = __builtin_elementwise_max(dm, halves(vd[s][x][y]));
-      const float dtop = fmaxf((float)dm[0], (float)dm[1]);
       float top = w[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, w[j]);
@@ -307,11 +373,17 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       if (__ballot(top > m || dtop > most)) {
         float shrink = up;
         if (__ballot(dtop > most)) {
-          float d = dtop;
+          uint32_t d = dtop < 0x7c00u ? dtop : 0;
 #pragma unroll
-          for (int x = 1; x < 64; x <<= 1) d = fmaxf(d, __shfl_xor(d, x));
-          up = (float)(ilogbf(d) + 1);
-          most = ldexpf(1.f, (int)up);
+          for (int x = 1; x < 64; x <<= 1) {
+            const uint32_t other = __shfl_xor(d, x);
+            d = other > d ? other : d;
+          }
+          if (d > most) {
+            const int e = d < 0x400u ? -14 : (int)(d >> 10) - 14;  // 2^e is above it
+            up = (float)e;
+            most = (uint32_t)(e + 14) << 10 | 0x3ffu;
+          }
         }
         top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
         shrink = m == minus_inf() ? 0.f : exp2_((m - top) + (shrink - up));
@@ -327,29 +399,72 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         p[j] = exp2_(w[j] - from + shift);
         l += p[j];
       }
+      h2 ph[4];
+      if constexpr (NW == 1)
 #pragma unroll
-      for (int x = 0; x < GT; ++x) {
-        if (kPad && x >= groups) break;
-        h8 pd[NP];
+        for (int n = 0; n < 4; ++n) ph[n] = h2{(_Float16)p[2 * n], (_Float16)p[2 * n + 1]};
+      auto values = [&](auto all) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const h2 d = halves(vd[j >> 2][x][(j & 3) / 2]);
-          split<NP>(settled(p[j] * (float)d[j & 1]), pd, j);
+        for (int x = 0; x < GT; ++x) {
+          if (kPad && x >= groups) break;
+          u4 d;  // of this lane's 8 keys
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const u2 r = factors_of(GT + x, s);
+            d[2 * s] = r[0];
+            d[2 * s + 1] = r[1];
+          }
+          // (what this row does not see may be NaN, which its weight of 0 would not
+          // keep out)
+          if constexpr (!all)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              d[n] &= ((vis >> (2 * n)) & 1 ? 0xffffu : 0u) | ((vis >> (2 * n + 1)) & 1 ? 0xffff0000u : 0u);
+          h8 pd[NW];
+          if constexpr (NW == 1) {
+            u4 r;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) r[n] = __builtin_bit_cast(uint32_t, ph[n] * halves(d[n]));
+            pd[0] = __builtin_bit_cast(h8, r);
+          } else {
+            float pw[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[j], (float)halves(d[j / 2])[j & 1], 0.f);
+            in_two(pw, pd);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            u4 codes;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) codes[n] = value_codes<kBits>(vc[B][2 * n], vc[B][2 * n + 1], x, h);
+#pragma unroll
+            for (int n = NW - 1; n >= 0; --n)
+              o[2 * x + h] = mma16(__builtin_bit_cast(h8, codes), pd[n], o[2 * x + h]);
+          }
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u4 codes;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) codes[n] = value_codes<kBits>(vc[2 * n], vc[2 * n + 1], x, h);
-#pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
-            o[2 * x + h] = mma16(__builtin_bit_cast(h8, codes), pd[n], o[2 * x + h]);
-        }
-      }
-      if (more) {
-        fetch_v(kb + kStep, step1);
-        step = step1;
-      }
+      };
+      if (whole)
+        values(Is<true>{});
+      else
+        values(Is<false>{});
+      if (more) fetch_v(set, kb + 2 * kStep);
+    };
+
+    int kb = k0 + wave * 32;
+    auto begin = [&](auto set, int at) {
+      constexpr int B = set;
+      if (at >= k1) return;
+      page[B] = pages_of(at, entries_at(at));
+      entry[B] = entries_at(at + 2 * kStep);
+      fetch_f(set, at);
+      fetch_k(set, at);
+      fetch_v(set, at);
+    };
+    begin(Nth<0>{}, kb);
+    begin(Nth<1>{}, kb + kStep);
+    for (; kb < k1; kb += 2 * kStep) {
+      body(Nth<0>{}, kb);
+      if (kb + kStep < k1) body(Nth<1>{}, kb + kStep);
     }
 
     // the waves' sums, relative to the largest of their maxima alone

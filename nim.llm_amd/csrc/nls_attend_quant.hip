@@ -8,7 +8,7 @@ namespace {
 constexpr int kThreads = 256;
 
 template <typename T, int kBits, int GT, bool kPad>
-__global__ __launch_bounds__(kThreads, GT == 8 ? 1 : 2) void few_quant_kernel(AttendArgs a, Parts parts, int tiles,
+__global__ __launch_bounds__(kThreads, GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2) void few_quant_kernel(AttendArgs a, Parts parts, int tiles,
                                                                               bool chunk_runs) {
   few_quant_rows<T, kBits, GT, kPad>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
 }
