@@ -175,7 +175,7 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
     // split: the second launch costs the host more than it saves the GPU (517 keys:
     // 13.2 us a call whole, 17.2 in three parts, 12.8 and 12.3 in a graph; 24
     // contexts of 517: 17.4 and 18.4, 17.8 and 18.8 in a graph).
-    p.few_parts = parts_of_keys(most, tasks, (512 + tasks - 1) / tasks, most <= 768 ? 768 : 256, 2048);
+    p.few_parts = parts_of_keys(most, tasks, (512 + tasks - 1) / tasks, most <= 768 ? 768 : 256, quant_type(a.cache_type) ? 4096 : 2048);
     p.few_parts.rows = tasks * 16;
     p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   }

@@ -94,11 +94,18 @@ template <typename T>
 constexpr int weight_parts() {
   return __is_same(T, __bf16) ? 1 : 2;
 }
-// Numbers and truth values as types.
-template <int N>
-struct Nth {
-  __device__ constexpr operator int() const { return N; }
-};
+// What is read once: bytes that leave the caches to others.
+template <int kBytes>
+__device__ __forceinline__ void past_caches(uint32_t* to, const char* from) {
+  typedef uint32_t words __attribute__((ext_vector_type(kBytes < 16 ? kBytes / 4 : 4)));
+#pragma unroll
+  for (int n = 0; n < kBytes; n += 16) {
+    const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(from + n));
+    __builtin_memcpy(to + n / 4, &x, sizeof x);
+  }
+}
+
+// A truth value as a type.
 template <bool B>
 struct Is {
   __device__ constexpr operator bool() const { return B; }
@@ -111,12 +118,13 @@ template <typename T, int kBits, int GT, bool kPad>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,
                                                int group_at, int part) {
   constexpr int NP = quant_parts<T>(), NW = weight_parts<T>(), D = 32 * GT, kWaves = 4, kThreads = 256;
+  constexpr int NR = 2, KT = 16 * NR;   // runs of 16 keys in a step of a wave, and its keys
   constexpr int KW = kBits / 4;                       // words of a key unit
   constexpr int kWide = GT < 4 ? GT : 4;              // blocks of a plane
   constexpr int VW = (GT * kBits / 4 + 3) / 4;        // words of a lane's piece of a value row
   extern __shared__ float quant_lds[];                // [wave][16][D + 4] sums
   __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
-  __shared__ __align__(16) uint32_t sh_f[kWaves][32 * GT];  // a step's factors, of keys, then of values: [2 GT][32 tokens]
+  __shared__ __align__(16) uint32_t sh_f[kWaves][KT * GT];  // a step's factors, of keys, then of values: [2 GT][KT]
 
   const int kvh = group_at % a.p.kv_heads, task = group_at / a.p.kv_heads;
   const int seq = task / tiles, tile = task - seq * tiles;
@@ -179,7 +187,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
       for (int b = 0; b < GT; ++b)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split<NP>(ldexpf(x[b][j], -e), q[b], j);
+        for (int j = 0; j < 8; ++j)
+          split<NP>(ldexpf(x[b][j], -e), q[b], j);
     }
     const float sc = a.scale * kLog2e;
 
@@ -192,17 +201,17 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f;
     uint32_t most = NW == 1 ? 0x3bffu : 0u;
 
-    // A step's 32 keys are two runs of 16, each within a page (-1: none; what is
-    // read there is page 0, and counts for nothing).
+    // A step's keys are runs of 16, each within a page (-1: none; what is read
+    // there is page 0, and counts for nothing).
     struct Pages {
-      int at[2];
+      int at[NR];
     };
     const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
     const char* base = static_cast<const char*>(a.p.kv) + quant_base(shape, kvh, 0);
     auto entries_at = [&](int kb) {
       Pages e;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NR; ++s) {
         const int key = kb + s * 16;
         e.at[s] = table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
       }
@@ -211,7 +220,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     auto pages_of = [&](int kb, const Pages& e) {
       Pages p;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NR; ++s) {
         const int page = __builtin_amdgcn_readfirstlane(e.at[s]);
         p.at[s] = kb + s * 16 < k1 && (uint32_t)page < (uint32_t)a.p.pages ? page : -1;
       }
@@ -219,53 +228,58 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     };
     auto home = [&](int page) { return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride; };
 
-    // Two steps of a wave are on their way while one is worked on.
-    uint32_t kc[2][2][GT][KW], vc[2][8][VW];
-    // A lane's factors: GT tokens' of one block, keys' for the first 32 lanes and
-    // values' for the others; 16 lanes of the operands want each, out of LDS.
-    constexpr int FW = GT / 2, kAcross = 32 / GT;
-    uint32_t fc[2][FW];
-    Pages page[2], entry[2];  // of the steps in flight; of those behind them
-    const int f_x = lane / kAcross % GT, f_token = lane % kAcross * GT;
+    uint32_t kc[NR][GT][KW], vc[4 * NR][VW];
+    // A lane's factors: KT GT / 32 tokens' of one block, keys' for the first 32
+    // lanes and values' for the others; 16 lanes of the operands want each, out of
+    // LDS.
+    constexpr int FT = KT * GT / 32, FW = FT / 2, kAcross = 32 / GT;
+    static_assert(FT <= 16, "within a run");
+    uint32_t fc[FW];
+    const int f_x = lane / kAcross % GT, f_token = lane % kAcross * FT;
     const bool f_there = !kPad || f_x < groups;
     uint32_t* factors = sh_f[wave];
-    // (one address for the wave and 32 bits for the lane)
-    const uint32_t lane_k = i * row_bytes + g * groups * kBits, lane_v = g * 4 * row_bytes + (kPad ? 0 : i * kWide * kBits / 4);
+    // Row 4 g + r of a run's scores is key 4 r + g, so that one load of values is of
+    // four neighbouring rows.  (One address for the wave and 32 bits for the lane.)
+    const uint32_t lane_k = (i % 4 * 4 + i / 4) * row_bytes + g * groups * kBits;
+    const uint32_t lane_v = g * row_bytes + (kPad ? 0 : i * kWide * kBits / 4);
     const uint32_t lane_f = (lane < 32 ? 0 : shape.half) + shape.codes + ((f_there ? f_x : 0) * size + (f_token & 15)) * 2;
-    auto fetch_k = [&](auto set, int kb) {
-      constexpr int B = set;
+    auto fetch_k = [&](int kb, const Pages& p) {
       const uint32_t at_k = here(lane_k);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
-        const char* codes = home(page[B].at[s]) + place * row_bytes;
+        const char* codes = home(p.at[s]) + place * row_bytes;
         if constexpr (!kPad) {
-          __builtin_memcpy(kc[B][s], __builtin_assume_aligned(codes + at_k, GT * kBits < 16 ? GT * kBits : 16), GT * kBits);
+          past_caches<GT * kBits>(&kc[s][0][0], codes + at_k);
         } else {
 #pragma unroll
           for (int x = 0; x < GT; ++x)
             if (x < groups)
-              __builtin_memcpy(kc[B][s][x], __builtin_assume_aligned(codes + x * kBits + at_k, kBits), kBits);
+              __builtin_memcpy(kc[s][x], __builtin_assume_aligned(codes + x * kBits + at_k, kBits), kBits);
         }
       }
     };
-    auto fetch_f = [&](auto set, int kb) {
-      constexpr int B = set;
-      const bool second = f_token >= 16;
-      const char* from = home(second ? page[B].at[1] : page[B].at[0]) + ((kb + (second ? 16 : 0)) & (size - 1)) * 2;
-      __builtin_memcpy(fc[B], __builtin_assume_aligned(from + lane_f, 2 * GT), 2 * GT);
+    // the run of this lane's factors
+    auto run_page = [&](const Pages& p) {
+      int page = p.at[0];
+#pragma unroll
+      for (int s = 1; s < NR; ++s) page = f_token >= 16 * s ? p.at[s] : page;
+      return page;
     };
-    auto fetch_v = [&](auto set, int kb) {
-      constexpr int B = set;
+    auto fetch_f = [&](int kb, const Pages& p) {
+      const char* from = home(run_page(p)) + ((kb + (f_token & ~15)) & (size - 1)) * 2;
+      __builtin_memcpy(fc, __builtin_assume_aligned(from + lane_f, 2 * FT < 16 ? 2 * FT : 16), 2 * FT);
+    };
+    auto fetch_v = [&](int kb, const Pages& p) {
       const uint32_t at_v = here(lane_v);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
-        const char* codes = home(page[B].at[s]) + shape.half + place * row_bytes;
+        const char* codes = home(p.at[s]) + shape.half + place * row_bytes;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          uint32_t* to = vc[B][s * 4 + r];
-          const char* from = codes + r * row_bytes;
+          uint32_t* to = vc[s * 4 + r];
+          const char* from = codes + r * 4 * row_bytes;
           if constexpr (!kPad) {
             constexpr int kBytes = kWide * kBits / 4;  // of a plane
             if constexpr (kBytes == 2) {
@@ -273,7 +287,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
             } else {
 #pragma unroll
               for (int n = 0; n < GT / kWide; ++n)
-                __builtin_memcpy(to + n * kBytes / 4, __builtin_assume_aligned(from + n * 16 * kBytes + at_v, kBytes), kBytes);
+                past_caches<kBytes>(to + n * kBytes / 4, from + n * 16 * kBytes + at_v);
             }
           } else {
 #pragma unroll
@@ -293,47 +307,62 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         }
       }
     };
-    // 4 tokens' factors of a plane of sh_f
-    auto factors_of = [&](int plane, int s) { return *reinterpret_cast<const u2*>(factors + plane * 16 + s * 8 + g * 2); };
+    // a lane's 4 tokens' factors of a plane of sh_f (token 4 r + g of a run is at 4 g + r)
+    auto factors_of = [&](int plane, int s) { return *reinterpret_cast<const u2*>(factors + plane * (KT / 2) + s * 8 + g * 2); };
 
-    constexpr int kStep = kWaves * 32;
-    auto body = [&](auto set, const int kb) {
-      constexpr int B = set;
-      const Pages now = page[B];
-      const bool both = now.at[0] >= 0 && now.at[1] >= 0 && kb + 32 <= k1;
-      const bool whole = kb >= all_lo && kb + 31 <= all_hi && both;
-      const bool more = kb + 2 * kStep < k1;
+    constexpr int kStep = kWaves * KT;
+    int kb = k0 + wave * KT;
+    Pages now, entry;
+    if (kb < k1) {
+      now = pages_of(kb, entries_at(kb));
+      entry = entries_at(kb + kStep);
+      fetch_f(kb, now);
+      fetch_k(kb, now);
+      fetch_v(kb, now);
+    }
+    for (; kb < k1; kb += kStep) {
+      bool all = kb + KT <= k1;
+#pragma unroll
+      for (int s = 0; s < NR; ++s) all = all && now.at[s] >= 0;
+      const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && all;
+      const bool more = kb + kStep < k1;
       // The factors, those of tokens that are not there as 0 (the memory there may
       // hold anything).
-      if (!f_there || (!both && (f_token < 16 ? now.at[0] : now.at[1]) < 0)) {
+      if (!f_there || (!all && run_page(now) < 0)) {
 #pragma unroll
-        for (int n = 0; n < FW; ++n) fc[B][n] = 0;
-      } else if (!both) {
+        for (int n = 0; n < FW; ++n) fc[n] = 0;
+      } else if (!all) {
         const int left = k1 - kb - f_token;  // of this lane's tokens
 #pragma unroll
-        for (int n = 0; n < FW; ++n) fc[B][n] &= (2 * n < left ? 0xffffu : 0u) | (2 * n + 1 < left ? 0xffff0000u : 0u);
+        for (int n = 0; n < FW; ++n) fc[n] &= (2 * n < left ? 0xffffu : 0u) | (2 * n + 1 < left ? 0xffff0000u : 0u);
       }
       // (bits of numbers that are not negative, in order; a block that is not finite
       // is above them all, and has no say)
       typedef uint16_t us2 __attribute__((ext_vector_type(2)));
       us2 dm{0, 0};
 #pragma unroll
-      for (int n = 0; n < FW; ++n) dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[B][n])));
+      for (int n = 0; n < FW; ++n) dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[n])));
       uint32_t dtop = dm[0] > dm[1] ? dm[0] : dm[1];
       dtop = lane < 32 ? 0 : dtop;
-      __builtin_memcpy(__builtin_assume_aligned(factors + (lane < 32 ? 0 : GT * 16) + (f_x * 32 + f_token) / 2, 2 * GT), fc[B],
-                       2 * GT);
+      {
+        uint16_t* to = reinterpret_cast<uint16_t*>(factors) + (lane < 32 ? 0 : GT * KT) + f_x * KT + (f_token & ~15);
+#pragma unroll
+        for (int n = 0; n < FT; ++n) {
+          const int token = (f_token & 15) + n;
+          to[token % 4 * 4 + token / 4] = (uint16_t)(fc[n / 2] >> (16 * (n & 1)));
+        }
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
 
-      float w[8];
+      float w[4 * NR];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NR; ++s) {
         f4 sum{0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < GT; ++x) {
           if (kPad && x >= groups) break;
-          const h8 codes = key_codes<kBits>(kc[B][s][x]);
+          const h8 codes = key_codes<kBits>(kc[s][x]);
           f4 acc{0, 0, 0, 0};
 #pragma unroll
           for (int n = NP - 1; n >= 0; --n) acc = mma16(codes, q[x][n], acc);
@@ -347,19 +376,20 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
         for (int r = 0; r < 4; ++r) w[s * 4 + r] = sum[r] * qs * sc;
       }
+      const Pages then = now;
       if (more) {
-        page[B] = pages_of(kb + 2 * kStep, entry[B]);
-        entry[B] = entries_at(kb + 4 * kStep);
-        fetch_f(set, kb + 2 * kStep);
-        fetch_k(set, kb + 2 * kStep);
+        now = pages_of(kb + kStep, entry);
+        entry = entries_at(kb + 2 * kStep);
+        fetch_f(kb + kStep, now);
+        fetch_k(kb + kStep, now);
       }
-      uint32_t vis = 0xff;  // bit j: this row sees key j of this lane
+      uint32_t vis = 0xffff;  // bit j: this row sees key j of this lane
       if (!whole) {
         const int from = low - kb, to = (pos < k1 ? pos : k1 - 1) - kb;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int n = (j >> 2) * 16 + g * 4 + (j & 3);
-          if (now.at[j >> 2] < 0 || n < from || n > to) {
+        for (int j = 0; j < 4 * NR; ++j) {
+          const int n = (j >> 2) * 16 + (j & 3) * 4 + g;
+          if (then.at[j >> 2] < 0 || n < from || n > to) {
             w[j] = minus_inf();
             vis &= ~(1u << j);
           }
@@ -367,7 +397,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       }
       float top = w[0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, w[j]);
+      for (int j = 1; j < 4 * NR; ++j) top = fmaxf(top, w[j]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       if (__ballot(top > m || dtop > most)) {
@@ -393,78 +423,63 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         for (int t = 0; t < 2 * GT; ++t) o[t] *= shrink;
       }
       const float from = m == minus_inf() ? 0.f : m, shift = kQuantShift - up;
-      float p[8];
+      float p[4 * NR];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4 * NR; ++j) {
         p[j] = exp2_(w[j] - from + shift);
         l += p[j];
       }
-      h2 ph[4];
+      h2 ph[2 * NR];
       if constexpr (NW == 1)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) ph[n] = h2{(_Float16)p[2 * n], (_Float16)p[2 * n + 1]};
-      auto values = [&](auto all) {
+        for (int n = 0; n < 2 * NR; ++n) ph[n] = h2{(_Float16)p[2 * n], (_Float16)p[2 * n + 1]};
+      auto values = [&](auto seen) {
 #pragma unroll
-        for (int x = 0; x < GT; ++x) {
-          if (kPad && x >= groups) break;
-          u4 d;  // of this lane's 8 keys
+        for (int b = 0; b < NR; b += 2)  // 32 keys: the depth of one product
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const u2 r = factors_of(GT + x, s);
-            d[2 * s] = r[0];
-            d[2 * s + 1] = r[1];
+          for (int x = 0; x < GT; ++x) {
+            if (kPad && x >= groups) break;
+            u4 d;  // of this lane's 8 keys
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const u2 r = factors_of(GT + x, b + s);
+              d[2 * s] = r[0];
+              d[2 * s + 1] = r[1];
+            }
+            // (what this row does not see may be NaN, which its weight of 0 would not
+            // keep out)
+            if constexpr (!seen)
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                d[n] &= ((vis >> (4 * b + 2 * n)) & 1 ? 0xffffu : 0u) | ((vis >> (4 * b + 2 * n + 1)) & 1 ? 0xffff0000u : 0u);
+            h8 pd[NW];
+            if constexpr (NW == 1) {
+              u4 r;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) r[n] = __builtin_bit_cast(uint32_t, ph[2 * b + n] * halves(d[n]));
+              pd[0] = __builtin_bit_cast(h8, r);
+            } else {
+              float pw[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[4 * b + j], (float)halves(d[j / 2])[j & 1], 0.f);
+              in_two(pw, pd);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              u4 codes;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) codes[n] = value_codes<kBits>(vc[4 * b + 2 * n], vc[4 * b + 2 * n + 1], x, h);
+#pragma unroll
+              for (int n = NW - 1; n >= 0; --n)
+                o[2 * x + h] = mma16(__builtin_bit_cast(h8, codes), pd[n], o[2 * x + h]);
+            }
           }
-          // (what this row does not see may be NaN, which its weight of 0 would not
-          // keep out)
-          if constexpr (!all)
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-              d[n] &= ((vis >> (2 * n)) & 1 ? 0xffffu : 0u) | ((vis >> (2 * n + 1)) & 1 ? 0xffff0000u : 0u);
-          h8 pd[NW];
-          if constexpr (NW == 1) {
-            u4 r;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) r[n] = __builtin_bit_cast(uint32_t, ph[n] * halves(d[n]));
-            pd[0] = __builtin_bit_cast(h8, r);
-          } else {
-            float pw[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[j], (float)halves(d[j / 2])[j & 1], 0.f);
-            in_two(pw, pd);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            u4 codes;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) codes[n] = value_codes<kBits>(vc[B][2 * n], vc[B][2 * n + 1], x, h);
-#pragma unroll
-            for (int n = NW - 1; n >= 0; --n)
-              o[2 * x + h] = mma16(__builtin_bit_cast(h8, codes), pd[n], o[2 * x + h]);
-          }
-        }
       };
       if (whole)
         values(Is<true>{});
       else
         values(Is<false>{});
-      if (more) fetch_v(set, kb + 2 * kStep);
-    };
-
-    int kb = k0 + wave * 32;
-    auto begin = [&](auto set, int at) {
-      constexpr int B = set;
-      if (at >= k1) return;
-      page[B] = pages_of(at, entries_at(at));
-      entry[B] = entries_at(at + 2 * kStep);
-      fetch_f(set, at);
-      fetch_k(set, at);
-      fetch_v(set, at);
-    };
-    begin(Nth<0>{}, kb);
-    begin(Nth<1>{}, kb + kStep);
-    for (; kb < k1; kb += 2 * kStep) {
-      body(Nth<0>{}, kb);
-      if (kb + kStep < k1) body(Nth<1>{}, kb + kStep);
+      if (more) fetch_v(kb + kStep, now);
     }
 
     // the waves' sums, relative to the largest of their maxima alone

@@ -7,9 +7,15 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Waves per SIMD that registers are kept for.
+template <typename T, int kBits, int GT>
+constexpr int few_quant_waves() {
+  return GT == 8 ? 1 : GT == 4 ? 2 : 3;
+}
+
 template <typename T, int kBits, int GT, bool kPad>
-__global__ __launch_bounds__(kThreads, GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2) void few_quant_kernel(AttendArgs a, Parts parts, int tiles,
-                                                                              bool chunk_runs) {
+__global__ __launch_bounds__(kThreads, (few_quant_waves<T, kBits, GT>())) void few_quant_kernel(AttendArgs a, Parts parts,
+                                                                                               int tiles, bool chunk_runs) {
   few_quant_rows<T, kBits, GT, kPad>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
 }
 
