@@ -9,9 +9,9 @@ namespace nls {
 
 constexpr int kMaxBeams = 64;
 constexpr int kBeamThreads = 256;
-constexpr int kBeamSlice = 32 * kBeamThreads;  // logits of a workgroup
+constexpr int kBeamPer = 32, kBeamPerFew = 8;  // logits of a thread
 
-// The largest logit of a slice, the sum of exp(l - max), and behind them (in
+// The largest logit of a slice, the sum of exp(l - max), and behind the parts (in
 // the workspace) its `beams` largest logits in order.
 struct BeamPart {
   float max, sum;
@@ -32,12 +32,21 @@ struct BeamArgs {
   int32_t *parents, *tokens;
   float* out_scores;
   int32_t* out_ended;
-  int slices;  // of a row
+  int per, slices;  // logits of a thread, slices of a row
   BeamPart* parts;
   BeamEntry* entries;
 };
 
-inline int beam_slices(int64_t vocab) { return (int)((vocab + kBeamSlice - 1) / kBeamSlice); }
+// 32 logits to a thread, 32 KB on their way to each workgroup; 8 where that leaves
+// less than a workgroup for a CU (4 x 32000: 7.0 us with 32, 5.3 with 8).
+inline int beam_per(int64_t rows, int64_t vocab) {
+  const int64_t slice = (int64_t)kBeamPer * kBeamThreads;
+  return rows * ((vocab + slice - 1) / slice) < 256 ? kBeamPerFew : kBeamPer;
+}
+inline int64_t beam_slices(int64_t rows, int64_t vocab) {
+  const int64_t slice = (int64_t)beam_per(rows, vocab) * kBeamThreads;
+  return (vocab + slice - 1) / slice;
+}
 hipError_t launch_beam(const BeamArgs& a, hipStream_t s);
 
 }  // namespace nls

@@ -13,13 +13,11 @@
 // lists in the same way.
 #include "nls_beam.h"
 #include "nls_primitives.h"
-#include "nls_rowsplit.h"
 
 namespace nls {
 namespace {
 
 constexpr int kNT = kBeamThreads, kWaves = kNT / kWave;
-constexpr int kPer = kBeamSlice / kNT;  // logits of a thread
 constexpr int kList = 512;              // logits of a slice that reach the bound, at most
 constexpr int kMerge = 1024;            // candidates of a group likewise
 
@@ -29,7 +27,9 @@ __device__ __forceinline__ bool takes_part(const BeamArgs& a, int row) {
   return a.scores[row] > -__builtin_inff() && !(a.ended && a.ended[row]);
 }
 
+template <int kPer>
 __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
+  constexpr int kSlice = kPer * kNT;
   __shared__ float sh_max[kWaves], sh_sum[kWaves];
   __shared__ uint32_t sh_bound[kWaves];
   __shared__ int count;
@@ -39,13 +39,13 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   if (!takes_part(a, row)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float none = -__builtin_inff();
-  const float* x = a.logits + (int64_t)row * a.vocab + (int64_t)slice * kBeamSlice;
-  const int n = (int)(a.vocab - (int64_t)slice * kBeamSlice < kBeamSlice ? a.vocab - (int64_t)slice * kBeamSlice : kBeamSlice);
+  const float* x = a.logits + (int64_t)row * a.vocab + (int64_t)slice * kSlice;
+  const int n = (int)(a.vocab - (int64_t)slice * kSlice < kSlice ? a.vocab - (int64_t)slice * kSlice : kSlice);
   float l[kPer];  // element (k, e) of a thread: logit (k 256 + thread) 4 + e of the slice
 #pragma unroll
   for (int k = 0; k < kPer / 4; ++k) {
     const int at = (k * kNT + (int)threadIdx.x) * 4;
-    if (n == kBeamSlice || at + 4 <= n) {
+    if (n == kSlice || at + 4 <= n) {
       f4v v;
       __builtin_memcpy(&v, x + at, 16);
 #pragma unroll
@@ -57,10 +57,7 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   }
   float top = none;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    l[j] = fmaxf(l[j], none);  // (NaN: -infinity)
-    top = fmaxf(top, l[j]);
-  }
+  for (int j = 0; j < kPer; ++j) top = fmaxf(top, l[j]);  // (NaN is passed over)
   const uint32_t key = top == none ? 0u : f2key(top);
   const uint32_t wave_top = wave_max_u32(key), wave_bound = wave_kth_largest(key, a.beams);
   if (lane == 0) {
@@ -76,13 +73,21 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
     mx = fmaxf(mx, sh_max[w]);
     bound = max(bound, sh_bound[w]);
   }
+  // (the largest term is exactly 1; a product rounded once in the exponent of the
+  // others is 2^-24 of a number that weighs exp(-it))
+  auto term = [&](float v) {
+    if (mx == __builtin_inff()) return v == mx ? 1.f : 0.f;  // those of +infinity, each as much
+    return __builtin_amdgcn_exp2f((v - mx) * 1.44269504f);
+  };
   float sum = 0.f;
-  if (mx == __builtin_inff()) {  // those of +infinity, each as much
+  if (mx > none) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += l[j] == mx ? 1.f : 0.f;
-  } else if (mx > none) {
+    for (int j = 0; j < kPer; ++j) sum += term(l[j]);
+    if (__ballot(!(sum < __builtin_inff()))) {  // a NaN among them
+      sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += expf_estimate(l[j] - mx);
+      for (int j = 0; j < kPer; ++j) sum += l[j] > none ? term(l[j]) : 0.f;
+    }
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -92,7 +97,7 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   for (int j = 0; j < kPer; ++j)
     if (l[j] >= least && l[j] > none) {
       const int at = atomicAdd(&count, 1);
-      if (at < kList) list[at] = {l[j], (int32_t)(slice * kBeamSlice + ((j >> 2) * kNT + threadIdx.x) * 4 + (j & 3))};
+      if (at < kList) list[at] = {l[j], (int32_t)(slice * kSlice + ((j >> 2) * kNT + threadIdx.x) * 4 + (j & 3))};
     }
   __syncthreads();
   const int64_t part = blockIdx.x;
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
     BeamEntry e{none, 0x7fffffff};
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int v = slice * kBeamSlice + ((j >> 2) * kNT + threadIdx.x) * 4 + (j & 3);
+      const int v = slice * kSlice + ((j >> 2) * kNT + threadIdx.x) * 4 + (j & 3);
       const bool behind = l[j] < last.l || (l[j] == last.l && v > last.v);
       if (behind && l[j] > none) argmax_merge(e.l, e.v, l[j], v);
     }
@@ -145,85 +150,109 @@ __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
 }
 
 __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
-  __shared__ float s_score[kMaxBeams], s_max[kMaxBeams];
-  __shared__ double s_lse[kMaxBeams];
-  __shared__ int s_kind[kMaxBeams];  // 0 no candidates, 1 the row's, 2 itself
-  __shared__ Candidate s_top[kNT];
-  __shared__ Candidate s_bound, s_wave[kWaves];
+  __shared__ float s_score[kMaxBeams];
+  __shared__ double s_of[kMaxBeams], s_sum[kMaxBeams];  // ln sum exp(l): of + sum
+  __shared__ int s_kind[kMaxBeams];  // 0 no candidates, 1 the row's, 2 itself, 3 the row's of +infinity
+  __shared__ uint32_t s_bound[kWaves];
+  __shared__ Candidate s_wave[kWaves];
   __shared__ Candidate list[kMerge];
-  __shared__ int count, s_found;
+  __shared__ int32_t s_eog[kNT];
+  __shared__ int count;
   const int g = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const double none = -__builtin_inf();
-  for (int b = wave; b < a.beams; b += kWaves) {
-    const int row = g * a.beams + b;
+  const int lists = a.beams * a.slices;
+  const BeamEntry* entries = a.entries + (int64_t)g * lists * a.beams;
+  // (what does not wait for the sums is requested before them)
+  constexpr int kHeld = 8;
+  BeamEntry held[kHeld];  // of list threadIdx.x
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    held[k] = {-__builtin_inff(), -1};
+    if ((int)threadIdx.x < lists && k < a.beams) held[k] = entries[(int64_t)threadIdx.x * a.beams + k];
+  }
+  if ((int)threadIdx.x < a.n_eog) s_eog[threadIdx.x] = a.eog[threadIdx.x];
+  // a row's parts: 16 lanes
+  for (int b = threadIdx.x / 16; b < a.beams; b += kNT / 16) {
+    const int row = g * a.beams + b, part = threadIdx.x & 15;
     const float score = a.scores[row];
     const bool live = score > -__builtin_inff(), ended = a.ended && a.ended[row];
-    float mx = -__builtin_inff();
-    double sum = 0.0;
+    double of = none, sum = 0.0;
+    const BeamPart* p = a.parts + (int64_t)row * a.slices;
+    BeamPart next = p[part < a.slices ? part : 0];
+    // sums of exp(l - of) together; what is against +infinity stands alone
+    auto add = [&](double of2, double sum2) {
+      if (!(of2 > none)) return;
+      const double most = of2 > of ? of2 : of;
+      sum = (of == most ? sum : sum * exp(of - most)) + (of2 == most ? sum2 : sum2 * exp(of2 - most));
+      of = most;
+    };
     if (live && !ended) {
-      const BeamPart* p = a.parts + (int64_t)row * a.slices;
-      for (int s = lane; s < a.slices; s += kWave) mx = fmaxf(mx, p[s].max);
-#pragma unroll
-      for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-      if (mx > -__builtin_inff())
-        for (int s = lane; s < a.slices; s += kWave) {
-          const BeamPart q = p[s];
-          sum += q.max == mx ? (double)q.sum : (double)q.sum * exp((double)q.max - (double)mx);
-        }
-#pragma unroll
-      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+      for (int s = part; s < a.slices; s += 16) {
+        const BeamPart q = next;
+        if (s + 16 < a.slices) next = p[s + 16];
+        add((double)q.max, (double)q.sum);
+      }
     }
-    if (lane == 0) {
+#pragma unroll
+    for (int d = 8; d; d >>= 1) {
+      const double of2 = __shfl_xor(of, d), sum2 = __shfl_xor(sum, d);
+      add(of2, sum2);
+    }
+    if (part == 0) {
       s_score[b] = score;
-      s_max[b] = mx;
-      s_lse[b] = log(sum);
-      s_kind[b] = !live ? 0 : ended ? 2 : mx > -__builtin_inff() ? 1 : 0;
+      s_of[b] = of;
+      s_sum[b] = log(sum);
+      s_kind[b] = !live ? 0 : ended ? 2 : of == __builtin_inf() ? 3 : of > none ? 1 : 0;
     }
   }
-  if (threadIdx.x == 0) {
-    count = 0;
-    s_found = 0;
-  }
+  if (threadIdx.x == 0) count = 0;
   __syncthreads();
-  const int lists = a.beams * a.slices;
   // entry i of a list, or none
+  auto worth = [&](const BeamEntry& e, int b) {
+    const int kind = s_kind[b];
+    if (e.v < 0 || (kind == 3 && e.l != __builtin_inff())) return Candidate{none, 0};
+    const double x = kind == 3 ? 0.0 : (double)e.l - s_of[b];
+    return Candidate{(x - s_sum[b]) + (double)s_score[b], (int64_t)b << 32 | (uint32_t)(e.v + 1)};
+  };
   auto candidate = [&](int which, int i) {
     const int b = which / a.slices, s = which - b * a.slices, kind = s_kind[b];
-    if (kind == 1) {
-      const BeamEntry e = a.entries[((int64_t)g * lists + which) * a.beams + i];
-      if (e.v < 0) return Candidate{none, 0};
-      const double x = e.l == s_max[b] ? 0.0 : (double)e.l - (double)s_max[b];
-      return Candidate{(x - s_lse[b]) + (double)s_score[b], (int64_t)b << 32 | (uint32_t)(e.v + 1)};
-    }
+    if (kind & 1) return worth(entries[(int64_t)which * a.beams + i], b);
     if (kind == 2 && s == 0 && i == 0) return Candidate{(double)s_score[b], (int64_t)b << 32};
     return Candidate{none, 0};
   };
-  // The bound: the beams-th of the threads' best, each of another list or more.
-  Candidate mine{none, 0};
+  // The bound, as the slices': the beams-th largest of a wave's lanes' best, each
+  // of another list or more.  (Its number is rounded down to fp32.)
+  auto key_of = [&](const Candidate& c) { return c.c > none ? f2key(__double2float_rd(c.c)) : 0u; };
+  uint32_t mine = 0;
   for (int i = threadIdx.x; i < lists; i += kNT) {
-    const Candidate c = candidate(i, 0);
-    if (c.c > none && (mine.c == none || before(c, mine))) mine = c;
+    const int b = i / a.slices;
+    const uint32_t k = key_of(i < kNT && (s_kind[b] & 1) ? worth(held[0], b) : candidate(i, 0));
+    mine = k > mine ? k : mine;
   }
-  s_top[threadIdx.x] = mine;
+  const uint32_t wave_bound = wave_kth_largest(mine, a.beams);
+  if (lane == 0) s_bound[wave] = wave_bound;
   __syncthreads();
-  if (mine.c > none) {
-    int rank = 0;
-    for (int j = 0; j < kNT; ++j) rank += s_top[j].c > none && before(s_top[j], mine);
-    if (rank == a.beams - 1) {
-      s_bound = mine;
-      s_found = 1;
+  uint32_t bound = s_bound[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) bound = max(bound, s_bound[w]);
+  // (a list is in order)
+  auto take = [&](const Candidate& c) {
+    if (!(c.c > none) || key_of(c) < bound) return false;
+    const int at = atomicAdd(&count, 1);
+    if (at < kMerge) list[at] = c;
+    return true;
+  };
+  for (int i = threadIdx.x; i < lists; i += kNT) {
+    const int b = i / a.slices;
+    bool more = true;
+    if (i < kNT && (s_kind[b] & 1)) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) more = more && k < a.beams && take(worth(held[k], b));
+      for (int k = kHeld; more && k < a.beams; ++k) more = take(candidate(i, k));
+    } else {
+      for (int k = 0; more && k < a.beams; ++k) more = take(candidate(i, k));
     }
   }
-  __syncthreads();
-  const bool bounded = s_found;
-  const Candidate bound = s_bound;
-  for (int i = threadIdx.x; i < lists; i += kNT)
-    for (int k = 0; k < a.beams; ++k) {
-      const Candidate c = candidate(i, k);
-      if (!(c.c > none) || (bounded && before(bound, c))) break;
-      const int at = atomicAdd(&count, 1);
-      if (at < kMerge) list[at] = c;
-    }
   __syncthreads();
   const int n = count, row0 = g * a.beams;
   auto put = [&](int place, const Candidate& c) {
@@ -233,7 +262,7 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
     a.out_scores[row0 + place] = (float)c.c;
     if (a.out_ended) {
       int over = s_kind[b] == 2;
-      for (int i = 0; i < a.n_eog; ++i) over |= v >= 0 && v == a.eog[i];
+      for (int i = 0; i < a.n_eog; ++i) over |= v >= 0 && v == (i < kNT ? s_eog[i] : a.eog[i]);
       a.out_ended[row0 + place] = over;
     }
   };
@@ -284,7 +313,10 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
 }  // namespace
 
 hipError_t launch_beam(const BeamArgs& a, hipStream_t s) {
-  beam_slice_kernel<<<a.groups * a.beams * a.slices, kNT, 0, s>>>(a);
+  if (a.per == kBeamPer)
+    beam_slice_kernel<kBeamPer><<<a.groups * a.beams * a.slices, kNT, 0, s>>>(a);
+  else
+    beam_slice_kernel<kBeamPerFew><<<a.groups * a.beams * a.slices, kNT, 0, s>>>(a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   beam_merge_kernel<<<a.groups, kNT, 0, s>>>(a);

@@ -20,7 +20,7 @@ const char* check_sizes(int32_t groups, int32_t beams, int64_t vocab) {
   if ((int64_t)groups * beams >= 1 << 24) return "beams: 2^24 rows or more";
   if (vocab < 0 || vocab >= int64_t{1} << 29) return "beams: vocab is negative or 2^29 or more";
   // (a launch has fewer than 2^32 threads)
-  if ((int64_t)groups * beams * beam_slices(vocab) >= 1 << 24) return "beams: rows times vocab is too large";
+  if ((int64_t)groups * beams * beam_slices((int64_t)groups * beams, vocab) >= 1 << 24) return "beams: rows times vocab is too large";
   return nullptr;
 }
 size_t align256(size_t n) { return (n + 255) & ~size_t{255}; }
@@ -32,7 +32,7 @@ extern "C" {
 
 size_t nls_beam_workspace(int32_t groups, int32_t beams, int64_t vocab) {
   if (check_sizes(groups, beams, vocab)) return 0;
-  const int64_t parts = (int64_t)groups * beams * beam_slices(vocab);
+  const int64_t rows = (int64_t)groups * beams, parts = rows * beam_slices(rows, vocab);
   return part_bytes(parts) + align256(parts * beams * sizeof(BeamEntry));
 }
 
@@ -64,7 +64,8 @@ int32_t nls_beam_select(const float* d_logits, int32_t groups, int32_t beams, in
   a.tokens = d_tokens;
   a.out_scores = d_out_scores;
   a.out_ended = d_out_ended;
-  a.slices = beam_slices(vocab);
+  a.per = beam_per((int64_t)groups * beams, vocab);
+  a.slices = (int)beam_slices((int64_t)groups * beams, vocab);
   a.parts = static_cast<BeamPart*>(d_work);
   a.entries = reinterpret_cast<BeamEntry*>(static_cast<char*>(d_work) + part_bytes((int64_t)groups * beams * a.slices));
   const hipError_t e = launch_beam(a, reinterpret_cast<hipStream_t>(stream));
