@@ -21,7 +21,7 @@ constexpr int kNT = kBeamThreads, kWaves = kNT / kWave;
 constexpr int kList = 512;              // logits of a slice that reach the bound, at most
 constexpr int kMerge = 1024;            // candidates of a group likewise
 
-typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4v __attribute__((ext_vector_type(4), aligned(4)));  // (rows may start off 16 bytes)
 
 __device__ __forceinline__ bool takes_part(const BeamArgs& a, int row) {
   return a.scores[row] > -__builtin_inff() && !(a.ended && a.ended[row]);
@@ -46,8 +46,7 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   for (int k = 0; k < kPer / 4; ++k) {
     const int at = (k * kNT + (int)threadIdx.x) * 4;
     if (n == kSlice || at + 4 <= n) {
-      f4v v;
-      __builtin_memcpy(&v, x + at, 16);
+      const f4v v = __builtin_nontemporal_load(reinterpret_cast<const f4v*>(x + at));
 #pragma unroll
       for (int e = 0; e < 4; ++e) l[4 * k + e] = v[e];
     } else {

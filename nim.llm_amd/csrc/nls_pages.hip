@@ -407,19 +407,31 @@ __device__ __forceinline__ int settled(const int32_t* p) {
 
 // What goes where.  A page is free for a copy when nobody held it, or only
 // slots whose contexts end here: it is marked by those, and the mark is taken off
-// by every row as it will be.
+// by every row as it will be.  One workgroup: what bounds it are the two passes
+// over the table: a wave takes eight rows at a time, with the slots' numbers in LDS
+// (512 slots of 73 entries: 47 us when entries are dealt out to threads by a
+// division each, TIME so).
+constexpr int kSlotsHeld = 2048;
 __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, const int32_t* src, int32_t* status,
                                                                int32_t* work) {
   __shared__ int sh[kPlanWaves];
+  __shared__ int s_src[kSlotsHeld], s_len[kSlotsHeld], s_first[kSlotsHeld];
   const PlanLds lds = plan_lds(t.pages);
   const ReorderWork w(work, t.slots);
   const int mask = (1 << t.page_shift) - 1;
+  const bool held = t.slots <= kSlotsHeld;
   int bad = 0;
   for (int s = threadIdx.x; s < t.slots; s += kPlanThreads) {
     const int len = t.lens[s], p = src[s];
     if (p < -1 || p >= t.slots || len < 0 || ((int64_t)len + mask) >> t.page_shift > t.max_pages) bad = 1;
     w.len[s] = len;
-    __hip_atomic_store(&w.first[s], t.slots, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (held) {
+      s_src[s] = p;
+      s_len[s] = len;
+      s_first[s] = t.slots;
+    } else {
+      __hip_atomic_store(&w.first[s], t.slots, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
   bad = __syncthreads_or(bad);
   if (bad) {
@@ -427,49 +439,110 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (t.pages + 63) >> 6;
-  for (int i = wave; i < words; i += kPlanWaves) {
-    const int p = i * 64 + lane;
-    const uint64_t b = __ballot(p < t.pages && t.refs[p < t.pages ? p : 0] == 0);
-    if (lane == 0) lds.bits[i] = b;
+  constexpr int kWords = 8;
+  for (int i0 = wave * kWords; i0 < words; i0 += kPlanWaves * kWords) {
+    int refs[kWords];
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) {
+      const int p = (i0 + u) * 64 + lane;
+      refs[u] = p < t.pages ? t.refs[p] : 1;
+    }
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) {
+      const uint64_t b = __ballot(refs[u] == 0);
+      if (lane == 0 && i0 + u < words) lds.bits[i0 + u] = b;
+    }
   }
   // the partial page of a parent stays with itself, else with its first child
-  for (int s = threadIdx.x; s < t.slots; s += kPlanThreads)
-    if (src[s] >= 0) atomicMin(&w.first[src[s]], src[s] == s ? -1 : s);
-  __syncthreads();
-  const uint32_t all = (uint32_t)t.slots * (uint32_t)t.max_pages, per = t.max_pages;  // (below 2^31)
-  uint32_t* marks = reinterpret_cast<uint32_t*>(lds.bits);
-  for (uint32_t e = threadIdx.x; e < all; e += kPlanThreads) {
-    const int s = (int)(e / per), j = (int)(e % per);
-    if (j >= pages_of(w.len[s], t.page_shift)) continue;
-    const int page = t.table[s * t.table_stride + j];
-    w.rows[e] = page;
-    if (src[s] != s && (uint32_t)page < (uint32_t)t.pages) atomicOr(&marks[page >> 5], 1u << (page & 31));
+  for (int s = threadIdx.x; s < t.slots; s += kPlanThreads) {
+    const int p = held ? s_src[s] : src[s];
+    if (p >= 0) atomicMin(held ? &s_first[p] : &w.first[p], p == s ? -1 : s);
   }
   __syncthreads();
-  for (uint32_t e = threadIdx.x; e < all; e += kPlanThreads) {
-    const int s = (int)(e / per), j = (int)(e % per), p = src[s];
-    if (p < 0) continue;
-    const int len = w.len[p], whole = len >> t.page_shift;
-    const int first = settled(&w.first[p]);
-    if (j >= whole + ((len & mask) != 0 && (first == s || p == s))) continue;
-    const int page = t.table[p * t.table_stride + j];
-    if ((uint32_t)page < (uint32_t)t.pages) atomicAnd(&marks[page >> 5], ~(1u << (page & 31)));
+  auto src_of = [&](int s) { return held ? s_src[s] : src[s]; };
+  auto len_of = [&](int s) { return held ? s_len[s] : w.len[s]; };
+  auto first_of = [&](int s) { return held ? s_first[s] : settled(&w.first[s]); };
+  uint32_t* marks = reinterpret_cast<uint32_t*>(lds.bits);
+  // eight rows at a time to a wave, 128 entries of each
+  constexpr int kRows = 8, kCols = 2;
+  for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
+    int used[kRows], most = 0;
+    bool ends[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int s = s0 + u;
+      used[u] = s < t.slots ? pages_of(len_of(s), t.page_shift) : 0;
+      ends[u] = s < t.slots && src_of(s) != s;
+      most = used[u] > most ? used[u] : most;
+    }
+    for (int j0 = lane; j0 < most; j0 += 64 * kCols) {
+      int page[kRows][kCols];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int j = j0 + 64 * c;
+          page[u][c] = j < used[u] ? t.table[(s0 + u) * t.table_stride + j] : -1;
+        }
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int j = j0 + 64 * c, p = page[u][c];
+          if (j < used[u]) w.rows[(int64_t)(s0 + u) * t.max_pages + j] = p;
+          if (ends[u] && (uint32_t)p < (uint32_t)t.pages) atomicOr(&marks[p >> 5], 1u << (p & 31));
+        }
+    }
+  }
+  __syncthreads();
+  for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
+    int from[kRows], keep[kRows], most = 0;
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int s = s0 + u;
+      from[u] = s < t.slots ? src_of(s) : -1;
+      keep[u] = 0;
+      if (from[u] >= 0) {
+        // (a parent's pages once, by the child that keeps them all)
+        if (from[u] == s || first_of(from[u]) == s) keep[u] = pages_of(len_of(from[u]), t.page_shift);
+      }
+      most = keep[u] > most ? keep[u] : most;
+    }
+    for (int j0 = lane; j0 < most; j0 += 64 * kCols) {
+      int page[kRows][kCols];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int j = j0 + 64 * c;
+          page[u][c] = j < keep[u] ? t.table[from[u] * t.table_stride + j] : -1;
+        }
+#pragma unroll
+      for (int u = 0; u < kRows; ++u)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int p = page[u][c];
+          if ((uint32_t)p < (uint32_t)t.pages) atomicAnd(&marks[p >> 5], ~(1u << (p & 31)));
+        }
+    }
   }
   __syncthreads();
   const int free_pages = rank_bitmap(words, lds.bits, lds.ranks, sh);
   int total = 0;
   for (int s0 = 0; s0 < t.slots; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
-    int copies = 0, p = -1;
-    if (s < t.slots && (p = src[s]) >= 0)
-      copies = (w.len[p] & mask) != 0 && p != s && settled(&w.first[p]) != s;
+    int copies = 0, p = -1, len = 0;
+    if (s < t.slots && (p = src_of(s)) >= 0) {
+      len = len_of(p);
+      copies = (len & mask) != 0 && p != s && first_of(p) != s;
+    }
     int sum;
     const int r = total + block_scan(copies, sh, &sum);
     if (s < t.slots) {
       int mine = -1;
       if (copies && r < free_pages) {
         mine = free_page(lds.bits, lds.ranks, t.pages, r);
-        w.from[r] = t.table[p * t.table_stride + (w.len[p] >> t.page_shift)];
+        w.from[r] = t.table[(int64_t)p * t.table_stride + (len >> t.page_shift)];
         w.to[r] = mine;
       }
       w.fresh[s] = mine;

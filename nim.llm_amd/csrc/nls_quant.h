@@ -73,6 +73,58 @@ NLS_HD int key_at(const QuantShape& s, int x, int g) { return (g * s.groups + x)
 NLS_HD int nibble_of(int e) { return e / 2 + 4 * (e & 1); }
 
 #ifdef __HIPCC__
+// Tokens of a workgroup: one where there are few, so that they run side by side;
+// else enough that their look-ups, a chain of four loads, are one wait among many.
+constexpr int kTokensMost = 8;
+inline int tokens_of_group(int tokens) { return tokens < 2048 ? 1 : kTokensMost; }
+
+struct TokenPlace {
+  int seq;      // -1: the row is of no sequence
+  int page;     // -1: none
+  int64_t pos;  // in its slot
+};
+// Where tokens first .. first + n - 1 belong, by the first wave; a barrier is the
+// caller's.
+__device__ __forceinline__ void find_places(const PagedArgs& a, int first, int n, TokenPlace* places) {
+  if (threadIdx.x >= 64) return;
+  const int lane = threadIdx.x;
+  // the starts not behind the first token, 64 at a time; then each lane goes on
+  // from there for its own
+  int seq = -1;
+  for (int s0 = 0; s0 < a.seqs + 1; s0 += 64) {
+    const int s = s0 + lane;
+    const int m = __popcll(__ballot(s <= a.seqs && a.starts[s <= a.seqs ? s : a.seqs] <= first));
+    seq += m;
+    if (m < 64) break;
+  }
+  if (lane >= n) return;
+  const int token = first + lane;
+  while (seq < a.seqs && a.starts[seq + 1] <= token) ++seq;
+  TokenPlace p{-1, -1, 0};
+  if (seq >= 0 && seq < a.seqs) {
+    const Chunk c = chunk_of(a, seq);
+    p.seq = seq;
+    p.pos = position_of(a, c, token - c.begin);
+    p.page = page_of(a, c.slot, p.pos);
+  }
+  places[lane] = p;
+}
+
+// f(Width<blocks>) for a plane's width.
+template <int W>
+struct Width {
+  __device__ constexpr operator int() const { return W; }
+};
+template <typename F>
+__device__ __forceinline__ void by_width(int wide, F&& f) {
+  if (wide == 4)
+    f(Width<4>{});
+  else if (wide == 2)
+    f(Width<2>{});
+  else
+    f(Width<1>{});
+}
+
 // cache_append and cache_read over such pages (nls_rope.hip, nls_quant.hip)
 hipError_t launch_append_quant(const TurnArgs& t, const PagedArgs& a, int type, int cache_type, bool wide, hipStream_t s);
 struct ReadArgs {

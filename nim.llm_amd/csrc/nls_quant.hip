@@ -2,7 +2,9 @@
 // as [tokens, kv_heads, head_dim], from pages of any type.
 //
 // Bound by the bytes: a row's elements are converted (blocks: one product with
-// the factor, rounded once) as they pass.  One workgroup takes one token.
+// the factor, rounded once) as they pass.  16 contexts of up to 4000 tokens, 8
+// heads of 128, Q4_0 to bf16 (220 MB): TIME us; a workgroup for each token, whose
+// look-ups are a wait of their own, 76.
 #include "nls_quant.h"
 
 namespace nls {
@@ -10,141 +12,123 @@ namespace {
 
 constexpr int kReadThreads = 256;
 
-template <typename T, int N>
+template <typename T, int N, bool kWide>
 __device__ __forceinline__ void put(T* to, const float* x) {
-  typedef T vec __attribute__((ext_vector_type(N)));
-  vec r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) r[i] = (T)x[i];
-  __builtin_memcpy(__builtin_assume_aligned(to, sizeof(T) * N < 16 ? sizeof(T) * N : 16), &r, sizeof r);
-}
-template <typename T, bool kWide>
-__device__ __forceinline__ void put8(T* to, const float (&x)[8]) {
   if constexpr (kWide) {
-    put<T, 8>(to, x);
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = (T)x[i];
+    __builtin_memcpy(__builtin_assume_aligned(to, sizeof(T) * N < 16 ? sizeof(T) * N : 16), &r, sizeof r);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) to[i] = (T)x[i];
+    for (int i = 0; i < N; ++i) to[i] = (T)x[i];
   }
 }
 
-// Where a token's keys and values lie: its page's first byte (NULL: it has no
-// place) and its place there.
-struct Place {
-  char* page;
-  int place;
-  bool row;  // it belongs to a sequence
-};
-__device__ __forceinline__ Place place_of(const PagedArgs& a, int token, int64_t page_bytes) {
-  const int lane = threadIdx.x & 63;
-  int seq = -1;
-  for (int s0 = 0; s0 < a.seqs + 1; s0 += 64) {
-    const int s = s0 + lane;
-    const int n = __popcll(__ballot(s <= a.seqs && a.starts[s <= a.seqs ? s : a.seqs] <= token));
-    seq += n;
-    if (n < 64) break;
-  }
-  if (seq < 0 || seq >= a.seqs) return {nullptr, 0, false};
-  const Chunk c = chunk_of(a, seq);
-  const int64_t pos = position_of(a, c, token - c.begin);
-  const int page = page_of(a, c.slot, pos);
-  return {page < 0 ? nullptr : static_cast<char*>(a.kv) + (int64_t)page * page_bytes,
-          (int)(pos & ((1 << a.page_shift) - 1)), true};
-}
-
-// A token without a place reads as zeros.
+// Tokens without a place read as zeros.
 template <typename T, typename TC, bool kWide>
-__global__ __launch_bounds__(kReadThreads) void read_kernel(ReadArgs r) {
+__global__ __launch_bounds__(kReadThreads) void read_kernel(ReadArgs r, int tokens) {
+  __shared__ TokenPlace places[kTokensMost];
   const PagedArgs& a = r.p;
-  const int token = blockIdx.x;
-  const Place at = place_of(a, token, a.page_stride * (int64_t)sizeof(TC));
-  if (!at.row) return;
+  const int first = blockIdx.x * tokens, n = a.tokens - first < tokens ? a.tokens - first : tokens;
+  find_places(a, first, n, places);
+  __syncthreads();
   const int per = a.dim / 8, all = 2 * per * a.kv_heads;
-  for (int w = threadIdx.x; w < all; w += kReadThreads) {
-    const int k = w >= per * a.kv_heads, u = k ? w - per * a.kv_heads : w, head = u / per, d = u % per * 8;
+  for (int w = threadIdx.x; w < all * n; w += kReadThreads) {
+    const int j = w / all, i = w % all, k = i >= per * a.kv_heads, u = k ? i - per * a.kv_heads : i;
+    const int head = u / per, d = u % per * 8;
+    const TokenPlace p = places[j];
+    if (p.seq < 0) continue;
     const HeadsView& to = k ? r.v : r.k;
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (at.page) {
+    if (p.page >= 0) {
       typedef TC vec __attribute__((ext_vector_type(8)));
-      const TC* from = reinterpret_cast<const TC*>(at.page) + at.place * a.token_stride + head * a.head_stride +
+      const TC* from = static_cast<const TC*>(a.kv) + token_offset(a, p.page, p.pos) + head * a.head_stride +
                        (k ? a.value_offset : 0) + d;
-      vec p;
-      __builtin_memcpy(&p, __builtin_assume_aligned(from, 16), sizeof p);
+      vec y;
+      __builtin_memcpy(&y, __builtin_assume_aligned(from, 16), sizeof y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+      for (int z = 0; z < 8; ++z) x[z] = (float)y[z];
     }
-    put8<T, kWide>(static_cast<T*>(to.d) + token * to.token_stride + head * to.head_stride + d, x);
+    put<T, 8, kWide>(static_cast<T*>(to.d) + (first + j) * to.token_stride + head * to.head_stride + d, x);
   }
 }
 
+// A thread takes 8 neighbouring elements of a key, or 4 neighbours of either half
+// of each block of a value's plane, whose codes are one piece of the row.
 template <typename T, int kBits, bool kWide>
-__global__ __launch_bounds__(kReadThreads) void read_quant_kernel(ReadArgs r) {
+__global__ __launch_bounds__(kReadThreads) void read_quant_kernel(ReadArgs r, int tokens) {
+  __shared__ TokenPlace places[kTokensMost];
   const PagedArgs& a = r.p;
-  const int token = blockIdx.x;
-  const Place at = place_of(a, token, a.page_stride);
-  if (!at.row) return;
+  const int first = blockIdx.x * tokens, n = a.tokens - first < tokens ? a.tokens - first : tokens;
+  find_places(a, first, n, places);
+  __syncthreads();
   const int size = 1 << a.page_shift;
   const QuantShape s = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, a.dim, size);
   const int planes = plane_count(s.groups);
-  const int nk = 4 * s.groups * a.kv_heads, all = nk + 16 * planes * a.kv_heads;
-  for (int w = threadIdx.x; w < all; w += kReadThreads) {
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (w < nk) {
-      const int head = w / (4 * s.groups), u = w % (4 * s.groups), b = u >> 2, g = u & 3;
-      if (at.page) {
-        const char* from = at.page + quant_base(s, head, 0);
-        const float d = (float)reinterpret_cast<const _Float16*>(from + s.codes)[b * size + at.place];
-        uint32_t c[kBits / 4];
-        __builtin_memcpy(c, __builtin_assume_aligned(from + at.place * s.row + key_at(s, b, g), kBits), kBits);
+  const int nk = 4 * s.groups * a.kv_heads, nv = 4 * planes * a.kv_heads;
+  for (int w = threadIdx.x; w < (nk + nv) * n; w += kReadThreads) {
+    const bool key = w < nk * n;
+    const int j = key ? w / nk : (w - nk * n) / nv, u = key ? w % nk : (w - nk * n) % nv, g = u & 3;
+    const TokenPlace p = places[j];
+    if (p.seq < 0) continue;
+    const int place = (int)(p.pos & (size - 1));
+    const char* home = static_cast<const char*>(a.kv) + (int64_t)(p.page < 0 ? 0 : p.page) * a.page_stride;
+    if (key) {
+      const int head = u / (4 * s.groups), b = u % (4 * s.groups) >> 2;
+      const char* from = home + quant_base(s, head, 0);
+      const float d = (float)reinterpret_cast<const _Float16*>(from + s.codes)[b * size + place];
+      uint32_t c[kBits / 4];
+      __builtin_memcpy(c, __builtin_assume_aligned(from + place * s.row + key_at(s, b, g), kBits), kBits);
+      float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = d * (kBits == 8 ? (float)(int)((c[e / 4 * (kBits / 8)] >> (8 * (e & 3))) & 255) - 128.f
-                                 : (float)(int)((c[0] >> (4 * nibble_of(e))) & 15) - 8.f);
+      for (int e = 0; e < 8; ++e) {
+        const float code = kBits == 8 ? (float)(int)((c[e / 4 * (kBits / 8)] >> (8 * (e & 3))) & 255) - 128.f
+                                      : (float)(int)((c[0] >> (4 * nibble_of(e))) & 15) - 8.f;
+        x[e] = p.page < 0 ? 0.f : d * code;
       }
-      put8<T, kWide>(static_cast<T*>(r.k.d) + token * r.k.token_stride + head * r.k.head_stride + 32 * b + 8 * g, x);
+      put<T, 8, kWide>(static_cast<T*>(r.k.d) + (first + j) * r.k.token_stride + head * r.k.head_stride + 32 * b + 8 * g, x);
     } else {
-      const int n = (w - nk) >> 4, i = (w - nk) & 15, head = n / planes;
-      const Plane p = plane_of(s.groups, n % planes);
-      T* to = static_cast<T*>(r.v.d) + token * r.v.token_stride + head * r.v.head_stride + 32 * p.first + i;
-      if (at.page) {
-        const char* from = at.page + quant_base(s, head, 1);
-        const char* row = from + at.place * s.row + value_at(s, p, i);
-        const int bytes = p.wide * kBits / 4;
-        uint32_t c[2] = {0, 0};
-        if (bytes == 8)
-          __builtin_memcpy(c, __builtin_assume_aligned(row, 8), 8);
-        else
-          c[0] = bytes == 4 ? *reinterpret_cast<const uint32_t*>(row)
-                 : bytes == 2 ? *reinterpret_cast<const uint16_t*>(row) : *reinterpret_cast<const uint8_t*>(row);
+      const int head = u / (4 * planes);
+      const Plane plane = plane_of(s.groups, u % (4 * planes) >> 2);
+      const char* from = home + quant_base(s, head, 1);
+      T* to = static_cast<T*>(r.v.d) + (first + j) * r.v.token_stride + head * r.v.head_stride + 32 * plane.first + 4 * g;
+      by_width(plane.wide, [&](auto wide) {
+        constexpr int W = wide, kBytes = W * kBits;
+        uint32_t c[kBytes / 4];
+        __builtin_memcpy(c, __builtin_assume_aligned(from + place * s.row + value_at(s, plane, 4 * g), kBytes < 16 ? kBytes : 16),
+                         kBytes);
+        float d[W];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (b >= p.wide) break;
-          const float d = (float)reinterpret_cast<const _Float16*>(from + s.codes)[(p.first + b) * size + at.place];
+        for (int b = 0; b < W; ++b) d[b] = (float)reinterpret_cast<const _Float16*>(from + s.codes)[(plane.first + b) * size + place];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            x[2 * b + h] = d * (kBits == 8 ? (float)(int)((c[b / 2] >> (16 * (b & 1) + 8 * h)) & 255) - 128.f
-                                           : (float)(int)((c[0] >> (8 * b + 4 * h)) & 15) - 8.f);
-        }
-      }
+        for (int b = 0; b < W; ++b)
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b >= p.wide) break;
-        to[32 * b] = (T)x[2 * b];
-        to[32 * b + 16] = (T)x[2 * b + 1];
-      }
+          for (int h = 0; h < 2; ++h) {
+            float x[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const int byte = (z * W + b) * (kBits / 4) + (kBits == 8 ? h : 0);
+              const uint32_t code = c[byte / 4] >> (8 * (byte % 4) + (kBits == 8 ? 0 : 4 * h));
+              x[z] = p.page < 0 ? 0.f : d[b] * ((float)(int)(code & (kBits == 8 ? 255 : 15)) - (kBits == 8 ? 128.f : 8.f));
+            }
+            put<T, 4, kWide>(to + 32 * b + 16 * h, x);
+          }
+      });
     }
   }
 }
 
 template <typename T, bool kWide>
 hipError_t read_of(const ReadArgs& a, int cache_type, hipStream_t s) {
-  const int n = a.p.tokens;
+  const int per = tokens_of_group(a.p.tokens), n = (a.p.tokens + per - 1) / per;
   switch (cache_type) {
-    case kF32: read_kernel<T, float, kWide><<<n, kReadThreads, 0, s>>>(a); break;
-    case kF16: read_kernel<T, _Float16, kWide><<<n, kReadThreads, 0, s>>>(a); break;
-    case kBF16: read_kernel<T, __bf16, kWide><<<n, kReadThreads, 0, s>>>(a); break;
-    case kQ8_0: read_quant_kernel<T, 8, kWide><<<n, kReadThreads, 0, s>>>(a); break;
-    default: read_quant_kernel<T, 4, kWide><<<n, kReadThreads, 0, s>>>(a); break;
+    case kF32: read_kernel<T, float, kWide><<<n, kReadThreads, 0, s>>>(a, per); break;
+    case kF16: read_kernel<T, _Float16, kWide><<<n, kReadThreads, 0, s>>>(a, per); break;
+    case kBF16: read_kernel<T, __bf16, kWide><<<n, kReadThreads, 0, s>>>(a, per); break;
+    case kQ8_0: read_quant_kernel<T, 8, kWide><<<n, kReadThreads, 0, s>>>(a, per); break;
+    default: read_quant_kernel<T, 4, kWide><<<n, kReadThreads, 0, s>>>(a, per); break;
   }
   return hipGetLastError();
 }

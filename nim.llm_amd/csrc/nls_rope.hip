@@ -223,12 +223,19 @@ hipError_t append_width(const TurnArgs& t, const PagedArgs& a, bool wide, hipStr
 
 // ---------------------------------------------------------------- pages of blocks
 
-// The largest and least of a block's elements, whose lanes are `lanes`
-// neighbours, and whether one is not finite.
-template <int kLanes>
-__device__ __forceinline__ void over_block(float& hi, float& lo, int& odd) {
+// The largest and least of a block's elements, and whether one is not finite: of
+// 8 in each of 4 neighbouring lanes.
+__device__ __forceinline__ void over_block(const float* x, float& hi, float& lo, int& odd) {
+  hi = lo = x[0];
+  odd = 0;
 #pragma unroll
-  for (int d = 1; d < kLanes; d <<= 1) {
+  for (int j = 0; j < 8; ++j) {
+    hi = fmaxf(hi, x[j]);
+    lo = fminf(lo, x[j]);
+    odd |= !(fabsf(x[j]) < __builtin_inff());
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
     hi = fmaxf(hi, __shfl_xor(hi, d));
     lo = fminf(lo, __shfl_xor(lo, d));
     odd |= __shfl_xor(odd, d);
@@ -288,130 +295,121 @@ __device__ __forceinline__ void turned8(const T* row, int d, int rot, const floa
   }
 }
 
-// One token's k and v into a page of blocks, and its q turned.  A key's block
-// is four lanes of 8 elements, a value's 16 lanes of 2; each lane's codes are
-// one piece of the row (nls_quant.h).  Factors and codes come of fp32 products
-// alone, each rounded once, so that they are the same numbers wherever they
-// are computed.
+// Tokens' k and v into pages of blocks, and their q turned.  A block is four
+// lanes of 8 elements: a key's of neighbours, a value's of 4 neighbours in either
+// half, whose codes are one piece of the row (nls_quant.h).  Factors and codes
+// come of fp32 products alone, each rounded once, so that they are the same
+// numbers wherever they are computed.
+// Bound by the bytes: prompts of 6102 tokens, 8 heads of 128, bf16 to Q8_0
+// (38 MB): TIME us.
 template <typename T, int kBits, bool kWide, Turn kTurn>
-__global__ __launch_bounds__(kTurnThreads) void append_quant_kernel(TurnArgs t, PagedArgs a) {
+__global__ __launch_bounds__(kTurnThreads) void append_quant_kernel(TurnArgs t, PagedArgs a, int tokens) {
   constexpr int N = kWide ? 8 : 1;
   constexpr bool kInterleaved = kTurn == kNeighbours;
-  __shared__ float2 cs[kMaxHeadDim / 2];
-  const int token = blockIdx.x;
+  __shared__ float2 turns[kTurn == kNoTurn ? 1 : kTokensMost][kMaxHeadDim / 2];
+  __shared__ TokenPlace places[kTokensMost];
+  const int first = blockIdx.x * tokens, n = t.tokens - first < tokens ? t.tokens - first : tokens;
   const int rot = kTurn == kNoTurn ? 0 : t.rot;
   const int pairs = rot / (2 * N), units = pairs + (t.dim - rot) / N;
   const int qu = t.heads ? (t.x.d == t.y.d ? pairs : units) : 0;
-  const int lane = threadIdx.x & 63;
-  int seq = -1;
-  for (int s0 = 0; s0 < a.seqs + 1; s0 += 64) {
-    const int s = s0 + lane;
-    const int n = __popcll(__ballot(s <= a.seqs && a.starts[s <= a.seqs ? s : a.seqs] <= token));
-    seq += n;
-    if (n < 64) break;
-  }
-  if (seq < 0 || seq >= a.seqs) return;  // a row of no sequence
-  const Chunk c = chunk_of(a, seq);
-  const int64_t pos = position_of(a, c, token - c.begin);
-  const int page = page_of(a, c.slot, pos);
+  find_places(a, first, n, places);
+  __syncthreads();
   if constexpr (kTurn != kNoTurn) {
-    turn_table(t, pos, cs);
+    for (int j = 0; j < n; ++j)
+      if (places[j].seq >= 0) turn_table(t, places[j].pos, turns[j]);
     __syncthreads();
   }
   if (qu) {
-    const T* x = static_cast<const T*>(t.x.d) + token * t.x.token_stride;
-    T* y = static_cast<T*>(t.y.d) + token * t.y.token_stride;
-    for (int w = threadIdx.x; w < qu * t.heads; w += kTurnThreads)
-      store_unit<T, T, N, kInterleaved>(load_unit<T, N, kInterleaved>(x + w / qu * t.x.head_stride, w % qu, rot),
-                                        y + w / qu * t.y.head_stride, w % qu, rot, cs);
+    const int per = qu * t.heads;
+    for (int w = threadIdx.x; w < per * n; w += kTurnThreads) {
+      const int j = w / per, u = w % per;
+      if (places[j].seq < 0) continue;
+      const T* x = static_cast<const T*>(t.x.d) + (first + j) * t.x.token_stride + u / qu * t.x.head_stride;
+      T* y = static_cast<T*>(t.y.d) + (first + j) * t.y.token_stride + u / qu * t.y.head_stride;
+      store_unit<T, T, N, kInterleaved>(load_unit<T, N, kInterleaved>(x, u % qu, rot), y, u % qu, rot,
+                                        turns[kTurn == kNoTurn ? 0 : j]);
+    }
   }
-  if (page < 0) return;
-  const QuantShape s = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, t.dim, 1 << a.page_shift);
-  const int place = (int)(pos & ((1 << a.page_shift) - 1)), size = 1 << a.page_shift;
-  char* home = static_cast<char*>(a.kv) + (int64_t)page * a.page_stride;
+  const int size = 1 << a.page_shift;
+  const QuantShape s = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, t.dim, size);
   const int planes = plane_count(s.groups);
-  // keys by four lanes to a block, then (from a multiple of 16 on) values by 16 to a plane
-  const int nk = 4 * s.groups * a.kv_heads, v0 = (nk + 15) & ~15, all = v0 + 16 * planes * a.kv_heads;
-  for (int w = threadIdx.x; w < all; w += kTurnThreads) {
-    if (w < nk) {
-      const int head = w / (4 * s.groups), u = w % (4 * s.groups), x = u >> 2, g = u & 3;
-      float e[8];
-      turned8<T, kWide, kTurn>(static_cast<const T*>(t.k.d) + token * t.k.token_stride + head * t.k.head_stride,
-                               32 * x + 8 * g, rot, cs, e);
-      float hi = e[0], lo = e[0];
-      int odd = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        hi = fmaxf(hi, e[j]);
-        lo = fminf(lo, e[j]);
-        odd |= !(fabsf(e[j]) < __builtin_inff());
-      }
-      over_block<4>(hi, lo, odd);
-      float step;
+  // keys of all tokens, then values: four lanes to a block (a plane)
+  const int nk = 4 * s.groups * a.kv_heads, nv = 4 * planes * a.kv_heads;
+  for (int w = threadIdx.x; w < (nk + nv) * n; w += kTurnThreads) {
+    const bool key = w < nk * n;
+    const int j = key ? w / nk : (w - nk * n) / nv, u = key ? w % nk : (w - nk * n) % nv;
+    const TokenPlace p = places[j];
+    if (p.page < 0) continue;
+    const int place = (int)(p.pos & (size - 1)), g = u & 3;
+    char* home = static_cast<char*>(a.kv) + (int64_t)p.page * a.page_stride;
+    if (key) {
+      const int head = u / (4 * s.groups), x = u % (4 * s.groups) >> 2;
+      float e[8], hi, lo, step;
+      int odd;
+      turned8<T, kWide, kTurn>(static_cast<const T*>(t.k.d) + (first + j) * t.k.token_stride + head * t.k.head_stride,
+                               32 * x + 8 * g, rot, turns[kTurn == kNoTurn ? 0 : j], e);
+      over_block(e, hi, lo, odd);
       const _Float16 d = factor_of<kBits>(hi, lo, odd, &step);
       char* to = home + quant_base(s, head, 0);
-      if constexpr (kBits == 8) {
-        uint32_t r[2] = {0, 0};
+      uint32_t r[kBits / 4] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j / 4] |= code_of<8>(e[j], step) << (8 * (j & 3));
-        __builtin_memcpy(__builtin_assume_aligned(to + place * s.row + key_at(s, x, g), 8), r, 8);
-      } else {
-        uint32_t r = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r |= code_of<4>(e[j], step) << (4 * nibble_of(j));
-        *reinterpret_cast<uint32_t*>(to + place * s.row + key_at(s, x, g)) = r;
-      }
+      for (int z = 0; z < 8; ++z)
+        r[kBits == 8 ? z / 4 : 0] |= code_of<kBits>(e[z], step) << (kBits == 8 ? 8 * (z & 3) : 4 * nibble_of(z));
+      __builtin_memcpy(__builtin_assume_aligned(to + place * s.row + key_at(s, x, g), kBits), r, kBits);
       if (g == 0) reinterpret_cast<_Float16*>(to + s.codes)[x * size + place] = d;
-    } else if (w >= v0) {
-      const int n = (w - v0) >> 4, i = w & 15, head = n / planes;
-      const Plane p = plane_of(s.groups, n % planes);
-      const T* row = static_cast<const T*>(t.v.d) + token * t.v.token_stride + head * t.v.head_stride + 32 * p.first + i;
+    } else {
+      const int head = u / (4 * planes);
+      const Plane plane = plane_of(s.groups, u % (4 * planes) >> 2);
+      const T* row = static_cast<const T*>(t.v.d) + (first + j) * t.v.token_stride + head * t.v.head_stride +
+                     32 * plane.first + 4 * g;
       char* to = home + quant_base(s, head, 1);
-      float e[8];
+      by_width(plane.wide, [&](auto wide) {
+        constexpr int W = wide;
+        float e[W][8];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        e[2 * x] = x < p.wide ? to_f(row[32 * x]) : 0.f;
-        e[2 * x + 1] = x < p.wide ? to_f(row[32 * x + 16]) : 0.f;
-      }
-      uint32_t r[2] = {0, 0};
+        for (int x = 0; x < W; ++x)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if (x >= p.wide) break;
-        float hi = fmaxf(e[2 * x], e[2 * x + 1]), lo = fminf(e[2 * x], e[2 * x + 1]);
-        int odd = !(fabsf(e[2 * x]) < __builtin_inff()) || !(fabsf(e[2 * x + 1]) < __builtin_inff());
-        over_block<16>(hi, lo, odd);
-        float step;
-        const _Float16 d = factor_of<kBits>(hi, lo, odd, &step);
-        const uint32_t a0 = code_of<kBits>(e[2 * x], step), a1 = code_of<kBits>(e[2 * x + 1], step);
-        if constexpr (kBits == 8)
-          r[x / 2] |= (a0 | a1 << 8) << (16 * (x & 1));
-        else
-          r[0] |= (a0 | a1 << 4) << (8 * x);
-        if (i == 0) reinterpret_cast<_Float16*>(to + s.codes)[(p.first + x) * size + place] = d;
-      }
-      char* at = to + place * s.row + value_at(s, p, i);
-      const int bytes = p.wide * kBits / 4;
-      if (bytes == 8) {
-        __builtin_memcpy(__builtin_assume_aligned(at, 8), r, 8);
-      } else if (bytes == 4) {
-        *reinterpret_cast<uint32_t*>(at) = r[0];
-      } else if (bytes == 2) {
-        *reinterpret_cast<uint16_t*>(at) = (uint16_t)r[0];
-      } else {
-        *reinterpret_cast<uint8_t*>(at) = (uint8_t)r[0];
-      }
+          for (int h = 0; h < 2; ++h)
+            if constexpr (kWide) {
+              const Pack<T, 4> four = load_pack<T, 4>(row + 32 * x + 16 * h);
+#pragma unroll
+              for (int z = 0; z < 4; ++z) e[x][4 * h + z] = to_f(four.v[z]);
+            } else {
+#pragma unroll
+              for (int z = 0; z < 4; ++z) e[x][4 * h + z] = to_f(row[32 * x + 16 * h + z]);
+            }
+        uint32_t r[W * kBits / 4] = {};
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+          float hi, lo, step;
+          int odd;
+          over_block(e[x], hi, lo, odd);
+          const _Float16 d = factor_of<kBits>(hi, lo, odd, &step);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {  // lane 4 g + z of the operands
+            const uint32_t low = code_of<kBits>(e[x][z], step), high = code_of<kBits>(e[x][4 + z], step);
+            const int byte = (z * W + x) * (kBits / 4);
+            r[byte / 4] |= (low | high << kBits) << (8 * (byte % 4));
+          }
+          if (g == 0) reinterpret_cast<_Float16*>(to + s.codes)[(plane.first + x) * size + place] = d;
+        }
+        constexpr int kBytes = W * kBits;
+        __builtin_memcpy(__builtin_assume_aligned(to + place * s.row + value_at(s, plane, 4 * g), kBytes < 16 ? kBytes : 16), r,
+                         kBytes);
+      });
     }
   }
 }
 
 template <typename T, int kBits, bool kWide>
 hipError_t append_quant_of(const TurnArgs& t, const PagedArgs& a, hipStream_t s) {
+  const int per = tokens_of_group(t.tokens), groups = (t.tokens + per - 1) / per;
   if (!t.freqs)
-    append_quant_kernel<T, kBits, kWide, kNoTurn><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+    append_quant_kernel<T, kBits, kWide, kNoTurn><<<groups, kTurnThreads, 0, s>>>(t, a, per);
   else if (t.interleaved)
-    append_quant_kernel<T, kBits, kWide, kNeighbours><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+    append_quant_kernel<T, kBits, kWide, kNeighbours><<<groups, kTurnThreads, 0, s>>>(t, a, per);
   else
-    append_quant_kernel<T, kBits, kWide, kHalves><<<t.tokens, kTurnThreads, 0, s>>>(t, a);
+    append_quant_kernel<T, kBits, kWide, kHalves><<<groups, kTurnThreads, 0, s>>>(t, a, per);
   return hipGetLastError();
 }
 template <typename T>
