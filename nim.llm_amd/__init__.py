@@ -19,10 +19,11 @@ point raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 from dataclasses import dataclass, field
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libnimllm_sampler.so")
@@ -850,8 +851,22 @@ def rope(x, positions, plan: RopePlan, inverse: bool = False, out=None):
     return out
 
 
-@dataclass(frozen=True)
-class PageFormat:
+@functools.lru_cache(maxsize=None)
+def _format_of(kind: str, kv_heads: int, page_size: int, head_dim: int):
+    """(type code, bytes of a page) of a PageFormat's sizes."""
+    t = {"q8_0": 8, "q4_0": 2}.get(kind)
+    if t is None:
+        raise SamplerError(f"page format {kind!r} is neither q8_0 nor q4_0")
+    n = -1
+    if 0 < kv_heads < 1 << 31 and 0 < page_size <= 4096 and 0 < head_dim <= 256:
+        n = int(lib().nls_cache_page_bytes(t, kv_heads, page_size, head_dim))
+    if n < 0:
+        raise SamplerError(f"page format {kind} of {kv_heads} heads of {head_dim}, {page_size} tokens: pages are of 16 to "
+                           "4096 tokens (a power of two), heads of a multiple of 32 up to 256")
+    return t, n
+
+
+class PageFormat(NamedTuple):
     """Pages whose keys and values are blocks of 32 elements of a head, an fp16
     factor and a code of 8 or 4 bits each: kind "q8_0" or "q4_0", as GGUF's types
     of those names hold.  One layer of such a cache is a uint8 tensor [pages,
@@ -864,33 +879,26 @@ class PageFormat:
 
     @property
     def type(self) -> int:
-        t = {"q8_0": 8, "q4_0": 2}.get(self.kind)
-        if t is None:
-            raise SamplerError(f"page format {self.kind!r} is neither q8_0 nor q4_0")
-        return t
+        return _format_of(*self)[0]
 
     @property
     def page_bytes(self) -> int:
-        n = -1
-        if 0 < self.kv_heads < 1 << 31 and 0 < self.page_size <= 4096 and 0 < self.head_dim <= 256:
-            n = int(lib().nls_cache_page_bytes(self.type, self.kv_heads, self.page_size, self.head_dim))
-        if n < 0:
-            raise SamplerError(f"{self}: pages of 16 to 4096 tokens (a power of two), heads of a multiple of 32 up to 256")
-        return n
+        return _format_of(*self)[1]
 
 
 def _kv_dims(kv, fmt):
     """(kv_heads, page_size, head_dim) of a layer."""
-    return (kv.shape[2], kv.shape[3], kv.shape[4]) if fmt is None else (fmt.kv_heads, fmt.page_size, fmt.head_dim)
+    return kv.shape[2:] if fmt is None else fmt[1:]
 
 
 def _paged_kv(dev: int, kv, table, lens, fmt=None):
     st = kv.stride()
     if fmt is not None:
-        if not (dev >= 0 and kv.dim() == 2 and kv.element_size() == 1 and st[1] == 1 and kv.shape[1] == fmt.page_bytes):
+        kind, size = _format_of(*fmt)
+        if not (dev >= 0 and len(st) == 2 and kv.element_size() == 1 and st[1] == 1 and kv.shape[1] == size):
             raise AssertionError("a layer of blocks on the GPU: uint8 [pages, page_bytes] of its format")
-        pages, kv_heads, page_size, dim = kv.shape[0], fmt.kv_heads, fmt.page_size, fmt.head_dim
-        st, kind = (st[0], 0, 0, 0), fmt.type
+        pages, (_, kv_heads, page_size, dim) = kv.shape[0], fmt
+        st = st[0], 0, 0, 0
     else:
         pages, two, kv_heads, page_size, dim = kv.shape
         if not (dev >= 0 and two == 2 and st[4] == 1):
@@ -960,7 +968,10 @@ def cache_read(kv, table, lens, starts, tokens: int, dtype=None, k=None, v=None,
     shape = (tokens, of[0], of[2])
     given = k if k is not None else v
     dt = dtype or (torch.float32 if given is None else given.dtype)
-    k, v = (torch.empty(shape, dtype=dt, device=kv.device) if x is None else x for x in (k, v))
+    if k is None:
+        k = torch.empty(shape, dtype=dt, device=kv.device)
+    if v is None:
+        v = torch.empty(shape, dtype=dt, device=kv.device) if given is not None else torch.empty_like(k)
     if not (k.shape == shape and v.shape == shape):
         raise AssertionError("k and v: [tokens, kv_heads, head_dim] of the cache's heads")
     _launch(dev, "nls_cache_read", _paged_kv(dev, kv, table, lens, fmt), _chunks(dev, tokens, starts, slots), _elem_type(k),
@@ -1210,7 +1221,7 @@ def beam_select(logits, scores, ended=None, eog=None, out=None, work=None):
         raise AssertionError("beams: V below 2^29, fewer than 2^24 rows")
     if out is None:
         # (one buffer: an allocation less for each of the others)
-        ints = torch.empty((3, groups, beams), dtype=torch.int32, device=logits.device)
+        ints = torch.empty((3, groups, beams), dtype=torch.int32, device=logits.device).unbind()
         out = ints[0], ints[1], torch.empty_like(scores), ints[2]
     parents, tokens, worth, over = out
     for x in (scores, worth):

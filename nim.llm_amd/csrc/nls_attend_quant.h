@@ -153,7 +153,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     const int all_lo = as_int(sees.low(sees.p0 + t1)), all_hi = as_int(sees.p0 + t0);
 
     h8 q[GT][NP];
-    float qs = 1.f;  // the row divided by a power of two
+    float sc, rest = 1.f;  // of a row's products, the power of two that the row was divided by among it
     {
       const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
                      (int64_t)(kvh * a.group + row % a.group) * a.q.head_stride;
@@ -177,20 +177,30 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
           top = fmaxf(top, fabsf(x[b][j]));
         }
       }
+      // the scale's sign goes to the queries: a largest score is a largest product
+      const float flip = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+      const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
       int e = 0;
       if constexpr (!__is_same(T, _Float16)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
+        // (the scale times the power stays a normal number: masked scores would be
+        // -infinity times 0)
+        const int least = -126 - ilogbf(scale2);
         e = query_exponent(top);
-        qs = ldexpf(1.f, e);
+        e = e < least ? least : e;
+      }
+      sc = scale2 * ldexpf(1.f, e);
+      // Nor does it pass fp32's range: the maximum gets back what was left out.
+      if (sc > 0x1p127f) {
+        sc = 0x1p127f;
+        rest = scale2 * 0x1p-127f * ldexpf(1.f, e);
       }
 #pragma unroll
       for (int b = 0; b < GT; ++b)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          split<NP>(ldexpf(x[b][j], -e), q[b], j);
+        for (int j = 0; j < 8; ++j) split<NP>(ldexpf(x[b][j] * flip, -e), q[b], j);
     }
-    const float sc = a.scale * kLog2e;
 
     f4 o[2 * GT];
 #pragma unroll
@@ -198,7 +208,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     // The weights are taken from m + up: 2^up is above any value's factor so far,
     // so that a weight times a factor is at most 1.  (One part: not below 2^0, so
     // that the weight itself is too.)  most: that bound as fp16's bits.
-    float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f;
+    float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f, back = kQuantShift - up;
     uint32_t most = NW == 1 ? 0x3bffu : 0u;
 
     // A step's keys are runs of 16, each within a page (-1: none; what is read
@@ -239,12 +249,21 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     const bool f_there = !kPad || f_x < groups;
     uint32_t* factors = sh_f[wave];
     // Row 4 g + r of a run's scores is key 4 r + g, so that one load of values is of
-    // four neighbouring rows.  (One address for the wave and 32 bits for the lane.)
-    const uint32_t lane_k = (i % 4 * 4 + i / 4) * row_bytes + g * groups * kBits;
-    const uint32_t lane_v = g * row_bytes + (kPad ? 0 : i * kWide * kBits / 4);
-    const uint32_t lane_f = (lane < 32 ? 0 : shape.half) + shape.codes + ((f_there ? f_x : 0) * size + (f_token & 15)) * 2;
+    // four neighbouring rows.  (One address for the wave and 32 bits for the lane,
+    // which are computed where they are used: registers are what waves are short of.)
+    auto lane_k = [&]() {
+      const int n = here(lane) & 15;
+      return (uint32_t)((n % 4 * 4 + n / 4) * row_bytes + (here(lane) >> 4) * groups * kBits);
+    };
+    auto lane_v = [&]() {
+      return (uint32_t)((here(lane) >> 4) * row_bytes + (kPad ? 0 : (here(lane) & 15) * (kWide * kBits / 4)));
+    };
+    auto lane_f = [&]() {
+      const int n = here(lane), x = n / kAcross % GT, token = n % kAcross * FT;
+      return (uint32_t)((n < 32 ? 0 : shape.half) + shape.codes + ((!kPad || x < groups ? x : 0) * size + (token & 15)) * 2);
+    };
     auto fetch_k = [&](int kb, const Pages& p) {
-      const uint32_t at_k = here(lane_k);
+      const uint32_t at_k = lane_k();
 #pragma unroll
       for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
@@ -268,10 +287,10 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     };
     auto fetch_f = [&](int kb, const Pages& p) {
       const char* from = home(run_page(p)) + ((kb + (f_token & ~15)) & (size - 1)) * 2;
-      __builtin_memcpy(fc, __builtin_assume_aligned(from + lane_f, 2 * FT < 16 ? 2 * FT : 16), 2 * FT);
+      __builtin_memcpy(fc, __builtin_assume_aligned(from + lane_f(), 2 * FT < 16 ? 2 * FT : 16), 2 * FT);
     };
     auto fetch_v = [&](int kb, const Pages& p) {
-      const uint32_t at_v = here(lane_v);
+      const uint32_t at_v = lane_v();
 #pragma unroll
       for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
@@ -320,12 +339,14 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       fetch_k(kb, now);
       fetch_v(kb, now);
     }
-    for (; kb < k1; kb += kStep) {
+    // (`more`, whether a step follows, is known when this is compiled: behind a
+    // branch the compiler does not know how many loads are on their way, and waits
+    // for the next step's with this one's.)
+    auto work = [&](auto more, const int kb) {
       bool all = kb + KT <= k1;
 #pragma unroll
       for (int s = 0; s < NR; ++s) all = all && now.at[s] >= 0;
       const bool whole = kb >= all_lo && kb + KT - 1 <= all_hi && all;
-      const bool more = kb + kStep < k1;
       // The factors, those of tokens that are not there as 0 (the memory there may
       // hold anything).
       if (!f_there || (!all && run_page(now) < 0)) {
@@ -374,10 +395,10 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
           sum[3] = __builtin_fmaf((float)d23[1], acc[3], sum[3]);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w[s * 4 + r] = sum[r] * qs * sc;
+        for (int r = 0; r < 4; ++r) w[s * 4 + r] = sum[r];
       }
       const Pages then = now;
-      if (more) {
+      if constexpr (more) {
         now = pages_of(kb + kStep, entry);
         entry = entries_at(kb + 2 * kStep);
         fetch_f(kb + kStep, now);
@@ -400,6 +421,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       for (int j = 1; j < 4 * NR; ++j) top = fmaxf(top, w[j]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
+      top *= sc;
       if (__ballot(top > m || dtop > most)) {
         float shrink = up;
         if (__ballot(dtop > most)) {
@@ -418,15 +440,27 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact
         shrink = m == minus_inf() ? 0.f : exp2_((m - top) + (shrink - up));
         m = top;
+        // (taken to be 0 where there is no score yet)
+        back = kQuantShift - up - (m == minus_inf() ? 0.f : m);
         l *= shrink;
 #pragma unroll
         for (int t = 0; t < 2 * GT; ++t) o[t] *= shrink;
       }
-      const float from = m == minus_inf() ? 0.f : m, shift = kQuantShift - up;
+      // A weight's exponent, the score less the maximum, is one fused product.  A
+      // maximum beyond 2^20 leaves no room for the shift beside it, and so large a
+      // product is off by whole numbers when rounded, as the maximum was: all are.
       float p[4 * NR];
+      if (__ballot(fabsf(back) > 1048576.f)) {
+        const float from = m == minus_inf() ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < 4 * NR; ++j) p[j] = w[j] * sc - from + (kQuantShift - up);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4 * NR; ++j) p[j] = __builtin_fmaf(w[j], sc, back);
+      }
 #pragma unroll
       for (int j = 0; j < 4 * NR; ++j) {
-        p[j] = exp2_(w[j] - from + shift);
+        p[j] = exp2_(p[j]);
         l += p[j];
       }
       h2 ph[2 * NR];
@@ -479,12 +513,15 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         values(Is<true>{});
       else
         values(Is<false>{});
-      if (more) fetch_v(kb + kStep, now);
-    }
+      if constexpr (more) fetch_v(kb + kStep, now);
+    };
+    for (; kb + kStep < k1; kb += kStep) work(Is<true>{}, kb);
+    if (kb < k1) work(Is<false>{}, kb);
 
     // the waves' sums, relative to the largest of their maxima alone
-    const float back = exp2_(up);
-    l *= back;
+    m *= rest;
+    const float full = exp2_(up);
+    l *= full;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g == 0) {
@@ -495,7 +532,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     float top = sh_m[0][i];
 #pragma unroll
     for (int x = 1; x < kWaves; ++x) top = fmaxf(top, sh_m[x][i]);
-    const float f = exp2_(m - (top == minus_inf() ? 0.f : top)) * back;
+    const float f = exp2_(m - (top == minus_inf() ? 0.f : top)) * full;
     float* mine = quant_lds + (wave * 16 + i) * (D + 4);
 #pragma unroll
     for (int t = 0; t < 2 * GT; ++t) *reinterpret_cast<f4*>(mine + t * 16 + g * 4) = o[t] * f;
