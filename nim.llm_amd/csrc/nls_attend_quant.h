@@ -498,15 +498,19 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
               for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[4 * b + j], (float)halves(d[j / 2])[j & 1], 0.f);
               in_two(pw, pd);
             }
+            h8 codes[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              u4 codes;
+              u4 r;
 #pragma unroll
-              for (int n = 0; n < 4; ++n) codes[n] = value_codes<kBits>(vc[4 * b + 2 * n], vc[4 * b + 2 * n + 1], x, h);
-#pragma unroll
-              for (int n = NW - 1; n >= 0; --n)
-                o[2 * x + h] = mma16(__builtin_bit_cast(h8, codes), pd[n], o[2 * x + h]);
+              for (int n = 0; n < 4; ++n) r[n] = value_codes<kBits>(vc[4 * b + 2 * n], vc[4 * b + 2 * n + 1], x, h);
+              codes[h] = __builtin_bit_cast(h8, r);
             }
+            // (one product does not wait for the other)
+#pragma unroll
+            for (int n = NW - 1; n >= 0; --n)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) o[2 * x + h] = mma16(codes[h], pd[n], o[2 * x + h]);
           }
       };
       if (whole)

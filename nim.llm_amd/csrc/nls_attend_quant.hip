@@ -10,7 +10,7 @@ constexpr int kThreads = 256;
 // Waves per SIMD that registers are kept for.
 template <typename T, int kBits, int GT>
 constexpr int few_quant_waves() {
-  return GT == 8 ? 1 : GT == 4 ? 2 : 3;
+  return GT == 8 ? 1 : GT == 4 || (sizeof(T) == 4 && kBits == 8) ? 2 : 3;
 }
 
 template <typename T, int kBits, int GT, bool kPad>
