@@ -40,8 +40,8 @@ constexpr int kJoinThreads = 256;
 // of few_rows; the others all of the call's, of chunk_rows.
 template <typename T, int D, int kWaves>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts few, Parts chunk, int64_t few_rows,
-                                                            int per, int tiles, bool alone, float few_shift,
-                                                            float chunk_shift) {
+                                                            int per, int tiles, bool alone, int chunk_tile,
+                                                            float few_shift, float chunk_shift) {
   constexpr int kAcross = D / 4, kSide = 64 * kWaves / kAcross;
   constexpr int kRows = kJoinThreads / (64 * kWaves);  // of a workgroup
   __shared__ f4 sums[kRows][kSide][kAcross];
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendArgs a, Parts 
   const int64_t index = (int64_t)blockIdx.x * kRows + sub;
   const bool is_few = index < few_rows;
   const int64_t rest = is_few ? index : index - few_rows;
-  const int head = (int)(rest % a.heads), kvh = head / a.group, size = is_few ? 16 : kChunkTile;
+  const int head = (int)(rest % a.heads), kvh = head / a.group, size = is_few ? 16 : chunk_tile;
   const Parts parts = is_few ? few : chunk;
   const float shift = is_few ? few_shift : chunk_shift;
   int token = (int)(rest / a.heads), seq = -1, parts_n = 0;
@@ -152,7 +152,7 @@ Parts parts_of_keys(int64_t most, int64_t tasks, int64_t n, int64_t least, int64
 }
 
 // How the call is dealt out, by its sizes and the caller's hints alone.
-AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
+AttendPlan plan_of(const AttendArgs& a, int type, int max_new, int64_t max_len) {
   AttendPlan p{};
   if (a.p.seqs < 1 || a.p.tokens < 1) return p;
   const int D = width_of(a.p.dim);
@@ -180,7 +180,9 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
     p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   }
   if (p.chunk) {
-    p.chunk_tiles = tile_count(a.p.tokens, a.group, kChunkTile, a.p.seqs);
+    const bool quant = quant_type(a.cache_type);
+    const int tile = !quant ? kChunkTile : type == kF32 ? quant_tile<float>(a.p.dim / 32) : quant_tile<__bf16>(a.p.dim / 32);
+    p.chunk_tiles = tile_count(a.p.tokens, a.group, tile, a.p.seqs);
     // Two workgroups per CU (heads of up to 64: three), of the tiles that have rows
     // when they are all of one sequence (509 tokens of 28 heads beside 16 that
     // decode: 141 us when the empty tiles of those count too, 126 us so); parts of
@@ -193,8 +195,8 @@ AttendPlan plan_of(const AttendArgs& a, int max_new, int64_t max_len) {
     // four run at once of 16-bit queries in heads of up to 64, two and one (heads of
     // 72 to 128) over an fp32 cache, one of wider heads (300 tokens over 4000 fp32
     // keys, heads of 128: 227 us when rounded up, 262 so).
-    const int64_t wgs = ((int64_t)a.p.tokens * a.group + kChunkTile - 1) / kChunkTile * a.p.kv_heads;
-    const int64_t places = D == 64 ? 768 : 512, down = places / wgs > 1 ? places / wgs : 1;
+    const int64_t wgs = ((int64_t)a.p.tokens * a.group + tile - 1) / tile * a.p.kv_heads;
+    const int64_t places = tile > kChunkTile || (quant && D == 256) ? 256 : D == 64 ? 768 : 512, down = places / wgs > 1 ? places / wgs : 1;
     // (tiles of no rows are launched too: sequences beyond number do not multiply)
     const int64_t n = down * wgs * 4 >= places * 3 ? down : down + 1, room = 16384 / (p.chunk_tiles * a.p.kv_heads);
     p.chunk_parts = parts_of_keys(most, wgs, n < room ? n : room > 1 ? room : 1, 512, most);
@@ -212,18 +214,18 @@ Parts placed(Parts p, void* work, int D) {
 
 // The rows whose keys were split.
 template <typename T, int D>
-hipError_t join(const AttendArgs& a, const AttendPlan& p, const Parts& few, const Parts& chunk, float few_shift,
-                float chunk_shift, hipStream_t s) {
+hipError_t join(const AttendArgs& a, const AttendPlan& p, const Parts& few, const Parts& chunk, int chunk_tile,
+                float few_shift, float chunk_shift, hipStream_t s) {
   const int per = a.group >= 16 ? 1 : 16 / a.group;  // tokens that few_rows takes of a sequence
   const int64_t few_rows = few.most > 1 ? (int64_t)a.p.seqs * per * a.heads : 0;
   const int64_t rows = few_rows + (chunk.most > 1 ? (int64_t)a.p.tokens * a.heads : 0);
   if (rows == 0) return hipSuccess;
   if (rows < 1024)
     join_kernel<T, D, 4><<<(unsigned)rows, kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
-                                                                few_shift, chunk_shift);
+                                                                chunk_tile, few_shift, chunk_shift);
   else
     join_kernel<T, D, 1><<<(unsigned)((rows + 3) / 4), kJoinThreads, 0, s>>>(a, few, chunk, few_rows, per, p.few_tiles, !p.few,
-                                                                          few_shift, chunk_shift);
+                                                                          chunk_tile, few_shift, chunk_shift);
   return hipGetLastError();
 }
 
@@ -246,7 +248,7 @@ hipError_t attend_width(const AttendArgs& a, const AttendPlan& p, int type, int 
   if (p.chunk &&
       (e = launch_chunk(a, type, cache_type, chunk, p.chunk_tiles, p.few ? &few : nullptr, p.few_tiles, s)) != hipSuccess)
     return e;
-  return join<T, D>(a, p, few, chunk, Elem<TC>::kShift, chunk_shift<TC>(), s);
+  return join<T, D>(a, p, few, chunk, kChunkTile, Elem<TC>::kShift, chunk_shift<TC>(), s);
 }
 
 template <typename T, typename TC>
@@ -269,7 +271,7 @@ hipError_t attend_quant_width(const AttendArgs& a, const AttendPlan& p, int type
   hipError_t e;
   if (p.few && (e = launch_few_quant(a, type, cache_type, few, p.few_tiles, p.chunk, s)) != hipSuccess) return e;
   if (p.chunk && (e = launch_chunk_quant(a, type, cache_type, chunk, p.chunk_tiles, !p.few, s)) != hipSuccess) return e;
-  return join<T, D>(a, p, few, chunk, kQuantShift, chunk_shift<_Float16>(), s);
+  return join<T, D>(a, p, few, chunk, quant_tile<T>(a.p.dim / 32), kQuantShift, chunk_shift<_Float16>(), s);
 }
 
 template <typename T>
@@ -282,13 +284,19 @@ hipError_t attend_quant(const AttendArgs& a, const AttendPlan& p, int type, int 
 }  // namespace
 
 size_t attend_workspace(const AttendArgs& a, int max_new, int64_t max_len) {
-  const AttendPlan p = plan_of(a, max_new, max_len);
-  return (p.few_bytes + 255) / 256 * 256 + p.chunk_bytes;
+  // (whatever type the queries will be: chunks over blocks are dealt out by it)
+  size_t most = 0;
+  for (int type : {kF32, kBF16}) {
+    const AttendPlan p = plan_of(a, type, max_new, max_len);
+    const size_t n = (p.few_bytes + 255) / 256 * 256 + p.chunk_bytes;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 hipError_t launch_attend(const AttendArgs& a, int type, int cache_type, int max_new, int64_t max_len, void* work,
                          hipStream_t s) {
-  const AttendPlan p = plan_of(a, max_new, max_len);
+  const AttendPlan p = plan_of(a, type, max_new, max_len);
   char* w = static_cast<char*>(work);
   if (quant_type(cache_type)) {
     if (a.p.seqs < 1 || a.p.tokens < 1) return hipSuccess;

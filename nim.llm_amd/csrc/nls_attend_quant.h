@@ -574,6 +574,16 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
   }
 }
 
+// Rows of a workgroup of the chunk kernel, 32 to a wave.  Turning codes into
+// operands is work that the waves share: fp32 queries in heads of 96 and 128, whose
+// values are two parts, take eight waves (2048 tokens over 16384 keys, Q4_0: 1530
+// us with four, 1424 so); elsewhere four are as fast (bf16, heads of 128: 814 and
+// 816) or faster (heads of 64: 157 and 186).
+template <typename T>
+constexpr int quant_tile(int groups) {
+  return sizeof(T) == 4 && (groups == 3 || groups == 4) ? 256 : 128;
+}
+
 // Launched by launch_attend (nls_attend.hip), which joins the parts.
 hipError_t launch_few_quant(const AttendArgs& a, int type, int cache_type, const Parts& parts, int few_tiles,
                             bool chunk_runs, hipStream_t s);

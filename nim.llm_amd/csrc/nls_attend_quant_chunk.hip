@@ -1,10 +1,10 @@
 // nls_attend_quant_chunk.hip -- attention of chunks over pages of blocks:
 // sequences of more than 16 rows (token, head of the group) per kv head.
 //
-// As for chunks over wide caches (nls_attend_chunk.hip), a workgroup takes 128
-// rows of one (sequence, kv head), 32 per wave, S^T = K Q^T and O^T = V^T P^T on
-// 32 x 32 products, tiles of keys in LDS two at a time, and the maximum follows
-// the scores only when it is passed by 2^8.  What differs:
+// As for chunks over wide caches (nls_attend_chunk.hip), a wave takes 32 rows of
+// one (sequence, kv head), S^T = K Q^T and O^T = V^T P^T are 32 x 32 products,
+// tiles of keys are in LDS two at a time, and the maximum follows the scores only
+// when it is passed by 2^8.  What differs:
 //
 //   K   LDS holds the codes as fp16, which is exact.  Two products over a block
 //       are its depth; their sums are multiplied by the block's factor in fp32
@@ -21,10 +21,6 @@
 namespace nls {
 namespace {
 
-constexpr int kChunkWaves = 4;
-constexpr int kChunkThreads = 64 * kChunkWaves;
-static_assert(kChunkTile == 32 * kChunkWaves, "32 rows per wave");
-
 __device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 typedef short s4x __attribute__((ext_vector_type(4)));
@@ -34,16 +30,17 @@ template <typename T, int kBits, int GT>
 struct QTile {
   static constexpr int D = 32 * GT;
   static constexpr int NP = quant_parts<T>();
-  static constexpr int KT = GT == 2 || (GT == 4 && NP == 1) ? 64 : 32;  // keys per tile
+  static constexpr int kRows = quant_tile<T>(GT), kWaves = kRows / 32, kThreads = 64 * kWaves;
+  static constexpr int KT = GT == 8 ? 32 : 64;                  // keys per tile
   static constexpr int kRuns = KT / 16;                 // of keys within a page
   static constexpr int kPieces = D / 8;                 // 16-byte pieces of a row
   static constexpr int kTiles = GT;                     // of O^T
   static constexpr int kBytes = KT * D * 2;             // of one of the three below
   static constexpr int kFactors = GT * KT * 2;
   static constexpr int kStage = kBytes * (1 + NP) + kFactors;  // K, V (and its rest), K's factors
-  static constexpr int kUnits = KT * 4 * GT / kChunkThreads;   // key units of a thread
+  static constexpr int kUnits = KT * 4 * GT / kThreads;        // key units of a thread
   static constexpr int kWide = GT < 4 ? GT : 4;                // blocks of a plane
-  static constexpr int kLanes = KT * 16 * (GT / kWide) / kChunkThreads;  // value pieces of a thread, side by side
+  static constexpr int kLanes = KT * 16 * (GT / kWide) / kThreads;  // value pieces of a thread, side by side
   static constexpr int kKeyWords = kUnits * kBits / 4, kValueBytes = kLanes * kWide * kBits / 4;
   static constexpr int kValueWords = (kValueBytes + 3) / 4;
   static_assert(kUnits <= GT && kUnits >= 1 && kLanes >= 2, "a thread's units are of one quarter, its pieces of one plane");
@@ -64,8 +61,8 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   constexpr float kShift = chunk_shift<_Float16>();
   extern __shared__ __align__(16) char chunk_lds[];  // [2][K, V, V's rest, K's factors]
   __shared__ uint8_t noted[2][KT];                   // bit x: block x of a value was not finite
-  __shared__ int has_noted[2][kChunkWaves];
-  __shared__ float max_times[kScaled ? kChunkTile : 1];
+  __shared__ int has_noted[2][L::kWaves];
+  __shared__ float max_times[kScaled ? L::kRows : 1];
 
   const int kvh = group_at % a.p.kv_heads, tile = (groups_n - 1 - group_at) / a.p.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
@@ -74,7 +71,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   int seq = -1;
   for (int s0 = 0; s0 < a.p.seqs; s0 += 64) {
     const int s = s0 + lane;
-    const int n = __popcll(__ballot(s < a.p.seqs && tile_base(a.p.starts[s < a.p.seqs ? s : 0], a.group, kChunkTile, s) <= tile));
+    const int n = __popcll(__ballot(s < a.p.seqs && tile_base(a.p.starts[s < a.p.seqs ? s : 0], a.group, L::kRows, s) <= tile));
     seq += n;
     if (n < 64) break;
   }
@@ -82,9 +79,9 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   const Chunk c = chunk_of(a.p, seq);
   const int rows = c.n * a.group;
   if (!alone && (rows <= 16 || c.n == 1)) return;  // few_quant_rows'
-  const int64_t r0l = (tile - tile_base(c.begin, a.group, kChunkTile, seq)) * kChunkTile;
+  const int64_t r0l = (tile - tile_base(c.begin, a.group, L::kRows, seq)) * L::kRows;
   if (r0l < 0 || r0l >= rows) return;
-  const int r0 = (int)r0l, rn = rows - r0 < kChunkTile ? rows - r0 : kChunkTile;
+  const int r0 = (int)r0l, rn = rows - r0 < L::kRows ? rows - r0 : L::kRows;
   const Sees sees = sees_of(a, c);
   const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
   const Span span = span_of(sees, t0, t1, parts.keys, parts.most);
@@ -157,26 +154,28 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   const bool f_mine = f_x < groups;
   const char* base = static_cast<const char*>(a.p.kv) + quant_base(shape, kvh, 0);
   const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
+  // The table's entries of a tile: its runs', and once more this wave's run's and
+  // that of this lane's factors.
   struct Entries {
-    int at[L::kRuns];
+    int at[L::kRuns], run, factors;
   };
+  auto entry_of = [&](int key) { return table[(key < k1 ? key : k1 - 1) >> a.p.page_shift]; };
   auto entries_at = [&](int kb) {
     Entries e;
 #pragma unroll
-    for (int r = 0; r < L::kRuns; ++r) {
-      const int key = kb + r * 16;
-      e.at[r] = table[(key < k1 ? key : k1 - 1) >> a.p.page_shift];
-    }
+    for (int r = 0; r < L::kRuns; ++r) e.at[r] = entry_of(kb + r * 16);
+    e.run = entry_of(kb + run * 16);
+    e.factors = f_mine ? entry_of(kb + f_key) : 0;
     return e;
   };
   // (from kb on; -1: none, and what is read there is page 0)
+  auto page_of_entry = [&](int key, int page) { return key < k1 && (uint32_t)page < (uint32_t)a.p.pages ? page : -1; };
   auto pages_at = [&](int kb, const Entries& e) {
     Entries p;
 #pragma unroll
-    for (int r = 0; r < L::kRuns; ++r) {
-      const int page = __builtin_amdgcn_readfirstlane(e.at[r]);
-      p.at[r] = kb + r * 16 < k1 && (uint32_t)page < (uint32_t)a.p.pages ? page : -1;
-    }
+    for (int r = 0; r < L::kRuns; ++r) p.at[r] = page_of_entry(kb + r * 16, __builtin_amdgcn_readfirstlane(e.at[r]));
+    p.run = page_of_entry(kb + run * 16, __builtin_amdgcn_readfirstlane(e.run));
+    p.factors = page_of_entry(kb + (f_key & ~15), e.factors);
     return p;
   };
   // bit n: key n of the tile is there
@@ -192,14 +191,9 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   uint32_t kc[L::kKeyWords], vc[L::kValueWords];
   u4 kf;             // factors of 8 keys
   _Float16 vd[L::kWide];
-  auto page_at = [&](const Entries& p, int r) {
-    int page = p.at[0];
-#pragma unroll
-    for (int n = 1; n < L::kRuns; ++n) page = r == n ? p.at[n] : page;
-    return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride;
-  };
+  auto home_of = [&](int page) { return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride; };
   auto fetch = [&](int kb, const Entries& p) {
-    const char* home = page_at(p, run);
+    const char* home = home_of(p.run);
     const int place = ((uint32_t)kb + run * 16) & (size - 1);  // of the run
     const char* keys = home + (place + (k_row & 15)) * row_bytes + (k_g * groups + k_x) * kBits;
     const char* values = home + shape.half + (place + (v_row & 15)) * row_bytes;
@@ -239,7 +233,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       }
     }
     if (f_mine) {
-      const char* there = page_at(p, f_key / 16);
+      const char* there = home_of(p.factors);
       kf = *reinterpret_cast<const u4*>(there + shape.codes + (f_x * size + (((uint32_t)kb + f_key) & (size - 1))) * 2);
     }
   };
@@ -516,7 +510,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
 
 // alone: sequences of few rows are its too
 template <typename T, int kBits, int GT, bool kPad>
-__global__ __launch_bounds__(kChunkThreads, GT == 8 ? 1 : 2) void chunk_quant_kernel(AttendArgs a, Parts parts, bool alone) {
+__global__ __launch_bounds__((QTile<T, kBits, GT>::kThreads), GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2) void chunk_quant_kernel(AttendArgs a, Parts parts, bool alone) {
   chunk_quant_rows<T, kBits, GT, kPad>(a, parts, alone, blockIdx.x, gridDim.x, blockIdx.z);
 }
 
@@ -529,7 +523,7 @@ hipError_t chunk_of(const AttendArgs& a, const Parts& parts, int64_t tiles, bool
     if (e != hipSuccess) return e;
   }
   chunk_quant_kernel<T, kBits, GT, kPad>
-      <<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), kChunkThreads, lds, s>>>(a, parts, alone);
+      <<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), QTile<T, kBits, GT>::kThreads, lds, s>>>(a, parts, alone);
   return hipGetLastError();
 }
 
