@@ -447,7 +447,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
     for (int sub = 0; sub < NS; ++sub)
       if (used) step(whole, sub, lk, kb, there);
     if (more) put(chunk_lds + (buf ^ 1) * L::kStage, there1, kb + KT, buf ^ 1);
-    if (used && mixed(kb) && (has_noted[buf][0] | has_noted[buf][1] | has_noted[buf][2] | has_noted[buf][3])) {
+    if (used && mixed(kb) && __ballot(lane < L::kWaves && has_noted[buf][lane % L::kWaves])) {
 #pragma unroll 1
       for (int n = 0; n < KT; ++n) {
         const int key = kb + n;

@@ -92,7 +92,9 @@ def attend(q, kv, kind, table, lens, starts, scale, window=0, first=None, slots=
     out = np.full(q.shape, np.nan)
     lse, ob, lb = np.full(q.shape[:2], np.nan), np.full(q.shape, np.nan), np.full(q.shape[:2], np.nan)
     most = 127 if kind == "q8_0" else 8
-    part = 2.0 ** -22 if q.dtype == torch.float32 else 2.0 ** -11  # of a weight times a factor
+    # of a weight times a factor or a value: two parts each, or one of eleven bits
+    # (few rows: of the weight times the factor; chunks: of the weight and of the value)
+    part = 2.0 ** -22 if q.dtype == torch.float32 else 2.0 ** -10
     for i in range(len(starts) - 1):
         a, b = starts[i], starts[i + 1]
         if a == b:
@@ -138,12 +140,13 @@ def attend(q, kv, kind, table, lens, starts, scale, window=0, first=None, slots=
                 # A weight: its score's error twice, the exponential, its product
                 # with the factor as parts; sums over the keys, joined parts
                 # among them.  And fp16's least step, at 2^14 for the largest
-                # weight times a power of two over the largest factor, per code.
+                # weight times a power of two over the largest factor, per code;
+                # for chunks, at 2^7 for a weight of 1, per value: half of 2^-24 2^-7.
                 count = int(m.sum())
                 dw = 2 * ds + 2.0 ** -21 + 2 * (count + 16) * e32
                 mean = p @ np.abs(vt)
                 big = np.abs(vt).max() * 2 if kind == "q8_0" else np.abs(vt).max() * 8
-                ob[a + t, h] = (mean * (dw * (1 + dw) + part) + count * 2.0 ** -38 * big
+                ob[a + t, h] = (mean * (dw * (1 + dw) + part) + count * (2.0 ** -38 * big + 2.0 ** -32 * np.abs(vt).max())
                                 + np.abs(out[a + t, h]) * HALF[q.dtype] * 2 + 1e-37 + (2.0 ** -25 if q.dtype == torch.float16 else 0))
                 lb[a + t, h] = dw + abs(l) * 4 * e32
     return out, lse, ob, lb

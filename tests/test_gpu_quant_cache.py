@@ -319,3 +319,484 @@ def test_attention_long_single_token(pkg, kind, dtype):
     m.check(pkg)
     m.check(pkg, window=4000)
     m.check(pkg, hints=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+def test_attention_rows_without_keys(pkg, kind, dtype):
+    """Empty slots, slots out of range, pages out of range, lengths of zero and
+    shorter than their rows, first keys behind the context."""
+    m = Made(pkg, kind, [40, 0, 70, 33], [3, 2, 20, 1, 4], 4, 2, 64, 16, dtype, seed=3, slots=[0, 1, 2, 7, 3])
+    m.table_l[0][1] = -1
+    m.table_l[2][2] = 10 ** 6
+    m.table_l[3][0] = -(2 ** 31)
+    m.table = torch.tensor(m.table_l, dtype=torch.int32)
+    m.check(pkg)
+    m.check(pkg, first=[41, 0, 69, 32], what="first")
+    m.check(pkg, window=1, what="itself alone")
+    m.lens_l[3] = 2  # four rows, two tokens
+    m.lens = torch.tensor(m.lens_l, dtype=torch.int32)
+    m.check(pkg, what="short")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAME.get)
+@pytest.mark.parametrize("lens,new,heads,d", [([100], [1], 4, 64), ([90], [3], 4, 128), ([150], [60], 8, 64), ([150], [90], 8, 128),
+                                              ([120, 40], [70, 1], 4, 256)])
+def test_attention_blocks_that_are_not_finite(pkg, kind, dtype, lens, new, heads, d):
+    """A value's factor of NaN reaches that block of the rows that see its key, a
+    key's all of them; others stay what they are."""
+    m = Made(pkg, kind, lens, new, heads, 2, d, 16, dtype, seed=d)
+    m.check(pkg)
+    bits = R.BITS[kind]
+    codes, half = 16 * d * bits // 8, 16 * d * bits // 8 + 16 * d // 32 * 2
+    n, c = lens[0], new[0]
+    for what, key, block in ((1, n - 1, 0), (1, n - max(1, c // 2), d // 32 - 1), (0, n - max(1, c // 3), 1), (1, 0, 1)):
+        raw = m.raw.copy()
+        page, place = m.table_l[0][key // 16], key % 16
+        o = (0 * 2 + what) * half + codes + (block * 16 + place) * 2  # kv head 0
+        raw[page, o:o + 2] = np.array([np.nan], dtype=np.float16).view(np.uint8)
+        for window in (0, 20):
+            want, wl, ob, lb = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, m.scale, window)  # all finite
+            got, lse = pkg.paged_attention(m.q.cuda(), torch.from_numpy(raw).cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(),
+                                           max(new), max(lens), window=window, lse=True, fmt=m.fmt)
+            got, lse = got.cpu(), lse.cpu()
+            pos = torch.arange(n - c, n)
+            sees = (pos >= key) & ((pos - key < window) if window else True)
+            hit = torch.zeros(got.shape, dtype=torch.bool)
+            if what == 0:
+                hit[:c, :heads // 2] = sees[:, None, None]
+                assert torch.equal(torch.isnan(lse[:c, :heads // 2]), sees[:, None].expand(-1, heads // 2))
+            else:
+                hit[:c, :heads // 2, block * 32:block * 32 + 32] = sees[:, None, None]
+            assert bool(torch.isnan(got[hit]).all()), (what, key, block, window)
+            near(got, np.where(hit, np.nan, want), ob, f"{what} {key} {block} {window} out")
+            if what == 1:
+                near(lse, wl, lb, f"{what} {key} {block} {window} lse")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+@pytest.mark.parametrize("spread", [1e-4, 30.0, "tokens", "blocks"])
+@pytest.mark.parametrize("lens,new", [([300], [1]), ([200], [3]), ([150], [70])])
+def test_attention_factors_of_any_size(pkg, kind, dtype, spread, lens, new):
+    """Small and large values, factors that differ by 2^10 between tokens or
+    blocks (what lies below 2^-38 of the largest is in the bound)."""
+
+    def contents(gen, shape):
+        x = gen.standard_normal(shape).astype(np.float32)
+        if spread == "tokens":
+            x *= 2.0 ** gen.integers(-10, 1, shape[:4] + (1,)).astype(np.float32)
+        elif spread == "blocks":
+            x *= np.repeat(2.0 ** gen.integers(-10, 1, shape[:4] + (shape[4] // 32,)).astype(np.float32), 32, -1)
+        else:
+            x[:, 1] *= np.float32(spread)
+        return x
+
+    Made(pkg, kind, lens, new, 4, 2, 128, 16, dtype, seed=7, contents=contents).check(pkg)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+@pytest.mark.parametrize("lens,new", [([60], [1]), ([130], [40])])
+def test_attention_scales(pkg, kind, dtype, lens, new):
+    m = Made(pkg, kind, lens, new, 4, 1, 64, 16, dtype, seed=9)
+    for scale in (0.0, -0.125, 1.0, 1e-30, 30.0):
+        m.check(pkg, scale=scale, what=f"scale {scale}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAME.get)
+@pytest.mark.parametrize("lens,new", [([90], [1]), ([150], [40])])
+def test_attention_one_key_far_above_the_others(pkg, kind, dtype, lens, new):
+    """Scores of up to 10^8: the row's largest has all the weight, whose value is
+    then the row (twice the output's half step, and the weight's part)."""
+    m = Made(pkg, kind, lens, new, 4, 2, 64, 16, dtype, seed=11)
+    for scale in (1e4, 1e7):
+        got, lse = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), max(new),
+                                       max(lens), scale=scale, lse=True, fmt=m.fmt)
+        v = m.values()
+        at = np.arange(lens[0])
+        k, x = (v[np.array(m.table_l[0])[at // 16], z, :, at % 16] for z in (0, 1))
+        for t in range(new[0]):
+            n = lens[0] - new[0] + t + 1
+            for h in range(4):
+                s = k[:n, h // 2] @ m.q[t, h].double().numpy() * scale
+                order = np.argsort(s)
+                # (what fp32 cannot tell apart: 80 products and sums of the row)
+                noise = np.abs(k[:n, h // 2]) @ np.abs(m.q[t, h].double().numpy()) * scale * 80 * 2.0 ** -24
+                if s[order[-1]] - s[order[-2]] < 2 * noise.max() + 120:
+                    continue
+                want = x[order[-1], h // 2]
+                off = np.abs(got[t, h].double().cpu().numpy() - want)
+                # (elements next to 0 beside larger ones of their block: the weight times
+                # the factor is rounded, not the element)
+                assert (off <= np.abs(want) * (2 * R.HALF[dtype] + 2.0 ** -11) + 1e-30).all()
+                assert abs(float(lse[t, h]) - s[order[-1]]) <= noise.max() + 2.0 ** -22 * abs(s[order[-1]])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAME.get)
+def test_attention_strided_rows_and_rows_of_no_sequence(pkg, kind, dtype):
+    m = Made(pkg, kind, [70, 55], [40, 3], 6, 2, 64, 16, dtype, seed=6)
+    tokens = m.starts_l[-1]
+    base = torch.zeros(6, tokens + 5, 64 + 3, dtype=dtype, device="cuda")
+    q = base.permute(1, 0, 2)[2:2 + tokens, :, 1:65]
+    q.copy_(m.q.cuda())
+    dest = torch.full((tokens + 5, 7, 67), 7.0, dtype=dtype, device="cuda")
+    m.check(pkg, q=q, out=dest[2:2 + tokens, :6, 1:65])
+    assert bool((dest[:2] == 7).all()) and bool((dest[2 + tokens:] == 7).all())
+    assert bool((dest[:, 6] == 7).all()) and bool((dest[..., 0] == 7).all()) and bool((dest[..., 65:] == 7).all())
+    # padding before, behind and as sequences of no rows
+    starts = torch.tensor([2, 2, 42, 42, 45], dtype=torch.int32).cuda()
+    slots = torch.tensor([1, 0, 0, 1], dtype=torch.int32).cuda()
+    pad = torch.zeros(tokens + 5, 6, 64, dtype=dtype, device="cuda")
+    pad[2:45] = m.q.cuda()
+    out, l = torch.full_like(pad, 7.0), torch.full((tokens + 5, 6), 7.0, device="cuda")
+    pkg.paged_attention(pad, m.kv_cuda(), m.table.cuda(), m.lens.cuda(), starts, 40, 70, slots=slots, out=out, lse=l, fmt=m.fmt)
+    right, rl, ob, lb = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, m.scale)
+    near(out[2:45], right, ob, "padded")
+    near(l[2:45], rl, lb, "padded lse")
+    for x in (out, l):
+        assert bool((x[:2] == 7).all()) and bool((x[45:] == 7).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,heads,kv_heads,d", [(F32, 8, 2, 128), (BF16, 8, 2, 64), (F16, 28, 4, 128), (F32, 4, 1, 256), (BF16, 6, 2, 96)])
+def test_attention_mixed_batches(pkg, kind, dtype, heads, kv_heads, d):
+    lens, new = [300, 41, 90, 700, 64, 5], [130, 1, 30, 1, 2, 5]
+    m = Made(pkg, kind, lens, new, heads, kv_heads, d, 32, dtype, seed=d)
+    m.check(pkg)
+    m.check(pkg, window=100, what="window")
+    m.check(pkg, hints=False, what="no hints")
+    # hints that are wrong either way
+    args = (m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda())
+    want, lse, ob, lb = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, m.scale)
+    for max_new, max_len in ((1, 10), (1, 1 << 40), (1 << 20, 64), (0, 700)):
+        got, l = pkg.paged_attention(*args, max_new, max_len, lse=True, fmt=m.fmt)
+        near(got, want, ob, f"hints {max_new} {max_len}")
+        near(l, lse, lb, f"hints {max_new} {max_len} lse")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_many_empty_sequences(pkg, kind):
+    m = Made(pkg, kind, [100], [30], 4, 2, 64, 16, F32, seed=1)
+    want, _, ob, _ = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, m.scale)
+    n = 3000
+    starts = torch.cat([torch.zeros(n, dtype=torch.int32), torch.tensor([0, 30], dtype=torch.int32), torch.full((n,), 30, dtype=torch.int32)]).cuda()
+    slots = torch.zeros(2 * n + 1, dtype=torch.int32).cuda()
+    args = (m.kv_cuda(), m.table.cuda(), m.lens.cuda(), starts)
+    got = pkg.paged_attention(m.q.cuda(), *args, 30, 100, slots=slots, fmt=m.fmt)
+    near(got, want, ob)
+    k, v = pkg.cache_read(*args, 30, slots=slots, fmt=m.fmt)
+    assert torch.equal(k, pkg.cache_read(m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), 30, fmt=m.fmt)[0])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_far_pages(pkg, kind):
+    """Offsets beyond 32 bits: pages 2^29 bytes apart."""
+    fmt = pkg.PageFormat(kind, 2, 16, 64)
+    apart, pages = 1 << 29, 12
+    far = torch.zeros(apart * (pages - 1) + fmt.page_bytes, dtype=torch.uint8, device="cuda").as_strided((pages, fmt.page_bytes), (apart, 1))
+    near_ = torch.zeros(pages, fmt.page_bytes, dtype=torch.uint8, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    table = torch.tensor([[11, 9, 10, 8, 1]], dtype=torch.int32).cuda()
+    lens, n = torch.tensor([75], dtype=torch.int32).cuda(), 75
+    k, v = (torch.randn(n, 2, 64, generator=g).cuda() for _ in range(2))
+    q = torch.randn(n, 4, 64, generator=g).cuda()
+    starts = torch.tensor([0, n], dtype=torch.int32).cuda()
+    out = []
+    for kv in (far, near_):
+        pkg.cache_append(kv, table, lens, starts, k, v, fmt=fmt)
+        one = torch.tensor([0, 1], dtype=torch.int32).cuda()
+        out.append([*pkg.cache_read(kv, table, lens, starts, n, fmt=fmt), pkg.paged_attention(q, kv, table, lens, starts, n, n, fmt=fmt),
+                    pkg.paged_attention(q[:1], kv, table, lens, one, 1, n, fmt=fmt)])
+    assert torch.equal(far, near_)
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and bool(a.abs().sum() > 0)
+
+
+# ---------------------------------------------------------------- streams, graphs, refusals
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_step_captured_and_replayed(pkg, kind):
+    """Append, read and attention of a chunk and of single tokens in one graph,
+    replayed over other inputs between eager work."""
+    m = Made(pkg, kind, [150, 60, 2100], [40, 1, 1], 4, 2, 64, 16, F32, seed=4)
+    kv, table, lens, starts = m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda()
+    g = torch.Generator().manual_seed(8)
+    ins = [(torch.randn(42, 4, 64, generator=g).cuda(), torch.randn(42, 2, 64, generator=g).cuda(), torch.randn(42, 2, 64, generator=g).cuda())
+           for _ in range(4)]
+    q, k, v = (x.clone() for x in ins[0])
+    plan = pkg.rope_plan(64)
+
+    def step():
+        turned = pkg.cache_append(kv, table, lens, starts, k, v, q=q, plan=plan, fmt=m.fmt)
+        return (turned, *pkg.cache_read(kv, table, lens, starts, 42, fmt=m.fmt),
+                *pkg.paged_attention(turned, kv, table, lens, starts, 40, 2100, lse=True, fmt=m.fmt))
+
+    want = []
+    for x in ins:
+        for to, fr in zip((q, k, v), x):
+            to.copy_(fr)
+        want.append([y.clone() for y in step()])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step()
+    torch.cuda.current_stream().wait_stream(stream)
+    for again in range(2):
+        for x, w in zip(ins, want):
+            for to, fr in zip((q, k, v), x):
+                to.copy_(fr)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got, w):
+                assert torch.equal(a, b)
+            torch.randn(1000, 1000, device="cuda").sum().item()
+
+
+def test_two_streams_at_once_and_same_bits(pkg):
+    made = [Made(pkg, k, [500, 3000], [40, 1], 8, 2, 128, 32, t, seed=s) for s, (k, t) in enumerate([("q4_0", F32), ("q8_0", BF16)])]
+    args = [(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), 40, 3000) for m in made]
+    want = [pkg.paged_attention(*a, fmt=m.fmt).clone() for m, a in zip(made, args)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(pkg.paged_attention(*args[i], fmt=made[i].fmt))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
+
+
+def test_refused_calls(pkg):
+    m = Made(pkg, "q4_0", [40], [3], 4, 2, 64, 16, F32)
+    kv, table, lens, starts, q = m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), m.q.cuda()
+    k = torch.zeros(3, 2, 64).cuda()
+    bad = pkg.SamplerError, AssertionError
+    for kw in (dict(kv=kv[:, :-16]), dict(kv=kv.view(kv.shape[0], -1, 16)), dict(kv=kv.cpu()), dict(fmt=pkg.PageFormat("q8_0", 2, 16, 64)),
+               dict(fmt=pkg.PageFormat("q4_0", 2, 8, 64)), dict(fmt=pkg.PageFormat("q4_0", 2, 16, 60)), dict(fmt=pkg.PageFormat("q5_0", 2, 16, 64)),
+               dict(fmt=pkg.PageFormat("q4_0", 2, 24, 64)), dict(fmt=pkg.PageFormat("q4_0", 0, 16, 64)), dict(fmt=pkg.PageFormat("q4_0", 2, 16, 288))):
+        a = dict(kv=kv, fmt=m.fmt)
+        a.update(kw)
+        with pytest.raises(bad):
+            pkg.paged_attention(q, a["kv"], table, lens, starts, fmt=a["fmt"])
+        with pytest.raises(bad):
+            pkg.cache_append(a["kv"], table, lens, starts, k, k, fmt=a["fmt"])
+        with pytest.raises(bad):
+            pkg.cache_read(a["kv"], table, lens, starts, 3, fmt=a["fmt"])
+    for kw in (dict(k=k.double()), dict(k=k[:, :1]), dict(v=k[:2]), dict(k=k.int())):
+        a = dict(k=k, v=k)
+        a.update(kw)
+        with pytest.raises(bad):
+            pkg.cache_append(kv, table, lens, starts, a["k"], a["v"], fmt=m.fmt)
+        with pytest.raises(bad):
+            pkg.cache_read(kv, table, lens, starts, 3, k=a["k"], v=a["v"], fmt=m.fmt)
+    with pytest.raises(bad):
+        pkg.cache_read(kv, table, lens, starts, 3, dtype=torch.float64, fmt=m.fmt)
+    with pytest.raises(bad):
+        pkg.paged_attention(q[..., :32], kv, table, lens, starts, fmt=m.fmt)
+    with pytest.raises(bad):
+        pkg.paged_attention(q, kv, table, lens, starts, scale=math.inf, fmt=m.fmt)
+    # nothing to do is no error
+    none = torch.zeros(1, dtype=torch.int32).cuda()
+    pkg.cache_append(kv, table, lens, none, k[:0], k[:0], fmt=m.fmt)
+    assert pkg.cache_read(kv, table, lens, none, 0, fmt=m.fmt)[0].shape == (0, 2, 64)
+    assert pkg.paged_attention(q[:0], kv, table, lens, none, fmt=m.fmt).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------- together
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_pages_of_blocks_forked_compacted_and_copied(pkg, kind):
+    """The calls that move whole pages move pages of blocks as they are."""
+    heads, d, page, layers = 2, 64, 16, 2
+    cache = pkg.PagedCache(layers, 20, page, heads, d, 4, 6, dtype=kind)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(3)
+    lens = [40, 33, 0, 16]
+    starts = ints([0, 40, 73, 73, 89])
+    assert int(cache.reserve(ints(lens))) == pkg.PAGES_DONE
+    rows = [[torch.randn(89, heads, d, generator=g).cuda() for _ in range(2)] for _ in range(layers)]
+    for i, (k, v) in enumerate(rows):
+        cache.append(i, k, v, starts)
+    before = [cache.read(i, starts, 89) for i in range(layers)]
+    for (k, v), (a, b) in zip(rows, before):
+        for x, y in ((k, a), (v, b)):
+            codes, f = R.blocks(x.cpu().numpy(), kind)
+            assert np.array_equal(y.cpu().double().numpy(), R.values(codes, f))
+    assert int(cache.fork(ints([0]), ints([2]))) == pkg.PAGES_DONE
+    assert cache.lens.tolist() == [40, 33, 40, 16]
+    assert int(cache.release(ints([0]))) == pkg.PAGES_DONE
+    assert int(cache.compact()) == 7 and cache.refs.tolist() == [1] * 7 + [0] * 13
+    again, slots = ints([0, 33, 73, 89]), ints([1, 2, 3])
+    for i, (a, b) in enumerate(before):
+        for x, y in zip(cache.read(i, again, 89, slots=slots), (a, b)):
+            assert torch.equal(x, torch.cat([y[40:73], y[:40], y[73:]]))
+    used = cache.kv[:, :7].clone()
+    pkg.cache_copy_pages(cache.kv, ints([0, 6]), ints([19, 10]), fmt=cache.fmt)
+    assert torch.equal(cache.kv[:, [19, 10]], used[:, [0, 6]]) and torch.equal(cache.kv[:, :7], used)
+
+
+@pytest.mark.parametrize("kind,dtype", [("q8_0", F32), ("q4_0", F32), ("q4_0", BF16)])
+def test_beam_search_over_blocks(pkg, kind, dtype):
+    """Prompts read as chunks, then steps of beam search over one cache of blocks:
+    room, append, attention, logits by an F32 head, the best continuations, the
+    contexts that follow them; each step against definitions over the contexts'
+    own tokens, and in the end every context read back."""
+    groups, beams, heads, kvh, d, page, vocab, layers = 2, 4, 4, 2, 64, 16, 501, 2
+    rows, steps, prompts = groups * beams, 9, [37, 19]
+    g = torch.Generator().manual_seed(12)
+    # a model of its own: a token's q, k and v by tables, the layers' outputs summed
+    tq, tk, tv = (torch.randn(layers, vocab, n, d, generator=g).to(dtype).cuda() for n in (heads, kvh, kvh))
+    head = (torch.randn(vocab, heads * d, generator=g) / 8).cuda()
+    raw = head.view(torch.uint8).reshape(-1)
+    eog = torch.tensor([3], dtype=torch.int32).cuda()
+    cache = pkg.PagedCache(layers, 64, page, kvh, d, rows, 10, dtype=kind)
+
+    def run(tokens, starts, slots, max_new):
+        hidden = 0
+        for i in range(layers):
+            cache.append(i, tk[i][tokens], tv[i][tokens], starts, slots=slots)
+            hidden = hidden + cache.attend(i, tq[i][tokens], starts, slots=slots, max_new=max_new).float()
+        return hidden.reshape(len(tokens), -1)
+
+    def defined(context):
+        """The logits after a context, in float64, and their bound."""
+        t = torch.tensor(context)
+        n, total, bound = len(context), 0, 0
+        for i in range(layers):
+            kv = np.empty((1, 2, kvh, n, d))
+            for z, x in ((0, tk), (1, tv)):
+                kv[0, z] = np.swapaxes(R.values(*R.blocks(x[i].cpu()[t].float().numpy(), kind)), 0, 1)
+            out, _, ob, _ = R.attend(tq[i].cpu()[t[-1:]], kv, kind, [[0]], [n], [0, 1], d ** -0.5)
+            total, bound = total + out, bound + ob
+        w = head.cpu().double().numpy()
+        total, bound = total.reshape(-1), bound.reshape(-1)
+        size = np.abs(w) @ np.abs(total)  # the sums of the layers and of the products
+        return w @ total, np.abs(w) @ bound + size * (heads * d + 4) * 2.0 ** -24
+
+    contexts = [torch.randint(0, vocab, (n,), generator=g).tolist() for n in prompts]
+    slots = torch.tensor([0, beams], dtype=torch.int32).cuda()
+    need = torch.zeros(rows, dtype=torch.int32)
+    need[0], need[beams] = prompts
+    assert int(cache.reserve(need.cuda())) == pkg.PAGES_DONE
+    starts = torch.tensor([0, prompts[0], sum(prompts)], dtype=torch.int32).cuda()
+    hidden = run(torch.tensor(sum(contexts, [])).cuda(), starts, slots, max(prompts))
+    first = hidden[(starts[1:] - 1).long()]
+    # every beam of a group starts as its first one; the others are worth nothing
+    parents = (torch.arange(rows) // beams * beams).int().cuda()
+    assert int(cache.reorder(parents)) == pkg.PAGES_DONE
+    contexts = [list(contexts[r // beams]) for r in range(rows)]
+    scores = torch.full((groups, beams), -math.inf).cuda()
+    scores[:, 0] = 0
+    ended = torch.zeros(groups, beams, dtype=torch.int32).cuda()
+    logits = pkg.lm_head(raw, 0, vocab, heads * d, first.repeat_interleave(beams, 0), exact=True)
+    one = torch.arange(rows + 1, dtype=torch.int32).cuda()
+    for step in range(steps):
+        say(f"[beam search] {kind} {NAME[dtype]} step {step}")
+        old, was = scores.cpu().double().numpy(), ended.cpu().numpy().reshape(-1)
+        parents, tokens, scores, ended = pkg.beam_select(logits, scores, ended=ended, eog=eog)
+        p, t, s, e = (x.reshape(-1).cpu() for x in (parents, tokens, scores, ended))
+        # what was chosen is worth what the definitions say, and nothing left out is worth more
+        for k in range(groups):
+            worth, bound = np.full((beams, vocab + 1), -np.inf), np.zeros((beams, vocab + 1))  # (last: itself)
+            for b in range(beams):
+                r = k * beams + b
+                if was[r]:
+                    worth[b, -1] = old[k, b]
+                elif old[k, b] > -math.inf:
+                    y, by = defined(contexts[r])
+                    assert (np.abs(logits[r].cpu().double().numpy() - y) <= by).all()
+                    top = y.max()
+                    lse = top + math.log(np.exp(y - top).sum())
+                    worth[b, :-1], bound[b, :-1] = old[k, b] + y - lse, by + by.max() + (np.abs(old[k, b]) + np.abs(y) + abs(lse) + 8) * 2.0 ** -20
+            mine = [(int(p[k * beams + b]), int(t[k * beams + b])) for b in range(beams)]
+            assert len(set(mine)) == beams and all(x // beams == k for x, _ in mine)
+            for b, (x, v) in enumerate(mine):
+                assert abs(float(s[k * beams + b]) - worth[x % beams, v]) <= bound[x % beams, v]
+                assert int(e[k * beams + b]) == int(bool(was[x]) or v == 3) and bool(was[x]) == (v == -1)
+            least = min(float(s[k * beams + b]) for b in range(beams))
+            rest = worth - bound
+            for x, v in mine:
+                rest[x % beams, v] = -np.inf
+            assert rest.max() <= least + bound.max()
+        assert int(cache.reorder(parents.reshape(-1))) == pkg.PAGES_DONE
+        contexts = [contexts[int(x)] + ([] if was[int(x)] else [int(v)]) for x, v in zip(p, t)]
+        # the ended ones wait: no new token of theirs
+        going = [r for r in range(rows) if not was[int(p[r])]]
+        need = torch.zeros(rows, dtype=torch.int32)
+        need[going] = 1
+        assert int(cache.reserve(need.cuda())) == pkg.PAGES_DONE
+        assert cache.lens.tolist() == [len(c) for c in contexts]
+        at = torch.tensor(going).cuda()
+        hidden = run(t[going].cuda().long(), one[:len(going) + 1], at.int(), 1)
+        logits = torch.zeros(rows, vocab, device="cuda")
+        logits[at] = pkg.lm_head(raw, 0, vocab, heads * d, hidden, exact=True)
+    starts = torch.tensor(np.concatenate([[0], np.cumsum([len(c) for c in contexts])]), dtype=torch.int32).cuda()
+    t = torch.tensor(sum(contexts, []))
+    for i in range(layers):
+        for got, x in zip(cache.read(i, starts, len(t)), (tk, tv)):
+            assert np.array_equal(got.cpu().double().numpy(), R.values(*R.blocks(x[i].cpu()[t].float().numpy(), kind)))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_beam_step_captured_and_replayed(pkg, kind):
+    """A step of beam search as one graph: room, append, attention, choice and the
+    contexts that follow, replayed over several steps beside the same steps alone."""
+    groups, beams, heads, kvh, d, page, vocab = 2, 3, 4, 2, 64, 16, 300
+    rows = groups * beams
+    g = torch.Generator().manual_seed(1)
+    head = (torch.randn(vocab, heads * d, generator=g) / 4).cuda()
+    table = torch.randn(vocab, heads + 2 * kvh, d, generator=g).cuda()
+    one, need = torch.arange(rows + 1, dtype=torch.int32).cuda(), torch.ones(rows, dtype=torch.int32).cuda()
+
+    def made():
+        cache = pkg.PagedCache(1, 40, page, kvh, d, rows, 7, dtype=kind)
+        cache.reserve(torch.full((rows,), 13, dtype=torch.int32).cuda())
+        x = torch.randn(rows * 13, 2 * kvh, d, generator=torch.Generator().manual_seed(5)).cuda()
+        cache.append(0, x[:, :kvh], x[:, kvh:], one * 13)
+        return [cache, torch.arange(rows, dtype=torch.int32).cuda() + 7, torch.zeros(groups, beams).cuda()]
+
+    def step(cache, tokens, scores):
+        cache.reserve(need)
+        x = table.index_select(0, tokens)
+        cache.append(0, x[:, heads:heads + kvh], x[:, heads + kvh:], one)
+        y = cache.attend(0, x[:, :heads], one, max_new=1, max_len=112)
+        logits = pkg.lm_head(head.view(torch.uint8).reshape(-1), 0, vocab, heads * d, y.reshape(rows, -1))
+        parents, chosen, worth, _ = pkg.beam_select(logits, scores)
+        cache.reorder(parents.reshape(-1))
+        tokens.copy_(chosen.reshape(-1))
+        scores.copy_(worth)
+        return parents, y
+
+    alone, captured, spare = made(), made(), made()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*spare)  # (what the calls set up once)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step(*captured)
+    torch.cuda.current_stream().wait_stream(stream)
+    for i in range(20):
+        want = step(*alone)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*got, *captured[1:]), (*want, *alone[1:])):
+            assert torch.equal(a, b), i
+        assert torch.equal(captured[0].lens, alone[0].lens)
+    starts = (torch.arange(rows + 1, dtype=torch.int32) * 33).cuda()
+    for a, b in zip(captured[0].read(0, starts, rows * 33), alone[0].read(0, starts, rows * 33)):
+        assert torch.equal(a, b)
