@@ -96,9 +96,11 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
  * d_kv + p * page_stride + h * head_stride + t * token_stride (elements), the
  * value value_offset elements behind it.  All four strides are multiples of 8
  * (page_stride and token_stride below 2^30), d_kv is 16-byte aligned, head_dim a
- * multiple of 8 up to 256, page_size a power of two up to 4096.  A table entry outside [0, pages) is no page: what
- * it would hold is neither read nor written, and attention sees no key there. */
-/* type NLS_GGML_Q8_0 or NLS_GGML_Q4_0: blocks of 32 elements of a head, an fp16
+ * multiple of 8 up to 256, page_size a power of two up to 4096.  A table entry
+ * outside [0, pages) is no page: what it would hold is neither read nor written,
+ * and attention sees no key there.
+ *
+ * type NLS_GGML_Q8_0 or NLS_GGML_Q4_0: blocks of 32 elements of a head, an fp16
  * factor d and a whole number c each, value d c, as GGUF's types of those names
  * hold (Q8_0 -127 .. 127, Q4_0 -8 .. 7), but with codes and factors apart and in
  * the order that the kernels take them.  A page is then nls_cache_page_bytes()
@@ -150,8 +152,8 @@ typedef struct nls_chunks {
  *   Q8_0  d = fp16(max |x| * (1 / 127)),                  c = rint(x * (1 / d))
  *   Q4_0  d = fp16(max(max x * (1 / 7), min x * (-1 / 8))), c within -8 .. 7
  * in fp32, each operation rounded once.  d is at most 515.5 and 8188, so that
- * fp16 holds d c: elements beyond its range are cut.  All c are 0 where d is 0.  A block with an element that is not finite
- * has d = NaN.
+ * fp16 holds d c: elements beyond its range are cut.  All c are 0 where d is 0.  A
+ * block with an element that is not finite has d = NaN.
  */
 int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const nls_rope_plan* plan, int32_t type,
                          const nls_heads* q, const nls_heads* q_out, int32_t heads, const nls_heads* k,
@@ -180,7 +182,8 @@ int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t
  * value that it does see makes it infinite or NaN.  (An infinite key that it
  * sees makes its score infinite, or NaN where fp32 queries meet 16-bit keys.)
  * scale: finite, up to 2.3e38 either way (log2 e times it is finite too).
- * type (q and out): F32 with any cache type, F16 or BF16 with the same one.
+ * type (q and out): F32 with any cache type, F16 or BF16 with the same one or
+ * with blocks.
  * Scores, statistics and sums are fp32.  fp32 queries and weights meet 16-bit
  * keys and values as sums of 16-bit parts: three of bf16, which are exact, or two
  * of fp16, 22 bits (or 2^-38 of the row's largest element).  16-bit queries'
@@ -189,6 +192,13 @@ int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t
  * may come out a rounding apart in another batch.  Weighted values are summed
  * before they are divided: in an fp32 or bf16 cache, values beyond 2^88 may
  * overflow in long sums.
+ * Blocks: d c itself meets the queries and weights, nothing of the cache is
+ * rounded but for BF16 queries in sequences of more than 16 rows, where d c is
+ * rounded to fp16.  F32 queries are two parts of fp16 as above; weights, or their
+ * products with the factors, are two parts, 22 bits, for F32 and F16 queries, and
+ * rounded to fp16 for BF16.  Factors are taken to be as nls_cache_append writes
+ * them: 0 to 515.5 or 8188, or NaN.  A key's factor of NaN makes the rows that see
+ * the key NaN, a value's the 32 elements of its block in them.
  * max_new and max_len say what the caller expects of the longest chunk and
  * context (0: not known).  They choose how the work is split; results hold
  * whatever the true values are.

@@ -174,14 +174,16 @@ AttendPlan plan_of(const AttendArgs& a, int type, int max_new, int64_t max_len) 
     // token over 131071 keys: 94.1 us so, 96.8 with three); up to 768 keys are not
     // split: the second launch costs the host more than it saves the GPU (517 keys:
     // 13.2 us a call whole, 17.2 in three parts, 12.8 and 12.3 in a graph; 24
-    // contexts of 517: 17.4 and 18.4, 17.8 and 18.8 in a graph).
+    // contexts of 517: 17.4 and 18.4, 17.8 and 18.8 in a graph).  Blocks are fewer
+    // bytes a key: their parts end at 4096 (64 contexts of up to 16384, Q4_0: 203 us;
+    // at 2048 220, at 8192 223).
     p.few_parts = parts_of_keys(most, tasks, (512 + tasks - 1) / tasks, most <= 768 ? 768 : 256, quant_type(a.cache_type) ? 4096 : 2048);
     p.few_parts.rows = tasks * 16;
     p.few_bytes = p.few_parts.most > 1 ? p.few_parts.most * p.few_parts.rows * per_row : 0;
   }
   if (p.chunk) {
     const bool quant = quant_type(a.cache_type);
-    const int tile = !quant ? kChunkTile : type == kF32 ? quant_tile<float>(a.p.dim / 32) : quant_tile<__bf16>(a.p.dim / 32);
+    const int tile = !quant ? kChunkTile : type == kBF16 ? quant_tile<__bf16>(a.p.dim / 32) : quant_tile<float>(a.p.dim / 32);
     p.chunk_tiles = tile_count(a.p.tokens, a.group, tile, a.p.seqs);
     // Two workgroups per CU (heads of up to 64: three), of the tiles that have rows
     // when they are all of one sequence (509 tokens of 28 heads beside 16 that
@@ -194,7 +196,8 @@ AttendPlan plan_of(const AttendArgs& a, int type, int max_new, int64_t max_len) 
     // 1600 tokens over 16000: 582 and 516).  One number for all types: registers let
     // four run at once of 16-bit queries in heads of up to 64, two and one (heads of
     // 72 to 128) over an fp32 cache, one of wider heads (300 tokens over 4000 fp32
-    // keys, heads of 128: 227 us when rounded up, 262 so).
+    // keys, heads of 128: 227 us when rounded up, 262 so).  Over blocks one workgroup
+    // runs where it has eight waves or heads are beyond 128.
     const int64_t wgs = ((int64_t)a.p.tokens * a.group + tile - 1) / tile * a.p.kv_heads;
     const int64_t places = tile > kChunkTile || (quant && D == 256) ? 256 : D == 64 ? 768 : 512, down = places / wgs > 1 ? places / wgs : 1;
     // (tiles of no rows are launched too: sequences beyond number do not multiply)

@@ -8,6 +8,17 @@
 //   o_e  = sum_j (p_j d_jx) c_je        for e in block x
 // Codes are whole numbers, exact in fp16, so nothing of the cache is rounded;
 // a block is the depth of one 16 x 16 x 32 product.
+//
+// What bounds it: one pass over the blocks, at what this pattern of loads reaches
+// (6.2 TB/s with nothing done to what arrives), for 8 bits: 64 contexts of 8192,
+// heads of 128, bf16 6.0 TB/s.  For 4 bits the steps between a load and its use
+// take as long as the bytes: 4.4 TB/s there, 3.4 with fp32 queries; 64 contexts of
+// up to 16384 184 us, one of 131071 (fp32) 49.
+// Measured and left: three waves a SIMD, which do not fit and spill; steps of 64
+// keys, the same; two steps' loads in flight, no faster; codes as they are in the
+// mantissa of a denormal number, which saves the subtraction and no time.  Loads in
+// a branch are waited for at its end: the loop's body is compiled with and without
+// the next step's (202 -> 191 us).
 #pragma once
 #include "nls_attend.h"
 #include "nls_quant.h"
@@ -575,13 +586,13 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 }
 
 // Rows of a workgroup of the chunk kernel, 32 to a wave.  Turning codes into
-// operands is work that the waves share: fp32 queries in heads of 96 and 128, whose
-// values are two parts, take eight waves (2048 tokens over 16384 keys, Q4_0: 1530
-// us with four, 1424 so); elsewhere four are as fast (bf16, heads of 128: 814 and
-// 816) or faster (heads of 64: 157 and 186).
+// operands is work that the waves share: in heads of 96 and 128 whose values are
+// two parts eight waves take it (2048 tokens over 16384 keys, Q4_0: fp32 queries
+// 1530 us with four, 1424 so; fp16 1721 and 1246); elsewhere four are as fast (bf16,
+// heads of 128: 814 and 816) or faster (heads of 64, bf16: 157 and 186).
 template <typename T>
 constexpr int quant_tile(int groups) {
-  return sizeof(T) == 4 && (groups == 3 || groups == 4) ? 256 : 128;
+  return weight_parts<T>() == 2 && (groups == 3 || groups == 4) ? 256 : 128;
 }
 
 // Launched by launch_attend (nls_attend.hip), which joins the parts.

@@ -9,10 +9,18 @@
 //   K   LDS holds the codes as fp16, which is exact.  Two products over a block
 //       are its depth; their sums are multiplied by the block's factor in fp32
 //       as they are added up, 16 per lane and block.
-//   V   LDS holds d c: for 16-bit queries rounded to fp16 (2^-12 of a value, an
-//       eighth of a bf16 step), for fp32 queries as two fp16 parts, which are
-//       exact (both c and d are whole multiples of fp16's least step), and three
-//       products: hi hi, hi lo, lo hi.
+//   V   LDS holds d c: for bf16 queries rounded to fp16, as their weights are
+//       (2^-11 at most, an eighth of the output's own half step), for fp32 and
+//       fp16 queries as two fp16 parts, which are exact (both c and d are whole
+//       multiples of fp16's least step), their weights two parts as well, and
+//       three products: hi hi, hi lo, lo hi.  (fp16 queries with one of each: 924 us
+//       for 1246, and the error half as large again as the output's rounding.)
+//
+// What bounds it: the matrix cores, with the turning of codes into operands on
+// the vector units between their runs.  2048 tokens over 16384 keys, 32 heads on 8
+// of 128, Q4_0: fp32 queries 1370 us, 376 TFLOP/s of the mathematics in two and a
+// half times as many products (two and three for one and one); bf16 797 us, 647 TFLOP/s (a bf16 cache, which
+// has nothing to turn: 572); 4001 tokens of 32 heads of 64, Q8_0, bf16: 156 us.
 //
 // Factors outside of the second product as well would be 16 products, splits and
 // conversions per lane, block and part, more than the third matrix product costs.
@@ -29,7 +37,7 @@ typedef __attribute__((address_space(3))) s4x* lds_s4x;
 template <typename T, int kBits, int GT>
 struct QTile {
   static constexpr int D = 32 * GT;
-  static constexpr int NP = quant_parts<T>();
+  static constexpr int NP = quant_parts<T>(), NW = weight_parts<T>();
   static constexpr int kRows = quant_tile<T>(GT), kWaves = kRows / 32, kThreads = 64 * kWaves;
   static constexpr int KT = GT == 8 ? 32 : 64;                  // keys per tile
   static constexpr int kRuns = KT / 16;                 // of keys within a page
@@ -37,7 +45,7 @@ struct QTile {
   static constexpr int kTiles = GT;                     // of O^T
   static constexpr int kBytes = KT * D * 2;             // of one of the three below
   static constexpr int kFactors = GT * KT * 2;
-  static constexpr int kStage = kBytes * (1 + NP) + kFactors;  // K, V (and its rest), K's factors
+  static constexpr int kStage = kBytes * (1 + NW) + kFactors;  // K, V (and its rest), K's factors
   static constexpr int kUnits = KT * 4 * GT / kThreads;        // key units of a thread
   static constexpr int kWide = GT < 4 ? GT : 4;                // blocks of a plane
   static constexpr int kLanes = KT * 16 * (GT / kWide) / kThreads;  // value pieces of a thread, side by side
@@ -56,7 +64,7 @@ template <typename T, int kBits, int GT, bool kPad>
 __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Parts& parts, bool alone, int group_at,
                                                  int groups_n, int part) {
   using L = QTile<T, kBits, GT>;
-  constexpr int NP = L::NP, KT = L::KT, NS = KT / 32, D = L::D;
+  constexpr int NP = L::NP, NW = L::NW, KT = L::KT, NS = KT / 32, D = L::D;
   constexpr bool kScaled = !__is_same(T, _Float16);  // rows are divided by a power of two
   constexpr float kShift = chunk_shift<_Float16>();
   extern __shared__ __align__(16) char chunk_lds[];  // [2][K, V, V's rest, K's factors]
@@ -258,7 +266,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
         for (int n = 0; n < 4; ++n)
           f[n] &= ((ok >> (2 * n)) & 1 ? 0xffffu : 0u) | ((ok >> (2 * n + 1)) & 1 ? 0xffff0000u : 0u);
       }
-      *reinterpret_cast<u4*>(to + L::kBytes * (1 + NP) + (f_x * KT + f_key) * 2) = f;
+      *reinterpret_cast<u4*>(to + L::kBytes * (1 + NW) + (f_x * KT + f_key) * 2) = f;
     }
     if (there != kAll && !((there >> v_row) & 1)) {
 #pragma unroll
@@ -294,13 +302,13 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
           const uint32_t codes = kBits == 8 ? less(pair | 0x64006400u, 1152.f) : half ? high_nibbles(pair) : low_nibbles(pair);
           const h2 d{vd[b], vd[b]}, v = halves(codes) * d;
           w[z / 2] = __builtin_bit_cast(uint32_t, v);
-          if constexpr (NP == 2)
+          if constexpr (NW == 2)
             rest[z / 2] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(halves(codes), d, -v));
         }
         const int e = (v_plane * L::kWide + b) * 32 + half * 16 + v_i;
         char* at = hi + (v_row * L::kPieces + L::v_piece(v_row, e >> 3)) * 16 + (e & 7) * 2;
         __builtin_memcpy(__builtin_assume_aligned(at, 2 * L::kLanes), w, 2 * L::kLanes);
-        if constexpr (NP == 2)
+        if constexpr (NW == 2)
           __builtin_memcpy(__builtin_assume_aligned(at + L::kBytes, 2 * L::kLanes), rest, 2 * L::kLanes);
       }
     const bool wave_any = __ballot(any) != 0;
@@ -317,7 +325,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   // 32 keys from kb + sub * 32 on; whole: every row sees all of them
   auto step = [&](bool whole, int sub, const char* lk, int kb, uint64_t there) {
     const char* row_k = lk + (sub * 32 + i) * L::kPieces * 16;
-    const char* factors = lk + L::kBytes * (1 + NP) + (sub * 32 + 4 * h) * 2;
+    const char* factors = lk + L::kBytes * (1 + NW) + (sub * 32 + 4 * h) * 2;
     const char* lv = lk + L::kBytes;
     f16x s;
     __builtin_amdgcn_s_setprio(1);
@@ -394,10 +402,10 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {  // 16 keys
-      h8 p[NP];
+      h8 p[NW];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split<NP>(w[b * 8 + j], p, j);
-      if constexpr (NP == 1) lr = plus_all(p[0], lr);
+      for (int j = 0; j < 8; ++j) split<NW>(w[b * 8 + j], p, j);
+      if constexpr (NW == 1) lr = plus_all(p[0], lr);
 #pragma unroll
       for (int t = 0; t < L::kTiles; ++t) {
         // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
@@ -411,7 +419,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
           return __builtin_bit_cast(h8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         };
         const h8 v = operand(at);
-        if constexpr (NP == 2) {
+        if constexpr (NW == 2) {
           o[t] = mma32(operand(at + L::kBytes), p[0], o[t]);
           o[t] = mma32(v, p[1], o[t]);
         }
@@ -465,7 +473,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
 
   if (!row_ok) return;
   l += __shfl_xor(l, 32);
-  if constexpr (NP == 1)
+  if constexpr (NW == 1)
     lr += __shfl_xor(lr, 32);
   else
     lr = l;
@@ -508,9 +516,12 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
     a.lse[(int64_t)token * a.heads + head] = l == 0.f ? minus_inf() : (from + (__builtin_amdgcn_logf(l) - kShift)) * kLn2;
 }
 
-// alone: sequences of few rows are its too
+// alone: sequences of few rows are its too.  Registers for three workgroups of
+// 16-bit queries in heads of up to 64 (more of the waiting hidden), one of heads
+// beyond 128, whose sums alone are 128 registers.
 template <typename T, int kBits, int GT, bool kPad>
-__global__ __launch_bounds__((QTile<T, kBits, GT>::kThreads), GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2) void chunk_quant_kernel(AttendArgs a, Parts parts, bool alone) {
+__global__ __launch_bounds__((QTile<T, kBits, GT>::kThreads), GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2)
+void chunk_quant_kernel(AttendArgs a, Parts parts, bool alone) {
   chunk_quant_rows<T, kBits, GT, kPad>(a, parts, alone, blockIdx.x, gridDim.x, blockIdx.z);
 }
 

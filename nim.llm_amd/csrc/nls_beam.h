@@ -38,7 +38,7 @@ struct BeamArgs {
 };
 
 // 32 logits to a thread, 32 KB on their way to each workgroup; 8 where that leaves
-// less than a workgroup for a CU (4 x 32000: 7.0 us with 32, 5.3 with 8).
+// less than a workgroup for a CU (4 x 32000: 7.0 us with 32, 5.6 with 8).
 inline int beam_per(int64_t rows, int64_t vocab) {
   const int64_t slice = (int64_t)kBeamPer * kBeamThreads;
   return rows * ((vocab + slice - 1) / slice) < 256 ? kBeamPerFew : kBeamPer;

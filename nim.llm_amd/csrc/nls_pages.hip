@@ -410,7 +410,7 @@ __device__ __forceinline__ int settled(const int32_t* p) {
 // by every row as it will be.  One workgroup: what bounds it are the two passes
 // over the table: a wave takes eight rows at a time, with the slots' numbers in LDS
 // (512 slots of 73 entries: 47 us when entries are dealt out to threads by a
-// division each, TIME so).
+// division each, 33 so).
 constexpr int kSlotsHeld = 2048;
 __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, const int32_t* src, int32_t* status,
                                                                int32_t* work) {

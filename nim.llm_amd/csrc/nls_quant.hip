@@ -3,8 +3,9 @@
 //
 // Bound by the bytes: a row's elements are converted (blocks: one product with
 // the factor, rounded once) as they pass.  16 contexts of up to 4000 tokens, 8
-// heads of 128, Q4_0 to bf16 (220 MB): TIME us; a workgroup for each token, whose
-// look-ups are a wait of their own, 76.
+// heads of 128, Q4_0 to bf16 (220 MB): 53 us, 4.2 TB/s, nine tenths of what a large copy
+// reaches; a workgroup for each token, whose look-ups are a wait of their own, 76;
+// stores that pass the caches 58.
 #include "nls_quant.h"
 
 namespace nls {

@@ -94,7 +94,7 @@ def attend(q, kv, kind, table, lens, starts, scale, window=0, first=None, slots=
     most = 127 if kind == "q8_0" else 8
     # of a weight times a factor or a value: two parts each, or one of eleven bits
     # (few rows: of the weight times the factor; chunks: of the weight and of the value)
-    part = 2.0 ** -22 if q.dtype == torch.float32 else 2.0 ** -10
+    part = 2.0 ** -10 if q.dtype == torch.bfloat16 else 2.0 ** -22
     for i in range(len(starts) - 1):
         a, b = starts[i], starts[i + 1]
         if a == b:
