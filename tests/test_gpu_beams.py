@@ -336,3 +336,30 @@ def test_reorder_many_slots(pkg):
         assert c.reorder(torch.tensor(src, dtype=torch.int32).cuda()).item() == 0
         m.same(c)
         holds(c, m)
+
+
+def test_reorder_over_the_most_pages(pkg):
+    """524288 pages, contexts on the last ones, copies onto the lowest free one."""
+    pages = 1 << 19
+    c = pkg.PagedCache(1, pages, 1, 1, 8, 3, 5, dtype=torch.float16)
+    c.page_size = 1
+    c.refs.fill_(1)
+    c.refs[pages - 3] = 0
+    c.refs[7] = 0
+    c.table[0, :2] = torch.tensor([pages - 1, pages - 2], dtype=torch.int32)
+    c.lens[0] = 2
+    assert c.reorder(torch.tensor([0, 0, -1], dtype=torch.int32).cuda()).item() == pkg.PAGES_DONE
+    assert c.table.tolist() == [[pages - 1, pages - 2, -1, -1, -1]] * 2 + [[-1] * 5] and c.lens.tolist() == [2, 2, 0]
+    assert c.refs[pages - 2:].tolist() == [2, 2]
+    # pages of 2 tokens: the partial last one is copied to page 7
+    wide = torch.randn(1, pages, 2, 1, 2, 8, device="cuda", dtype=torch.float16)
+    before = wide[:, pages - 2].clone()
+    table, lens = c.table.clone(), torch.tensor([3, 0, 0], dtype=torch.int32).cuda()
+    table[1] = -1
+    refs = c.refs.clone()
+    refs[pages - 2:] = 1
+    parents = torch.tensor([0, 0, 0], dtype=torch.int32).cuda()
+    assert pkg.cache_reorder(wide, table, lens, refs, parents).item() == pkg.PAGES_DONE
+    assert table[:, :3].tolist() == [[pages - 1, pages - 2, -1], [pages - 1, 7, -1], [pages - 1, pages - 3, -1]]
+    assert torch.equal(wide[:, 7], before) and torch.equal(wide[:, pages - 3], before)
+    assert refs[pages - 3:].tolist() == [1, 1, 3] and int(refs[7]) == 1 and lens.tolist() == [3] * 3
