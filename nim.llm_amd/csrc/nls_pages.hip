@@ -407,10 +407,10 @@ __device__ __forceinline__ int settled(const int32_t* p) {
 
 // What goes where.  A page is free for a copy when nobody held it, or only
 // slots whose contexts end here: it is marked by those, and the mark is taken off
-// by every row as it will be.  One workgroup: what bounds it are the two passes
+// by every row as it will be.  The first workgroup: what bounds it are the two passes
 // over the table: a wave takes eight rows at a time, with the slots' numbers in LDS
 // (512 slots of 73 entries: 47 us when entries are dealt out to threads by a
-// division each, 33 so).
+// division each, 33 by rows, 30 since the other workgroups keep the table).
 constexpr int kSlotsHeld = 2048;
 __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, const int32_t* src, int32_t* status,
                                                                int32_t* work) {
@@ -418,6 +418,12 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
   __shared__ int s_src[kSlotsHeld], s_len[kSlotsHeld], s_first[kSlotsHeld];
   const PlanLds lds = plan_lds(t.pages);
   const ReorderWork w(work, t.slots);
+  if (blockIdx.x > 0) {  // the table as it was, by the other workgroups
+    const uint32_t n = (uint32_t)t.slots * (uint32_t)t.max_pages, per = t.max_pages;  // (below 2^31)
+    for (uint32_t e = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; e < n; e += (gridDim.x - 1) * kPlanThreads)
+      w.rows[e] = t.table[(int64_t)(e / per) * t.table_stride + e % per];
+    return;
+  }
   const int mask = (1 << t.page_shift) - 1;
   const bool held = t.slots <= kSlotsHeld;
   int bad = 0;
@@ -466,13 +472,11 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
   // eight rows at a time to a wave, 128 entries of each
   constexpr int kRows = 8, kCols = 2;
   for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
-    int used[kRows], most = 0;
-    bool ends[kRows];
+    int used[kRows], most = 0;  // (of those that end here)
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       const int s = s0 + u;
-      used[u] = s < t.slots ? pages_of(len_of(s), t.page_shift) : 0;
-      ends[u] = s < t.slots && src_of(s) != s;
+      used[u] = s < t.slots && src_of(s) != s ? pages_of(len_of(s), t.page_shift) : 0;
       most = used[u] > most ? used[u] : most;
     }
     for (int j0 = lane; j0 < most; j0 += 64 * kCols) {
@@ -488,9 +492,8 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
       for (int u = 0; u < kRows; ++u)
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
-          const int j = j0 + 64 * c, p = page[u][c];
-          if (j < used[u]) w.rows[(int64_t)(s0 + u) * t.max_pages + j] = p;
-          if (ends[u] && (uint32_t)p < (uint32_t)t.pages) atomicOr(&marks[p >> 5], 1u << (p & 31));
+          const int p = page[u][c];
+          if ((uint32_t)p < (uint32_t)t.pages) atomicOr(&marks[p >> 5], 1u << (p & 31));
         }
     }
   }
@@ -636,9 +639,10 @@ hipError_t launch_reorder(const PoolArgs& p, const TableArgs& t, const int32_t* 
                           hipStream_t s) {
   hipError_t e = allow_lds(reinterpret_cast<const void*>(reorder_kernel), t.pages);
   if (e != hipSuccess) return e;
-  reorder_kernel<<<1, kPlanThreads, plan_lds_bytes(t.pages), s>>>(t, src, status, work);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
   const int64_t entries = (int64_t)t.slots * t.max_pages;
+  const int copying = (int)(entries > 64 * kPlanThreads ? 64 : (entries + kPlanThreads - 1) / kPlanThreads);
+  reorder_kernel<<<1 + copying, kPlanThreads, plan_lds_bytes(t.pages), s>>>(t, src, status, work);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
   const int tb = (int)(entries > 256 * kCopyThreads ? 256 : (entries + kCopyThreads - 1) / kCopyThreads);
   reorder_apply_kernel<<<tb + copy_blocks(copy_items(p, t.slots)), kCopyThreads, 0, s>>>(p, t, src, work, tb);
   return hipGetLastError();
