@@ -177,28 +177,23 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
     const int row = g * a.beams + b, part = threadIdx.x & 15;
     const float score = a.scores[row];
     const bool live = score > -__builtin_inff(), ended = a.ended && a.ended[row];
-    double of = none, sum = 0.0;
     const BeamPart* p = a.parts + (int64_t)row * a.slices;
-    BeamPart next = p[part < a.slices ? part : 0];
-    // sums of exp(l - of) together; what is against +infinity stands alone
-    auto add = [&](double of2, double sum2) {
-      if (!(of2 > none)) return;
-      const double most = of2 > of ? of2 : of;
-      sum = (of == most ? sum : sum * exp(of - most)) + (of2 == most ? sum2 : sum2 * exp(of2 - most));
-      of = most;
-    };
-    if (live && !ended) {
-      for (int s = part; s < a.slices; s += 16) {
-        const BeamPart q = next;
-        if (s + 16 < a.slices) next = p[s + 16];
-        add((double)q.max, (double)q.sum);
-      }
-    }
+    const BeamPart held_part = p[part < a.slices ? part : 0];
+    // the maximum first, so that a part's exponential is one (what is against
+    // +infinity stands alone)
+    const bool asks = live && !ended;
+    float top = asks && part < a.slices ? held_part.max : -__builtin_inff();
+    if (asks)
+      for (int s = part + 16; s < a.slices; s += 16) top = fmaxf(top, p[s].max);
 #pragma unroll
-    for (int d = 8; d; d >>= 1) {
-      const double of2 = __shfl_xor(of, d), sum2 = __shfl_xor(sum, d);
-      add(of2, sum2);
-    }
+    for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const double of = top;
+    auto share = [&](const BeamPart& q) { return q.max == top ? (double)q.sum : (double)q.sum * exp((double)q.max - of); };
+    double sum = asks && part < a.slices ? share(held_part) : 0.0;
+    if (asks)
+      for (int s = part + 16; s < a.slices; s += 16) sum += share(p[s]);
+#pragma unroll
+    for (int d = 8; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (part == 0) {
       s_score[b] = score;
       s_of[b] = of;
