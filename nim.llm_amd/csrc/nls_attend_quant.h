@@ -105,15 +105,14 @@ template <typename T>
 constexpr int weight_parts() {
   return __is_same(T, __bf16) ? 1 : 2;
 }
-// What is read once: bytes that leave the caches to others.
-template <int kBytes>
+// What is read once: bytes that leave the caches to others (kAlign: 4 or more).
+template <int kBytes, int kAlign>
 __device__ __forceinline__ void past_caches(uint32_t* to, const char* from) {
-  typedef uint32_t words __attribute__((ext_vector_type(kBytes < 16 ? kBytes / 4 : 4)));
-#pragma unroll
-  for (int n = 0; n < kBytes; n += 16) {
-    const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(from + n));
-    __builtin_memcpy(to + n / 4, &x, sizeof x);
-  }
+  constexpr int kPiece = kBytes >= 16 ? 16 : kBytes >= 8 ? 8 : 4;
+  typedef uint32_t words __attribute__((ext_vector_type(kPiece / 4), aligned(kAlign < kPiece ? kAlign : kPiece)));
+  const words x = __builtin_nontemporal_load(reinterpret_cast<const words*>(from));
+  __builtin_memcpy(to, &x, kPiece);
+  if constexpr (kBytes > kPiece) past_caches<kBytes - kPiece, kAlign>(to + kPiece / 4, from + kPiece);
 }
 
 // A truth value as a type.
@@ -124,15 +123,19 @@ struct Is {
 
 constexpr float kQuantShift = 14.f;  // log2 of the largest weight times factor
 
-// kPad: heads of fewer than GT blocks
-template <typename T, int kBits, int GT, bool kPad>
+// Heads of NG blocks, at most GT (2, 4 or 8: what the factors are dealt out by).
+// Each number of blocks has its own loads, plane by plane: 32 contexts of 8192, bf16
+// over Q4_0, heads of 96 61 us and of 192 133 (a byte at a time, for any number
+// below GT, 182 and 518).
+template <typename T, int kBits, int GT, int NG>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,
                                                int group_at, int part) {
   constexpr int NP = quant_parts<T>(), NW = weight_parts<T>(), D = 32 * GT, kWaves = 4, kThreads = 256;
   constexpr int NR = 2, KT = 16 * NR;   // runs of 16 keys in a step of a wave, and its keys
   constexpr int KW = kBits / 4;                       // words of a key unit
-  constexpr int kWide = GT < 4 ? GT : 4;              // blocks of a plane
+  constexpr bool kPad = NG < GT;
   constexpr int VW = (GT * kBits / 4 + 3) / 4;        // words of a lane's piece of a value row
+  constexpr bool kApart = kBits == 4 && (NG & 3) == 3;  // a last byte that joins its word when it is used
   extern __shared__ float quant_lds[];                // [wave][16][D + 4] sums
   __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
   __shared__ __align__(16) uint32_t sh_f[kWaves][KT * GT];  // a step's factors, of keys, then of values: [2 GT][KT]
@@ -145,10 +148,9 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
   const bool over = rows > 16 && c.n != 1;
   if (over && (chunk_runs || part > 0)) return;
   const Sees sees = sees_of(a, c);
-  const int dim = a.p.dim, groups = kPad ? dim / 32 : GT;
+  constexpr int groups = NG, dim = 32 * NG, row_bytes = 4 * NG * kBits;
   const int size = 1 << a.p.page_shift;
-  const QuantShape shape = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, kPad ? dim : D, size);
-  const int row_bytes = kPad ? shape.row : D * kBits / 8;
+  const QuantShape shape = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, dim, size);
   for (int r0 = tile * 16; r0 < rows; r0 += tiles * 16) {
     const int rn = rows - r0 < 16 ? rows - r0 : 16;
     const int t0 = r0 / a.group, t1 = (r0 + rn - 1) / a.group;
@@ -249,7 +251,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     };
     auto home = [&](int page) { return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride; };
 
-    uint32_t kc[NR][GT][KW], vc[4 * NR][VW];
+    uint32_t kc[NR][GT][KW], vc[4 * NR][VW + kApart];
     // A lane's factors: KT GT / 32 tokens' of one block, keys' for the first 32
     // lanes and values' for the others; 16 lanes of the operands want each, out of
     // LDS.
@@ -266,9 +268,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       const int n = here(lane) & 15;
       return (uint32_t)((n % 4 * 4 + n / 4) * row_bytes + (here(lane) >> 4) * groups * kBits);
     };
-    auto lane_v = [&]() {
-      return (uint32_t)((here(lane) >> 4) * row_bytes + (kPad ? 0 : (here(lane) & 15) * (kWide * kBits / 4)));
-    };
+    auto lane_v = [&](int wide) { return (uint32_t)((here(lane) >> 4) * row_bytes + (here(lane) & 15) * (wide * kBits / 4)); };
     auto lane_f = [&]() {
       const int n = here(lane), x = n / kAcross % GT, token = n % kAcross * FT;
       return (uint32_t)((n < 32 ? 0 : shape.half) + shape.codes + ((!kPad || x < groups ? x : 0) * size + (token & 15)) * 2);
@@ -279,14 +279,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
         const char* codes = home(p.at[s]) + place * row_bytes;
-        if constexpr (!kPad) {
-          past_caches<GT * kBits>(&kc[s][0][0], codes + at_k);
-        } else {
-#pragma unroll
-          for (int x = 0; x < GT; ++x)
-            if (x < groups)
-              __builtin_memcpy(kc[s][x], __builtin_assume_aligned(codes + x * kBits + at_k, kBits), kBits);
-        }
+        past_caches<NG * kBits, (NG * kBits) & -(NG * kBits)>(&kc[s][0][0], codes + at_k);
       }
     };
     // the run of this lane's factors
@@ -301,7 +294,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       __builtin_memcpy(fc, __builtin_assume_aligned(from + lane_f(), 2 * FT < 16 ? 2 * FT : 16), 2 * FT);
     };
     auto fetch_v = [&](int kb, const Pages& p) {
-      const uint32_t at_v = lane_v();
+      const uint32_t at_4 = lane_v(4), at_2 = lane_v(2), at_1 = lane_v(1);
 #pragma unroll
       for (int s = 0; s < NR; ++s) {
         const int place = (kb + s * 16) & (size - 1);
@@ -310,29 +303,23 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         for (int r = 0; r < 4; ++r) {
           uint32_t* to = vc[s * 4 + r];
           const char* from = codes + r * 4 * row_bytes;
-          if constexpr (!kPad) {
-            constexpr int kBytes = kWide * kBits / 4;  // of a plane
-            if constexpr (kBytes == 2) {
-              to[0] = *reinterpret_cast<const uint16_t*>(from + at_v);
-            } else {
+          // planes of four blocks, of two, of one; block x's codes are bytes of to in its order
+          constexpr int kFours = NG / 4, kLast = NG - 1;
 #pragma unroll
-              for (int n = 0; n < GT / kWide; ++n)
-                past_caches<kBytes>(to + n * kBytes / 4, from + n * 16 * kBytes + at_v);
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) to[w] = 0;
-#pragma unroll
-            for (int x = 0; x < GT; ++x) {
-              if (x >= groups) break;
-              const int fours = groups & ~3, first = x < fours ? x & ~3 : x < fours + (groups & 2) ? fours : x;
-              const int wide = x < fours ? 4 : x < fours + (groups & 2) ? 2 : 1;
-              const char* at = from + (first * 16 + x - first) * (kBits / 4) + (at_v + i * (uint32_t)wide * (kBits / 4));
-              if constexpr (kBits == 8)
-                to[x / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(at) << (16 * (x & 1));
-              else
-                to[x / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(at) << (8 * (x & 3));
-            }
+          for (int n = 0; n < kFours; ++n) past_caches<kBits, kBits>(to + n * kBits / 4, from + n * 16 * kBits + at_4);
+          if constexpr ((NG & 2) != 0) {
+            const char* at = from + kFours * 16 * kBits + at_2;
+            if constexpr (kBits == 8)
+              past_caches<4, 4>(to + kFours * 2, at);
+            else
+              to[kFours] = *reinterpret_cast<const uint16_t*>(at);
+          }
+          if constexpr ((NG & 1) != 0) {
+            const char* at = from + kLast * 4 * kBits + at_1;
+            if constexpr (kBits == 8)
+              to[kLast / 2] = *reinterpret_cast<const uint16_t*>(at);
+            else
+              to[kApart ? VW : kLast / 4] = *reinterpret_cast<const uint8_t*>(at);
           }
         }
       }
@@ -524,6 +511,9 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
               for (int h = 0; h < 2; ++h) o[2 * x + h] = mma16(codes[h], pd[n], o[2 * x + h]);
           }
       };
+      if constexpr (kApart)
+#pragma unroll
+        for (int n = 0; n < 4 * NR; ++n) vc[n][VW - 1] |= vc[n][VW] << 16;
       if (whole)
         values(Is<true>{});
       else

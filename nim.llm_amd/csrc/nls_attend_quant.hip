@@ -13,21 +13,21 @@ constexpr int few_quant_waves() {
   return GT == 8 ? 1 : GT == 4 || (sizeof(T) == 4 && kBits == 8) ? 2 : 3;
 }
 
-template <typename T, int kBits, int GT, bool kPad>
+template <typename T, int kBits, int GT, int NG>
 __global__ __launch_bounds__(kThreads, (few_quant_waves<T, kBits, GT>())) void few_quant_kernel(AttendArgs a, Parts parts,
                                                                                                int tiles, bool chunk_runs) {
-  few_quant_rows<T, kBits, GT, kPad>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
+  few_quant_rows<T, kBits, GT, NG>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
 }
 
-template <typename T, int kBits, int GT, bool kPad>
+template <typename T, int kBits, int GT, int NG>
 hipError_t few_of(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs, hipStream_t s) {
   constexpr size_t lds = (size_t)4 * 16 * (32 * GT + 4) * sizeof(float);
   if (lds > 60000) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_quant_kernel<T, kBits, GT, kPad>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(few_quant_kernel<T, kBits, GT, NG>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  few_quant_kernel<T, kBits, GT, kPad>
+  few_quant_kernel<T, kBits, GT, NG>
       <<<dim3(a.p.kv_heads * a.p.seqs * tiles, 1, parts.most), kThreads, lds, s>>>(a, parts, tiles, chunk_runs);
   return hipGetLastError();
 }
@@ -35,12 +35,14 @@ hipError_t few_of(const AttendArgs& a, const Parts& parts, int tiles, bool chunk
 template <typename T, int kBits>
 hipError_t few_width(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs, hipStream_t s) {
   switch (a.p.dim / 32) {
-    case 1: return few_of<T, kBits, 2, true>(a, parts, tiles, chunk_runs, s);
-    case 2: return few_of<T, kBits, 2, false>(a, parts, tiles, chunk_runs, s);
-    case 3: return few_of<T, kBits, 4, true>(a, parts, tiles, chunk_runs, s);
-    case 4: return few_of<T, kBits, 4, false>(a, parts, tiles, chunk_runs, s);
-    case 8: return few_of<T, kBits, 8, false>(a, parts, tiles, chunk_runs, s);
-    default: return few_of<T, kBits, 8, true>(a, parts, tiles, chunk_runs, s);
+    case 1: return few_of<T, kBits, 2, 1>(a, parts, tiles, chunk_runs, s);
+    case 2: return few_of<T, kBits, 2, 2>(a, parts, tiles, chunk_runs, s);
+    case 3: return few_of<T, kBits, 4, 3>(a, parts, tiles, chunk_runs, s);
+    case 4: return few_of<T, kBits, 4, 4>(a, parts, tiles, chunk_runs, s);
+    case 5: return few_of<T, kBits, 8, 5>(a, parts, tiles, chunk_runs, s);
+    case 6: return few_of<T, kBits, 8, 6>(a, parts, tiles, chunk_runs, s);
+    case 7: return few_of<T, kBits, 8, 7>(a, parts, tiles, chunk_runs, s);
+    default: return few_of<T, kBits, 8, 8>(a, parts, tiles, chunk_runs, s);
   }
 }
 

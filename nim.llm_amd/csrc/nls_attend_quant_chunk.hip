@@ -42,7 +42,6 @@ struct QTile {
   static constexpr int KT = GT == 8 ? 32 : 64;                  // keys per tile
   static constexpr int kRuns = KT / 16;                 // of keys within a page
   static constexpr int kPieces = D / 8;                 // 16-byte pieces of a row
-  static constexpr int kTiles = GT;                     // of O^T
   static constexpr int kBytes = KT * D * 2;             // of one of the three below
   static constexpr int kFactors = GT * KT * 2;
   static constexpr int kStage = kBytes * (1 + NW) + kFactors;  // K, V (and its rest), K's factors
@@ -60,10 +59,16 @@ struct QTile {
   }
 };
 
-template <typename T, int kBits, int GT, bool kPad>
+// Heads of NG blocks, in tiles of GT.  Where NG is less a thread's values come in
+// pieces of the planes that there are, and become a whole plane's order on their way
+// to LDS (512 tokens over 8192, heads of 96 and 192, bf16 over Q4_0: 136 and 383 us;
+// with a load for each lane and block, and products over the blocks that are not
+// there, 185 and 619).
+template <typename T, int kBits, int GT, int NG>
 __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Parts& parts, bool alone, int group_at,
                                                  int groups_n, int part) {
   using L = QTile<T, kBits, GT>;
+  constexpr bool kPad = NG < GT;
   constexpr int NP = L::NP, NW = L::NW, KT = L::KT, NS = KT / 32, D = L::D;
   constexpr bool kScaled = !__is_same(T, _Float16);  // rows are divided by a power of two
   constexpr float kShift = chunk_shift<_Float16>();
@@ -106,12 +111,12 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   const int all_lo = as_int(sees.low(sees.p0 + last / a.group)), all_hi = as_int(sees.p0 + (r0 + w0) / a.group);
   const int any_lo = as_int(sees.low(sees.p0 + (r0 + w0) / a.group)), any_hi = as_int(sees.p0 + last / a.group);  // and by some row
   const int tile_lo = as_int(sees.low(sees.p0 + t1)), tile_hi = as_int(sees.p0 + t0);  // and by all of the workgroup's
-  const int dim = a.p.dim, groups = kPad ? dim / 32 : GT;
+  constexpr int dim = 32 * NG, row_bytes = 4 * NG * kBits;
 
   // the scale's sign goes to the queries: a largest score is a largest product
   const float flip = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
   const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
-  h8 q[2 * GT][NP];
+  h8 q[2 * NG][NP];
   float qs = 1.f;
   {
     const T* src = static_cast<const T*>(a.q.d) + (int64_t)(c.begin + row / a.group) * a.q.token_stride +
@@ -130,7 +135,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       qs = ldexpf(1.f, e);
     }
 #pragma unroll
-    for (int k = 0; k < 2 * GT; ++k)
+    for (int k = 0; k < 2 * NG; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int d = (k * 2 + h) * 8 + j;
@@ -152,14 +157,13 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
 
   // This thread's part of a tile.  A wave's rows are of one run of 16 keys.
   const int size = 1 << a.p.page_shift;
-  const QuantShape shape = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, kPad ? dim : D, size);
-  const int row_bytes = kPad ? shape.row : D * kBits / 8;
+  const QuantShape shape = quant_shape(kBits == 8 ? kQ8_0 : kQ4_0, dim, size);
   const int unit = threadIdx.x * L::kUnits, k_row = unit / (4 * GT), k_g = unit % (4 * GT) / GT, k_x = unit % GT;
   constexpr int kPlanes = GT / L::kWide;
   const int piece = threadIdx.x * L::kLanes, v_row = piece / (16 * kPlanes), v_plane = piece / 16 % kPlanes, v_i = piece % 16;
   const int run = __builtin_amdgcn_readfirstlane(k_row / 16);  // (v_row's too)
   const int f_x = threadIdx.x / (KT / 8), f_key = threadIdx.x % (KT / 8) * 8;  // K's factors: the first GT KT / 8 threads
-  const bool f_mine = f_x < groups;
+  const bool f_mine = f_x < NG;
   const char* base = static_cast<const char*>(a.p.kv) + quant_base(shape, kvh, 0);
   const int32_t* table = a.p.table + (int64_t)c.slot * a.p.table_stride;  // (no keys without a slot)
   // The table's entries of a tile: its runs', and once more this wave's run's and
@@ -199,11 +203,28 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   uint32_t kc[L::kKeyWords], vc[L::kValueWords];
   u4 kf;             // factors of 8 keys
   _Float16 vd[L::kWide];
+  // (kPad) the pieces of a row's planes, which vc is made of when they are there
+  uint32_t v4[L::kLanes * kBits / 4], v2[L::kLanes * kBits / 8], v1[(L::kLanes * kBits + 15) / 16];
+  auto join_planes = [&]() {
+    constexpr int kBytes = kBits / 4;  // of a lane and block
+    auto bytes_of = [](const uint32_t* from, int n) { return from[n * kBytes / 4] >> (8 * (n * kBytes % 4)) & ((1u << 8 * kBytes) - 1); };
+#pragma unroll
+    for (int w = 0; w < L::kValueWords; ++w) {
+      uint32_t r = 0;
+#pragma unroll
+      for (int n = 4 / kBytes * w; n < 4 / kBytes * (w + 1); ++n) {
+        const int z = n / L::kWide, b = n % L::kWide;
+        if ((NG & 2) && b < 2) r |= bytes_of(v2, z * 2 + b) << (8 * (n * kBytes % 4));
+        if ((NG & 1) && b == (NG & 2)) r |= bytes_of(v1, z) << (8 * (n * kBytes % 4));
+      }
+      vc[w] = NG > 4 && v_plane == 0 ? v4[w] : r;
+    }
+  };
   auto home_of = [&](int page) { return base + (int64_t)(page < 0 ? 0 : page) * a.p.page_stride; };
   auto fetch = [&](int kb, const Entries& p) {
     const char* home = home_of(p.run);
     const int place = ((uint32_t)kb + run * 16) & (size - 1);  // of the run
-    const char* keys = home + (place + (k_row & 15)) * row_bytes + (k_g * groups + k_x) * kBits;
+    const char* keys = home + (place + (k_row & 15)) * row_bytes + (k_g * NG + (kPad ? 0 : k_x)) * kBits;
     const char* values = home + shape.half + (place + (v_row & 15)) * row_bytes;
     const char* factors = home + shape.half + shape.codes + (place + (v_row & 15)) * 2;
     if constexpr (!kPad) {
@@ -214,31 +235,23 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       for (int b = 0; b < L::kWide; ++b)
         vd[b] = *reinterpret_cast<const _Float16*>(factors + (v_plane * L::kWide + b) * size * 2);
     } else {
+      // (in the place of blocks that are not there the last one, which nothing reads)
 #pragma unroll
       for (int u = 0; u < L::kUnits; ++u)
-        if (k_x + u < groups)
-          __builtin_memcpy(kc + u * kBits / 4, __builtin_assume_aligned(keys + u * kBits, kBits), kBits);
-      // block by block, into the order of whole planes
+        __builtin_memcpy(kc + u * kBits / 4, __builtin_assume_aligned(keys + min(k_x + u, NG - 1) * kBits, kBits), kBits);
+      // pieces of the planes of four blocks, of two, of one
+      constexpr int kFours = NG / 4;
+      if constexpr (kFours != 0)
+        __builtin_memcpy(v4, __builtin_assume_aligned(values + v_i * kBits, L::kLanes * kBits < 16 ? L::kLanes * kBits : 16), L::kLanes * kBits);
+      if constexpr ((NG & 2) != 0)
+        __builtin_memcpy(v2, __builtin_assume_aligned(values + kFours * 16 * kBits + v_i * kBits / 2, L::kLanes * kBits / 2),
+                         L::kLanes * kBits / 2);
+      if constexpr ((NG & 1) != 0)
+        __builtin_memcpy(v1, __builtin_assume_aligned(values + (NG - 1) * 4 * kBits + v_i * kBits / 4, L::kLanes * kBits / 4),
+                         L::kLanes * kBits / 4);
 #pragma unroll
-      for (int w = 0; w < L::kValueWords; ++w) vc[w] = 0;
-#pragma unroll
-      for (int b = 0; b < L::kWide; ++b) {
-        const int x = v_plane * L::kWide + b;
-        vd[b] = (_Float16)0.f;
-        if (x >= groups) continue;
-        const int fours = groups & ~3, first = x < fours ? x & ~3 : x < fours + (groups & 2) ? fours : x;
-        const int wide = x < fours ? 4 : x < fours + (groups & 2) ? 2 : 1;
-        vd[b] = *reinterpret_cast<const _Float16*>(factors + x * size * 2);
-#pragma unroll
-        for (int z = 0; z < L::kLanes; ++z) {
-          const char* from = values + (first * 16 + (v_i + z) * wide + x - first) * (kBits / 4);
-          const int byte = (z * L::kWide + b) * (kBits / 4);
-          if constexpr (kBits == 8)
-            vc[byte / 4] |= (uint32_t)*reinterpret_cast<const uint16_t*>(from) << (8 * (byte % 4));
-          else
-            vc[byte / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(from) << (8 * (byte % 4));
-        }
-      }
+      for (int b = 0; b < L::kWide; ++b)
+        vd[b] = *reinterpret_cast<const _Float16*>(factors + min(v_plane * L::kWide + b, NG - 1) * size * 2);
     }
     if (f_mine) {
       const char* there = home_of(p.factors);
@@ -254,9 +267,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
 #pragma unroll
     for (int u = 0; u < L::kUnits; ++u) {
       const u4 codes = __builtin_bit_cast(u4, key_codes<kBits>(kc + u * kBits / 4));
-      const bool none = kPad && k_x + u >= groups;
-      *reinterpret_cast<u4*>(to + (k_row * L::kPieces + L::k_piece(k_row, (k_x + u) * 4 + k_g)) * 16) =
-          none ? u4{0, 0, 0, 0} : codes;
+      *reinterpret_cast<u4*>(to + (k_row * L::kPieces + L::k_piece(k_row, (k_x + u) * 4 + k_g)) * 16) = codes;
     }
     if (f_x < GT) {
       u4 f = f_mine ? kf : u4{0, 0, 0, 0};
@@ -287,6 +298,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       if (v_i == 0 && v_plane == 0) noted[buf][v_row] = (uint8_t)bits;
       any = bits != 0;
     }
+    if constexpr (kPad) join_planes();
     // pairs of lanes z, z + 1: elements 32 x + 16 half + v_i + z
     char* hi = to + L::kBytes;
 #pragma unroll
@@ -315,9 +327,9 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
     if (lane == 0) has_noted[buf][wave] = wave_any;
   };
 
-  f16x o[L::kTiles];
+  f16x o[NG];
 #pragma unroll
-  for (int t = 0; t < L::kTiles; ++t) o[t] = f16x{};
+  for (int t = 0; t < NG; ++t) o[t] = f16x{};
   float m = minus_inf(), l = 0.f, lr = 0.f;  // (lr: of the rounded weights)
   float back = __builtin_inff();             // kShift - m: what turns a score into its weight's exponent
   constexpr float kSlack = 32768.f;          // 2^8, kShift included
@@ -330,7 +342,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
     f16x s;
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int x = 0; x < GT; ++x) {
+    for (int x = 0; x < NG; ++x) {
       f16x acc{};
 #pragma unroll
       for (int k = 2 * x; k < 2 * x + 2; ++k) {
@@ -386,7 +398,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       l *= shrink;
       lr *= shrink;
 #pragma unroll
-      for (int t = 0; t < L::kTiles; ++t) o[t] *= shrink;
+      for (int t = 0; t < NG; ++t) o[t] *= shrink;
       // So large a product is off by whole numbers when rounded, as `top` was and
       // the fused one is not: all are rounded, so that none passes the largest.
       float times = sc;
@@ -407,7 +419,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
       for (int j = 0; j < 8; ++j) split<NW>(w[b * 8 + j], p, j);
       if constexpr (NW == 1) lr = plus_all(p[0], lr);
 #pragma unroll
-      for (int t = 0; t < L::kTiles; ++t) {
+      for (int t = 0; t < NG; ++t) {
         // a lane reads 4 elements of one of 4 keys, and gets 4 keys of one element
         const int r = 4 * h + ((lane >> 2) & 3), e = t * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
         const char* at = lv + (sub * 32 + b * 16) * L::kPieces * 16 + (e & 7) * 2;
@@ -462,7 +474,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
         const bool sees_it = ((there >> n) & 1) && key >= low && key <= pos;
         const uint32_t note = noted[buf][n];
 #pragma unroll
-        for (int t = 0; t < L::kTiles; ++t)
+        for (int t = 0; t < NG; ++t)
           if (sees_it && ((note >> t) & 1))
 #pragma unroll
             for (int y = 0; y < 16; ++y) o[t][y] = __builtin_nanf("");
@@ -483,7 +495,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   if (span.parts > 1) {
     const int64_t to = part * parts.rows + (int64_t)token * a.heads + head;
 #pragma unroll
-    for (int t = 0; t < L::kTiles; ++t)
+    for (int t = 0; t < NG; ++t)
 #pragma unroll
       for (int y = 0; y < 16; y += 4)
         *reinterpret_cast<f4*>(parts.o + to * D + t * 32 + 2 * y + 4 * h) = f4{o[t][y], o[t][y + 1], o[t][y + 2], o[t][y + 3]};
@@ -495,8 +507,7 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
   const bool wide_out = ((reinterpret_cast<uintptr_t>(a.out.d) / sizeof(T) | (uint64_t)a.out.token_stride |
                           (uint64_t)a.out.head_stride) & 3) == 0;
 #pragma unroll
-  for (int t = 0; t < L::kTiles; ++t) {
-    if (kPad && t >= groups) break;
+  for (int t = 0; t < NG; ++t) {
 #pragma unroll
     for (int y = 0; y < 16; y += 4) {
       typedef T run_of __attribute__((ext_vector_type(4)));
@@ -519,21 +530,21 @@ __device__ __forceinline__ void chunk_quant_rows(const AttendArgs& a, const Part
 // alone: sequences of few rows are its too.  Registers for three workgroups of
 // 16-bit queries in heads of up to 64 (more of the waiting hidden), one of heads
 // beyond 128, whose sums alone are 128 registers.
-template <typename T, int kBits, int GT, bool kPad>
+template <typename T, int kBits, int GT, int NG>
 __global__ __launch_bounds__((QTile<T, kBits, GT>::kThreads), GT == 8 ? 1 : GT == 2 && sizeof(T) == 2 ? 3 : 2)
 void chunk_quant_kernel(AttendArgs a, Parts parts, bool alone) {
-  chunk_quant_rows<T, kBits, GT, kPad>(a, parts, alone, blockIdx.x, gridDim.x, blockIdx.z);
+  chunk_quant_rows<T, kBits, GT, NG>(a, parts, alone, blockIdx.x, gridDim.x, blockIdx.z);
 }
 
-template <typename T, int kBits, int GT, bool kPad>
+template <typename T, int kBits, int GT, int NG>
 hipError_t chunk_of(const AttendArgs& a, const Parts& parts, int64_t tiles, bool alone, hipStream_t s) {
   constexpr size_t lds = 2 * QTile<T, kBits, GT>::kStage;
   if (lds > 60000) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_quant_kernel<T, kBits, GT, kPad>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(chunk_quant_kernel<T, kBits, GT, NG>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  chunk_quant_kernel<T, kBits, GT, kPad>
+  chunk_quant_kernel<T, kBits, GT, NG>
       <<<dim3((unsigned)(tiles * a.p.kv_heads), 1, parts.most), QTile<T, kBits, GT>::kThreads, lds, s>>>(a, parts, alone);
   return hipGetLastError();
 }
@@ -541,12 +552,14 @@ hipError_t chunk_of(const AttendArgs& a, const Parts& parts, int64_t tiles, bool
 template <typename T, int kBits>
 hipError_t chunk_width(const AttendArgs& a, const Parts& parts, int64_t tiles, bool alone, hipStream_t s) {
   switch (a.p.dim / 32) {
-    case 1: return chunk_of<T, kBits, 2, true>(a, parts, tiles, alone, s);
-    case 2: return chunk_of<T, kBits, 2, false>(a, parts, tiles, alone, s);
-    case 3: return chunk_of<T, kBits, 4, true>(a, parts, tiles, alone, s);
-    case 4: return chunk_of<T, kBits, 4, false>(a, parts, tiles, alone, s);
-    case 8: return chunk_of<T, kBits, 8, false>(a, parts, tiles, alone, s);
-    default: return chunk_of<T, kBits, 8, true>(a, parts, tiles, alone, s);
+    case 1: return chunk_of<T, kBits, 2, 1>(a, parts, tiles, alone, s);
+    case 2: return chunk_of<T, kBits, 2, 2>(a, parts, tiles, alone, s);
+    case 3: return chunk_of<T, kBits, 4, 3>(a, parts, tiles, alone, s);
+    case 4: return chunk_of<T, kBits, 4, 4>(a, parts, tiles, alone, s);
+    case 5: return chunk_of<T, kBits, 8, 5>(a, parts, tiles, alone, s);
+    case 6: return chunk_of<T, kBits, 8, 6>(a, parts, tiles, alone, s);
+    case 7: return chunk_of<T, kBits, 8, 7>(a, parts, tiles, alone, s);
+    default: return chunk_of<T, kBits, 8, 8>(a, parts, tiles, alone, s);
   }
 }
 

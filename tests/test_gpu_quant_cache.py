@@ -800,3 +800,16 @@ def test_beam_step_captured_and_replayed(pkg, kind):
     starts = (torch.arange(rows + 1, dtype=torch.int32) * 33).cuda()
     for a, b in zip(captured[0].read(0, starts, rows * 33), alone[0].read(0, starts, rows * 33)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+@pytest.mark.parametrize("d", [32, 96, 160, 192, 224])
+def test_attention_of_every_number_of_blocks_in_parts(pkg, kind, dtype, d):
+    """Heads that fill no tile, keys split over workgroups, rows with gaps behind
+    them that stay as they are, blocks that are not finite in unseen places."""
+    m = Made(pkg, kind, [2100, 1300], [1, 70], 4, 2, d, 16, dtype, seed=d)
+    dest = torch.full((71, 5, d + 8), 7.0, dtype=dtype, device="cuda")
+    m.check(pkg, out=dest[:, :4, :d])
+    assert bool((dest[:, 4] == 7).all()) and bool((dest[..., d:] == 7).all())
+    m.check(pkg, window=300, first=[1900, 1000], what="window")
