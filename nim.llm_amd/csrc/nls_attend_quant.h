@@ -125,8 +125,8 @@ constexpr float kQuantShift = 14.f;  // log2 of the largest weight times factor
 
 // Heads of NG blocks, at most GT (2, 4 or 8: what the factors are dealt out by).
 // Each number of blocks has its own loads, plane by plane: 32 contexts of 8192, bf16
-// over Q4_0, heads of 96 61 us and of 192 133 (a byte at a time, for any number
-// below GT, 182 and 518).
+// over Q4_0, heads of 96 61 us and of 192 100 (a byte at a time, for any number
+// below GT, 182 and 518; of the 418 off 192, 34 are its second wave a SIMD).
 template <typename T, int kBits, int GT, int NG>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,
                                                int group_at, int part) {

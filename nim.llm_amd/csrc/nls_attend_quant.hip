@@ -7,14 +7,19 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Waves per SIMD that registers are kept for.
-template <typename T, int kBits, int GT>
+// Waves per SIMD that registers are kept for.  Heads beyond 128 want more than two
+// waves have; over 4 bits two are faster all the same (32 contexts of 8192, bf16,
+// heads of 160, 192, 224 and 256: 89, 100, 114 and 137 us with two, 126, 134, 148 and
+// 161 with one; fp32 of 160 and 192 120 and 137, 167 and 185), but for fp32 queries
+// in heads of 224 and 256 (214 either way); over 8 bits one is (192: 179, with two
+// 198; fp32 191 and 239).  Three for heads of 96 gain nothing (62 us, 63.5 so).
+template <typename T, int kBits, int GT, int NG>
 constexpr int few_quant_waves() {
-  return GT == 8 ? 1 : GT == 4 || (sizeof(T) == 4 && kBits == 8) ? 2 : 3;
+  return GT == 8 ? (kBits == 4 && (sizeof(T) == 2 || NG <= 6) ? 2 : 1) : GT == 4 || (sizeof(T) == 4 && kBits == 8) ? 2 : 3;
 }
 
 template <typename T, int kBits, int GT, int NG>
-__global__ __launch_bounds__(kThreads, (few_quant_waves<T, kBits, GT>())) void few_quant_kernel(AttendArgs a, Parts parts,
+__global__ __launch_bounds__(kThreads, (few_quant_waves<T, kBits, GT, NG>())) void few_quant_kernel(AttendArgs a, Parts parts,
                                                                                                int tiles, bool chunk_runs) {
   few_quant_rows<T, kBits, GT, NG>(a, parts, tiles, chunk_runs, blockIdx.x, blockIdx.z);
 }
