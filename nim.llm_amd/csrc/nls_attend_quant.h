@@ -99,8 +99,9 @@ template <typename T>
 constexpr int quant_parts() {
   return sizeof(T) == 4 ? 2 : 1;
 }
-// Weights times factors, likewise; for bf16 queries they are rounded to fp16 (an
-// eighth of the output's own step).
+// Weights times factors, likewise; for bf16 queries the weights and then the products
+// are rounded to fp16 (each an eighth of the output's own rounding.  Two parts: 64
+// contexts of up to 16384 257 us for 204; 32 of 8192, heads of 128 91 for 71).
 template <typename T>
 constexpr int weight_parts() {
   return __is_same(T, __bf16) ? 1 : 2;
@@ -218,11 +219,15 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     f4 o[2 * GT];
 #pragma unroll
     for (int t = 0; t < 2 * GT; ++t) o[t] = f4{0, 0, 0, 0};
-    // The weights are taken from m + up: 2^up is above any value's factor so far,
-    // so that a weight times a factor is at most 1.  (One part: not below 2^0, so
-    // that the weight itself is too.)  most: that bound as fp16's bits.
+    // A weight times a value's factor is at most 1: 2^e is above any factor so far,
+    // most is that bound as fp16's bits.  Two parts: the weights are taken from m + e.
+    // One part, where weight and factor are rounded by themselves: half of e is taken
+    // off each while it is above 0; else the factors are brought up to 1 (exactly).
+    // So small weights keep clear of fp16's denormal numbers, and so does their product
+    // with small factors.
     float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f, back = kQuantShift - up;
-    uint32_t most = NW == 1 ? 0x3bffu : 0u;
+    int e_of = NW == 1 ? -15 : -24;
+    uint32_t most = NW == 1 ? 0x1ffu : 0u, lift = 0x78007800u;  // (2^15 twice)
 
     // A step's keys are runs of 16, each within a page (-1: none; what is read
     // there is page 0, and counts for nothing).
@@ -324,6 +329,17 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         }
       }
     };
+    // the largest factor of the lanes that is a number, and the power of two above it
+    auto wave_top = [&](uint32_t d) {
+      d = d < 0x7c00u ? d : 0;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) {
+        const uint32_t other = __shfl_xor(d, x);
+        d = other > d ? other : d;
+      }
+      return d;
+    };
+    auto above = [](uint32_t d) { return d < 0x400u ? -14 : (int)(d >> 10) - 14; };
     // a lane's 4 tokens' factors of a plane of sh_f (token 4 r + g of a run is at 4 g + r)
     auto factors_of = [&](int plane, int s) { return *reinterpret_cast<const u2*>(factors + plane * (KT / 2) + s * 8 + g * 2); };
 
@@ -363,6 +379,27 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       for (int n = 0; n < FW; ++n) dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[n])));
       uint32_t dtop = dm[0] > dm[1] ? dm[0] : dm[1];
       dtop = lane < 32 ? 0 : dtop;
+      if (NW == 1) {
+        if (__ballot(dtop > most)) {
+          const uint32_t d = wave_top(dtop);
+          if (d > most) {
+            const int e = above(d), off = e > 0 ? (e + 1) / 2 : 0;  // of the weights' exponents
+            const float shrink = ldexpf(1.f, e_of - e);
+            l *= exp2_(up - off);
+            back += up - off;
+            up = (float)off;
+#pragma unroll
+            for (int t = 0; t < 2 * GT; ++t) o[t] *= shrink;
+            e_of = e;
+            most = (uint32_t)(e + 14) << 10 | 0x3ffu;
+            lift = (uint32_t)(15 + off - e) << 10;
+            lift |= lift << 16;
+          }
+        }
+        if (lane >= 32)
+#pragma unroll
+          for (int n = 0; n < FW; ++n) fc[n] = __builtin_bit_cast(uint32_t, halves(fc[n]) * halves(lift));
+      }
       {
         uint16_t* to = reinterpret_cast<uint16_t*>(factors) + (lane < 32 ? 0 : GT * KT) + f_x * KT + (f_token & ~15);
 #pragma unroll
@@ -420,17 +457,12 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       top *= sc;
-      if (__ballot(top > m || dtop > most)) {
+      if (__ballot(top > m || (NW == 2 && dtop > most))) {
         float shrink = up;
-        if (__ballot(dtop > most)) {
-          uint32_t d = dtop < 0x7c00u ? dtop : 0;
-#pragma unroll
-          for (int x = 1; x < 64; x <<= 1) {
-            const uint32_t other = __shfl_xor(d, x);
-            d = other > d ? other : d;
-          }
+        if (NW == 2 && __ballot(dtop > most)) {
+          const uint32_t d = wave_top(dtop);
           if (d > most) {
-            const int e = d < 0x400u ? -14 : (int)(d >> 10) - 14;  // 2^e is above it
+            const int e = above(d);
             up = (float)e;
             most = (uint32_t)(e + 14) << 10 | 0x3ffu;
           }
@@ -525,8 +557,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 
     // the waves' sums, relative to the largest of their maxima alone
     m *= rest;
-    const float full = exp2_(up);
-    l *= full;
+    const float full = NW == 1 ? ldexpf(1.f, e_of) : exp2_(up);
+    l *= exp2_(up);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g == 0) {

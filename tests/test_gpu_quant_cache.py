@@ -813,3 +813,39 @@ def test_attention_of_every_number_of_blocks_in_parts(pkg, kind, dtype, d):
     m.check(pkg, out=dest[:, :4, :d])
     assert bool((dest[:, 4] == 7).all()) and bool((dest[..., d:] == 7).all())
     m.check(pkg, window=300, first=[1900, 1000], what="window")
+
+
+# The outputs' bound where small weights add up: a weight times its factor is one
+# part of eleven bits (2^-11, and its factor or weight another's at most), scores and
+# exponentials in fp32 are some 2^-18 of it, and sums of that many equal terms in
+# fp32 lose at most 16384 2^-24.
+SMALL = 2.0 ** -10 + 2.0 ** -10 + 2.0 ** -16
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+@pytest.mark.parametrize("value", [1.0, 1e-3, 1e-4, 4e-5, 7000.0])
+def test_attention_many_small_weights_and_values(pkg, kind, dtype, value):
+    """Some keys of nearly all the weight whose values are 0, four of any 256 so that
+    whoever sums has one, and 16128 equal ones of 2^-14.5 each, whose values are all
+    alike: rounded one by one the same way, their sum would be off by as much as each."""
+    page, d, lens = 4096, 64, [16384]
+
+    def contents(gen, shape):
+        x = np.zeros(shape, dtype=np.float32)
+        x[:, 1] = value
+        for far in (7, 39, 71, 103):
+            x[:, 0, :, far::256] = 1.0
+            x[:, 1, :, far::256] = 0.0
+        return x
+
+    m = Made(pkg, kind, lens, [1], 4, 1, d, page, dtype, seed=3, contents=contents)
+    m.q = torch.ones(1, 4, d, dtype=dtype)
+    scale = 14.5 * math.log(2.0) / d / float(m.values()[m.table_l[0][0], 0, 0, 7, 0])
+    say(f"[small weights] {kind} {NAME[dtype]} {value}")
+    want, lse, _, lb = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, scale)
+    got, l = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), 1, 16384,
+                                 scale=scale, lse=True, fmt=m.fmt)
+    # (fp16 outputs have a least step: half of 2^-24)
+    near(got, want, np.abs(want) * (SMALL + R.HALF[dtype]) + (2.0 ** -25 if dtype == F16 else 0), f"{kind} {value}")
+    near(l, lse, lb, "lse")
