@@ -329,9 +329,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         }
       }
     };
-    // the largest factor of the lanes that is a number, and the power of two above it
+    // the largest factor of the lanes, and the power of two above it
     auto wave_top = [&](uint32_t d) {
-      d = d < 0x7c00u ? d : 0;
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) {
         const uint32_t other = __shfl_xor(d, x);
@@ -371,12 +370,14 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
         for (int n = 0; n < FW; ++n) fc[n] &= (2 * n < left ? 0xffffu : 0u) | (2 * n + 1 < left ? 0xffff0000u : 0u);
       }
-      // (bits of numbers that are not negative, in order; a block that is not finite
-      // is above them all, and has no say)
+      // (bits of numbers that are not negative, in order.  One that is not finite has no
+      // say, and hides none: it wraps to below the others, which are taken down again.)
       typedef uint16_t us2 __attribute__((ext_vector_type(2)));
       us2 dm{0, 0};
 #pragma unroll
-      for (int n = 0; n < FW; ++n) dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[n])));
+      for (int n = 0; n < FW; ++n)
+        dm = __builtin_elementwise_max(dm, __builtin_bit_cast(us2, halves(fc[n])) + us2{0x8400, 0x8400});
+      dm = __builtin_elementwise_sub_sat(dm, us2{0x8400, 0x8400});
       uint32_t dtop = dm[0] > dm[1] ? dm[0] : dm[1];
       dtop = lane < 32 ? 0 : dtop;
       if (NW == 1) {

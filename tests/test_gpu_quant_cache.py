@@ -849,3 +849,23 @@ def test_attention_many_small_weights_and_values(pkg, kind, dtype, value):
     # (fp16 outputs have a least step: half of 2^-24)
     near(got, want, np.abs(want) * (SMALL + R.HALF[dtype]) + (2.0 ** -25 if dtype == F16 else 0), f"{kind} {value}")
     near(l, lse, lb, "lse")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=NAME.get)
+@pytest.mark.parametrize("d", [32, 128, 256])
+@pytest.mark.parametrize("lens,new", [([2], [2]), ([8], [7]), ([4, 40], [3, 2])])
+def test_attention_a_neighbour_that_is_not_finite(pkg, kind, dtype, d, lens, new):
+    """The last token's values are NaN in every block, and the tokens before it have
+    the only finite ones or by far the largest: rows that do not see it are as without it."""
+    def contents(gen, shape):
+        x = gen.standard_normal(shape).astype(np.float32)
+        x[:, 1] *= 1e-3
+        x[:, 1, :, min(lens) - 2] = 50.0
+        x[:, 1, :, min(lens) - 1] = np.nan
+        return x
+
+    m = Made(pkg, kind, lens, new, 2, 1, d, 64, dtype, seed=d, contents=contents)
+    say(f"[nan neighbour] {kind} {NAME[dtype]} d={d} {lens}")
+    got, _ = m.check(pkg)
+    assert torch.isfinite(got[:new[0] - 1].float()).all() and torch.isnan(got[new[0] - 1].float()).all()
