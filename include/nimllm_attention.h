@@ -273,8 +273,10 @@ int32_t nls_cache_release(const nls_page_tables* tables, const int32_t* d_slots,
  * one, or, where that is -1, empty.  Full pages are shared.  The partial last
  * page of a parent stays with the parent if it is its own child, else goes to
  * its first child; the other children take copies, in the order of the slots, on
- * the lowest pages that nobody holds any more.  What no slot goes on from is let
- * go of.  A status as above: BAD_ENTRY for a parent or a length out of range.
+ * the lowest pages that nobody holds any more (whose counts are 0, or as high as the
+ * entries that let go of them here: a page that someone outside of these rows counts
+ * on stays as it is).  What no slot goes on from is let go of.  A status as above:
+ * BAD_ENTRY for a parent or a length out of range.
  * d_work: nls_cache_reorder_workspace() bytes, 256-byte aligned. */
 size_t nls_cache_reorder_workspace(const nls_page_tables* tables);
 int32_t nls_cache_reorder(const nls_page_pool* pool, const nls_page_tables* tables, const int32_t* d_parents,

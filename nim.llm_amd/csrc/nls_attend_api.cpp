@@ -428,7 +428,7 @@ int32_t nls_cache_compact(const nls_page_pool* p, const nls_page_tables* t, int3
 
 size_t nls_cache_reorder_workspace(const nls_page_tables* t) {
   if (check_tables(t, true)) return 0;
-  return align256(4 * (2 + 5 * (size_t)t->slots + (size_t)t->slots * t->max_pages));
+  return align256(4 * (2 + 5 * (size_t)t->slots + (size_t)t->pages + (size_t)t->slots * t->max_pages));
 }
 
 int32_t nls_cache_reorder(const nls_page_pool* p, const nls_page_tables* t, const int32_t* d_parents, int32_t* d_status,

@@ -391,12 +391,13 @@ __global__ __launch_bounds__(kCopyThreads) void move_kernel(PoolArgs p, TableArg
 
 // Where reorder's work area has what: [0] the status, [1] pairs to copy, then
 // their sources and destinations, each slot's old length, the page its partial
-// last one is copied to (-1: none), its first child, and the old table.
+// last one is copied to (-1: none), its first child, how many entries let go of a
+// page (of those whose count is above 1), and the old table.
 struct ReorderWork {
-  int32_t *head, *from, *to, *len, *fresh, *first, *rows;
-  __device__ __host__ ReorderWork(int32_t* w, int slots)
+  int32_t *head, *from, *to, *len, *fresh, *first, *gone, *rows;
+  __device__ __host__ ReorderWork(int32_t* w, int slots, int pages)
       : head(w), from(w + 2), to(from + slots), len(to + slots), fresh(len + slots), first(fresh + slots),
-        rows(first + slots) {}
+        gone(first + slots), rows(gone + pages) {}
 };
 // Pages of a context (whose length may be all that an int holds).
 __device__ __forceinline__ int pages_of(int len, int shift) { return (int)(((uint32_t)len + ((1u << shift) - 1)) >> shift); }
@@ -407,17 +408,20 @@ __device__ __forceinline__ int settled(const int32_t* p) {
 
 // What goes where.  A page is free for a copy when nobody held it, or only
 // slots whose contexts end here: it is marked by those, and the mark is taken off
-// by every row as it will be.  The first workgroup: what bounds it are the two passes
+// by every row as it will be.  Where its count is above the entries that let go of it
+// someone else holds it, outside of these rows: those of a count above 1 are counted,
+// if any is marked still (which LDS tells for up to 65536 pages: 2 us of 78 less).  The first workgroup: what bounds it are the two passes
 // over the table: a wave takes eight rows at a time, with the slots' numbers in LDS
 // (512 slots of 73 entries: 47 us when entries are dealt out to threads by a
 // division each, 33 by rows, 30 since the other workgroups keep the table).
-constexpr int kSlotsHeld = 2048;
+constexpr int kSlotsHeld = 2048, kWordsHeld = 1024;
 __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, const int32_t* src, int32_t* status,
                                                                int32_t* work) {
   __shared__ int sh[kPlanWaves];
   __shared__ int s_src[kSlotsHeld], s_len[kSlotsHeld], s_first[kSlotsHeld];
+  __shared__ uint64_t s_many[kWordsHeld];  // pages of counts above 1
   const PlanLds lds = plan_lds(t.pages);
-  const ReorderWork w(work, t.slots);
+  const ReorderWork w(work, t.slots, t.pages);
   if (blockIdx.x > 0) {  // the table as it was, by the other workgroups
     const uint32_t n = (uint32_t)t.slots * (uint32_t)t.max_pages, per = t.max_pages;  // (below 2^31)
     for (uint32_t e = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; e < n; e += (gridDim.x - 1) * kPlanThreads)
@@ -445,20 +449,26 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (t.pages + 63) >> 6;
-  constexpr int kWords = 8;
-  for (int i0 = wave * kWords; i0 < words; i0 += kPlanWaves * kWords) {
-    int refs[kWords];
+  // f(word, this lane's page, its count) for all words of the bitmap
+  auto over_counts = [&](auto f) {
+    constexpr int kWords = 8;
+    for (int i0 = wave * kWords; i0 < words; i0 += kPlanWaves * kWords) {
+      int refs[kWords];
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      const int p = (i0 + u) * 64 + lane;
-      refs[u] = p < t.pages ? t.refs[p] : 1;
-    }
+      for (int u = 0; u < kWords; ++u) {
+        const int p = (i0 + u) * 64 + lane;
+        refs[u] = p < t.pages ? t.refs[p] : 1;
+      }
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) {
-      const uint64_t b = __ballot(refs[u] == 0);
-      if (lane == 0 && i0 + u < words) lds.bits[i0 + u] = b;
+      for (int u = 0; u < kWords; ++u)
+        if (i0 + u < words) f(i0 + u, (i0 + u) * 64 + lane, refs[u]);
     }
-  }
+  };
+  over_counts([&](int word, int, int refs) {
+    const uint64_t b = __ballot(refs == 0), many = __ballot(refs > 1);
+    if (lane == 0) lds.bits[word] = b;
+    if (lane == 0 && word < kWordsHeld) s_many[word] = many;
+  });
   // the partial page of a parent stays with itself, else with its first child
   for (int s = threadIdx.x; s < t.slots; s += kPlanThreads) {
     const int p = held ? s_src[s] : src[s];
@@ -469,34 +479,36 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
   auto len_of = [&](int s) { return held ? s_len[s] : w.len[s]; };
   auto first_of = [&](int s) { return held ? s_first[s] : settled(&w.first[s]); };
   uint32_t* marks = reinterpret_cast<uint32_t*>(lds.bits);
-  // eight rows at a time to a wave, 128 entries of each
+  // f(page) for the entries of the rows that end here: eight rows at a time to a
+  // wave, 128 entries of each
   constexpr int kRows = 8, kCols = 2;
-  for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
-    int used[kRows], most = 0;  // (of those that end here)
+  auto over_ending = [&](auto f) {
+    for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
+      int used[kRows], most = 0;
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) {
-      const int s = s0 + u;
-      used[u] = s < t.slots && src_of(s) != s ? pages_of(len_of(s), t.page_shift) : 0;
-      most = used[u] > most ? used[u] : most;
+      for (int u = 0; u < kRows; ++u) {
+        const int s = s0 + u;
+        used[u] = s < t.slots && src_of(s) != s ? pages_of(len_of(s), t.page_shift) : 0;
+        most = used[u] > most ? used[u] : most;
+      }
+      for (int j0 = lane; j0 < most; j0 += 64 * kCols) {
+        int page[kRows][kCols];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            const int j = j0 + 64 * c;
+            page[u][c] = j < used[u] ? t.table[(s0 + u) * t.table_stride + j] : -1;
+          }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if ((uint32_t)page[u][c] < (uint32_t)t.pages) f(page[u][c]);
+      }
     }
-    for (int j0 = lane; j0 < most; j0 += 64 * kCols) {
-      int page[kRows][kCols];
-#pragma unroll
-      for (int u = 0; u < kRows; ++u)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int j = j0 + 64 * c;
-          page[u][c] = j < used[u] ? t.table[(s0 + u) * t.table_stride + j] : -1;
-        }
-#pragma unroll
-      for (int u = 0; u < kRows; ++u)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int p = page[u][c];
-          if ((uint32_t)p < (uint32_t)t.pages) atomicOr(&marks[p >> 5], 1u << (p & 31));
-        }
-    }
-  }
+  };
+  over_ending([&](int p) { atomicOr(&marks[p >> 5], 1u << (p & 31)); });
   __syncthreads();
   for (int s0 = wave * kRows; s0 < t.slots; s0 += kPlanWaves * kRows) {
     int from[kRows], keep[kRows], most = 0;
@@ -530,6 +542,26 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
     }
   }
   __syncthreads();
+  int several = words > kWordsHeld;
+  if (!several)
+    for (int i = threadIdx.x; i < words; i += kPlanThreads) several |= (lds.bits[i] & s_many[i]) != 0;
+  if (__syncthreads_or(several)) {
+    over_counts([&](int word, int p, int refs) {
+      if (refs > 1 && (lds.bits[word] >> lane) & 1)
+        __hip_atomic_store(&w.gone[p], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    });
+    __syncthreads();
+    over_ending([&](int p) {
+      if (((marks[p >> 5] >> (p & 31)) & 1) && t.refs[p] > 1) atomicAdd(&w.gone[p], 1);
+    });
+    __syncthreads();
+    over_counts([&](int word, int p, int refs) {
+      const bool mine = refs > 1 && (lds.bits[word] >> lane) & 1;
+      const uint64_t stays = __ballot(mine && settled(&w.gone[mine ? p : 0]) < refs);
+      if (lane == 0) lds.bits[word] &= ~stays;
+    });
+    __syncthreads();
+  }
   const int free_pages = rank_bitmap(words, lds.bits, lds.ranks, sh);
   int total = 0;
   for (int s0 = 0; s0 < t.slots; s0 += kPlanThreads) {
@@ -562,7 +594,7 @@ __global__ __launch_bounds__(kPlanThreads) void reorder_kernel(TableArgs t, cons
 // The tables as planned, and the copies.
 __global__ __launch_bounds__(kCopyThreads) void reorder_apply_kernel(PoolArgs p, TableArgs t, const int32_t* src,
                                                                      int32_t* work, int table_blocks) {
-  const ReorderWork w(work, t.slots);
+  const ReorderWork w(work, t.slots, t.pages);
   if (w.head[0]) return;
   if ((int)blockIdx.x >= table_blocks) {
     copy_pairs(p, t.pages, w.from, w.to, w.head[1], blockIdx.x - table_blocks, gridDim.x - table_blocks);

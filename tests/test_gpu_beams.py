@@ -363,3 +363,59 @@ def test_reorder_over_the_most_pages(pkg):
     assert table[:, :3].tolist() == [[pages - 1, pages - 2, -1], [pages - 1, 7, -1], [pages - 1, pages - 3, -1]]
     assert torch.equal(wide[:, 7], before) and torch.equal(wide[:, pages - 3], before)
     assert refs[pages - 3:].tolist() == [1, 1, 3] and int(refs[7]) == 1 and lens.tolist() == [3] * 3
+
+
+@pytest.mark.parametrize("slots,pages", [(5, 18), (2100, 4208), (5, 70001)])
+def test_reorder_leaves_pages_that_others_hold(pkg, slots, pages):
+    """Pages of contexts that end here, with more on their counts than the entries
+    that let them go (a caller's own, or of slots outside of the given rows): no copy
+    takes them, and the counts go down by what was let go."""
+    ps, per = 16, 3
+    c = pkg.PagedCache(2, pages, ps, 1, 32, slots, per, dtype=torch.float32)
+    counts = [20, 18, 16, 32, 7] + [0] * (slots - 5)
+    assert c.reserve(torch.tensor(counts, dtype=torch.int32).cuda()).item() == pkg.PAGES_DONE
+    # 0: pages 0, 1; 1: pages 2, 3; 2: page 4; 3: pages 5, 6; 4: page 7
+    c.kv.normal_()
+    c.refs[2] = 2                  # one more holder
+    c.refs[3] = 5
+    c.refs[8:] = 1
+    c.refs[pages - 3] = 0
+    c.table[3, 0] = 4              # page 4 by two slots: 2 and 3 (page 5 is free then)
+    c.refs[4], c.refs[5] = 2, 1    # 5: only someone else
+    kv = c.kv.clone()
+    parents = [0, 0, 0, 0, 0] + [-1] * (slots - 5)
+    if slots > 2050:
+        parents[2050] = 0
+    # copies for slots 1, 2, 3, 4 (and 2050): the pages that were slot 2's and 3's alone
+    # (4, held twice and let go twice, and 6), slot 4's, the free one, and no other
+    n = sum(p == 0 for p in parents) - 1
+    st = c.reorder(torch.tensor(parents, dtype=torch.int32).cuda()).item()
+    if n > 4:
+        assert st == pkg.PAGES_NONE_LEFT and torch.equal(c.kv, kv) and c.lens.tolist() == counts
+        parents[2050] = -1
+        st = c.reorder(torch.tensor(parents, dtype=torch.int32).cuda()).item()
+    assert st == pkg.PAGES_DONE
+    fresh = [4, 6, 7, pages - 3]
+    assert c.table[:5].tolist() == [[0, 1, -1]] + [[0, p, -1] for p in fresh]
+    assert c.refs[:8].tolist() == [5, 1, 1, 4, 1, 1, 1, 1] and int(c.refs[pages - 3]) == 1
+    assert c.lens.tolist() == [20] * 5 + [0] * (slots - 5)
+    kv[:, fresh] = kv[:, 1:2]
+    assert torch.equal(c.kv, kv)
+
+
+def test_reorder_of_some_rows_of_a_table(pkg):
+    """Rows 2 and on of a table whose first two slots share pages with them."""
+    c = pkg.PagedCache(1, 9, 16, 2, 32, 6, 3, dtype="q8_0")
+    assert c.reserve(torch.tensor([37, 0, 0, 0, 5, 0], dtype=torch.int32).cuda()).item() == pkg.PAGES_DONE
+    c.kv.random_(0, 255)
+    to = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()
+    assert c.fork(to(0, 0), to(2, 3)).item() == pkg.PAGES_DONE  # pages 0, 1 three times; 2, 4, 5 theirs; slot 4: 3
+    assert c.table.tolist()[:5] == [[0, 1, 2], [-1] * 3, [0, 1, 4], [0, 1, 5], [3, -1, -1]]
+    kv = c.kv.clone()
+    # slots 2 and 3 end, 4 and 5 go on from 4, with a copy
+    st = pkg.cache_reorder(c.kv, c.table[2:], c.lens[2:], c.refs, to(-1, -1, 2, 2), fmt=c.fmt)
+    assert st.item() == pkg.PAGES_DONE
+    assert c.table.tolist() == [[0, 1, 2], [-1] * 3, [-1] * 3, [-1] * 3, [3, -1, -1], [4, -1, -1]]
+    assert c.refs.tolist() == [1, 1, 1, 1, 1, 0, 0, 0, 0] and c.lens.tolist() == [37, 0, 0, 0, 5, 5]
+    kv[:, 4] = kv[:, 3]
+    assert torch.equal(c.kv, kv)
