@@ -14,7 +14,8 @@ constexpr int kBeamPer = 32, kBeamPerFew = 8;  // logits of a thread
 // The largest logit of a slice, the sum of exp(l - max), and behind the parts (in
 // the workspace) its `beams` largest logits in order.
 struct BeamPart {
-  float max, sum;
+  double sum;
+  float max;
 };
 struct BeamEntry {
   float l;

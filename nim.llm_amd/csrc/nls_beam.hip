@@ -32,7 +32,8 @@ __device__ __forceinline__ bool takes_part(const BeamArgs& a, int row) {
 template <int kPer>
 __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   constexpr int kSlice = kPer * kNT;
-  __shared__ float sh_max[kWaves], sh_sum[kWaves];
+  __shared__ float sh_max[kWaves];
+  __shared__ double sh_sum[kWaves];
   __shared__ uint32_t sh_bound[kWaves];
   __shared__ int count;
   __shared__ BeamEntry list[kList];
@@ -90,9 +91,10 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
       for (int j = 0; j < kPer; ++j) sum += l[j] > none ? term(l[j]) : 0.f;
     }
   }
+  double all = sum;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  if (lane == 0) sh_sum[wave] = sum;
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+  if (lane == 0) sh_sum[wave] = all;
   const float least = bound ? key2f(bound) : none;
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
@@ -103,7 +105,7 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
   __syncthreads();
   const int64_t part = blockIdx.x;
   BeamEntry* out = a.entries + part * a.beams;
-  if (threadIdx.x == 0) a.parts[part] = {mx, sh_sum[0] + sh_sum[1] + sh_sum[2] + sh_sum[3]};
+  if (threadIdx.x == 0) a.parts[part] = {sh_sum[0] + sh_sum[1] + sh_sum[2] + sh_sum[3], mx};
   const int m = count;
   if (m <= kList) {
     // a place for each by the number of those before it
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
 #pragma unroll
     for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const double of = top;
-    auto share = [&](const BeamPart& q) { return q.max == top ? (double)q.sum : (double)q.sum * exp((double)q.max - of); };
+    auto share = [&](const BeamPart& q) { return q.max == top ? q.sum : q.sum * exp((double)q.max - of); };
     double sum = asks && part < a.slices ? share(held_part) : 0.0;
     if (asks)
       for (int s = part + 16; s < a.slices; s += 16) sum += share(p[s]);

@@ -419,3 +419,18 @@ def test_reorder_of_some_rows_of_a_table(pkg):
     assert c.refs.tolist() == [1, 1, 1, 1, 1, 0, 0, 0, 0] and c.lens.tolist() == [37, 0, 0, 0, 5, 5]
     kv[:, 4] = kv[:, 3]
     assert torch.equal(c.kv, kv)
+
+
+def test_sums_of_a_row_across_lanes(pkg):
+    """One logit of weight 1 and 255 of 2^-26, no two within a thread's run: a lane
+    that adds another's 2^-26 to its 1 in fp32 loses them one by one."""
+    vocab = 1024
+    logits = np.full((1, vocab), -np.inf, dtype=np.float32)
+    logits[0, ::4] = -26 * math.log(2.0)
+    logits[0, 0] = 0.0
+    (parents, tokens, worth, over), _ = select(logits, np.zeros((1, 1), dtype=np.float32))
+    assert -4e-6 < worth[0, 0] < -3e-6
+    got = pkg.beam_select(torch.from_numpy(logits).cuda(), torch.zeros(1, 1, device="cuda"))
+    assert got[0].item() == 0 and got[1].item() == 0
+    # an exponential: its argument of 18 rounded twice (2 * 18 * 2^-24) and two units of its own
+    assert abs(got[2].item() - worth[0, 0]) <= abs(worth[0, 0]) * (36 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -24)
