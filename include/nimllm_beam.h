@@ -44,7 +44,10 @@ extern "C" {
  * or NaN (a first step, say, has score 0 for one beam and -infinity for the
  * others).  Logits of +infinity share the probability of their row.
  *
- * A row takes part with its `beams` largest logits (of equal ones the lowest v).
+ * A row takes part with its `beams` largest logits (of equal ones the lowest v);
+ * where it is read in parts, of 2048 or 8192, with as many of each.  (It shows only
+ * where so many unlike logits are worth the same in float64, beside scores 10^15
+ * times their difference.)
  * Candidates are compared in float64: the exponentials of a row and the sums
  * of up to 32 of them are fp32, everything after that is float64; scores are
  * rounded once to fp32.  d_out_scores may be d_scores, and d_out_ended d_ended.

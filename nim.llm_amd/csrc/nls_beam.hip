@@ -284,14 +284,15 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
   Candidate last{__builtin_inf(), -1};
   for (int r = 0; r < a.beams; ++r) {
     Candidate c{none, 0};
-    for (int i = threadIdx.x; i < lists; i += kNT)
+    for (int i = threadIdx.x; i < lists; i += kNT) {
+      Candidate first{none, 0};  // of this list, which is in the order of its logits: equal worths may not be
       for (int k = 0; k < a.beams; ++k) {
         const Candidate o = candidate(i, k);
-        if (!(o.c > none)) break;
-        if (!before(last, o)) continue;
-        if (c.c == none || before(o, c)) c = o;
-        break;  // (a list is in order)
+        if (!(o.c > none) || o.c < first.c) break;
+        if (before(last, o) && (first.c == none || before(o, first))) first = o;
       }
+      if (first.c > none && (c.c == none || before(first, c))) c = first;
+    }
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
       const Candidate o{__shfl_xor(c.c, d), __shfl_xor(c.at, d)};

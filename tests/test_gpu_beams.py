@@ -434,3 +434,17 @@ def test_sums_of_a_row_across_lanes(pkg):
     assert got[0].item() == 0 and got[1].item() == 0
     # an exponential: its argument of 18 rounded twice (2 * 18 * 2^-24) and two units of its own
     assert abs(got[2].item() - worth[0, 0]) <= abs(worth[0, 0]) * (36 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -24)
+
+
+def test_equal_candidates_of_unequal_logits_beyond_the_lists(pkg):
+    """Logits that are equal beside the rest of a candidate, in float64, and more
+    candidates than the merge holds: the lowest ids come first all the same."""
+    beams, vocab = 64, 40000
+    logits, scores = np.zeros((beams, vocab), dtype=np.float32), np.full((1, beams), -3.0, dtype=np.float32)
+    far = np.arange(1000, 1010)
+    logits[:, far] = 1e-20
+    p, t, s, e = (x.cpu().numpy() for x in pkg.beam_select(torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda()))
+    # a row's 64 largest logits: the ten, and the lowest 54 of the others
+    assert np.array_equal(t[0], np.concatenate([np.arange(54), far])) and (p == 0).all() and (e == 0).all()
+    want = -3.0 - math.log(vocab)
+    assert (np.abs(s - want) <= LSE + 2.0 ** -24 * abs(want)).all()
