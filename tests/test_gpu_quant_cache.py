@@ -869,3 +869,61 @@ def test_attention_a_neighbour_that_is_not_finite(pkg, kind, dtype, d, lens, new
     say(f"[nan neighbour] {kind} {NAME[dtype]} d={d} {lens}")
     got, _ = m.check(pkg)
     assert torch.isfinite(got[:new[0] - 1].float()).all() and torch.isnan(got[new[0] - 1].float()).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,rot,interleaved,off", [(F32, 64, False, 0), (BF16, 64, True, 0), (F16, 32, False, 1), (BF16, 0, False, 0)])
+def test_many_tokens_are_written_and_read_as_few_are(pkg, kind, dtype, rot, interleaved, off):
+    """A call of so many tokens that a workgroup takes several at a time, of ragged
+    and empty sequences, against the same sequences in calls that do not."""
+    d, kvh, heads, page, seqs, slots = 96, 2, 3, 16, 190, 200
+    rng, g = random.Random(rot + off), torch.Generator().manual_seed(rot)
+    new = [rng.choice([0, 0, 1, 2, 7, 19, 40]) for _ in range(seqs - 1)] + [600]
+    cut = 90
+    lens = [rng.randint(0, 60) for _ in range(slots)]
+    slot_of = rng.sample(range(slots), seqs)
+    slot_of[3], slot_of[5] = -1, slots + 4
+    for i in range(seqs):
+        if 0 <= slot_of[i] < slots and i % 7:
+            lens[slot_of[i]] += new[i]  # else some are shorter than their rows
+    per = 45
+    table = [[rng.choice([-1, 10 ** 6]) if rng.random() < 0.05 else s * per + j for j in range(per)] for s in range(slots)]
+    starts = [5]
+    for n in new:
+        starts.append(starts[-1] + n)
+    tokens = starts[-1] + 9
+    assert tokens > 2048
+    fmt = pkg.PageFormat(kind, kvh, page, d)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    rows = [torch.randn(tokens, h, d + off, generator=g).to(dtype).cuda()[..., off:] for h in (heads, kvh, kvh)]
+    plan = pkg.rope_plan(rot, interleaved=interleaved) if rot else None
+    tb, ln, sl = ints(table), ints(lens), ints(slot_of)
+    fill = torch.randint(0, 120, (slots * per, fmt.page_bytes), dtype=torch.uint8, generator=g).cuda()  # (no factor is NaN)
+    whole, parts = fill.clone(), fill.clone()
+    out, k, v = (torch.full_like(x, 7) for x in rows)
+    pkg.cache_append(whole, tb, ln, ints(starts), rows[1], rows[2], q=rows[0], plan=plan, slots=sl, out=out, fmt=fmt)
+    pkg.cache_read(whole, tb, ln, ints(starts), tokens, k=k, v=v, slots=sl, fmt=fmt)
+    out2, k2, v2 = (torch.full_like(x, 7) for x in rows)
+    for a, b in ((0, cut), (cut, seqs)):
+        lo, hi = (0 if a == 0 else starts[a]), (tokens if b == seqs else starts[b])
+        assert hi - lo < 2048
+        st, part = ints([s - lo for s in starts[a:b + 1]]), slice(lo, hi)
+        pkg.cache_append(parts, tb, ln, st, rows[1][part], rows[2][part], q=rows[0][part], plan=plan, slots=sl[a:b], out=out2[part], fmt=fmt)
+        pkg.cache_read(parts, tb, ln, st, hi - lo, k=k2[part], v=v2[part], slots=sl[a:b], fmt=fmt)
+    assert torch.equal(whole, parts) and not torch.equal(whole, fill)
+    for x, y in ((out, out2), (k, k2), (v, v2)):
+        assert torch.equal(x, y) and bool((x[:5] == 7).all()) and bool((x[-9:] == 7).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAME.get)
+@pytest.mark.parametrize("max_new,max_len", [(1, 1), (1, 100000), (4096, 1), (7, 600)])
+def test_attention_hints_that_are_wrong(pkg, kind, dtype, max_new, max_len):
+    m = Made(pkg, kind, [700, 90, 1, 1300], [50, 3, 1, 1], 8, 2, 64, 32, dtype, seed=max_new)
+    for window, first in ((0, None), (65, [3, 0, 0, 1200])):
+        want, lse, ob, lb = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, m.scale, window, first)
+        f = None if first is None else torch.tensor(first, dtype=torch.int32).cuda()
+        got, l = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), max_new=max_new,
+                                     max_len=max_len, window=window, first=f, lse=True, fmt=m.fmt)
+        near(got, want, ob, "out")
+        near(l, lse, lb, "lse")
