@@ -329,7 +329,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         }
       }
     };
-    // the largest factor of the lanes, and the power of two above it
+    // the largest factor of the lanes, the power of two above it (of denormal ones too),
+    // and the largest one below that
     auto wave_top = [&](uint32_t d) {
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) {
@@ -338,7 +339,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       }
       return d;
     };
-    auto above = [](uint32_t d) { return d < 0x400u ? -14 : (int)(d >> 10) - 14; };
+    auto above = [](uint32_t d) { return d < 0x400u ? 8 - __builtin_clz(d) : (int)(d >> 10) - 14; };
+    auto below = [](int e) { return e < -14 ? (1u << (e + 24)) - 1 : (uint32_t)(e + 14) << 10 | 0x3ffu; };
     // a lane's 4 tokens' factors of a plane of sh_f (token 4 r + g of a run is at 4 g + r)
     auto factors_of = [&](int plane, int s) { return *reinterpret_cast<const u2*>(factors + plane * (KT / 2) + s * 8 + g * 2); };
 
@@ -384,7 +386,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         if (__ballot(dtop > most)) {
           const uint32_t d = wave_top(dtop);
           if (d > most) {
-            const int e = above(d), off = e > 0 ? (e + 1) / 2 : 0;  // of the weights' exponents
+            const int e = max(above(d), -15), off = e > 0 ? (e + 1) / 2 : 0;  // off: of the weights' exponents
             const float shrink = ldexpf(1.f, e_of - e);
             l *= exp2_(up - off);
             back += up - off;
@@ -392,7 +394,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
             for (int t = 0; t < 2 * GT; ++t) o[t] *= shrink;
             e_of = e;
-            most = (uint32_t)(e + 14) << 10 | 0x3ffu;
+            most = below(e);
             lift = (uint32_t)(15 + off - e) << 10;
             lift |= lift << 16;
           }
@@ -465,7 +467,7 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
           if (d > most) {
             const int e = above(d);
             up = (float)e;
-            most = (uint32_t)(e + 14) << 10 | 0x3ffu;
+            most = below(e);
           }
         }
         top = ceilf(fmaxf(top, m));  // whole: what it is taken from is exact

@@ -927,3 +927,29 @@ def test_attention_hints_that_are_wrong(pkg, kind, dtype, max_new, max_len):
                                      max_len=max_len, window=window, first=f, lse=True, fmt=m.fmt)
         near(got, want, ob, "out")
         near(l, lse, lb, "lse")
+
+
+@pytest.mark.parametrize("kind,value", [("q8_0", 7.6e-6), ("q4_0", 4.2e-7), ("q4_0", 3e-6)])
+def test_attention_factors_of_denormal_size(pkg, kind, value):
+    """Values whose factors are the least that fp16 holds, and small weights: their
+    product is 22 bits of fp32 queries' all the same."""
+    d, n = 64, 512
+
+    def contents(gen, shape):
+        x = np.zeros(shape, dtype=np.float32)
+        x[:, 0], x[:, 1] = -0.027, value
+        for far in (7, 39, 71, 103):
+            x[:, 0, :, far::256] = 1.0
+            x[:, 1, :, far::256] = 0.0
+        return x
+
+    m = Made(pkg, kind, [n], [1], 4, 1, d, 512, F32, seed=3, contents=contents)
+    m.q = torch.ones(1, 4, d)
+    scale = 20.3 * math.log(2.0) / d / float(m.values()[m.table_l[0][0], 0, 0, 7, 0])
+    want, _, _, _ = R.attend(m.q, m.values(), kind, m.table_l, m.lens_l, m.starts_l, scale)
+    assert (want > 0).all()
+    got = pkg.paged_attention(m.q.cuda(), m.kv_cuda(), m.table.cuda(), m.lens.cuda(), m.starts.cuda(), 1, n, scale=scale, fmt=m.fmt)
+    # scores of 20 (in exponents of base 2): 64 products and sums, a rounding each of
+    # factor, scale and exponent, 70 * 20 * 2^-24; exponentials, the two parts, and
+    # sums of 512 terms in fp32
+    near(got, want, np.abs(want) * (70 * 20 * 2.0 ** -24 + 2.0 ** -21 + 2 * 528 * 2.0 ** -24 + 2.0 ** -23), kind)
