@@ -448,3 +448,18 @@ def test_equal_candidates_of_unequal_logits_beyond_the_lists(pkg):
     assert np.array_equal(t[0], np.concatenate([np.arange(54), far])) and (p == 0).all() and (e == 0).all()
     want = -3.0 - math.log(vocab)
     assert (np.abs(s - want) <= LSE + 2.0 ** -24 * abs(want)).all()
+
+
+@pytest.mark.parametrize("groups,beams,vocab", [(2, 48, 32000), (2, 56, 128256), (3, 64, 8000), (2, 64, 32000), (1, 64, 128256),
+                                                (1, 33, 262144)])
+def test_selection_of_many_beams(pkg, groups, beams, vocab):
+    """Ordinary logits with as many beams as overflow the slices' lists and the
+    merge's."""
+    logits, scores = made(groups + beams + vocab, groups, beams, vocab)
+    say(f"[beams] {groups}x{beams}x{vocab}")
+    check(pkg, logits, scores)
+    # beams of one score, as after a first step, and logits whose mass is on a few ids
+    g = np.random.default_rng(beams)
+    scores = (g.standard_normal((groups, beams)) * 0.1 - 3).astype(np.float32)
+    logits[:, g.integers(0, vocab, 300)] += np.abs(g.standard_normal(300) * 4).astype(np.float32)
+    check(pkg, logits, scores, (g.random((groups, beams)) < 0.2).astype(np.int32), [5, 7])
