@@ -102,10 +102,12 @@ int32_t nls_rope(const nls_rope_plan* plan, int32_t type, const nls_heads* x, co
  *
  * type NLS_GGML_Q8_0 or NLS_GGML_Q4_0: blocks of 32 elements of a head, an fp16
  * factor d and a whole number c each, value d c, as GGUF's types of those names
- * hold (Q8_0 -127 .. 127, Q4_0 -8 .. 7), but with codes and factors apart and in
- * the order that the kernels take them.  A page is then nls_cache_page_bytes()
- * bytes; page_stride counts bytes (a multiple of 16), the three strides within a
- * page are 0, head_dim is a multiple of 32 and page_size at least 16. */
+ * hold (Q8_0 -127 .. 127, Q4_0 -8 .. 7), but with codes and factors apart, in the
+ * order that the kernels take them, and d never negative (a file's Q4_0 has the
+ * element largest in magnitude at -8 d, whatever its sign).  A page is then
+ * nls_cache_page_bytes() bytes; page_stride counts bytes (a multiple of 16), the
+ * three strides within a page are 0, head_dim is a multiple of 32 and page_size at
+ * least 16. */
 typedef struct nls_paged_kv {
   void* d_kv;
   int32_t type;
@@ -147,13 +149,16 @@ typedef struct nls_chunks {
  * 0; q_out may be q), k turned and v as it is to the pages of their positions,
  * converted to the cache's type.  plan may be NULL (nothing is turned).
  * `type` is that of q, k and v.  Two tokens never share a place, unless a slot
- * is named twice or a page is held twice: then either's row may stay.
+ * is named twice or a page is held twice: then either's row may stay, or parts of
+ * each (of blocks, codes of one with the factor of the other).
  * Blocks (type is then any of the three): the turned elements, unrounded, give
  *   Q8_0  d = fp16(max |x| * (1 / 127)),                  c = rint(x * (1 / d))
  *   Q4_0  d = fp16(max(max x * (1 / 7), min x * (-1 / 8))), c within -8 .. 7
  * in fp32, each operation rounded once.  d is at most 515.5 and 8188, so that
  * fp16 holds d c: elements beyond its range are cut.  All c are 0 where d is 0.  A
- * block with an element that is not finite has d = NaN.
+ * block with an element that is not finite has d = NaN.  (Q4_0: a block's largest
+ * positive element becomes 7 d, where a file's is -8 d of a negative d: normal
+ * elements' mean square error is 1.14 times as large.)
  */
 int32_t nls_cache_append(const nls_paged_kv* kv, const nls_chunks* chunks, const nls_rope_plan* plan, int32_t type,
                          const nls_heads* q, const nls_heads* q_out, int32_t heads, const nls_heads* k,
@@ -197,9 +202,12 @@ int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t
  * rounded to fp16.  F32 queries are two parts of fp16 as above; weights, or their
  * products with the factors, are two parts, 22 bits, for F32 and F16 queries; for
  * BF16 weights and products are rounded to fp16 each (with what both are relative to
- * in exponents of their own, so that small ones keep its 11 bits).  Factors are taken to be as nls_cache_append writes
- * them: 0 to 515.5 or 8188, or NaN.  A key's factor of NaN makes the rows that see
- * the key NaN, a value's the 32 elements of its block in them.
+ * in exponents of their own, so that small ones keep its 11 bits).  A product below
+ * 2^-28 of the largest factor near its key, seen or not, keeps fewer, to 2^-38 of it;
+ * in sequences of more than 16 rows a weight below 2^-21 does, to 2^-32, and values
+ * below 2^-14 are taken to within some 2^-38.  Factors are taken to be as
+ * nls_cache_append writes them: 0 to 515.5 or 8188, or NaN.  A key's factor of NaN
+ * makes the rows that see the key NaN, a value's the 32 elements of its block in them.
  * max_new and max_len say what the caller expects of the longest chunk and
  * context (0: not known).  They choose how the work is split; results hold
  * whatever the true values are.

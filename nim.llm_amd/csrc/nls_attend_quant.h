@@ -12,8 +12,8 @@
 // What bounds it: one pass over the blocks, at what this pattern of loads reaches
 // (6.2 TB/s with nothing done to what arrives), for 8 bits: 64 contexts of 8192,
 // heads of 128, bf16 6.0 TB/s.  For 4 bits the steps between a load and its use
-// take as long as the bytes: 4.4 TB/s there, 3.4 with fp32 queries; 64 contexts of
-// up to 16384 184 us, one of 131071 (fp32) 49.
+// take as long as the bytes: 4.6 TB/s there, 3.6 with fp32 queries; 64 contexts of
+// up to 16384 188 us, one of 131071 (fp32) 49.
 // Measured and left: three waves a SIMD, which do not fit and spill; steps of 64
 // keys, the same; two steps' loads in flight, no faster; codes as they are in the
 // mantissa of a denormal number, which saves the subtraction and no time.  Loads in
@@ -107,6 +107,9 @@ constexpr int weight_parts() {
   return __is_same(T, __bf16) ? 1 : 2;
 }
 // What is read once: bytes that leave the caches to others (kAlign: 4 or more).
+// (Pages that contexts share are read once for each: 8 x 8 contexts of 8000, 7888 of
+// them shared by eight, bf16 over Q4_0 heads of 128 121 us, 132 unshared; a bf16
+// cache, whose keys stay in the caches, 181 and 337.)
 template <int kBytes, int kAlign>
 __device__ __forceinline__ void past_caches(uint32_t* to, const char* from) {
   constexpr int kPiece = kBytes >= 16 ? 16 : kBytes >= 8 ? 8 : 4;
@@ -126,7 +129,7 @@ constexpr float kQuantShift = 14.f;  // log2 of the largest weight times factor
 
 // Heads of NG blocks, at most GT (2, 4 or 8: what the factors are dealt out by).
 // Each number of blocks has its own loads, plane by plane: 32 contexts of 8192, bf16
-// over Q4_0, heads of 96 61 us and of 192 100 (a byte at a time, for any number
+// over Q4_0, heads of 96 63 us and of 192 100 (a byte at a time, for any number
 // below GT, 182 and 518; of the 418 off 192, 34 are its second wave a SIMD).
 template <typename T, int kBits, int GT, int NG>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,

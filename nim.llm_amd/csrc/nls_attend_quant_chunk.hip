@@ -16,11 +16,18 @@
 //       three products: hi hi, hi lo, lo hi.  (fp16 queries with one of each: 924 us
 //       for 1246, and the error half as large again as the output's rounding.)
 //
-// What bounds it: the matrix cores, with the turning of codes into operands on
-// the vector units between their runs.  2048 tokens over 16384 keys, 32 heads on 8
-// of 128, Q4_0: fp32 queries 1370 us, 376 TFLOP/s of the mathematics in two and a
-// half times as many products (two and three for one and one); bf16 797 us, 647 TFLOP/s (a bf16 cache, which
-// has nothing to turn: 572); 4001 tokens of 32 heads of 64, Q8_0, bf16: 156 us.
+// What bounds it: for fp32 queries the matrix cores, with the turning of codes into
+// operands on the vector units between their runs; for 16-bit ones, of half as many
+// products or fewer, that turning and the exponentials as much.  2048 tokens over
+// 16384 keys, 32 heads on 8 of 128, Q4_0: fp32 1320 us, 390 TFLOP/s of the mathematics
+// in two and a half times as many products (two and three for one and one); fp16
+// (one and three) 1125; bf16 (one and one) 805, 640 TFLOP/s (a bf16 cache, which has
+// nothing to turn: 572); 4001 tokens of 32 heads of 64, Q8_0, bf16: 156 us.  Heads
+// beyond 128 have one wave a SIMD and tiles of 32 keys: 512 tokens over 8192, bf16,
+// heads of 128 148 us, of 160 345.
+//
+// Values below fp16's normal numbers (2^-14) leave the products' sums fewer bits: they
+// are taken to within some 2^-38 (measured: 2^-41), whatever their size.
 //
 // Factors outside of the second product as well would be 16 products, splits and
 // conversions per lane, block and part, more than the third matrix product costs.

@@ -10,9 +10,13 @@
 // comes of the lanes' own maxima: the beams-th largest of a wave's 64 is
 // reached by that many logits, and few others reach it.  The second launch, a
 // workgroup per group, joins the slices' sums in float64 and merges their
-// lists in the same way.  64 groups of 8 beams over 128256 (263 MB): 44 us, 6.0
-// TB/s, and 7 for the second launch (whose bound by ballots and lists requested
-// ahead, with fewer instructions a logit in the first, took both from 80 to 51).
+// lists in the same way.  64 groups of 8 beams over 128256, a fifth of them ended
+// (210 MB): 44 us, 4.8 TB/s, and 7 for the second launch (whose bound by ballots and
+// lists requested ahead, with fewer instructions a logit in the first, took both from
+// 80 to 51).  That is what up to 16 beams cost (16 groups of 16 over 128256: 54 us for
+// both).  With more the lists grow long, and are ranked by counting, or pass what LDS
+// holds and are taken one after another: 16 groups of 32 272 us, 8 of 48 495, 8 of 64
+// 2930, where the logits are read in 56, 42 and 56.
 #include "nls_beam.h"
 #include "nls_primitives.h"
 
@@ -20,7 +24,7 @@ namespace nls {
 namespace {
 
 constexpr int kNT = kBeamThreads, kWaves = kNT / kWave;
-constexpr int kList = 512;              // logits of a slice that reach the bound, at most
+constexpr int kList = 512;              // logits of a slice that reach the bound, as held
 constexpr int kMerge = 1024;            // candidates of a group likewise
 
 typedef float f4v __attribute__((ext_vector_type(4), aligned(4)));  // (rows may start off 16 bytes)
@@ -121,8 +125,9 @@ __global__ __launch_bounds__(kNT, 4) void beam_slice_kernel(BeamArgs a) {
     for (int i = m + threadIdx.x; i < a.beams; i += kNT) out[i] = {none, -1};
     return;
   }
-  // Too many reach the bound (equal ones): one after another, each the first
-  // behind the one before it.
+  // Too many reach the bound (equal ones, or nearly as many beams as a wave has
+  // lanes, whose least maximum is a low one: two slices of normal logits in a hundred
+  // at 56 beams, all at 64): one after another, each the first behind the one before it.
   BeamEntry last{__builtin_inff(), -1};
   for (int r = 0; r < a.beams; ++r) {
     BeamEntry e{none, 0x7fffffff};
@@ -280,7 +285,7 @@ __global__ __launch_bounds__(kNT) void beam_merge_kernel(BeamArgs a) {
     for (int i = n + threadIdx.x; i < a.beams; i += kNT) put_none(i);
     return;
   }
-  // More than the list holds: one after another.
+  // More than the list holds (most groups of 48 beams and more): one after another.
   Candidate last{__builtin_inf(), -1};
   for (int r = 0; r < a.beams; ++r) {
     Candidate c{none, 0};

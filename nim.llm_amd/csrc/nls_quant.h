@@ -4,6 +4,11 @@
 //   Q8_0  c in -127 .. 127, held as c + 128 in a byte
 //   Q4_0  c in -8 .. 7, held as c + 8 in half a byte
 //
+// (d is not negative; of a file's Q4_0 it may be, so that the largest element is
+// always -8 d.  Here a block whose largest element is positive has that at 7 d: the
+// mean square error of normal elements is 1.27 times theirs there and 1.14 over all.
+// Attention counts on that sign: it compares factors as bits.)
+//
 // A page holds, for each kv head, its keys and then its values: the codes of
 // page_size rows, then the factors, block by block, page_size of each (so that
 // the factors of neighbouring tokens come in one load).  Within a row of codes
