@@ -200,14 +200,13 @@ int32_t nls_cache_read(const nls_paged_kv* kv, const nls_chunks* chunks, int32_t
  * Blocks: d c itself meets the queries and weights, nothing of the cache is
  * rounded but for BF16 queries in sequences of more than 16 rows, where d c is
  * rounded to fp16.  F32 queries are two parts of fp16 as above; weights, or their
- * products with the factors, are two parts, 22 bits, for F32 and F16 queries; for
- * BF16 weights and products are rounded to fp16 each (with what both are relative to
- * in exponents of their own, so that small ones keep its 11 bits).  A product below
- * 2^-28 of the largest factor near its key, seen or not, keeps fewer, to 2^-38 of it;
- * in sequences of more than 16 rows a weight below 2^-21 does, to 2^-32, and values
- * below 2^-14 are taken to within some 2^-38.  Factors are taken to be as
- * nls_cache_append writes them: 0 to 515.5 or 8188, or NaN.  A key's factor of NaN
- * makes the rows that see the key NaN, a value's the 32 elements of its block in them.
+ * products with the factors, are two parts, 22 bits, for F32 and F16 queries, and
+ * rounded to fp16 for BF16.  A product below 2^-28 of the largest factor near its key,
+ * seen or not, keeps fewer bits, to 2^-38 of it; in sequences of more than 16 rows a
+ * weight below 2^-21 does, to 2^-32, and values below 2^-14 are taken to within some
+ * 2^-38.  Factors are taken to be as nls_cache_append writes them: 0 to 515.5 or 8188,
+ * or NaN.  A key's factor of NaN makes the rows that see the key NaN, a value's the 32
+ * elements of its block in them.
  * max_new and max_len say what the caller expects of the longest chunk and
  * context (0: not known).  They choose how the work is split; results hold
  * whatever the true values are.

@@ -13,7 +13,7 @@
 // (6.2 TB/s with nothing done to what arrives), for 8 bits: 64 contexts of 8192,
 // heads of 128, bf16 6.0 TB/s.  For 4 bits the steps between a load and its use
 // take as long as the bytes: 4.6 TB/s there, 3.6 with fp32 queries; 64 contexts of
-// up to 16384 188 us, one of 131071 (fp32) 49.
+// up to 16384 190 us, one of 131071 (fp32) 49.
 // Measured and left: three waves a SIMD, which do not fit and spill; steps of 64
 // keys, the same; two steps' loads in flight, no faster; codes as they are in the
 // mantissa of a denormal number, which saves the subtraction and no time.  Loads in
@@ -99,9 +99,11 @@ template <typename T>
 constexpr int quant_parts() {
   return sizeof(T) == 4 ? 2 : 1;
 }
-// Weights times factors, likewise; for bf16 queries the weights and then the products
-// are rounded to fp16 (each an eighth of the output's own rounding.  Two parts: 64
-// contexts of up to 16384 257 us for 204; 32 of 8192, heads of 128 91 for 71).
+// Weights times factors, likewise; for bf16 queries they are rounded to fp16, once (an
+// eighth of the output's own rounding.  Two parts: 64 contexts of up to 16384 257 us
+// for 204, 32 of 8192, heads of 128 91 for 71.  Weights rounded first, a packed product
+// for two keys then: 192 and 69 for 199 and 72, and twice the error; and small products
+// were lost in fp16's denormal numbers unless the factors were scaled, 195 and 71).
 template <typename T>
 constexpr int weight_parts() {
   return __is_same(T, __bf16) ? 1 : 2;
@@ -129,7 +131,7 @@ constexpr float kQuantShift = 14.f;  // log2 of the largest weight times factor
 
 // Heads of NG blocks, at most GT (2, 4 or 8: what the factors are dealt out by).
 // Each number of blocks has its own loads, plane by plane: 32 contexts of 8192, bf16
-// over Q4_0, heads of 96 63 us and of 192 100 (a byte at a time, for any number
+// over Q4_0, heads of 96 62 us and of 192 101 (a byte at a time, for any number
 // below GT, 182 and 518; of the 418 off 192, 34 are its second wave a SIMD).
 template <typename T, int kBits, int GT, int NG>
 __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts& parts, int tiles, bool chunk_runs,
@@ -222,15 +224,10 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
     f4 o[2 * GT];
 #pragma unroll
     for (int t = 0; t < 2 * GT; ++t) o[t] = f4{0, 0, 0, 0};
-    // A weight times a value's factor is at most 1: 2^e is above any factor so far,
-    // most is that bound as fp16's bits.  Two parts: the weights are taken from m + e.
-    // One part, where weight and factor are rounded by themselves: half of e is taken
-    // off each while it is above 0; else the factors are brought up to 1 (exactly).
-    // So small weights keep clear of fp16's denormal numbers, and so does their product
-    // with small factors.
-    float m = minus_inf(), l = 0.f, up = NW == 1 ? 0.f : -24.f, back = kQuantShift - up;
-    int e_of = NW == 1 ? -15 : -24;
-    uint32_t most = NW == 1 ? 0x1ffu : 0u, lift = 0x78007800u;  // (2^15 twice)
+    // The weights are taken from m + up: 2^up is above any value's factor so far,
+    // so that a weight times a factor is at most 1.  most: that bound as fp16's bits.
+    float m = minus_inf(), l = 0.f, up = -24.f, back = kQuantShift - up;
+    uint32_t most = 0u;
 
     // A step's keys are runs of 16, each within a page (-1: none; what is read
     // there is page 0, and counts for nothing).
@@ -385,27 +382,6 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       dm = __builtin_elementwise_sub_sat(dm, us2{0x8400, 0x8400});
       uint32_t dtop = dm[0] > dm[1] ? dm[0] : dm[1];
       dtop = lane < 32 ? 0 : dtop;
-      if (NW == 1) {
-        if (__ballot(dtop > most)) {
-          const uint32_t d = wave_top(dtop);
-          if (d > most) {
-            const int e = max(above(d), -15), off = e > 0 ? (e + 1) / 2 : 0;  // off: of the weights' exponents
-            const float shrink = ldexpf(1.f, e_of - e);
-            l *= exp2_(up - off);
-            back += up - off;
-            up = (float)off;
-#pragma unroll
-            for (int t = 0; t < 2 * GT; ++t) o[t] *= shrink;
-            e_of = e;
-            most = below(e);
-            lift = (uint32_t)(15 + off - e) << 10;
-            lift |= lift << 16;
-          }
-        }
-        if (lane >= 32)
-#pragma unroll
-          for (int n = 0; n < FW; ++n) fc[n] = __builtin_bit_cast(uint32_t, halves(fc[n]) * halves(lift));
-      }
       {
         uint16_t* to = reinterpret_cast<uint16_t*>(factors) + (lane < 32 ? 0 : GT * KT) + f_x * KT + (f_token & ~15);
 #pragma unroll
@@ -463,9 +439,9 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       top *= sc;
-      if (__ballot(top > m || (NW == 2 && dtop > most))) {
+      if (__ballot(top > m || dtop > most)) {
         float shrink = up;
-        if (NW == 2 && __ballot(dtop > most)) {
+        if (__ballot(dtop > most)) {
           const uint32_t d = wave_top(dtop);
           if (d > most) {
             const int e = above(d);
@@ -499,10 +475,6 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
         p[j] = exp2_(p[j]);
         l += p[j];
       }
-      h2 ph[2 * NR];
-      if constexpr (NW == 1)
-#pragma unroll
-        for (int n = 0; n < 2 * NR; ++n) ph[n] = h2{(_Float16)p[2 * n], (_Float16)p[2 * n + 1]};
       auto values = [&](auto seen) {
 #pragma unroll
         for (int b = 0; b < NR; b += 2)  // 32 keys: the depth of one product
@@ -522,16 +494,14 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 #pragma unroll
               for (int n = 0; n < 4; ++n)
                 d[n] &= ((vis >> (4 * b + 2 * n)) & 1 ? 0xffffu : 0u) | ((vis >> (4 * b + 2 * n + 1)) & 1 ? 0xffff0000u : 0u);
+            float pw[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[4 * b + j], (float)halves(d[j / 2])[j & 1], 0.f);
             h8 pd[NW];
             if constexpr (NW == 1) {
-              u4 r;
 #pragma unroll
-              for (int n = 0; n < 4; ++n) r[n] = __builtin_bit_cast(uint32_t, ph[2 * b + n] * halves(d[n]));
-              pd[0] = __builtin_bit_cast(h8, r);
+              for (int j = 0; j < 8; ++j) pd[0][j] = (_Float16)pw[j];  // (one instruction with the product)
             } else {
-              float pw[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) pw[j] = __builtin_fmaf(p[4 * b + j], (float)halves(d[j / 2])[j & 1], 0.f);
               in_two(pw, pd);
             }
             h8 codes[2];
@@ -563,8 +533,8 @@ __device__ __forceinline__ void few_quant_rows(const AttendArgs& a, const Parts&
 
     // the waves' sums, relative to the largest of their maxima alone
     m *= rest;
-    const float full = NW == 1 ? ldexpf(1.f, e_of) : exp2_(up);
-    l *= exp2_(up);
+    const float full = exp2_(up);
+    l *= full;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g == 0) {
